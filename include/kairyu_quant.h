@@ -403,6 +403,77 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
                                     const float* s2, int32_t* topk_idx, float* topk_w, void* out,
                                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------- paged e4m3 key/value cache
+ * k_cache and v_cache are e4m3 [pages, kv_heads, page_size, dim] and their
+ * scales fp32 [pages, kv_heads]: a stored element is code * scale.  Page size
+ * 16, 32, 64 or 128 tokens, dim 64, 128 or 256.  Rows [cu[s], cu[s + 1]) of the
+ * packed activations are sequence s's new tokens, the last ones of its
+ * lengths[s] tokens (new ones included); token t lies in page
+ * table[s][t / page_size].  cu int32 [seqs + 1], lengths int32 [seqs], table
+ * int32 [seqs, table_width] with row pitch table_ld, all read on the device
+ * only: nothing synchronizes, so the calls can be captured.  A table entry
+ * outside [0, pages) holds no tokens (they are neither stored nor seen), nor
+ * does a position past the table.  Rows of no sequence are padding: their
+ * outputs are zero and nothing is stored for them.  `*_ld` and `*_hs` are the
+ * pitches in elements from row to row and from head to head (multiples of 8;
+ * rows 16-byte aligned). */
+
+/* Rotation of queries and keys by position and the append of keys and values.
+ * cos_sin fp32 [positions, rotary] holds each position's rotary / 2 cosines,
+ * then its sines (null: no rotation; a position past the table becomes NaN);
+ * rotary a multiple of 16 up to dim, pairs rotary / 2 apart or (interleaved)
+ * neighbouring; q_norm / k_norm [dim] of the activations' dtype, or null, are
+ * weights of a per-head RMS norm before it.  q_out [rows, heads, dim] receives
+ * the queries.  A page's scale is 2^e with the smallest e that holds
+ * max(amax, 1e-12) <= 448 * 2^e over its tokens of this call, and not below the
+ * scale it has where it holds earlier tokens, which move to the new scale.  A
+ * token whose rotated key or whose value has a non-finite element in a head is
+ * stored there as a key of NaN codes, and those elements of its value as 0.  No
+ * page may be written for two sequences by one call.  Replaces the rotary and
+ * paged-write kernels (kairyu/kernels/rope_gpu.py, paged_kv_write_gpu.py) for
+ * an 8-bit cache. */
+int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld, int64_t k_hs,
+                        const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
+                        int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                        float* v_scale, int64_t pages, int64_t page_size, const int32_t* table, int64_t table_ld,
+                        int64_t table_width, const int32_t* cu, const int32_t* lengths, int64_t seqs,
+                        const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
+                        const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream);
+
+/* out[r, h] = sum_t softmax_t(scale * q[r, h] . k_t) v_t over the tokens t that
+ * row r sees in its sequence's pages, kv head h / (heads / kv_heads): all of
+ * them, or (causal) those up to its own position, at most the last `window`
+ * where that is positive.  A row that sees none is zero.  Stored values must not
+ * be NaN codes in slots that hold tokens (slots past a sequence's end may hold
+ * anything); NaN keys make the rows that see them NaN and no other.  out
+ * [rows, heads, dim].  Workspace: kq_kv_attention_workspace_size bytes.
+ * Replaces the paged attention backends (kairyu/engine/core/attention/) for an
+ * 8-bit cache. */
+int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
+                    int64_t kv_heads, int64_t dim, const uint8_t* k_cache, const uint8_t* v_cache,
+                    const float* k_scale, const float* v_scale, int64_t pages, int64_t page_size,
+                    const int32_t* table, int64_t table_ld, int64_t table_width, const int32_t* cu,
+                    const int32_t* lengths, int64_t seqs, float scale, int causal, int64_t window, void* out,
+                    void* workspace, size_t workspace_bytes, void* stream);
+size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size,
+                                      int64_t table_width, int64_t seqs);
+
+/* The norms around a decoder block, rows of `hidden` <= 32768 elements:
+ * r = residual + residual_scale * gate * (x / rms(x) * (offset + post)) and
+ * y = r / rms(r) * (offset + weight), rms(z) = sqrt(mean(z^2) + eps), all in
+ * fp32.  post null: x as it is; gate null: 1 (gate_ld 0: one row for all);
+ * residual null: 0.  r_out [rows, hidden] of residual_dtype (dtype or fp32);
+ * y_out [rows, hidden] by mode: 0 in dtype, 1 e4m3 and 2 int8 with a scale per
+ * row in scales [rows] (max(amax, 1e-12) / 448 and / 127), 3 e4m3 with a scale
+ * per 128 elements in scales [rows, ceil(hidden / 128)]: the forms of
+ * kq_act_quant_fp8, kq_act_quant_i8 and kq_act_quant_fp8_blocks, of y before
+ * its rounding to 16 bits.  Replaces the RMS norm kernels
+ * (kairyu/kernels/rms_norm_gpu.py). */
+int kq_block_norm(const void* x, int dtype, int64_t rows, int64_t hidden, int64_t x_ld, const void* residual,
+                  int residual_dtype, int64_t residual_ld, const void* post, const void* gate, int64_t gate_ld,
+                  float residual_scale, const void* weight, float offset, float eps, int mode, void* r_out,
+                  void* y_out, float* scales, void* stream);
+
 /* ---------------------------------------------------------------- ceilings
  * Measurement aids, no counterpart in the reference: the box's own ceilings
  * that bench.py --peaks reports next to the vendor peaks.  `sink` is device

@@ -38,6 +38,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 
 _SIGNATURES: dict[str, list] = {
     "kq_version": [],
@@ -99,6 +100,18 @@ _SIGNATURES: dict[str, list] = {
     "kq_moe_routed_block_fp8_experts": [
         _P, _I, _I, _P, _I, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P,
     ],
+    "kq_kv_rotate_append": [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
+        _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I, _P, _P, _F, _P, _P,
+    ],
+    "kq_kv_attention": [
+        _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
+        _F, _I, _I64, _P, _P, _SZ, _P,
+    ],
+    "kq_kv_attention_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "kq_block_norm": [
+        _P, _I, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _I64, _F, _P, _F, _F, _I, _P, _P, _P, _P,
+    ],
 }
 
 _lock = threading.Lock()
@@ -133,7 +146,8 @@ def _load() -> ctypes.CDLL:
                           "kq_w8a8_linear_workspace_size": ctypes.c_size_t,
                           "kq_w8a8_swiglu_workspace_size": ctypes.c_size_t,
                           "kq_block_fp8_workspace_size": ctypes.c_size_t,
-                          "kq_moe_workspace_size": ctypes.c_size_t}.get(name, ctypes.c_int)
+                          "kq_moe_workspace_size": ctypes.c_size_t,
+                          "kq_kv_attention_workspace_size": ctypes.c_size_t}.get(name, ctypes.c_int)
         _lib = lib
         return lib
 

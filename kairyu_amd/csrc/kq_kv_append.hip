@@ -1,0 +1,387 @@
+// Rotary positions and the append to a paged e4m3 cache in one launch.
+//
+// Query and key heads (optionally normed per head, x / rms(x) * weight) turn by
+// their position's angles, x1' = x1 cos - x2 sin, x2' = x2 cos + x1 sin, from the
+// caller's fp32 table of cos and sin; rotated queries are written in 16 bits, keys
+// and values as e4m3 codes of x * 2^-e with one exponent per page and head: the
+// smallest e with max |x| <= 448 * 2^e over what the page is given, and never below
+// the exponent it has already where it holds earlier tokens.  A page whose exponent
+// grows has its earlier codes moved to the new scale.  Powers of two make that move
+// exact (but for codes that fall below e4m3's normal range, which round once more),
+// and dividing by the scale as well; a floating-point code loses nothing to a scale
+// that is up to twice as large as it had to be.
+//
+// A token whose rotated key or whose value is not finite in a head is stored there
+// as a key of NaN codes, and such elements of its value as 0: every row that attends
+// to it becomes NaN and no row that does not, since no 0 * NaN enters a sum of values.
+#include "kq_kv.h"
+
+#include <algorithm>
+
+namespace kq {
+
+struct AppendArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_ld, k_ld, v_ld;  // elements from one row to the next
+  int64_t q_hs, k_hs, v_hs;  // and from one head to the next
+  uint16_t* q_out;           // [rows][heads][D]
+  const float* cos_sin;      // [positions][rotary]: cos, then sin; null: no rotation
+  int64_t positions;
+  const uint16_t* q_norm;
+  const uint16_t* k_norm;
+  float eps;
+  int heads, rotary, interleaved;
+  int page_units;  // workgroups of the append (the rest rotate queries)
+};
+
+KQ_DEV void widen(u32x4 raw, int dtype, float v[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = act_lo(raw[j], dtype);
+    v[2 * j + 1] = act_hi(raw[j], dtype);
+  }
+}
+
+// 8 elements [8c, 8c + 8) of one head's row, normed and rotated.  `row` points at
+// the row; D / 8 neighbouring lanes hold one row (all of them active), so the norm's
+// sum goes over lanes.  Half-split pairs lie rotary / 2 apart: the partner chunk is
+// read again (from L1) instead of exchanged, which keeps any rotary width.
+template <int D>
+KQ_DEV void turn(const uint16_t* row, int c, int pos, const AppendArgs& a, const uint16_t* norm, int dtype, float x[8]) {
+  widen(*(const u32x4*)(row + 8 * c), dtype, x);
+  const int half = a.rotary >> 1;
+  const bool turned = a.cos_sin != nullptr && 8 * c < a.rotary;
+  float y[8];
+  const int pc = 8 * c < half ? 8 * c + half : 8 * c - half;  // partner chunk's first element
+  const bool split = turned && !a.interleaved;
+  if (split) widen(*(const u32x4*)(row + pc), dtype, y);
+  if (norm != nullptr) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+#pragma unroll
+    for (int off = 1; off < D / 8; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
+    float w[8];
+    widen(*(const u32x4*)(norm + 8 * c), dtype, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+    if (split) {
+      widen(*(const u32x4*)(norm + pc), dtype, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * w[e];
+    }
+  }
+  if (!turned) return;
+  if (pos >= a.positions) {  // no angle for it
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
+    return;
+  }
+  const float* cs = a.cos_sin + (int64_t)pos * a.rotary;
+  if (a.interleaved) {
+    const f32x4 co = *(const f32x4*)(cs + 4 * c), si = *(const f32x4*)(cs + half + 4 * c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = x[2 * e], r = x[2 * e + 1];
+      x[2 * e] = p * co[e] - r * si[e];
+      x[2 * e + 1] = r * co[e] + p * si[e];
+    }
+  } else {
+    const bool low = 8 * c < half;
+    const float* at = cs + (low ? 8 * c : 8 * c - half);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float co = at[e], si = at[half + e];
+      x[e] = low ? x[e] * co - y[e] * si : x[e] * co + y[e] * si;
+    }
+  }
+}
+
+// 2^e, the smallest with amax <= 448 * 2^e (448 = 7 * 2^6); amax at least 1e-12
+KQ_DEV float kv_scale_for(float amax) {
+  const uint32_t u = __float_as_uint(fmaxf(amax, 1e-12f));
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);  // 448 = 1.75 * 2^8
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+KQ_DEV bool finite8(const float v[8]) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ok = ok && fabsf(v[e]) <= 3.402823466e38f;
+  return ok;
+}
+
+KQ_DEV u32x2 encode8(const float v[8], float inv) {
+  u32x2 w;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = fminf(fmaxf(v[4 * h + e] * inv, -448.0f), 448.0f);
+    w[h] = pack4_e4m3(t[0], t[1], t[2], t[3]);
+  }
+  return w;
+}
+
+// Four codes of earlier tokens on a new scale: code * ratio, rounded again.
+KQ_DEV uint32_t move4(uint32_t w, float ratio) {
+  float t[4];
+  uint32_t nan = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t b = (w >> (8 * e)) & 0xffu;
+    t[e] = e4m3_to_f32(b);
+    if ((b & 0x7fu) == 0x7fu) {
+      nan |= 0xffu << (8 * e);
+      t[e] = 0.0f;
+    }
+    t[e] = fminf(fmaxf(t[e] * ratio, -448.0f), 448.0f);
+  }
+  return (pack4_e4m3(t[0], t[1], t[2], t[3]) & ~nan) | (w & nan);
+}
+
+// Workgroups [0, page_units) : one page of one sequence and one kv head each, its
+// new tokens in registers (NCH chunks of 8 elements a thread, keys and values).
+// The others: query rows, 2048 / D heads each.
+template <int D, int NCH, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
+  constexpr int CPR = D / 8;             // chunks (threads) of a head's row
+  constexpr int ROWS = THREADS / CPR;    // rows a workgroup holds at once
+  const int tid = (int)threadIdx.x, c = tid % CPR, rr = tid / CPR;
+  if ((int)blockIdx.x >= a.page_units) {
+    const int64_t unit = (int64_t)(blockIdx.x - a.page_units) * ROWS + rr;
+    const int64_t row_ = unit / a.heads;
+    const int head = (int)(unit - row_ * a.heads);
+    const int row = (int)(row_ < batch.rows ? row_ : batch.rows - 1);
+    // the sequence of the wave's first row, then a few steps from it
+    const int row0 = __builtin_amdgcn_readfirstlane(row);
+    int s = 0;
+    for (int s0 = 0; s0 < batch.seqs; s0 += 64) {
+      const bool past = s0 + lane_id() < batch.seqs && batch.cu[s0 + lane_id() + 1] <= row0;
+      s += (int)__popcll(__ballot(past));
+    }
+    while (s < batch.seqs && batch.cu[s + 1] <= row) ++s;
+    const bool padding = s >= batch.seqs || row < batch.cu[s];
+    const int pos = padding ? -1 : batch.lengths[s] - (batch.cu[s + 1] - row);
+    float x[8];
+    turn<D>(a.q + (int64_t)row * a.q_ld + (int64_t)head * a.q_hs, c, max(pos, 0), a, a.q_norm, dtype, x);
+    if (row_ < batch.rows) {
+      u32x4 w = {0, 0, 0, 0};
+      if (pos >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pack_act2(x[2 * j], x[2 * j + 1], dtype);
+      }
+      *(u32x4*)(a.q_out + ((int64_t)row * a.heads + head) * D + 8 * c) = w;
+    }
+    return;
+  }
+
+  __shared__ uint32_t red[2][THREADS / 64];
+  const int shift = cache.page_shift, page_size = 1 << shift;
+  const int head = (int)blockIdx.x % cache.kv_heads;
+  int nth;
+  const int s = kv_find((int)blockIdx.x / cache.kv_heads, batch.seqs, nth, [&](int i) {
+    const KvSeq q = kv_seq(batch, i, shift);
+    const int lo = max(q.first, 0);
+    return q.rows > 0 && lo < q.tokens ? ((q.tokens - 1) >> shift) - (lo >> shift) + 1 : 0;
+  });
+  if (s < 0) return;
+  const KvSeq q = kv_seq(batch, s, shift);
+  const int slot = (max(q.first, 0) >> shift) + nth;
+  const int page = kv_page(batch, cache, s, slot);
+  if (page < 0) return;
+  const int lo = max(max(q.first, 0), slot << shift), hi = min(q.tokens, (slot + 1) << shift);  // positions stored here
+  const int kept = lo & (page_size - 1);                                                        // earlier tokens
+
+  float k[NCH][8], v[NCH][8];
+  uint32_t bad = 0;
+  float ka = 0.0f, va = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int pos = lo + i * ROWS + rr;
+    if (pos >= hi) continue;  // (whole rows: a row's lanes stay together)
+    const int64_t row = q.row0 + (pos - q.first);
+    turn<D>(a.k + row * a.k_ld + (int64_t)head * a.k_hs, c, pos, a, a.k_norm, dtype, k[i]);
+    widen(*(const u32x4*)(a.v + row * a.v_ld + (int64_t)head * a.v_hs + 8 * c), dtype, v[i]);
+    int ok = finite8(k[i]) && finite8(v[i]);
+#pragma unroll
+    for (int off = 1; off < CPR; off <<= 1) ok &= __shfl_xor(ok, off, 64);
+    if (!ok) bad |= 1u << i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!(fabsf(v[i][e]) <= 3.402823466e38f)) v[i][e] = 0.0f;
+      if (ok) ka = fmaxf(ka, fabsf(k[i][e]));
+      va = fmaxf(va, fabsf(v[i][e]));
+    }
+  }
+  const uint32_t kb = wave_max_u32_dpp(__float_as_uint(ka)), vb = wave_max_u32_dpp(__float_as_uint(va));
+  if (lane_id() == 0) {
+    red[0][wave_id()] = kb;
+    red[1][wave_id()] = vb;
+  }
+  __syncthreads();
+  uint32_t kt = 0, vt = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    kt = max(kt, red[0][w]);
+    vt = max(vt, red[1][w]);
+  }
+  const int64_t tile = (int64_t)page * cache.kv_heads + head;
+  uint8_t* kc = cache.k + (tile << shift) * D;
+  uint8_t* vc = cache.v + (tile << shift) * D;
+  float ks = kv_scale_for(__uint_as_float(kt)), vs = kv_scale_for(__uint_as_float(vt));
+  if (kept > 0) {
+    const float ko = cache.k_scale[tile], vo = cache.v_scale[tile];
+    // (every thread has read the scales before one writes them)
+    __syncthreads();
+    const float kn = fmaxf(ks, ko), vn = fmaxf(vs, vo);
+    if (kn != ko)
+      for (int i = tid; i < kept * CPR; i += THREADS) {
+        u32x2 w = *(const u32x2*)(kc + 8 * i);
+        w[0] = move4(w[0], ko / kn);
+        w[1] = move4(w[1], ko / kn);
+        *(u32x2*)(kc + 8 * i) = w;
+      }
+    if (vn != vo)
+      for (int i = tid; i < kept * CPR; i += THREADS) {
+        u32x2 w = *(const u32x2*)(vc + 8 * i);
+        w[0] = move4(w[0], vo / vn);
+        w[1] = move4(w[1], vo / vn);
+        *(u32x2*)(vc + 8 * i) = w;
+      }
+    ks = kn;
+    vs = vn;
+  }
+  if (tid == 0) {
+    cache.k_scale[tile] = ks;
+    cache.v_scale[tile] = vs;
+  }
+  const float ki = 1.0f / ks, vi = 1.0f / vs;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int pos = lo + i * ROWS + rr;
+    if (pos >= hi) continue;
+    const int at = (pos & (page_size - 1)) * D + 8 * c;
+    *(u32x2*)(kc + at) = (bad >> i) & 1 ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : encode8(k[i], ki);
+    *(u32x2*)(vc + at) = encode8(v[i], vi);
+  }
+}
+
+int kv_check(const char* what, int dtype, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+             int64_t page_size, int64_t pages, int64_t seqs, int64_t table_width, int64_t table_ld) {
+  if (dtype != KQ_DTYPE_F16 && dtype != KQ_DTYPE_BF16) {
+    set_error("%s: activation dtype must be fp16 or bf16 (code %d)", what, dtype);
+    return KQ_EUNSUPPORTED;
+  }
+  if (dim != 64 && dim != 128 && dim != 256) {
+    set_error("%s: head dim must be 64, 128 or 256, got %lld", what, (long long)dim);
+    return KQ_EINVAL;
+  }
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) {
+    set_error("%s: page size must be 16, 32, 64 or 128 tokens, got %lld", what, (long long)page_size);
+    return KQ_EINVAL;
+  }
+  if (rows < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || pages < 0 || seqs < 0 || table_width < 0 ||
+      table_ld < table_width) {
+    set_error("%s: bad shape rows=%lld heads=%lld kv_heads=%lld pages=%lld seqs=%lld table=[%lld, pitch %lld]", what,
+              (long long)rows, (long long)heads, (long long)kv_heads, (long long)pages, (long long)seqs,
+              (long long)table_width, (long long)table_ld);
+    return KQ_EINVAL;
+  }
+  // 32-bit row, page and unit counts inside the kernels
+  if (rows > (1 << 24) || heads > 1024 || pages > 0x7fffffffLL || seqs > (1 << 24) || table_width > (1 << 24) / page_size * 64) {
+    set_error("%s: rows=%lld, heads=%lld, pages=%lld, seqs=%lld or table width %lld past the supported range", what,
+              (long long)rows, (long long)heads, (long long)pages, (long long)seqs, (long long)table_width);
+    return KQ_EINVAL;
+  }
+  return KQ_OK;
+}
+
+template <int D, int NCH, int THREADS>
+static void launch_append(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+  const int rows = THREADS / (D / 8);
+  const int64_t query = ((int64_t)b.rows * a.heads + rows - 1) / rows;
+  hipLaunchKernelGGL((kv_append_kernel<D, NCH, THREADS>), dim3((unsigned)(a.page_units + query)), dim3(THREADS), 0, st, a, c, b,
+                     dtype);
+}
+
+// A page's tokens in registers: 256 threads hold 2048 elements a chunk; pages of 8
+// chunks and more go to 1024 threads instead of more registers.
+template <int D>
+static void pick_append(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+  const int chunks = (D << c.page_shift) / 2048;
+  if (chunks <= 1)
+    launch_append<D, 1, 256>(a, c, b, dtype, st);
+  else if (chunks == 2)
+    launch_append<D, 2, 256>(a, c, b, dtype, st);
+  else if (chunks <= 4)
+    launch_append<D, 4, 256>(a, c, b, dtype, st);
+  else if (chunks <= 8)
+    launch_append<D, 2, 1024>(a, c, b, dtype, st);
+  else
+    launch_append<D, 4, 1024>(a, c, b, dtype, st);
+}
+
+}  // namespace kq
+
+using namespace kq;
+
+extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld, int64_t k_hs,
+                                   const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                                   float* v_scale, int64_t pages, int64_t page_size, const int32_t* table, int64_t table_ld,
+                                   int64_t table_width, const int32_t* cu, const int32_t* lengths, int64_t seqs,
+                                   const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
+                                   const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream) {
+  const char* what = "kq_kv_rotate_append";
+  int rc = kv_check(what, dtype, rows, heads, kv_heads, dim, page_size, pages, seqs, table_width, table_ld);
+  if (rc) return rc;
+  if (cos_sin != nullptr && (rotary < 16 || rotary > dim || rotary % 16 != 0 || positions < 0)) {
+    set_error("%s: rotary width must be a multiple of 16 up to the head dim, got %lld", what, (long long)rotary);
+    return KQ_EINVAL;
+  }
+  const uintptr_t align = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_cache | (uintptr_t)v_cache |
+                          (uintptr_t)cos_sin | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)q_out;
+  if (align % 16 != 0 || (q_ld | q_hs | k_ld | k_hs | v_ld | v_hs) % 8 != 0) {
+    set_error("%s: tensors need 16-byte aligned rows and heads", what);
+    return KQ_EINVAL;
+  }
+  if (rows == 0) return KQ_OK;
+  AppendArgs a{};
+  a.q = (const uint16_t*)q;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.q_ld = q_ld, a.q_hs = q_hs, a.k_ld = k_ld, a.k_hs = k_hs, a.v_ld = v_ld, a.v_hs = v_hs;
+  a.q_out = (uint16_t*)q_out;
+  a.cos_sin = cos_sin;
+  a.positions = positions;
+  a.rotary = cos_sin != nullptr ? (int)rotary : 0;
+  a.interleaved = interleaved;
+  a.q_norm = (const uint16_t*)q_norm;
+  a.k_norm = (const uint16_t*)k_norm;
+  a.eps = eps;
+  a.heads = (int)heads;
+  int shift = 4;
+  while ((1 << shift) < page_size) ++shift;
+  // a sequence of n rows touches at most 1 + ceil((n - 1) / page) pages, and a row at most one
+  const int64_t units = seqs == 0 || pages == 0 ? 0 : std::min<int64_t>(rows, 2 * seqs + rows / page_size);
+  if ((units * kv_heads + rows * heads * dim / 2048 + 1) * 1024 >= (1LL << 32)) {  // threads of one launch
+    set_error("%s: %lld rows of %lld heads are past the supported range", what, (long long)rows, (long long)heads);
+    return KQ_EINVAL;
+  }
+  a.page_units = (int)(units * kv_heads);
+  const KvCache c{k_cache, v_cache, k_scale, v_scale, pages, (int)kv_heads, shift};
+  const KvBatch b{table, cu, lengths, table_ld, (int)seqs, (int)table_width, (int)rows};
+  hipStream_t st = (hipStream_t)stream;
+  if (dim == 64)
+    pick_append<64>(a, c, b, dtype, st);
+  else if (dim == 128)
+    pick_append<128>(a, c, b, dtype, st);
+  else
+    pick_append<256>(a, c, b, dtype, st);
+  return check_launch(what);
+}

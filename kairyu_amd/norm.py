@@ -1,0 +1,132 @@
+"""The norms around a decoder block, fused with its gate and residual scale.
+
+``block_norm`` runs what lies between a block's output projection and the next
+block's first one: the norm after the block, its gate and residual scale, the
+residual sum, and the norm before the next block, whose rows come out in 16 bits
+or already quantized as that projection's kernels take them.  Counterpart of the
+reference's RMS norm kernels (kairyu/kernels/rms_norm_gpu.py) next to this
+package's activation quantizers.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from kairyu_amd import _native
+
+__all__ = ["block_norm"]
+
+MODES = {None: 0, "fp8": 1, "int8": 2, "fp8_block": 3}
+MAX_HIDDEN = 32768
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *,
+               post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               residual_scale: float = 1.0, eps: float = 1e-6, unit_offset: bool = False,
+               quantize: str | None = None) -> tuple[torch.Tensor, ...]:
+    """``r = residual + residual_scale * gate * (x / rms(x) * post_weight)`` and
+    ``y = r / rms(r) * weight`` for rows ``x [..., H]``, ``rms(z) =
+    sqrt(mean(z^2) + eps)``.
+
+    ``x``, the weights ``[H]`` and ``gate`` (``[H]``, or a row for each of ``x``'s)
+    are fp16 or bf16 alike; ``residual`` is of that dtype or fp32 and shaped like
+    ``x`` (None: zero, and ``r`` of ``x``'s dtype).  Without ``post_weight`` the
+    block's output is not normed, without ``gate`` not gated; ``unit_offset`` keeps
+    the norms' weights as their difference from one.  All is computed in fp32; ``r``
+    and ``y`` are each rounded once.
+
+    Returns ``(r, y)``, or with ``quantize`` ``(r, yq, scales)`` as the activation
+    quantizers lay them out: ``"fp8"`` / ``"int8"`` per row (scales ``[..., 1]``),
+    ``"fp8_block"`` per 128 elements (scales ``[..., ceil(H / 128)]``)."""
+
+    if quantize not in MODES:
+        raise ValueError(f"quantize must be one of {tuple(MODES)}, got {quantize!r}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_HIDDEN:
+        raise ValueError(f"rows must have 1 to {MAX_HIDDEN} elements, got {tuple(x.shape)}")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"block_norm supports float16/bfloat16 rows, got {x.dtype}")
+    hidden = x.shape[-1]
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
+        if t is None:
+            continue
+        if t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"{name} must have the rows' dtype and device, got {t.dtype} on {t.device}")
+        if t.shape != (hidden,) and not (name == "gate" and t.shape == x.shape):
+            raise ValueError(f"{name} {tuple(t.shape)} does not match rows {tuple(x.shape)}")
+    if residual is not None:
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match rows "
+                             f"{tuple(x.shape)} on {x.device}")
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"residual must be {x.dtype} or float32, got {residual.dtype}")
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
+        raise RuntimeError("block_norm is for inference: an input requires a gradient")
+    if not x.is_cuda:
+        return _plain(x, residual, weight, post_weight, gate, residual_scale, eps, unit_offset, quantize)
+    from kairyu_amd.kernels import kv_cache_hip as hip
+
+    hip.require_device(x.device, "block_norm")
+    flat = _rows(x, hidden)
+    res = None if residual is None else _rows(residual, hidden)
+    per_row = gate is not None and (gate.dim() > 1 or x.dim() == 1)
+    gates = None if gate is None else _rows(gate, hidden) if per_row else gate.contiguous()
+    rows = flat.shape[0]
+    dtype = x.dtype if residual is None else residual.dtype
+    r = torch.empty(x.shape, device=x.device, dtype=dtype)
+    form = {None: x.dtype, "int8": torch.int8}.get(quantize, torch.float8_e4m3fn)
+    y = torch.empty(x.shape, device=x.device, dtype=form)
+    scales = None
+    if quantize is not None:
+        wide = -(-hidden // 128) if quantize == "fp8_block" else 1
+        scales = torch.empty((*x.shape[:-1], wide), device=x.device, dtype=torch.float32)
+    weight = weight.contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    hip.call_on(
+        x.device, "kq_block_norm", flat.data_ptr(), _native.dtype_code(x.dtype), rows, hidden, flat.stride(0),
+        _native.ptr(res), _native.dtype_code(dtype), 0 if res is None else res.stride(0), _native.ptr(post_weight),
+        _native.ptr(gates), gates.stride(0) if per_row else 0, residual_scale, weight.data_ptr(),
+        1.0 if unit_offset else 0.0, eps, MODES[quantize], r.data_ptr(), y.data_ptr(), _native.ptr(scales),
+    )
+    return (r, y) if scales is None else (r, y, scales)
+
+
+def _rows(x: torch.Tensor, hidden: int) -> torch.Tensor:
+    """``[rows, hidden]`` with unit stride along the row and a pitch of at least its
+    width: a view where ``x`` has one, else a copy."""
+
+    if x.dim() != 2:
+        x = x.reshape(-1, hidden)
+    if x.stride(1) == 1 and (x.stride(0) >= hidden or x.shape[0] <= 1):
+        return x if x.stride(0) >= hidden else x.as_strided(x.shape, (hidden, 1))
+    return x.contiguous()
+
+
+def _rms(x, weight, offset, eps):
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * (weight.to(torch.float32) + offset)
+
+
+def _plain(x, residual, weight, post_weight, gate, residual_scale, eps, unit_offset, quantize):
+    """The definition in fp32 torch operations (CPU tensors)."""
+
+    offset = 1.0 if unit_offset else 0.0
+    b = x.to(torch.float32)
+    if post_weight is not None:
+        b = _rms(b, post_weight, offset, eps)
+    if gate is not None:
+        b = b * gate.to(torch.float32)
+    r = residual_scale * b if residual is None else residual.to(torch.float32) + residual_scale * b
+    y = _rms(r, weight, offset, eps)
+    r = r.to(x.dtype if residual is None else residual.dtype)
+    if quantize is None:
+        return r, y.to(x.dtype)
+    if quantize == "fp8_block":
+        hidden = y.shape[-1]
+        y = torch.nn.functional.pad(y, (0, -hidden % 128)).unflatten(-1, (-1, 128))
+    most = 127.0 if quantize == "int8" else 448.0
+    scales = y.abs().amax(-1, keepdim=True).clamp(min=1e-12) / most
+    z = (y / scales).clamp(-most, most)
+    if quantize == "int8":
+        return r, z.round().to(torch.int8), scales
+    z = z.to(torch.float8_e4m3fn)
+    return (r, z.flatten(-2)[..., :hidden].contiguous(), scales[..., 0]) if quantize == "fp8_block" else (r, z, scales)

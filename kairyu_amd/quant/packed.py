@@ -29,6 +29,11 @@ operand), for W8A8 in one call whose streaming GEMM (M <= 64), panel GEMM (M
 the packed weight per 16-row tile, or gate rows [n0, n0 + 128) paired with up
 rows [I + n0, ...); no second copy).
 
+``attend(x, cache, ...)`` of a (q, k, v) pack returns what the layer's output
+projection takes: the projections, rotary positions and the append to a paged
+8-bit cache, and attention over it (``kairyu_amd/attention.py``; the reference's
+``Attention.forward_decode_tensors``, ``kairyu/models/attention.py:315-351``).
+
 ``create`` returns ``None`` for anything it cannot pack exactly (mixed
 formats, in-features, devices, biases, group sizes, static input scales,
 ``g_idx``; hooked or re-bound modules; ``N`` not a multiple of 16 for the
@@ -267,6 +272,34 @@ class QuantLinearPack:
         out = self._packed(hidden)
         lead = hidden.shape[:-1]
         return tuple(part.reshape(*lead, part.shape[-1]) for part in out.split(self._out_features, -1))
+
+    def attend(self, hidden: torch.Tensor, cache, block_table: torch.Tensor, cu_rows: torch.Tensor,
+               lengths: torch.Tensor, cos_sin: torch.Tensor | None = None, *, scale: float | None = None,
+               causal: bool = True, window: int = 0, interleaved: bool = False, q_norm: torch.Tensor | None = None,
+               k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+        """What the output projection of a decoder layer takes, from a (q, k, v)
+        pack's input: the projections, the rotation of queries and keys and the
+        append of keys and values to ``cache``, and attention over it
+        (:func:`kairyu_amd.attention.rotate_append` and
+        :func:`~kairyu_amd.attention.paged_attention`, whose arguments these are).
+        ``hidden [..., K]`` holds the batch's rows in order; returns ``[...,
+        q_features]``."""
+
+        from kairyu_amd.attention import paged_attention, rotate_append
+
+        heads, dim = cache.k.shape[1], cache.k.shape[3]
+        widths = self._out_features
+        if len(widths) != 3 or widths[1] != heads * dim or widths[2] != heads * dim or widths[0] % (heads * dim):
+            raise ValueError(f"attend needs a (q, k, v) pack of whole head groups over {heads} kv heads of {dim}, "
+                             f"got widths {widths}")
+        if torch.is_grad_enabled() and hidden.requires_grad:
+            raise RuntimeError("attend is for inference: the hidden states require a gradient")
+        with torch.no_grad():
+            q, k, v = (part.reshape(-1, part.shape[-1]).unflatten(-1, (-1, dim)) for part in self(hidden))
+            q = rotate_append(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved=interleaved,
+                              q_norm=q_norm, k_norm=k_norm, eps=eps)
+            out = paged_attention(q, cache, block_table, cu_rows, lengths, scale=scale, causal=causal, window=window)
+        return out.reshape(*hidden.shape[:-1], widths[0])
 
     def swiglu(self, hidden: torch.Tensor) -> torch.Tensor:
         """``silu(gate(x)) * up(x)`` of a (gate, up) pack, as the reference's
