@@ -57,6 +57,21 @@ KQ_DEV int kv_page(const KvBatch& b, const KvCache& c, int s, int slot) {
   return p >= 0 && p < c.pages ? p : -1;
 }
 
+// Sum over lanes 0..l, in registers (DPP row shifts, then the rows' last lanes
+// broadcast to the rows behind them).
+template <int CTRL, int ROWS>
+KQ_DEV int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, ROWS == 0xf);
+}
+KQ_DEV int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15
+  return dpp_add<0x143, 0xc>(v);  // row_bcast:31
+}
+
 // The sequence that unit `u` falls to when sequence s has count(s) units, found by
 // a wave together (64 sequences at a time: one load and a scan, where a binary
 // search would wait for a load at each of its steps), and its index there; -1 past
@@ -64,26 +79,40 @@ KQ_DEV int kv_page(const KvBatch& b, const KvCache& c, int s, int slot) {
 template <typename F>
 KQ_DEV int kv_find(int u, int seqs, int& local, F count) {
   int base = 0;
-  const int lane = lane_id();
   for (int s0 = 0; s0 < seqs; s0 += 64) {
-    const int s = s0 + lane;
+    const int s = s0 + lane_id();
     const int c = s < seqs ? count(s) : 0;
-    int incl = c;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int up = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += up;
-    }
+    const int incl = wave_scan(c);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (u < base + total) {
-      const uint64_t past = __ballot(base + incl > u);
-      const int at = __builtin_ctzll(past);
+      const int at = (int)__builtin_ctzll(__ballot(base + incl > u));
       local = u - base - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
       return s0 + at;
     }
     base += total;
   }
   local = 0;
+  return -1;
+}
+
+// The sequence of `row` and, in `units`, sum of count(s) over those before it; -1
+// for padding.
+template <typename F>
+KQ_DEV int kv_of_row(int row, const KvBatch& b, int page_shift, int& units, F count) {
+  units = 0;
+  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+    const int s = s0 + lane_id();
+    const KvSeq q = kv_seq(b, min(s, b.seqs - 1), page_shift);
+    const int c = s < b.seqs ? count(s) : 0;
+    const int incl = wave_scan(c);
+    const uint64_t here = __ballot(s < b.seqs && row >= q.row0 && row < q.row0 + q.rows);
+    if (here != 0) {
+      const int at = (int)__builtin_ctzll(here);
+      units += __builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at);
+      return s0 + at;
+    }
+    units += __builtin_amdgcn_readlane(incl, 63);
+  }
   return -1;
 }
 

@@ -14,14 +14,17 @@
 namespace kq {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 struct AttendArgs {
   const uint16_t* q;
   int64_t q_ld, q_hs;
   uint16_t* out;  // [rows][heads][D]
+  float* part;    // partial outputs of split sequences, null: none can be split
   float scale;    // times log2 e
   int heads, causal, window;
+  int units;      // grid width: units of work per kv head there is room for
+  int target;     // units of work per kv head to split into
+  int sum_shift;  // keeps the sum of all steps within 31 bits
 };
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
@@ -59,54 +62,122 @@ KQ_DEV void transpose4(const uint32_t in[4], uint32_t out[4]) {
   out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// max over the four lanes that hold one column (lanes l, l ^ 16, l ^ 32, l ^ 48)
+// Maximum and sum over the four lanes that hold one column (l, l ^ 16, l ^ 32, l ^ 48).
 KQ_DEV float column_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 KQ_DEV float column_sum(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
 
-// One workgroup: 16 rows (new tokens x the group's query heads) of one sequence and
-// kv head; its four waves take the sequence's tokens apart, 64 at a step.
+// Rows of a sequence go to tiles of 16 (new tokens x the group's query heads), and a
+// tile's tokens to units of `span` tokens.
+struct Split {
+  int span;    // tokens of a unit, a multiple of 256
+  KQ_DEV int chunks(const AttendArgs& a, const KvSeq& q) const { return (steps(a, q) * 64 + span - 1) / span; }
+  // 64-token steps from the first that any row sees to the last; at least one, so
+  // that a sequence without tokens has its rows written as well
+  KQ_DEV static int first(const AttendArgs& a, const KvSeq& q) {
+    return a.window > 0 ? max(q.first + 1 - a.window, 0) >> 6 : 0;
+  }
+  KQ_DEV static int steps(const AttendArgs& a, const KvSeq& q) { return max(((q.tokens + 63) >> 6) - first(a, q), 1); }
+  KQ_DEV static int tiles(const KvSeq& q, int group) { return (q.rows * group + 15) >> 4; }
+};
+
+// The same span in every workgroup: all steps of the batch over the units to fill.
+KQ_DEV Split split_of(const AttendArgs& a, const KvBatch& b, int shift, int group) {
+  int total = 0;
+  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+    const int s = s0 + lane_id();
+    int v = 0;
+    if (s < b.seqs) {
+      const KvSeq q = kv_seq(b, s, shift);
+      const int t = Split::tiles(q, group);
+      if (t > 0) v = (int)(((int64_t)t * Split::steps(a, q) >> a.sum_shift) + 1);
+    }
+    total += __builtin_amdgcn_readlane(wave_scan(v), 63);
+  }
+  const int64_t steps = ((int64_t)total << a.sum_shift) / a.target + 1;
+  Split r;
+  r.span = (int)min((steps + 3) / 4 * 256, (int64_t)1 << 30);
+  return r;
+}
+
+// Keys and values of one step of 16 * NT tokens in registers, and their scales.
+template <int D, int NT, int PP>
+struct Step {
+  u32x4 k[NT][D / 64];
+  uint32_t v[NT * 4][D / 64];
+  float ks[PP], vs[PP];  // scale times log2 e; value scale (0: no tokens here)
+};
+
+// One workgroup: a tile of 16 rows of one sequence and kv head, and a unit of its
+// tokens; its four waves take the steps of 16 * NT tokens in turn.
 //
 // Products run transposed, S^T = K Q^T and O^T = V^T P^T, on 16x16x32 MFMAs: lane
 // (c, b) = (l % 16, l / 16) then holds scores of query row c for tokens 4b..4b+3 of
 // each 16-token tile, which are, for two tiles, just the eight tokens that it has to
 // hand over as its part of P^T: no score leaves its lane.  Keys and values go from
-// memory to registers; a lane loads D / 16 bytes of each of its 16 tokens' values and
+// memory to registers; a lane loads D / 16 bytes of each of its tokens' values and
 // transposes them by bytes (the order of d within an output tile is free: row c of
 // tile j is d = c * D / 16 + j, so a lane ends up with neighbouring elements).
-template <int D, int DT>
-__global__ void __launch_bounds__(256)
-kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
-  constexpr int KS = D / 32;  // MFMA steps along a key
-  constexpr int VD = D / 64;  // dwords of a token's value a lane holds
-  constexpr int OT = D / 16;  // output tiles
-  extern __shared__ float lds[];  // [4][16][D + 2]
+//
+// Loads go through buffer resources of one page's tile whose size ends at the
+// sequence's last token: slots past it, pages that are none and steps past the unit
+// read as zero without a branch.
+template <int D, int DT, int NT, int PP>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
+                      const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
+  constexpr int KS = D / 32;   // MFMA steps along a key
+  constexpr int VD = D / 64;   // dwords of a token's value a lane holds
+  constexpr int OT = D / 16;   // output tiles
+  constexpr int ST = 16 * NT;  // tokens of a step
+  constexpr int LD = D + 4;
+  extern __shared__ float lds[];  // [4][16][LD]
   const int lane = lane_id(), wave = wave_id(), c = lane & 15, b = lane >> 4;
   const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
   const int head = (int)blockIdx.y;
-  int tile;
-  const int s = kv_find((int)blockIdx.x, batch.seqs, tile, [&](int i) {
+
+  {  // rows of no sequence
+    const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
+    const int first = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
+    const int words = group * D / 2;
+    for (int i = (int)blockIdx.x; i < first + batch.rows - last; i += (int)gridDim.x) {
+      const int64_t row = i < first ? i : last + (i - first);
+      uint32_t* dst = (uint32_t*)(a.out + (row * a.heads + head * group) * D);
+      for (int j = (int)threadIdx.x; j < words; j += 256) dst[j] = 0;
+    }
+  }
+
+  const Split split = split_of(a, batch, shift, group);
+  int unit;
+  const int s = kv_find((int)blockIdx.x, batch.seqs, unit, [&](int i) {
     const KvSeq q = kv_seq(batch, i, shift);
-    return (q.rows * group + 15) >> 4;
+    return Split::tiles(q, group) * split.chunks(a, q);
   });
   if (s < 0) return;
   const KvSeq q = kv_seq(batch, s, shift);
+  const int chunks = split.chunks(a, q), tile = unit / chunks, chunk = unit - tile * chunks;
   const int item = tile * 16 + c;  // this lane's column: row item / group, head item % group
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
   const int pos = q.first + row;
-  // tokens [from, to) of this column, [lo, hi) of the tile
-  int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
-  int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-  if (!real) to = from = 0;
+  // tokens [from, to) of this column; [lo, hi) of the tile; [lo_all, hi_all) of every row
+  const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
+  const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
   const int row_lo = (tile * 16) / group, row_hi = min(q.rows - 1, (tile * 16 + 15) / group);
-  const int hi = a.causal ? min(q.tokens, q.first + row_hi + 1) : q.tokens;
-  const int lo = a.window > 0 ? max(q.first + row_lo + 1 - a.window, 0) : 0;
+  int hi = a.causal ? min(q.tokens, q.first + row_hi + 1) : q.tokens;
+  int lo = a.window > 0 ? max(q.first + row_lo + 1 - a.window, 0) : 0;
+  const int hi_all = a.causal ? min(q.tokens, q.first + row_lo + 1) : q.tokens;
+  const int lo_all = a.window > 0 ? max(q.first + row_hi + 1 - a.window, 0) : 0;
+  const int begin = Split::first(a, q) * 64 + chunk * split.span;
+  hi = min(hi, begin + split.span);
+  lo = max(lo & ~63, begin);
 
   u32x4 qf[KS];
 #pragma unroll
@@ -117,97 +188,157 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
     for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1));
   }
 
+  const int32_t* pages = table + (int64_t)s * batch.table_ld;
+  const int64_t tile_bytes = (int64_t)D << shift;
+  const int in_page = (1 << shift) - 1;
+  const int k_lane = c * D + 16 * b, v_lane = 4 * b * D + c * (D / 16);
+  // pages of the step at t (-1 past the tile's last token)
+  auto pages_of = [&](int t, int (&id)[PP]) {
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      const int at = t + p * (ST / PP);
+      const int got = pages[min(at, max(hi - 1, 0)) >> shift];
+      id[p] = at < hi ? got : -1;
+    }
+  };
+  auto load = [&](int t, const int (&id)[PP], Step<D, NT, PP>& x) {
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      const int at = t + p * (ST / PP);
+      const int page = __builtin_amdgcn_readfirstlane(id[p]);
+      const bool there = page >= 0 && page < cache.pages;
+      const int64_t head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
+      const int left = min(q.tokens - (at & ~in_page), in_page + 1);
+      const uint32_t size = there ? (uint32_t)(left * D) : 0u;
+      const i32x4 kr = make_rsrc(cache.k + head_tile * tile_bytes, size);
+      const i32x4 vr = make_rsrc(cache.v + head_tile * tile_bytes, size);
+      const int off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
+#pragma unroll
+      for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i) {
+        const int so = off + (i - p * (NT / PP)) * 16 * D;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          x.k[i][h] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(kr, k_lane + 64 * h, so, 0));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (VD == 1) {
+            x.v[4 * i + r][0] = (uint32_t)kq_rbl_i32(vr, v_lane + r * D, so, 0);
+          } else if constexpr (VD == 2) {
+            const i32x2 w = kq_rbl_v2i32(vr, v_lane + r * D, so, 0);
+            x.v[4 * i + r][0] = (uint32_t)w[0];
+            x.v[4 * i + r][1] = (uint32_t)w[1];
+          } else {
+            const i32x4 w = kq_rbl_v4i32(vr, v_lane + r * D, so, 0);
+#pragma unroll
+            for (int d = 0; d < VD; ++d) x.v[4 * i + r][d] = (uint32_t)w[d];
+          }
+        }
+      }
+      x.ks[p] = there ? k_scale[head_tile] * a.scale : 0.0f;
+      x.vs[p] = there ? v_scale[head_tile] : 0.0f;
+    }
+  };
+
   f32x4 o[OT];
 #pragma unroll
   for (int j = 0; j < OT; ++j) o[j] = f32x4{0, 0, 0, 0};
   float top = -__builtin_inff(), sum = 0.0f;
-  const int64_t tile_bytes = (int64_t)D << shift;
-  for (int t0 = (lo & ~63) + 64 * wave; t0 < hi; t0 += 256) {
-    f32x4 w[4];
-    float inv_v[4];
-    u32x2 unused;
-    (void)unused;
-    uint32_t vr[16][VD];
+  auto compute = [&](int t, const Step<D, NT, PP>& x) {
+    f32x4 w[NT];
+    float m = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = t0 + 16 * i;
-      int page = t < hi ? kv_page(batch, cache, s, t >> shift) : -1;
-      page = __builtin_amdgcn_readfirstlane(page);
-      const bool there = page >= 0;
-      const int64_t at = (int64_t)max(page, 0) * cache.kv_heads + head;
-      const int off = (t & ((1 << shift) - 1)) * D;
-      const uint8_t* kp = cache.k + at * tile_bytes + off + c * D + 16 * b;
+    for (int i = 0; i < NT; ++i) {
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int h = 0; h < KS / 2; ++h) {
-        const u32x4 raw = *(const u32x4*)(kp + 64 * h);
-        acc = mfma16<DT>(widen_codes<DT>(raw[0], raw[1]), qf[2 * h], acc);
-        acc = mfma16<DT>(widen_codes<DT>(raw[2], raw[3]), qf[2 * h + 1], acc);
+        acc = mfma16<DT>(widen_codes<DT>(x.k[i][h][0], x.k[i][h][1]), qf[2 * h], acc);
+        acc = mfma16<DT>(widen_codes<DT>(x.k[i][h][2], x.k[i][h][3]), qf[2 * h + 1], acc);
       }
-      const uint8_t* vp = cache.v + at * tile_bytes + off + 4 * b * D + c * (D / 16);
+      const int p = i / (NT / PP);
+      const float shift_v = __builtin_amdgcn_logf(x.vs[p]);  // (-inf where there are no tokens)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int d = 0; d < VD; ++d) {
-          const uint32_t x = *(const uint32_t*)(vp + r * D + 4 * d);
-          // slots past the end hold whatever was there, NaN perhaps
-          vr[4 * i + r][d] = there && t + 4 * b + r < q.tokens ? x : 0u;
-        }
-      const float ks = there ? cache.k_scale[at] * a.scale : 0.0f;
-      const float vs = there ? cache.v_scale[at] : 1.0f;
-      inv_v[i] = 1.0f / vs;
-      const float shift_v = __builtin_amdgcn_logf(vs);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int token = t + 4 * b + r;
-        w[i][r] = there && token >= from && token < to ? acc[r] * ks + shift_v : -__builtin_inff();
-      }
+      for (int r = 0; r < 4; ++r) w[i][r] = fmaf(acc[r], x.ks[p], shift_v);
     }
-    float m = top;
+    if (t < lo_all || t + ST > hi_all) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int token = t + 16 * i + 4 * b + r;
+          if (token < from || token >= to) w[i][r] = -__builtin_inff();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, w[i][r]);
     m = column_max(m);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    const float keep = __builtin_amdgcn_exp2f(top - base);
-    top = m;
-    sum *= keep;
+    if (__ballot(m > top) != 0) {
+      m = fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
+      sum *= keep;
 #pragma unroll
-    for (int j = 0; j < OT; ++j) o[j] *= keep;
-    u32x4 p[2];
+      for (int j = 0; j < OT; ++j) o[j] *= keep;
+      top = m;
+    }
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    u32x4 p[NT / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) w[i][r] = __builtin_amdgcn_exp2f(w[i][r] - base);
-      sum += (w[i][0] + w[i][1] + w[i][2] + w[i][3]) * inv_v[i];
+      const float vs = x.vs[i / (NT / PP)];
+      sum += (w[i][0] + w[i][1] + w[i][2] + w[i][3]) * (vs > 0.0f ? 1.0f / vs : 0.0f);
       p[i >> 1][2 * (i & 1)] = pack_act2(w[i][0], w[i][1], KQ_DTYPE_F16);
       p[i >> 1][2 * (i & 1) + 1] = pack_act2(w[i][2], w[i][3], KQ_DTYPE_F16);
     }
 #pragma unroll
     for (int d = 0; d < VD; ++d)
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < NT / 2; ++g) {
         uint32_t in[2][4], out[2][4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) in[e][r] = vr[8 * g + 4 * e + r][d];
+          for (int r = 0; r < 4; ++r) in[e][r] = x.v[8 * g + 4 * e + r][d];
           transpose4(in[e], out[e]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           o[4 * d + j] = mfma16<KQ_DTYPE_F16>(widen_codes<KQ_DTYPE_F16>(out[0][j], out[1][j]), p[g], o[4 * d + j]);
       }
+  };
+
+  // one step in flight while another is computed, the pages of a third looked up
+  int t = lo + ST * wave;
+  if (t < hi) {
+    int id[PP];
+    Step<D, NT, PP> x, y;
+    pages_of(t, id);
+    load(t, id, x);
+    pages_of(t + 4 * ST, id);
+    while (true) {
+      load(t + 4 * ST, id, y);
+      pages_of(t + 8 * ST, id);
+      compute(t, x);
+      t += 4 * ST;
+      if (t >= hi) break;
+      load(t + 4 * ST, id, x);
+      pages_of(t + 8 * ST, id);
+      compute(t, y);
+      t += 4 * ST;
+      if (t >= hi) break;
+    }
   }
   sum = column_sum(sum);
 
   // the waves' parts meet in LDS, added in wave order
-  float* mine = lds + (wave * 16 + c) * (D + 2);
+  float* mine = lds + (wave * 16 + c) * LD;
 #pragma unroll
-  for (int j = 0; j < OT; ++j)
+  for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) mine[(4 * b + r) * OT + j] = o[j][r];
+    for (int j = 0; j < OT; j += 4)
+      *(f32x4*)(mine + (4 * b + r) * OT + j) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
   if (b == 0) {
     mine[D] = top;
     mine[D + 1] = sum;
@@ -219,16 +350,22 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
     if (it >= q.rows * group) break;
     float m = -__builtin_inff();
 #pragma unroll
-    for (int v = 0; v < 4; ++v) m = fmaxf(m, lds[(v * 16 + col) * (D + 2) + D]);
+    for (int v = 0; v < 4; ++v) m = fmaxf(m, lds[(v * 16 + col) * LD + D]);
     const float base = m == -__builtin_inff() ? 0.0f : m;
     float x = 0.0f, y = 0.0f, l = 0.0f;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const float* part = lds + (v * 16 + col) * (D + 2);
+      const float* part = lds + (v * 16 + col) * LD;
       const float f = __builtin_amdgcn_exp2f(part[D] - base);
       x += part[d] * f;
       y += part[d + 1] * f;
       l += part[D + 1] * f;
+    }
+    if (chunks > 1) {
+      float* dst = a.part + (((int64_t)head * a.units + (int)blockIdx.x) * 16 + col) * LD;
+      *(f32x2_t*)(dst + d) = f32x2_t{x, y};
+      if (d == 0) *(f32x2_t*)(dst + D) = f32x2_t{m, l};
+      continue;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees no token is zero)
     const int rw = it / group;
@@ -237,33 +374,112 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   }
 }
 
-// Rows past the last sequence are zero.
-__global__ void kv_pad_kernel(uint32_t* out, const int32_t* cu, int seqs, int rows, int row_words) {
-  const int row = (int)blockIdx.x;
-  const int first = seqs > 0 ? cu[0] : rows, last = seqs > 0 ? cu[seqs] : 0;
-  if (row >= first && row < last) return;
-  for (int i = (int)threadIdx.x; i < row_words; i += (int)blockDim.x) out[(int64_t)row * row_words + i] = 0;
+// The parts of split sequences joined in the order of their tokens: one wave per row
+// and query head.
+template <int D, int DT>
+__global__ void __launch_bounds__(256)
+kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
+  constexpr int LD = D + 4, PER = D / 64;
+  const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
+  const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
+  if (at >= (int64_t)batch.rows * a.heads) return;
+  const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads);
+  const Split split = split_of(a, batch, shift, group);
+  int unit;
+  const int s = kv_of_row(row, batch, shift, unit, [&](int i) {
+    const KvSeq q = kv_seq(batch, i, shift);
+    return Split::tiles(q, group) * split.chunks(a, q);
+  });
+  if (s < 0) return;
+  const KvSeq q = kv_seq(batch, s, shift);
+  const int chunks = split.chunks(a, q);
+  if (chunks == 1) return;  // written already
+  const int head = qh / group, item = (row - q.row0) * group + (qh - head * group);
+  unit += (item >> 4) * chunks;
+  const float* src = a.part + (((int64_t)head * a.units + unit) * 16 + (item & 15)) * LD;
+  float m = -__builtin_inff();
+  for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, src[(int64_t)i * 16 * LD + D]);
+  m = wave_max(m);
+  const float base = m == -__builtin_inff() ? 0.0f : m;
+  float x[PER], l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < PER; ++d) x[d] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < chunks; ++i) {
+    const float* p = src + (int64_t)i * 16 * LD;
+    const float f = __builtin_amdgcn_exp2f(p[D] - base);
+    l += p[D + 1] * f;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) x[d] += p[PER * lane_id() + d] * f;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* dst = a.out + ((int64_t)row * a.heads + qh) * D + PER * lane_id();
+#pragma unroll
+  for (int d = 0; d < PER; ++d) dst[d] = f32_to_out(x[d] * inv, DT);
+}
+
+// Units of work, of the whole grid, that split sequences are cut into.
+constexpr int kTargetUnits = 1024;
+
+struct RowsPlan {
+  int64_t tiles, target, units;
+  bool split;
+  int sum_shift;
+};
+
+static RowsPlan plan_rows(int64_t rows, int64_t heads, int64_t kv_heads, int64_t page_size, int64_t width, int64_t seqs) {
+  RowsPlan p{};
+  const int64_t group = heads / kv_heads;
+  p.tiles = std::min<int64_t>(rows * group, rows * group / 16 + seqs);
+  const int64_t steps = std::max<int64_t>((width * page_size + 63) / 64, 1);
+  p.split = steps > 4;
+  p.target = std::max<int64_t>((kTargetUnits + kv_heads - 1) / kv_heads, 1);
+  // a unit has `span` tokens but for the last of a tile: at most target + tiles of them
+  p.units = p.split ? p.target + p.tiles : p.tiles;
+  while (((p.tiles * steps) >> p.sum_shift) + p.tiles >= (1LL << 31)) ++p.sum_shift;
+  return p;
+}
+
+template <int D, int DT, int NT, int PP>
+static void launch_rows(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  const size_t lds = sizeof(float) * 4 * 16 * (D + 4);
+  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT, NT, PP>), dim3((unsigned)p.units, (unsigned)c.kv_heads), dim3(256), lds, st, a,
+                     c, b, b.table, c.k_scale, c.v_scale);
+  if (p.split)
+    hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0, st, a,
+                       c, b);
 }
 
 template <int D, int DT>
-static void launch_rows(const AttendArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  const int group = a.heads / c.kv_heads;
-  const int64_t tiles = std::min<int64_t>((int64_t)b.rows * group, (int64_t)b.rows * group / 16 + b.seqs);
-  const size_t lds = sizeof(float) * 4 * 16 * (D + 2);
-  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT>), dim3((unsigned)tiles, (unsigned)c.kv_heads), dim3(256), lds, st, a, c, b);
+static void pick_pages(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  constexpr int NT = D == 256 ? 2 : 4;  // (registers)
+  const int page = 1 << c.page_shift;
+  if (page >= 16 * NT)
+    launch_rows<D, DT, NT, 1>(a, p, c, b, st);
+  else if (page == 8 * NT)
+    launch_rows<D, DT, NT, 2>(a, p, c, b, st);
+  else if constexpr (NT == 4)
+    launch_rows<D, DT, NT, 4>(a, p, c, b, st);
 }
 
 template <int D>
-static void pick_rows(const AttendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+static void pick_rows(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
   if (dtype == KQ_DTYPE_BF16)
-    launch_rows<D, KQ_DTYPE_BF16>(a, c, b, st);
+    pick_pages<D, KQ_DTYPE_BF16>(a, p, c, b, st);
   else
-    launch_rows<D, KQ_DTYPE_F16>(a, c, b, st);
+    pick_pages<D, KQ_DTYPE_F16>(a, p, c, b, st);
 }
 
 }  // namespace kq
 
 using namespace kq;
+
+extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                                                 int64_t page_size, int64_t table_width, int64_t seqs) {
+  if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
+  const RowsPlan p = plan_rows(rows, heads, kv_heads, page_size, table_width, seqs);
+  return p.split ? sizeof(float) * (size_t)(p.units * kv_heads * 16 * (dim + 4)) : 0;
+}
 
 extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
                                int64_t kv_heads, int64_t dim, const uint8_t* k_cache, const uint8_t* v_cache,
@@ -272,40 +488,49 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
                                const int32_t* lengths, int64_t seqs, float scale, int causal, int64_t window, void* out,
                                void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "kq_kv_attention";
-  (void)workspace;
-  (void)workspace_bytes;
   int rc = kv_check(what, dtype, rows, heads, kv_heads, dim, page_size, pages, seqs, table_width, table_ld);
   if (rc) return rc;
   if (window < 0 || window > (1 << 30) || (window > 0 && !causal)) {
     set_error("%s: window %lld (a window is of causal attention)", what, (long long)window);
     return KQ_EINVAL;
   }
-  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16 != 0 || (q_ld | q_hs) % 8 != 0) {
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) % 16 != 0 ||
+      (q_ld | q_hs) % 8 != 0) {
     set_error("%s: tensors need 16-byte aligned rows and heads", what);
     return KQ_EINVAL;
   }
   if (rows == 0) return KQ_OK;
-  AttendArgs a{(const uint16_t*)q, q_ld, q_hs, (uint16_t*)out, scale * 1.44269504088896340736f, (int)heads, causal != 0,
-               (int)window};
+  const bool empty = seqs == 0 || pages == 0 || table_width == 0;  // every row is zero
+  RowsPlan p = plan_rows(rows, heads, kv_heads, page_size, table_width, seqs);
+  if (empty) p.split = false, p.units = std::min<int64_t>(rows, 1024);
+  if (p.split && (workspace == nullptr || workspace_bytes < kq_kv_attention_workspace_size(rows, heads, kv_heads, dim, page_size,
+                                                                                           table_width, seqs))) {
+    set_error("%s: workspace of %zu bytes is too small", what, workspace_bytes);
+    return KQ_EWORKSPACE;
+  }
+  if (p.units * kv_heads * 256 >= (1LL << 32) || rows * heads * 64 >= (1LL << 32)) {  // threads of one launch
+    set_error("%s: %lld rows of %lld heads are past the supported range", what, (long long)rows, (long long)heads);
+    return KQ_EINVAL;
+  }
+  AttendArgs a{};
+  a.q = (const uint16_t*)q;
+  a.q_ld = q_ld, a.q_hs = q_hs;
+  a.out = (uint16_t*)out;
+  a.part = (float*)workspace;
+  a.scale = scale * 1.44269504088896340736f;
+  a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
+  a.units = (int)p.units, a.target = (int)p.target, a.sum_shift = p.sum_shift;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
-  const KvBatch b{table, cu, lengths, table_ld, (int)seqs, (int)table_width, (int)rows};
+  // (without pages or table columns no sequence is looked at and all rows are padding)
+  const KvBatch b{table, cu, lengths, table_ld, empty ? 0 : (int)seqs, (int)table_width, (int)rows};
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(kv_pad_kernel, dim3((unsigned)rows), dim3(256), 0, st, (uint32_t*)out, cu, (int)seqs, (int)rows,
-                     (int)(heads * dim / 2));
-  if (seqs > 0 && pages > 0) {
-    if (dim == 64)
-      pick_rows<64>(a, c, b, dtype, st);
-    else if (dim == 128)
-      pick_rows<128>(a, c, b, dtype, st);
-    else
-      pick_rows<256>(a, c, b, dtype, st);
-  }
+  if (dim == 64)
+    pick_rows<64>(a, p, c, b, dtype, st);
+  else if (dim == 128)
+    pick_rows<128>(a, p, c, b, dtype, st);
+  else
+    pick_rows<256>(a, p, c, b, dtype, st);
   return check_launch(what);
-}
-
-extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
-                                                 int64_t page_size, int64_t table_width, int64_t seqs) {
-  return 0;
 }
