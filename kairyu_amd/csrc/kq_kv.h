@@ -77,8 +77,8 @@ KQ_DEV int wave_scan(int v) {
 // search would wait for a load at each of its steps), and its index there; -1 past
 // the last unit.  Uniform.
 template <typename F>
-KQ_DEV int kv_find(int u, int seqs, int& local, F count) {
-  int base = 0;
+KQ_DEV int kv_find(int64_t u, int seqs, int& local, F count) {
+  int64_t base = 0;
   for (int s0 = 0; s0 < seqs; s0 += 64) {
     const int s = s0 + lane_id();
     const int c = s < seqs ? count(s) : 0;
@@ -86,7 +86,7 @@ KQ_DEV int kv_find(int u, int seqs, int& local, F count) {
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (u < base + total) {
       const int at = (int)__builtin_ctzll(__ballot(base + incl > u));
-      local = u - base - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
+      local = (int)(u - base) - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
       return s0 + at;
     }
     base += total;
@@ -98,7 +98,7 @@ KQ_DEV int kv_find(int u, int seqs, int& local, F count) {
 // The sequence of `row` and, in `units`, sum of count(s) over those before it; -1
 // for padding.
 template <typename F>
-KQ_DEV int kv_of_row(int row, const KvBatch& b, int page_shift, int& units, F count) {
+KQ_DEV int kv_of_row(int row, const KvBatch& b, int page_shift, int64_t& units, F count) {
   units = 0;
   for (int s0 = 0; s0 < b.seqs; s0 += 64) {
     const int s = s0 + lane_id();

@@ -22,9 +22,7 @@ struct AttendArgs {
   float* part;    // partial outputs of split sequences, null: none can be split
   float scale;    // times log2 e
   int heads, causal, window;
-  int units;      // grid width: units of work per kv head there is room for
-  int target;     // units of work per kv head to split into
-  int sum_shift;  // keeps the sum of all steps within 31 bits
+  int shares;     // workgroups per kv head that the batch's tokens are dealt to
 };
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
@@ -74,36 +72,42 @@ KQ_DEV float column_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// Rows of a sequence go to tiles of 16 (new tokens x the group's query heads), and a
-// tile's tokens to units of `span` tokens.
-struct Split {
-  int span;    // tokens of a unit, a multiple of 256
-  KQ_DEV int chunks(const AttendArgs& a, const KvSeq& q) const { return (steps(a, q) * 64 + span - 1) / span; }
-  // 64-token steps from the first that any row sees to the last; at least one, so
-  // that a sequence without tokens has its rows written as well
+// A sequence's rows (new tokens x the group's query heads) go to tiles of 16, and the
+// tokens that they see to blocks of 256.  The blocks of all tiles, one after the
+// other, are dealt to `shares` workgroups per kv head in equal runs, so that every
+// workgroup streams the same number of bytes whatever the lengths are (units cut per
+// sequence left a third of the chip idle at the end of a ragged batch: 64 contexts of
+// up to 6000 tokens, XX us).  A run covers whole tiles, written at once, and
+// at most two parts of tiles: the end of one begun before it (part 0) and the
+// beginning of one that goes on behind it (part 1).
+struct Deal {
+  int64_t run;  // blocks of a workgroup
+
+  // 64-token step of the first token that any row sees
   KQ_DEV static int first(const AttendArgs& a, const KvSeq& q) {
     return a.window > 0 ? max(q.first + 1 - a.window, 0) >> 6 : 0;
   }
-  KQ_DEV static int steps(const AttendArgs& a, const KvSeq& q) { return max(((q.tokens + 63) >> 6) - first(a, q), 1); }
+  // at least one, so that rows that see nothing are written as well
+  KQ_DEV static int blocks(const AttendArgs& a, const KvSeq& q) {
+    return (max(((q.tokens + 63) >> 6) - first(a, q), 1) + 3) >> 2;
+  }
   KQ_DEV static int tiles(const KvSeq& q, int group) { return (q.rows * group + 15) >> 4; }
 };
 
-// The same span in every workgroup: all steps of the batch over the units to fill.
-KQ_DEV Split split_of(const AttendArgs& a, const KvBatch& b, int shift, int group) {
-  int total = 0;
+// The same run in every workgroup.
+KQ_DEV Deal deal_of(const AttendArgs& a, const KvBatch& b, int shift, int group) {
+  int64_t total = 0;
   for (int s0 = 0; s0 < b.seqs; s0 += 64) {
     const int s = s0 + lane_id();
     int v = 0;
     if (s < b.seqs) {
       const KvSeq q = kv_seq(b, s, shift);
-      const int t = Split::tiles(q, group);
-      if (t > 0) v = (int)(((int64_t)t * Split::steps(a, q) >> a.sum_shift) + 1);
+      v = Deal::tiles(q, group) * Deal::blocks(a, q);
     }
     total += __builtin_amdgcn_readlane(wave_scan(v), 63);
   }
-  const int64_t steps = ((int64_t)total << a.sum_shift) / a.target + 1;
-  Split r;
-  r.span = (int)min((steps + 3) / 4 * 256, (int64_t)1 << 30);
+  Deal r;
+  r.run = (total + a.shares - 1) / a.shares;
   return r;
 }
 
@@ -115,8 +119,8 @@ struct Step {
   float ks[PP], vs[PP];  // scale times log2 e; value scale (0: no tokens here)
 };
 
-// One workgroup: a tile of 16 rows of one sequence and kv head, and a unit of its
-// tokens; its four waves take the steps of 16 * NT tokens in turn.
+// One workgroup: its run of blocks of one kv head, tile by tile; its four waves take
+// a tile's steps of 16 * NT tokens in turn.
 //
 // Products run transposed, S^T = K Q^T and O^T = V^T P^T, on 16x16x32 MFMAs: lane
 // (c, b) = (l % 16, l / 16) then holds scores of query row c for tokens 4b..4b+3 of
@@ -127,7 +131,7 @@ struct Step {
 // tile j is d = c * D / 16 + j, so a lane ends up with neighbouring elements).
 //
 // Loads go through buffer resources of one page's tile whose size ends at the
-// sequence's last token: slots past it, pages that are none and steps past the unit
+// sequence's last token: slots past it, pages that are none and steps past the run
 // read as zero without a branch.
 template <int D, int DT, int NT, int PP>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
@@ -154,15 +158,23 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     }
   }
 
-  const Split split = split_of(a, batch, shift, group);
-  int unit;
-  const int s = kv_find((int)blockIdx.x, batch.seqs, unit, [&](int i) {
+  const Deal deal = deal_of(a, batch, shift, group);
+  const int64_t run_end = ((int64_t)blockIdx.x + 1) * deal.run;
+  int64_t block = (int64_t)blockIdx.x * deal.run;
+  int within = 0;  // blocks of the sequence before `block`
+  int s = kv_find(block, batch.seqs, within, [&](int i) {
     const KvSeq q = kv_seq(batch, i, shift);
-    return Split::tiles(q, group) * split.chunks(a, q);
+    return Deal::tiles(q, group) * Deal::blocks(a, q);
   });
   if (s < 0) return;
-  const KvSeq q = kv_seq(batch, s, shift);
-  const int chunks = split.chunks(a, q), tile = unit / chunks, chunk = unit - tile * chunks;
+  KvSeq q = kv_seq(batch, s, shift);
+  int blocks = Deal::blocks(a, q), tile = within / blocks;
+  within -= tile * blocks;
+  const int64_t tile_bytes = (int64_t)D << shift;
+  const int in_page = (1 << shift) - 1;
+  const int k_lane = c * D + 16 * b, v_lane = 4 * b * D + c * (D / 16);
+
+  while (true) {
   const int item = tile * 16 + c;  // this lane's column: row item / group, head item % group
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
@@ -175,8 +187,9 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   int lo = a.window > 0 ? max(q.first + row_lo + 1 - a.window, 0) : 0;
   const int hi_all = a.causal ? min(q.tokens, q.first + row_lo + 1) : q.tokens;
   const int lo_all = a.window > 0 ? max(q.first + row_hi + 1 - a.window, 0) : 0;
-  const int begin = Split::first(a, q) * 64 + chunk * split.span;
-  hi = min(hi, begin + split.span);
+  const int part_blocks = (int)min((int64_t)(blocks - within), run_end - block);
+  const int begin = Deal::first(a, q) * 64 + within * 256;
+  hi = min((int64_t)hi, (int64_t)begin + (int64_t)part_blocks * 256);
   lo = max(lo & ~63, begin);
 
   u32x4 qf[KS];
@@ -189,9 +202,6 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   }
 
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
-  const int64_t tile_bytes = (int64_t)D << shift;
-  const int in_page = (1 << shift) - 1;
-  const int k_lane = c * D + 16 * b, v_lane = 4 * b * D + c * (D / 16);
   // pages of the step at t (-1 past the tile's last token)
   auto pages_of = [&](int t, int (&id)[PP]) {
 #pragma unroll
@@ -333,6 +343,8 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   sum = column_sum(sum);
 
   // the waves' parts meet in LDS, added in wave order
+  const bool whole = part_blocks == blocks;
+  __syncthreads();  // (the last tile's parts have been read)
   float* mine = lds + (wave * 16 + c) * LD;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -361,8 +373,8 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
       y += part[d + 1] * f;
       l += part[D + 1] * f;
     }
-    if (chunks > 1) {
-      float* dst = a.part + (((int64_t)head * a.units + (int)blockIdx.x) * 16 + col) * LD;
+    if (!whole) {
+      float* dst = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (within == 0)) * 16 + col) * LD;
       *(f32x2_t*)(dst + d) = f32x2_t{x, y};
       if (d == 0) *(f32x2_t*)(dst + D) = f32x2_t{m, l};
       continue;
@@ -371,6 +383,19 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     const int rw = it / group;
     uint32_t* dst = (uint32_t*)(a.out + ((int64_t)(q.row0 + rw) * a.heads + head * group + (it - rw * group)) * D + d);
     *dst = pack_act2(x * inv, y * inv, DT);
+  }
+
+  block += part_blocks;
+  within = 0;
+  if (block >= run_end) return;
+  if (++tile >= Deal::tiles(q, group)) {
+    tile = 0;
+    do {
+      if (++s >= batch.seqs) return;
+      q = kv_seq(batch, s, shift);
+    } while (q.rows == 0);
+    blocks = Deal::blocks(a, q);
+  }
   }
 }
 
@@ -384,21 +409,24 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
   if (at >= (int64_t)batch.rows * a.heads) return;
   const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads);
-  const Split split = split_of(a, batch, shift, group);
-  int unit;
-  const int s = kv_of_row(row, batch, shift, unit, [&](int i) {
+  const Deal deal = deal_of(a, batch, shift, group);
+  int64_t block;
+  const int s = kv_of_row(row, batch, shift, block, [&](int i) {
     const KvSeq q = kv_seq(batch, i, shift);
-    return Split::tiles(q, group) * split.chunks(a, q);
+    return Deal::tiles(q, group) * Deal::blocks(a, q);
   });
   if (s < 0) return;
   const KvSeq q = kv_seq(batch, s, shift);
-  const int chunks = split.chunks(a, q);
-  if (chunks == 1) return;  // written already
+  const int blocks = Deal::blocks(a, q);
   const int head = qh / group, item = (row - q.row0) * group + (qh - head * group);
-  unit += (item >> 4) * chunks;
-  const float* src = a.part + (((int64_t)head * a.units + unit) * 16 + (item & 15)) * LD;
+  block += (int64_t)(item >> 4) * blocks;
+  const int x0 = (int)(block / deal.run), chunks = (int)((block + blocks - 1) / deal.run) - x0 + 1;
+  if (chunks == 1) return;  // written already
+  // part 1 of the run it begins in, then part 0 of those behind
+  const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
+  auto at_part = [&](int i) { return src + (int64_t)(i == 0 ? 0 : 2 * i - 1) * 16 * LD; };
   float m = -__builtin_inff();
-  for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, src[(int64_t)i * 16 * LD + D]);
+  for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
   m = wave_max(m);
   const float base = m == -__builtin_inff() ? 0.0f : m;
   float x[PER], l = 0.0f;
@@ -406,7 +434,7 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   for (int d = 0; d < PER; ++d) x[d] = 0.0f;
 #pragma unroll 4
   for (int i = 0; i < chunks; ++i) {
-    const float* p = src + (int64_t)i * 16 * LD;
+    const float* p = at_part(i);
     const float f = __builtin_amdgcn_exp2f(p[D] - base);
     l += p[D + 1] * f;
 #pragma unroll
@@ -418,56 +446,42 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   for (int d = 0; d < PER; ++d) dst[d] = f32_to_out(x[d] * inv, DT);
 }
 
-// Units of work, of the whole grid, that split sequences are cut into.
-constexpr int kTargetUnits = 1024;
+// Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
+constexpr int rows_slots(int64_t dim) { return 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1); }
 
-struct RowsPlan {
-  int64_t tiles, target, units;
-  bool split;
-  int sum_shift;
-};
+static int rows_shares(int64_t kv_heads, int64_t dim) { return (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1); }
 
-static RowsPlan plan_rows(int64_t rows, int64_t heads, int64_t kv_heads, int64_t page_size, int64_t width, int64_t seqs) {
-  RowsPlan p{};
-  const int64_t group = heads / kv_heads;
-  p.tiles = std::min<int64_t>(rows * group, rows * group / 16 + seqs);
-  const int64_t steps = std::max<int64_t>((width * page_size + 63) / 64, 1);
-  p.split = steps > 4;
-  p.target = std::max<int64_t>((kTargetUnits + kv_heads - 1) / kv_heads, 1);
-  // a unit has `span` tokens but for the last of a tile: at most target + tiles of them
-  p.units = p.split ? p.target + p.tiles : p.tiles;
-  while (((p.tiles * steps) >> p.sum_shift) + p.tiles >= (1LL << 31)) ++p.sum_shift;
-  return p;
-}
+// Whether a tile can have more than one block, and so be split.
+static bool rows_split(int64_t page_size, int64_t width) { return width * page_size > 256; }
 
 template <int D, int DT, int NT, int PP>
-static void launch_rows(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
+static void launch_rows(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, hipStream_t st) {
   const size_t lds = sizeof(float) * 4 * 16 * (D + 4);
-  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT, NT, PP>), dim3((unsigned)p.units, (unsigned)c.kv_heads), dim3(256), lds, st, a,
+  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT, NT, PP>), dim3((unsigned)a.shares, (unsigned)c.kv_heads), dim3(256), lds, st, a,
                      c, b, b.table, c.k_scale, c.v_scale);
-  if (p.split)
+  if (split)
     hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0, st, a,
                        c, b);
 }
 
 template <int D, int DT>
-static void pick_pages(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
+static void pick_pages(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, hipStream_t st) {
   constexpr int NT = D == 256 ? 2 : 4;  // (registers)
   const int page = 1 << c.page_shift;
   if (page >= 16 * NT)
-    launch_rows<D, DT, NT, 1>(a, p, c, b, st);
+    launch_rows<D, DT, NT, 1>(a, split, c, b, st);
   else if (page == 8 * NT)
-    launch_rows<D, DT, NT, 2>(a, p, c, b, st);
+    launch_rows<D, DT, NT, 2>(a, split, c, b, st);
   else if constexpr (NT == 4)
-    launch_rows<D, DT, NT, 4>(a, p, c, b, st);
+    launch_rows<D, DT, NT, 4>(a, split, c, b, st);
 }
 
 template <int D>
-static void pick_rows(const AttendArgs& a, const RowsPlan& p, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+static void pick_rows(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
   if (dtype == KQ_DTYPE_BF16)
-    pick_pages<D, KQ_DTYPE_BF16>(a, p, c, b, st);
+    pick_pages<D, KQ_DTYPE_BF16>(a, split, c, b, st);
   else
-    pick_pages<D, KQ_DTYPE_F16>(a, p, c, b, st);
+    pick_pages<D, KQ_DTYPE_F16>(a, split, c, b, st);
 }
 
 }  // namespace kq
@@ -477,8 +491,7 @@ using namespace kq;
 extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                                  int64_t page_size, int64_t table_width, int64_t seqs) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
-  const RowsPlan p = plan_rows(rows, heads, kv_heads, page_size, table_width, seqs);
-  return p.split ? sizeof(float) * (size_t)(p.units * kv_heads * 16 * (dim + 4)) : 0;
+  return rows_split(page_size, table_width) ? sizeof(float) * (size_t)(rows_shares(kv_heads, dim) * kv_heads * 2 * 16 * (dim + 4)) : 0;
 }
 
 extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
@@ -501,15 +514,17 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   }
   if (rows == 0) return KQ_OK;
   const bool empty = seqs == 0 || pages == 0 || table_width == 0;  // every row is zero
-  RowsPlan p = plan_rows(rows, heads, kv_heads, page_size, table_width, seqs);
-  if (empty) p.split = false, p.units = std::min<int64_t>(rows, 1024);
-  if (p.split && (workspace == nullptr || workspace_bytes < kq_kv_attention_workspace_size(rows, heads, kv_heads, dim, page_size,
+  const bool split = !empty && rows_split(page_size, table_width);
+  if (split && (workspace == nullptr || workspace_bytes < kq_kv_attention_workspace_size(rows, heads, kv_heads, dim, page_size,
                                                                                            table_width, seqs))) {
     set_error("%s: workspace of %zu bytes is too small", what, workspace_bytes);
     return KQ_EWORKSPACE;
   }
-  if (p.units * kv_heads * 256 >= (1LL << 32) || rows * heads * 64 >= (1LL << 32)) {  // threads of one launch
-    set_error("%s: %lld rows of %lld heads are past the supported range", what, (long long)rows, (long long)heads);
+  // threads of one launch, and blocks of all tiles
+  if (rows * heads * 64 >= (1LL << 32) ||
+      (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256) >= (1LL << 31)) {
+    set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
+              (long long)heads, (long long)(table_width * page_size));
     return KQ_EINVAL;
   }
   AttendArgs a{};
@@ -519,7 +534,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.part = (float*)workspace;
   a.scale = scale * 1.44269504088896340736f;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
-  a.units = (int)p.units, a.target = (int)p.target, a.sum_shift = p.sum_shift;
+  a.shares = rows_shares(kv_heads, dim);
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
@@ -527,10 +542,10 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   const KvBatch b{table, cu, lengths, table_ld, empty ? 0 : (int)seqs, (int)table_width, (int)rows};
   hipStream_t st = (hipStream_t)stream;
   if (dim == 64)
-    pick_rows<64>(a, p, c, b, dtype, st);
+    pick_rows<64>(a, split, c, b, dtype, st);
   else if (dim == 128)
-    pick_rows<128>(a, p, c, b, dtype, st);
+    pick_rows<128>(a, split, c, b, dtype, st);
   else
-    pick_rows<256>(a, p, c, b, dtype, st);
+    pick_rows<256>(a, split, c, b, dtype, st);
   return check_launch(what);
 }
