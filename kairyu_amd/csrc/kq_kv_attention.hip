@@ -23,6 +23,10 @@ struct AttendArgs {
   float scale;    // times log2 e
   int heads, causal, window;
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
+  float* big_part;  // partial outputs of the 128-row tiles, null: their tokens are not split
+  int few;          // rows * group up to which a sequence goes to tiles of 16 rows
+  int big_tiles;    // 128-row tiles per kv head that the grid has room for
+  int splits;       // parts that a 128-row tile's tokens are cut into
 };
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
@@ -91,8 +95,15 @@ struct Deal {
   KQ_DEV static int blocks(const AttendArgs& a, const KvSeq& q) {
     return (max(((q.tokens + 63) >> 6) - first(a, q), 1) + 3) >> 2;
   }
-  KQ_DEV static int tiles(const KvSeq& q, int group) { return (q.rows * group + 15) >> 4; }
+  KQ_DEV static int tiles(const AttendArgs& a, const KvSeq& q, int group) {
+    const int items = q.rows * group;
+    return items <= a.few ? (items + 15) >> 4 : 0;
+  }
 };
+KQ_DEV int big_tiles(const AttendArgs& a, const KvSeq& q, int group) {
+  const int items = q.rows * group;
+  return items > a.few ? (items + 127) >> 7 : 0;
+}
 
 // The same run in every workgroup.
 KQ_DEV Deal deal_of(const AttendArgs& a, const KvBatch& b, int shift, int group) {
@@ -102,13 +113,26 @@ KQ_DEV Deal deal_of(const AttendArgs& a, const KvBatch& b, int shift, int group)
     int v = 0;
     if (s < b.seqs) {
       const KvSeq q = kv_seq(b, s, shift);
-      v = Deal::tiles(q, group) * Deal::blocks(a, q);
+      v = Deal::tiles(a, q, group) * Deal::blocks(a, q);
     }
     total += __builtin_amdgcn_readlane(wave_scan(v), 63);
   }
   Deal r;
   r.run = (total + a.shares - 1) / a.shares;
   return r;
+}
+
+// Rows of no sequence are zero: those of one kv head, dealt to `of` workgroups.
+template <int D>
+KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, int group, int nth, int of) {
+  const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
+  const int first = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
+  const int words = group * D / 2;
+  for (int i = nth; i < first + batch.rows - last; i += of) {
+    const int64_t row = i < first ? i : last + (i - first);
+    uint32_t* dst = (uint32_t*)(a.out + (row * a.heads + head * group) * D);
+    for (int j = (int)threadIdx.x; j < words; j += 256) dst[j] = 0;
+  }
 }
 
 // Keys and values of one step of 16 * NT tokens in registers, and their scales.
@@ -142,29 +166,19 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   constexpr int OT = D / 16;   // output tiles
   constexpr int ST = 16 * NT;  // tokens of a step
   constexpr int LD = D + 4;
-  extern __shared__ float lds[];  // [4][16][LD]
+  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * LD];
   const int lane = lane_id(), wave = wave_id(), c = lane & 15, b = lane >> 4;
   const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
   const int head = (int)blockIdx.y;
 
-  {  // rows of no sequence
-    const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
-    const int first = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
-    const int words = group * D / 2;
-    for (int i = (int)blockIdx.x; i < first + batch.rows - last; i += (int)gridDim.x) {
-      const int64_t row = i < first ? i : last + (i - first);
-      uint32_t* dst = (uint32_t*)(a.out + (row * a.heads + head * group) * D);
-      for (int j = (int)threadIdx.x; j < words; j += 256) dst[j] = 0;
-    }
-  }
-
+  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x);
   const Deal deal = deal_of(a, batch, shift, group);
   const int64_t run_end = ((int64_t)blockIdx.x + 1) * deal.run;
   int64_t block = (int64_t)blockIdx.x * deal.run;
   int within = 0;  // blocks of the sequence before `block`
   int s = kv_find(block, batch.seqs, within, [&](int i) {
     const KvSeq q = kv_seq(batch, i, shift);
-    return Deal::tiles(q, group) * Deal::blocks(a, q);
+    return Deal::tiles(a, q, group) * Deal::blocks(a, q);
   });
   if (s < 0) return;
   KvSeq q = kv_seq(batch, s, shift);
@@ -388,19 +402,19 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   block += part_blocks;
   within = 0;
   if (block >= run_end) return;
-  if (++tile >= Deal::tiles(q, group)) {
+  if (++tile >= Deal::tiles(a, q, group)) {
     tile = 0;
     do {
       if (++s >= batch.seqs) return;
       q = kv_seq(batch, s, shift);
-    } while (q.rows == 0);
+    } while (Deal::tiles(a, q, group) == 0);
     blocks = Deal::blocks(a, q);
   }
   }
 }
 
-// The parts of split sequences joined in the order of their tokens: one wave per row
-// and query head.
+// The parts of split tiles joined in the order of their tokens: one wave per row and
+// query head.
 template <int D, int DT>
 __global__ void __launch_bounds__(256)
 kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
@@ -408,23 +422,35 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
   const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
   if (at >= (int64_t)batch.rows * a.heads) return;
-  const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads);
-  const Deal deal = deal_of(a, batch, shift, group);
-  int64_t block;
-  const int s = kv_of_row(row, batch, shift, block, [&](int i) {
-    const KvSeq q = kv_seq(batch, i, shift);
-    return Deal::tiles(q, group) * Deal::blocks(a, q);
-  });
+  const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads), head = qh / group;
+  int64_t before;  // 128-row tiles, or blocks, of the sequences before the row's
+  int s = kv_of_row(row, batch, shift, before, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
   if (s < 0) return;
   const KvSeq q = kv_seq(batch, s, shift);
-  const int blocks = Deal::blocks(a, q);
-  const int head = qh / group, item = (row - q.row0) * group + (qh - head * group);
-  block += (int64_t)(item >> 4) * blocks;
-  const int x0 = (int)(block / deal.run), chunks = (int)((block + blocks - 1) / deal.run) - x0 + 1;
-  if (chunks == 1) return;  // written already
-  // part 1 of the run it begins in, then part 0 of those behind
-  const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
-  auto at_part = [&](int i) { return src + (int64_t)(i == 0 ? 0 : 2 * i - 1) * 16 * LD; };
+  const int item = (row - q.row0) * group + (qh - head * group);
+  const float* src;
+  int chunks, step;  // part i > 0 lies (step * i - 1) * 16 rows behind the first, or i * 128
+  if (q.rows * group > a.few) {
+    if (a.splits == 1) return;
+    chunks = a.splits;
+    step = 0;
+    src = a.big_part + ((((int64_t)head * a.big_tiles + before + (item >> 7)) * a.splits) * 128 + (item & 127)) * LD;
+  } else {
+    const Deal deal = deal_of(a, batch, shift, group);
+    kv_of_row(row, batch, shift, before, [&](int i) {
+      const KvSeq q = kv_seq(batch, i, shift);
+      return Deal::tiles(a, q, group) * Deal::blocks(a, q);
+    });
+    const int blocks = Deal::blocks(a, q);
+    const int64_t block = before + (int64_t)(item >> 4) * blocks;
+    const int x0 = (int)(block / deal.run);
+    chunks = (int)((block + blocks - 1) / deal.run) - x0 + 1;
+    if (chunks == 1) return;  // written already
+    step = 2;
+    // part 1 of the run it begins in, then part 0 of those behind
+    src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
+  }
+  auto at_part = [&](int i) { return src + (step == 0 ? (int64_t)i * 128 : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
   float m = -__builtin_inff();
   for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
   m = wave_max(m);
@@ -446,42 +472,325 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   for (int d = 0; d < PER; ++d) dst[d] = f32_to_out(x[d] * inv, DT);
 }
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if (DT == KQ_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// One workgroup: a tile of 128 rows of one sequence and kv head (32 a wave), over the
+// tokens that it sees or one of `splits` parts of them, 64 at a step.
+//
+// The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
+// are shared by the four waves: they are widened once, keys to Q's type in rows of
+// one token, values to fp16 in rows of one d whose tokens stand in the order in which
+// the lanes of S^T hold them (for each 16: 0-3, 8-11, then 4-7, 12-15), so that both
+// are read as 16-byte MFMA operands; rows are padded by 16 bytes, which spreads eight
+// lanes' reads over all banks.  Two steps' worth of LDS: the next step's bytes travel
+// from memory while this one is computed, and one barrier a step suffices.  Row R of
+// the values is d = R % 16 * (D / 16) + R / 16 (any order does), which again leaves a
+// lane with neighbouring elements.
+template <int D, int DT>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
+                       const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
+  constexpr int KS = D / 16;            // MFMA steps along a key
+  constexpr int OT = D / 32;            // output tiles
+  constexpr int KLD = 2 * D + 16;       // bytes of a key's row
+  constexpr int VLD = 2 * 64 + 16;      // bytes of a d's row of values
+  constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale, its inverse)
+  constexpr int KC = D / 64;            // 16-byte chunks of keys a thread moves
+  constexpr int VC = D / 64;            // dwords of each of four tokens' values a thread moves
+  constexpr int LD = D + 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+  const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5, tid = (int)threadIdx.x;
+  const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
+  // kv heads side by side, so that (for up to 8 of them) an XCD's workgroups share
+  // theirs through its L2; the tiles with the most tokens first
+  const int head = (int)blockIdx.x % cache.kv_heads, rest = (int)blockIdx.x / cache.kv_heads;
+  const int part = rest % a.splits, nth = a.big_tiles - 1 - rest / a.splits;
+  if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits);  // (no other kernel does)
+  int tile;
+  const int s = kv_find(nth, batch.seqs, tile, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
+  if (s < 0) return;
+  const KvSeq q = kv_seq(batch, s, shift);
+  const int item = tile * 128 + wave * 32 + c;
+  const bool real = item < q.rows * group;
+  const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
+  const int pos = q.first + row;
+  // tokens [from, to) of this column, [lo_all, hi_all) of every row of the wave, [lo, hi) of the tile
+  const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
+  const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
+  const int last_row = min(q.rows - 1, (tile * 128 + 127) / group);
+  int hi = a.causal ? max(min(q.tokens, q.first + last_row + 1), 0) : q.tokens;
+  int lo = a.window > 0 ? max(q.first + tile * 128 / group + 1 - a.window, 0) & ~63 : 0;
+  const int w_lo = (tile * 128 + wave * 32) / group, w_hi = min(q.rows - 1, (tile * 128 + wave * 32 + 31) / group);
+  const int hi_all = a.causal ? min(q.tokens, q.first + w_lo + 1) : q.tokens;
+  const int lo_all = a.window > 0 ? max(q.first + w_hi + 1 - a.window, 0) : 0;
+  const int lo_wave = a.window > 0 ? max(q.first + w_lo + 1 - a.window, 0) : 0;
+  const int hi_wave = a.causal ? min(q.tokens, q.first + w_hi + 1) : q.tokens;
+  if (a.splits > 1) {
+    const int n = hi > lo ? (hi - lo + 63) >> 6 : 0, per = (n + a.splits - 1) / a.splits;
+    lo += part * per * 64;
+    hi = min(hi, lo + per * 64);
+  }
+
+  u32x4 qf[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) qf[i] = u32x4{0, 0, 0, 0};
+  if (real) {
+    const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h);
+  }
+
+  // what this thread moves: D / 4 bytes of one token's key, D / 16 of four tokens' values
+  const int k_tok = tid >> 2, k_at = (tid & 3) * (D / 4);
+  const int v_grp = tid >> 4, v_c = tid & 15;
+  const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
+  const int64_t tile_bytes = (int64_t)D << shift;
+  const int in_page = (1 << shift) - 1;
+  const int32_t* pages = table + (int64_t)s * batch.table_ld;
+  auto page_at = [&](int t) {
+    const int got = pages[min(t, max(hi - 1, 0)) >> shift];
+    return t < hi && got >= 0 && got < cache.pages ? got : -1;
+  };
+  u32x4 kr[KC];
+  uint32_t vr[4][VC];
+  float sc_k = 0.0f, sc_v = 0.0f;
+  int kp = page_at(lo + k_tok), vp = page_at(lo + 4 * v_grp);
+  auto fetch = [&](int t) {
+    const uint8_t* ks = cache.k + ((int64_t)max(kp, 0) * cache.kv_heads + head) * tile_bytes + ((t + k_tok) & in_page) * D + k_at;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const u32x4 x = *(const u32x4*)(ks + 16 * i);
+      kr[i] = kp >= 0 ? x : u32x4{0, 0, 0, 0};
+    }
+    const int64_t v_tile = (int64_t)max(vp, 0) * cache.kv_heads + head;
+    const uint8_t* vs = cache.v + v_tile * tile_bytes + ((t + 4 * v_grp) & in_page) * D + v_c * (D / 16);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      // slots past the end hold whatever was there, NaN perhaps
+      const bool there = vp >= 0 && t + 4 * v_grp + r < q.tokens;
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        const uint32_t x = *(const uint32_t*)(vs + r * D + 4 * i);
+        vr[r][i] = there ? x : 0u;
+      }
+    }
+    if (v_c == 0 && (v_grp & 3) == 0) {
+      sc_k = vp >= 0 ? k_scale[v_tile] * a.scale : 1.0f;
+      sc_v = vp >= 0 ? v_scale[v_tile] : 0.0f;
+    }
+    kp = page_at(t + 64 + k_tok);
+    vp = page_at(t + 64 + 4 * v_grp);
+  };
+  auto put = [&](char* buf) {
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      char* dst = buf + k_tok * KLD + 2 * (k_at + 16 * i);
+      *(u32x4*)dst = widen_codes<DT>(kr[i][0], kr[i][1]);
+      *(u32x4*)(dst + 16) = widen_codes<DT>(kr[i][2], kr[i][3]);
+    }
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+      const uint32_t in[4] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i]};
+      uint32_t out[4];
+      transpose4(in, out);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, false)),
+                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, true))};
+        *(u32x2*)(buf + KB + ((4 * i + j) * 16 + v_c) * VLD + 2 * v_pos) = w;
+      }
+    }
+    if (v_c == 0 && (v_grp & 3) == 0) {
+      float* dst = (float*)(buf + KB + VB) + (v_grp >> 2);
+      dst[0] = sc_k;
+      dst[4] = __builtin_amdgcn_logf(sc_v);
+      dst[8] = sc_v > 0.0f ? 1.0f / sc_v : 0.0f;
+    }
+  };
+
+  f32x16 o[OT];
+#pragma unroll
+  for (int j = 0; j < OT; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
+  float top = -__builtin_inff(), sum = 0.0f;
+
+  if (lo < hi) {
+    fetch(lo);
+    put(smem);
+  }
+  __syncthreads();
+  int which = 0;
+  for (int t = lo; t < hi; t += 64) {
+    const char* buf = smem + which * BUF;
+    if (t + 64 < hi) fetch(t + 64);
+    if (t < hi_wave && t + 64 > lo_wave) {
+      f32x16 w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[i][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          w[i] = mfma32<DT>(*(const u32x4*)(buf + (32 * i + c) * KLD + 32 * k + 16 * h), qf[k], w[i]);
+      }
+      const f32x4 ks = *(const f32x4*)(buf + KB + VB), lv = *(const f32x4*)(buf + KB + VB + 16),
+                  iv = *(const f32x4*)(buf + KB + VB + 32);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[i][e] = fmaf(w[i][e], ks[2 * i + (e >> 3)], lv[2 * i + (e >> 3)]);
+      if (t < lo_all || t + 64 > hi_all) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int token = t + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (token < from || token >= to) w[i][e] = -__builtin_inff();
+          }
+      }
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, w[i][e]);
+      const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+      m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+      if (__ballot(m > top) != 0) {
+        m = fmaxf(m, top);
+        const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
+        sum *= keep;
+#pragma unroll
+        for (int j = 0; j < OT; ++j) o[j] *= keep;
+        top = m;
+      }
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      u32x4 p[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float part_sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __builtin_amdgcn_exp2f(w[i][8 * g + 2 * e] - base);
+            const float y = __builtin_amdgcn_exp2f(w[i][8 * g + 2 * e + 1] - base);
+            part_sum += x + y;
+            p[2 * i + g][e] = pack_act2(x, y, KQ_DTYPE_F16);
+          }
+          sum = fmaf(part_sum, iv[2 * i + g], sum);
+        }
+#pragma unroll
+      for (int j = 0; j < OT; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          o[j] = mfma32<KQ_DTYPE_F16>(*(const u32x4*)(buf + KB + (32 * j + c) * VLD + 32 * k + 16 * h), p[k], o[j]);
+    }
+    if (t + 64 < hi) put(smem + (which ^ 1) * BUF);
+    __syncthreads();
+    which ^= 1;
+  }
+  sum += __shfl_xor(sum, 32, 64);
+
+  if (!real) return;
+  // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values
+  if (a.splits > 1) {
+    float* dst = a.big_part + ((((int64_t)head * a.big_tiles + nth) * a.splits + part) * 128 + wave * 32 + c) * LD;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int j = 0; j < OT; ++j)
+        *(f32x2_t*)(dst + (8 * (e >> 2) + 4 * h + (e & 3)) * (D / 16) + 2 * j) = f32x2_t{o[j][e], o[j][8 + e]};
+    if (h == 0) *(f32x2_t*)(dst + D) = f32x2_t{top, sum};
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees no token is zero)
+  uint16_t* dst = a.out + ((int64_t)(q.row0 + row) * a.heads + head * group + qh) * D;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+#pragma unroll
+    for (int j = 0; j < OT; ++j)
+      *(uint32_t*)(dst + (8 * (e >> 2) + 4 * h + (e & 3)) * (D / 16) + 2 * j) = pack_act2(o[j][e] * inv, o[j][8 + e] * inv, DT);
+}
+
 // Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
 constexpr int rows_slots(int64_t dim) { return 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1); }
 
-static int rows_shares(int64_t kv_heads, int64_t dim) { return (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1); }
+// rows * group up to which a sequence goes to tiles of 16 rows, which stream its
+// tokens once per tile
+constexpr int kFewItems = 32;
 
-// Whether a tile can have more than one block, and so be split.
-static bool rows_split(int64_t page_size, int64_t width) { return width * page_size > 256; }
+struct Plan {
+  bool rows, tiles;  // which kernels run
+  int few, shares, splits;
+  int64_t big_tiles;
+  size_t part, big_part;  // bytes
+};
+
+// From what the host knows: rows and sequences, not their lengths.
+static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
+                    int64_t seqs) {
+  Plan p{};
+  const int64_t group = heads / kv_heads, items = rows * group, tokens = width * page_size;
+  if (rows <= seqs || items <= kFewItems) {  // single tokens (no more rows than sequences)
+    p.rows = true;
+    p.few = 0x7fffffff;
+  } else {
+    p.rows = seqs > 1;
+    p.tiles = true;
+    p.few = p.rows ? kFewItems : 0;
+    p.big_tiles = items / 128 + std::min<int64_t>(seqs, items / (p.few + 1));
+    // few tiles: cut their tokens until two workgroups a CU have some
+    const int64_t most = std::max<int64_t>((tokens + 511) / 512, 1);
+    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, 512 / (p.big_tiles * kv_heads)));
+  }
+  p.splits = std::max(p.splits, 1);
+  p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
+  if (p.rows && tokens > 256) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
+  if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * 128 * (dim + 4));
+  return p;
+}
 
 template <int D, int DT, int NT, int PP>
-static void launch_rows(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  const size_t lds = sizeof(float) * 4 * 16 * (D + 4);
-  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT, NT, PP>), dim3((unsigned)a.shares, (unsigned)c.kv_heads), dim3(256), lds, st, a,
+static void launch_rows(const AttendArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  hipLaunchKernelGGL((kv_attend_rows_kernel<D, DT, NT, PP>), dim3((unsigned)a.shares, (unsigned)c.kv_heads), dim3(256), 0, st, a,
                      c, b, b.table, c.k_scale, c.v_scale);
-  if (split)
+}
+
+template <int D, int DT>
+static void launch(const AttendArgs& a, const Plan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  constexpr int NT = D == 256 ? 2 : 4;  // (registers)
+  const int page = 1 << c.page_shift;
+  if (p.rows) {
+    if (page >= 16 * NT)
+      launch_rows<D, DT, NT, 1>(a, c, b, st);
+    else if (page == 8 * NT)
+      launch_rows<D, DT, NT, 2>(a, c, b, st);
+    else if constexpr (NT == 4)
+      launch_rows<D, DT, NT, 4>(a, c, b, st);
+  }
+  if (p.tiles)
+    hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)), dim3(256), 0, st,
+                       a, c, b, b.table, c.k_scale, c.v_scale);
+  if (a.part != nullptr || a.big_part != nullptr)
     hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0, st, a,
                        c, b);
 }
 
-template <int D, int DT>
-static void pick_pages(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  constexpr int NT = D == 256 ? 2 : 4;  // (registers)
-  const int page = 1 << c.page_shift;
-  if (page >= 16 * NT)
-    launch_rows<D, DT, NT, 1>(a, split, c, b, st);
-  else if (page == 8 * NT)
-    launch_rows<D, DT, NT, 2>(a, split, c, b, st);
-  else if constexpr (NT == 4)
-    launch_rows<D, DT, NT, 4>(a, split, c, b, st);
-}
-
 template <int D>
-static void pick_rows(const AttendArgs& a, bool split, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+static void launch_dtype(const AttendArgs& a, const Plan& p, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
   if (dtype == KQ_DTYPE_BF16)
-    pick_pages<D, KQ_DTYPE_BF16>(a, split, c, b, st);
+    launch<D, KQ_DTYPE_BF16>(a, p, c, b, st);
   else
-    pick_pages<D, KQ_DTYPE_F16>(a, split, c, b, st);
+    launch<D, KQ_DTYPE_F16>(a, p, c, b, st);
 }
 
 }  // namespace kq
@@ -491,7 +800,8 @@ using namespace kq;
 extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                                  int64_t page_size, int64_t table_width, int64_t seqs) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
-  return rows_split(page_size, table_width) ? sizeof(float) * (size_t)(rows_shares(kv_heads, dim) * kv_heads * 2 * 16 * (dim + 4)) : 0;
+  const Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs);
+  return p.part + p.big_part;
 }
 
 extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
@@ -514,14 +824,18 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   }
   if (rows == 0) return KQ_OK;
   const bool empty = seqs == 0 || pages == 0 || table_width == 0;  // every row is zero
-  const bool split = !empty && rows_split(page_size, table_width);
-  if (split && (workspace == nullptr || workspace_bytes < kq_kv_attention_workspace_size(rows, heads, kv_heads, dim, page_size,
-                                                                                           table_width, seqs))) {
+  Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs);
+  if (empty) {
+    p = Plan{};
+    p.rows = true;
+    p.shares = (int)std::min<int64_t>(rows, 1024);
+  }
+  if (p.part + p.big_part > 0 && (workspace == nullptr || workspace_bytes < p.part + p.big_part)) {
     set_error("%s: workspace of %zu bytes is too small", what, workspace_bytes);
     return KQ_EWORKSPACE;
   }
   // threads of one launch, and blocks of all tiles
-  if (rows * heads * 64 >= (1LL << 32) ||
+  if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 256 >= (1LL << 32) ||
       (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256) >= (1LL << 31)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
@@ -531,10 +845,11 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.q = (const uint16_t*)q;
   a.q_ld = q_ld, a.q_hs = q_hs;
   a.out = (uint16_t*)out;
-  a.part = (float*)workspace;
+  a.part = p.part > 0 ? (float*)workspace : nullptr;
+  a.big_part = p.big_part > 0 ? (float*)((char*)workspace + p.part) : nullptr;
   a.scale = scale * 1.44269504088896340736f;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
-  a.shares = rows_shares(kv_heads, dim);
+  a.shares = p.shares, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.splits = p.splits;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
@@ -542,10 +857,10 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   const KvBatch b{table, cu, lengths, table_ld, empty ? 0 : (int)seqs, (int)table_width, (int)rows};
   hipStream_t st = (hipStream_t)stream;
   if (dim == 64)
-    pick_rows<64>(a, split, c, b, dtype, st);
+    launch_dtype<64>(a, p, c, b, dtype, st);
   else if (dim == 128)
-    pick_rows<128>(a, split, c, b, dtype, st);
+    launch_dtype<128>(a, p, c, b, dtype, st);
   else
-    pick_rows<256>(a, split, c, b, dtype, st);
+    launch_dtype<256>(a, p, c, b, dtype, st);
   return check_launch(what);
 }
