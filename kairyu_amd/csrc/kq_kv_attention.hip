@@ -20,7 +20,8 @@ struct AttendArgs {
   int64_t q_ld, q_hs;
   uint16_t* out;  // [rows][heads][D]
   float* part;    // partial outputs of split sequences, null: none can be split
-  float scale;    // times log2 e
+  float scale;    // magnitude times log2 e, at least 2^-60: times a page's scale it stays positive
+  uint32_t q_sign;  // the softmax scale's sign, for two 16-bit elements
   int heads, causal, window;
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
   float* big_part;  // partial outputs of the 128-row tiles, null: their tokens are not split
@@ -212,7 +213,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   if (real) {
     const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1));
+    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1)) ^ a.q_sign;
   }
 
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
@@ -545,54 +546,59 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   if (real) {
     const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h);
+    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h) ^ a.q_sign;
   }
 
-  // what this thread moves: D / 4 bytes of one token's key, D / 16 of four tokens' values
-  const int k_tok = tid >> 2, k_at = (tid & 3) * (D / 4);
-  const int v_grp = tid >> 4, v_c = tid & 15;
+  // what this thread moves: D / 4 bytes of one token's key, D / 16 of four tokens' values;
+  // a wave moves one 16-token tile, which lies in one page
+  const int k_tok = tid >> 2, v_grp = tid >> 4, v_c = tid & 15;
+  const int k_lane = (k_tok & 15) * D + (tid & 3) * (D / 4), v_lane = 4 * (v_grp & 3) * D + v_c * (D / 16);
   const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
   const int64_t tile_bytes = (int64_t)D << shift;
   const int in_page = (1 << shift) - 1;
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
   auto page_at = [&](int t) {
-    const int got = pages[min(t, max(hi - 1, 0)) >> shift];
-    return t < hi && got >= 0 && got < cache.pages ? got : -1;
+    const int at = t + 16 * wave;
+    const int got = pages[min(at, max(hi - 1, 0)) >> shift];
+    return at < hi ? got : -1;
   };
   u32x4 kr[KC];
   uint32_t vr[4][VC];
   float sc_k = 0.0f, sc_v = 0.0f;
-  int kp = page_at(lo + k_tok), vp = page_at(lo + 4 * v_grp);
+  int next_page = page_at(lo);
   auto fetch = [&](int t) {
-    const uint8_t* ks = cache.k + ((int64_t)max(kp, 0) * cache.kv_heads + head) * tile_bytes + ((t + k_tok) & in_page) * D + k_at;
+    const int page = __builtin_amdgcn_readfirstlane(next_page), at = t + 16 * wave;
+    const bool there = page >= 0 && page < cache.pages;
+    const int64_t head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
+    // slots past the end hold whatever was there, NaN perhaps: the resources end before them
+    const uint32_t size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
+    const i32x4 ksrc = make_rsrc(cache.k + head_tile * tile_bytes, size);
+    const i32x4 vsrc = make_rsrc(cache.v + head_tile * tile_bytes, size);
+    const int off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
 #pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const u32x4 x = *(const u32x4*)(ks + 16 * i);
-      kr[i] = kp >= 0 ? x : u32x4{0, 0, 0, 0};
-    }
-    const int64_t v_tile = (int64_t)max(vp, 0) * cache.kv_heads + head;
-    const uint8_t* vs = cache.v + v_tile * tile_bytes + ((t + 4 * v_grp) & in_page) * D + v_c * (D / 16);
+    for (int i = 0; i < KC; ++i) kr[i] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(ksrc, k_lane + 16 * i, off, 0));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      // slots past the end hold whatever was there, NaN perhaps
-      const bool there = vp >= 0 && t + 4 * v_grp + r < q.tokens;
+      if constexpr (VC == 1) {
+        vr[r][0] = (uint32_t)kq_rbl_i32(vsrc, v_lane + r * D, off, 0);
+      } else if constexpr (VC == 2) {
+        const i32x2 w = kq_rbl_v2i32(vsrc, v_lane + r * D, off, 0);
+        vr[r][0] = (uint32_t)w[0];
+        vr[r][1] = (uint32_t)w[1];
+      } else {
+        const i32x4 w = kq_rbl_v4i32(vsrc, v_lane + r * D, off, 0);
 #pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        const uint32_t x = *(const uint32_t*)(vs + r * D + 4 * i);
-        vr[r][i] = there ? x : 0u;
+        for (int i = 0; i < VC; ++i) vr[r][i] = (uint32_t)w[i];
       }
     }
-    if (v_c == 0 && (v_grp & 3) == 0) {
-      sc_k = vp >= 0 ? k_scale[v_tile] * a.scale : 1.0f;
-      sc_v = vp >= 0 ? v_scale[v_tile] : 0.0f;
-    }
-    kp = page_at(t + 64 + k_tok);
-    vp = page_at(t + 64 + 4 * v_grp);
+    sc_k = there ? k_scale[head_tile] * a.scale : 1.0f;
+    sc_v = there ? v_scale[head_tile] : 0.0f;
+    next_page = page_at(t + 64);
   };
   auto put = [&](char* buf) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      char* dst = buf + k_tok * KLD + 2 * (k_at + 16 * i);
+      char* dst = buf + k_tok * KLD + 2 * ((tid & 3) * (D / 4) + 16 * i);
       *(u32x4*)dst = widen_codes<DT>(kr[i][0], kr[i][1]);
       *(u32x4*)(dst + 16) = widen_codes<DT>(kr[i][2], kr[i][3]);
     }
@@ -608,11 +614,11 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         *(u32x2*)(buf + KB + ((4 * i + j) * 16 + v_c) * VLD + 2 * v_pos) = w;
       }
     }
-    if (v_c == 0 && (v_grp & 3) == 0) {
-      float* dst = (float*)(buf + KB + VB) + (v_grp >> 2);
+    if (lane == 0) {
+      float* dst = (float*)(buf + KB + VB) + wave;
       dst[0] = sc_k;
       dst[4] = __builtin_amdgcn_logf(sc_v);
-      dst[8] = sc_v > 0.0f ? 1.0f / sc_v : 0.0f;
+      dst[8] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
   };
 
@@ -635,20 +641,18 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     if (t < hi_wave && t + 64 > lo_wave) {
       f32x16 w[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[i][e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
           w[i] = mfma32<DT>(*(const u32x4*)(buf + (32 * i + c) * KLD + 32 * k + 16 * h), qf[k], w[i]);
-      }
       const f32x4 ks = *(const f32x4*)(buf + KB + VB), lv = *(const f32x4*)(buf + KB + VB + 16),
                   iv = *(const f32x4*)(buf + KB + VB + 32);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[i][e] = fmaf(w[i][e], ks[2 * i + (e >> 3)], lv[2 * i + (e >> 3)]);
       if (t < lo_all || t + 64 > hi_all) {
+        asm volatile("");  // (kept a branch: most steps have nothing to mask)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -657,11 +661,17 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
             if (token < from || token >= to) w[i][e] = -__builtin_inff();
           }
       }
+      // a 16-token tile's scale is positive, so its largest score is its largest dot product's
       float m = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, w[i][e]);
+        for (int g = 0; g < 2; ++g) {
+          float x = w[i][8 * g];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) x = fmaxf(x, w[i][8 * g + e]);
+          m = fmaxf(m, fmaf(x, ks[2 * i + g], lv[2 * i + g]));
+        }
       const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
       m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       if (__ballot(m > top) != 0) {
@@ -678,20 +688,21 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
+          const float scale = ks[2 * i + g], shift_v = lv[2 * i + g] - base;
           float part_sum = 0.0f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = __builtin_amdgcn_exp2f(w[i][8 * g + 2 * e] - base);
-            const float y = __builtin_amdgcn_exp2f(w[i][8 * g + 2 * e + 1] - base);
-            part_sum += x + y;
-            p[2 * i + g][e] = pack_act2(x, y, KQ_DTYPE_F16);
+            const uint32_t pair = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[i][8 * g + 2 * e], scale, shift_v)),
+                                            __builtin_amdgcn_exp2f(fmaf(w[i][8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
+            p[2 * i + g][e] = pair;
+            part_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, part_sum, false);
           }
           sum = fmaf(part_sum, iv[2 * i + g], sum);
         }
 #pragma unroll
-      for (int j = 0; j < OT; ++j)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int j = 0; j < OT; ++j)
           o[j] = mfma32<KQ_DTYPE_F16>(*(const u32x4*)(buf + KB + (32 * j + c) * VLD + 32 * k + 16 * h), p[k], o[j]);
     }
     if (t + 64 < hi) put(smem + (which ^ 1) * BUF);
@@ -847,7 +858,8 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.out = (uint16_t*)out;
   a.part = p.part > 0 ? (float*)workspace : nullptr;
   a.big_part = p.big_part > 0 ? (float*)((char*)workspace + p.part) : nullptr;
-  a.scale = scale * 1.44269504088896340736f;
+  a.scale = fmaxf(fabsf(scale) * 1.44269504088896340736f, 0x1p-60f);
+  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
   a.shares = p.shares, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.splits = p.splits;
   int shift = 4;
