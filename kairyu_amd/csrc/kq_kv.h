@@ -50,6 +50,16 @@ KQ_DEV KvSeq kv_seq(const KvBatch& b, int s, int page_shift) {
   return q;
 }
 
+// The same for one sequence of the whole wave, in scalar registers.
+KQ_DEV KvSeq kv_seq_uniform(const KvBatch& b, int s, int page_shift) {
+  KvSeq q = kv_seq(b, s, page_shift);
+  q.row0 = __builtin_amdgcn_readfirstlane(q.row0);
+  q.rows = __builtin_amdgcn_readfirstlane(q.rows);
+  q.first = __builtin_amdgcn_readfirstlane(q.first);
+  q.tokens = __builtin_amdgcn_readfirstlane(q.tokens);
+  return q;
+}
+
 // The page that holds `slot` of sequence s (slot < table_width), or -1 where the
 // entry names none.
 KQ_DEV int kv_page(const KvBatch& b, const KvCache& c, int s, int slot) {

@@ -24,10 +24,11 @@ struct AttendArgs {
   uint32_t q_sign;  // the softmax scale's sign, for two 16-bit elements
   int heads, causal, window;
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
-  float* big_part;  // partial outputs of the 128-row tiles, null: their tokens are not split
+  float* big_part;  // partial outputs of the large tiles, null: their tokens are not split
+  int big_rows;     // rows of such a tile
   int few;          // rows * group up to which a sequence goes to tiles of 16 rows
-  int big_tiles;    // 128-row tiles per kv head that the grid has room for
-  int splits;       // parts that a 128-row tile's tokens are cut into
+  int big_tiles;    // large tiles per kv head that the grid has room for
+  int splits;       // parts that a large tile's tokens are cut into
 };
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
@@ -103,7 +104,7 @@ struct Deal {
 };
 KQ_DEV int big_tiles(const AttendArgs& a, const KvSeq& q, int group) {
   const int items = q.rows * group;
-  return items > a.few ? (items + 127) >> 7 : 0;
+  return items > a.few ? (items + a.big_rows - 1) / a.big_rows : 0;
 }
 
 // The same run in every workgroup.
@@ -125,14 +126,14 @@ KQ_DEV Deal deal_of(const AttendArgs& a, const KvBatch& b, int shift, int group)
 
 // Rows of no sequence are zero: those of one kv head, dealt to `of` workgroups.
 template <int D>
-KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, int group, int nth, int of) {
+KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, int group, int nth, int of, int threads) {
   const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
   const int first = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
   const int words = group * D / 2;
   for (int i = nth; i < first + batch.rows - last; i += of) {
     const int64_t row = i < first ? i : last + (i - first);
     uint32_t* dst = (uint32_t*)(a.out + (row * a.heads + head * group) * D);
-    for (int j = (int)threadIdx.x; j < words; j += 256) dst[j] = 0;
+    for (int j = (int)threadIdx.x; j < words; j += threads) dst[j] = 0;
   }
 }
 
@@ -172,7 +173,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
   const int head = (int)blockIdx.y;
 
-  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x);
+  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 256);
   const Deal deal = deal_of(a, batch, shift, group);
   const int64_t run_end = ((int64_t)blockIdx.x + 1) * deal.run;
   int64_t block = (int64_t)blockIdx.x * deal.run;
@@ -182,7 +183,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     return Deal::tiles(a, q, group) * Deal::blocks(a, q);
   });
   if (s < 0) return;
-  KvSeq q = kv_seq(batch, s, shift);
+  KvSeq q = kv_seq_uniform(batch, s, shift);
   int blocks = Deal::blocks(a, q), tile = within / blocks;
   within -= tile * blocks;
   const int64_t tile_bytes = (int64_t)D << shift;
@@ -407,7 +408,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     tile = 0;
     do {
       if (++s >= batch.seqs) return;
-      q = kv_seq(batch, s, shift);
+      q = kv_seq_uniform(batch, s, shift);
     } while (Deal::tiles(a, q, group) == 0);
     blocks = Deal::blocks(a, q);
   }
@@ -424,18 +425,18 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
   const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
   if (at >= (int64_t)batch.rows * a.heads) return;
   const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads), head = qh / group;
-  int64_t before;  // 128-row tiles, or blocks, of the sequences before the row's
+  int64_t before;  // large tiles, or blocks, of the sequences before the row's
   int s = kv_of_row(row, batch, shift, before, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
   if (s < 0) return;
-  const KvSeq q = kv_seq(batch, s, shift);
+  const KvSeq q = kv_seq_uniform(batch, s, shift);
   const int item = (row - q.row0) * group + (qh - head * group);
   const float* src;
-  int chunks, step;  // part i > 0 lies (step * i - 1) * 16 rows behind the first, or i * 128
-  if (q.rows * group > a.few) {
+  int chunks;
+  const bool big = q.rows * group > a.few;
+  if (big) {
     if (a.splits == 1) return;
     chunks = a.splits;
-    step = 0;
-    src = a.big_part + ((((int64_t)head * a.big_tiles + before + (item >> 7)) * a.splits) * 128 + (item & 127)) * LD;
+    src = a.big_part + ((((int64_t)head * a.big_tiles + before + item / a.big_rows) * a.splits) * a.big_rows + item % a.big_rows) * LD;
   } else {
     const Deal deal = deal_of(a, batch, shift, group);
     kv_of_row(row, batch, shift, before, [&](int i) {
@@ -447,11 +448,10 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
     const int x0 = (int)(block / deal.run);
     chunks = (int)((block + blocks - 1) / deal.run) - x0 + 1;
     if (chunks == 1) return;  // written already
-    step = 2;
     // part 1 of the run it begins in, then part 0 of those behind
     src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
   }
-  auto at_part = [&](int i) { return src + (step == 0 ? (int64_t)i * 128 : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
+  auto at_part = [&](int i) { return src + (big ? (int64_t)i * a.big_rows : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
   float m = -__builtin_inff();
   for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
   m = wave_max(m);
@@ -482,29 +482,28 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// One workgroup: a tile of 128 rows of one sequence and kv head (32 a wave), over the
-// tokens that it sees or one of `splits` parts of them, 64 at a step.
+// One workgroup: a tile of 32 rows a wave of one sequence and kv head, over the tokens
+// that it sees or one of `splits` parts of them, 64 at a step.
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
-// are shared by the four waves: they are widened once, keys to Q's type in rows of
-// one token, values to fp16 in rows of one d whose tokens stand in the order in which
-// the lanes of S^T hold them (for each 16: 0-3, 8-11, then 4-7, 12-15), so that both
-// are read as 16-byte MFMA operands; rows are padded by 16 bytes, which spreads eight
-// lanes' reads over all banks.  Two steps' worth of LDS: the next step's bytes travel
-// from memory while this one is computed, and one barrier a step suffices.  Row R of
-// the values is d = R % 16 * (D / 16) + R / 16 (any order does), which again leaves a
-// lane with neighbouring elements.
-template <int D, int DT>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+// are shared by the waves: they are widened once, keys to Q's type in rows of one
+// token, values to fp16 in rows of one d whose tokens stand in the order in which the
+// lanes of S^T hold them (for each 16: 0-3, 8-11, then 4-7, 12-15), so that both are
+// read as 16-byte MFMA operands; rows are padded by 16 bytes, which spreads eight
+// lanes' reads over all banks.
+template <int D, int DT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2)
 kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
                        const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
   constexpr int KS = D / 16;            // MFMA steps along a key
   constexpr int OT = D / 32;            // output tiles
+  constexpr int ROWS = 32 * WAVES;
   constexpr int KLD = 2 * D + 16;       // bytes of a key's row
   constexpr int VLD = 2 * 64 + 16;      // bytes of a d's row of values
   constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale, its inverse)
-  constexpr int KC = D / 64;            // 16-byte chunks of keys a thread moves
-  constexpr int VC = D / 64;            // dwords of each of four tokens' values a thread moves
+  constexpr int KC = D / WAVES / 16;    // 16-byte chunks of one token's key a thread moves
+  constexpr int VW = 4 * WAVES;         // threads that move four tokens' values
+  constexpr int VY = D / VW, VC = VY / 4;  // bytes and dwords of each token's a thread moves
   constexpr int LD = D + 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   const int wave = __builtin_amdgcn_readfirstlane(wave_id());
@@ -514,22 +513,22 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   // theirs through its L2; the tiles with the most tokens first
   const int head = (int)blockIdx.x % cache.kv_heads, rest = (int)blockIdx.x / cache.kv_heads;
   const int part = rest % a.splits, nth = a.big_tiles - 1 - rest / a.splits;
-  if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits);  // (no other kernel does)
+  if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 64 * WAVES);  // (no other kernel does)
   int tile;
   const int s = kv_find(nth, batch.seqs, tile, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
   if (s < 0) return;
-  const KvSeq q = kv_seq(batch, s, shift);
-  const int item = tile * 128 + wave * 32 + c;
+  const KvSeq q = kv_seq_uniform(batch, s, shift);
+  const int item = tile * ROWS + wave * 32 + c;
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
   const int pos = q.first + row;
   // tokens [from, to) of this column, [lo_all, hi_all) of every row of the wave, [lo, hi) of the tile
   const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
   const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-  const int last_row = min(q.rows - 1, (tile * 128 + 127) / group);
+  const int last_row = min(q.rows - 1, (tile * ROWS + ROWS - 1) / group);
   int hi = a.causal ? max(min(q.tokens, q.first + last_row + 1), 0) : q.tokens;
-  int lo = a.window > 0 ? max(q.first + tile * 128 / group + 1 - a.window, 0) & ~63 : 0;
-  const int w_lo = (tile * 128 + wave * 32) / group, w_hi = min(q.rows - 1, (tile * 128 + wave * 32 + 31) / group);
+  int lo = a.window > 0 ? max(q.first + tile * ROWS / group + 1 - a.window, 0) & ~63 : 0;
+  const int w_lo = (tile * ROWS + wave * 32) / group, w_hi = min(q.rows - 1, (tile * ROWS + wave * 32 + 31) / group);
   const int hi_all = a.causal ? min(q.tokens, q.first + w_lo + 1) : q.tokens;
   const int lo_all = a.window > 0 ? max(q.first + w_hi + 1 - a.window, 0) : 0;
   const int lo_wave = a.window > 0 ? max(q.first + w_lo + 1 - a.window, 0) : 0;
@@ -549,59 +548,73 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h) ^ a.q_sign;
   }
 
-  // what this thread moves: D / 4 bytes of one token's key, D / 16 of four tokens' values;
-  // a wave moves one 16-token tile, which lies in one page
-  const int k_tok = tid >> 2, v_grp = tid >> 4, v_c = tid & 15;
-  const int k_lane = (k_tok & 15) * D + (tid & 3) * (D / 4), v_lane = 4 * (v_grp & 3) * D + v_c * (D / 16);
+  // what this thread moves: D / WAVES bytes of one token's key, VY of four tokens' values;
+  // a wave moves part of one 16-token tile, which lies in one page.  Row R of the values
+  // is d = R % VW * VY + R / VW: any order of d does, and neighbouring lanes then write
+  // neighbouring rows.
+  constexpr int TOK = 64 / WAVES;  // tokens a wave moves
+  const int k_tok = tid / WAVES, v_grp = tid / VW, v_c = tid % VW;
+  const int k_lane = (k_tok % TOK) * D + (tid % WAVES) * (D / WAVES), v_lane = 4 * (v_grp % (TOK / 4)) * D + v_c * VY;
   const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
   const int64_t tile_bytes = (int64_t)D << shift;
   const int in_page = (1 << shift) - 1;
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
-  auto page_at = [&](int t) {
-    const int at = t + 16 * wave;
-    const int got = pages[min(at, max(hi - 1, 0)) >> shift];
-    return at < hi ? got : -1;
-  };
+  const int tile_at = TOK * wave & ~15;  // (the waves that share a 16-token tile agree on its page)
+  auto page_at = [&](int t) { return pages[min(t + tile_at, max(hi - 1, 0)) >> shift]; };
   u32x4 kr[KC];
   uint32_t vr[4][VC];
   float sc_k = 0.0f, sc_v = 0.0f;
-  int next_page = page_at(lo);
-  auto fetch = [&](int t) {
-    const int page = __builtin_amdgcn_readfirstlane(next_page), at = t + 16 * wave;
-    const bool there = page >= 0 && page < cache.pages;
-    const int64_t head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
-    // slots past the end hold whatever was there, NaN perhaps: the resources end before them
-    const uint32_t size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
-    const i32x4 ksrc = make_rsrc(cache.k + head_tile * tile_bytes, size);
-    const i32x4 vsrc = make_rsrc(cache.v + head_tile * tile_bytes, size);
-    const int off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
+  // a step's page of this wave: its tile, the bytes before the sequence's end (slots past
+  // it hold whatever was there, NaN perhaps; the resources end before them) and the offset
+  struct Place {
+    int64_t head_tile;
+    uint32_t size;
+    int off;
+  };
+  auto place_of = [&](int t, int page_) {
+    const int page = __builtin_amdgcn_readfirstlane(page_), at = t + TOK * wave;
+    const bool there = page >= 0 && page < cache.pages && t + tile_at < hi;
+    Place p;
+    p.head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
+    p.size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
+    p.off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
+    return p;
+  };
+  auto fetch_k = [&](const Place& p) {
+    const i32x4 src = make_rsrc(cache.k + p.head_tile * tile_bytes, p.size);
 #pragma unroll
-    for (int i = 0; i < KC; ++i) kr[i] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(ksrc, k_lane + 16 * i, off, 0));
+    for (int i = 0; i < KC; ++i) kr[i] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(src, k_lane + 16 * i, p.off, 0));
+    // (a vector load, which the barriers do not wait for; 0 where there is no page)
+    sc_k = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
+  };
+  auto fetch_v = [&](const Place& p) {
+    const i32x4 src = make_rsrc(cache.v + p.head_tile * tile_bytes, p.size);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if constexpr (VC == 1) {
-        vr[r][0] = (uint32_t)kq_rbl_i32(vsrc, v_lane + r * D, off, 0);
+        vr[r][0] = (uint32_t)kq_rbl_i32(src, v_lane + r * D, p.off, 0);
       } else if constexpr (VC == 2) {
-        const i32x2 w = kq_rbl_v2i32(vsrc, v_lane + r * D, off, 0);
+        const i32x2 w = kq_rbl_v2i32(src, v_lane + r * D, p.off, 0);
         vr[r][0] = (uint32_t)w[0];
         vr[r][1] = (uint32_t)w[1];
       } else {
-        const i32x4 w = kq_rbl_v4i32(vsrc, v_lane + r * D, off, 0);
+        const i32x4 w = kq_rbl_v4i32(src, v_lane + r * D, p.off, 0);
 #pragma unroll
         for (int i = 0; i < VC; ++i) vr[r][i] = (uint32_t)w[i];
       }
     }
-    sc_k = there ? k_scale[head_tile] * a.scale : 1.0f;
-    sc_v = there ? v_scale[head_tile] : 0.0f;
-    next_page = page_at(t + 64);
+    sc_v = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
   };
-  auto put = [&](char* buf) {
+  auto put_k = [&](char* buf) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      char* dst = buf + k_tok * KLD + 2 * ((tid & 3) * (D / 4) + 16 * i);
+      char* dst = buf + k_tok * KLD + 2 * ((tid % WAVES) * (D / WAVES) + 16 * i);
       *(u32x4*)dst = widen_codes<DT>(kr[i][0], kr[i][1]);
       *(u32x4*)(dst + 16) = widen_codes<DT>(kr[i][2], kr[i][3]);
     }
+    if (lane == 0) ((float*)(buf + KB + VB))[wave * TOK / 16] = sc_k > 0.0f ? sc_k * a.scale : 1.0f;  // (waves of one tile write the same)
+  };
+  auto put_v = [&](char* buf) {
 #pragma unroll
     for (int i = 0; i < VC; ++i) {
       const uint32_t in[4] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i]};
@@ -611,15 +624,20 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       for (int j = 0; j < 4; ++j) {
         const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, false)),
                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, true))};
-        *(u32x2*)(buf + KB + ((4 * i + j) * 16 + v_c) * VLD + 2 * v_pos) = w;
+        *(u32x2*)(buf + KB + ((4 * i + j) * VW + v_c) * VLD + 2 * v_pos) = w;
       }
     }
     if (lane == 0) {
-      float* dst = (float*)(buf + KB + VB) + wave;
-      dst[0] = sc_k;
-      dst[4] = __builtin_amdgcn_logf(sc_v);
-      dst[8] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
+      float* dst = (float*)(buf + KB + VB) + 4 + wave * TOK / 16;
+      dst[0] = __builtin_amdgcn_logf(sc_v);
+      dst[4] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
+  };
+  // LDS is complete for every wave; loads from memory stay in flight
+  auto meet = [] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
 
   f32x16 o[OT];
@@ -629,111 +647,185 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
   float top = -__builtin_inff(), sum = 0.0f;
 
-  if (lo < hi) {
-    fetch(lo);
-    put(smem);
-  }
-  __syncthreads();
-  int which = 0;
-  for (int t = lo; t < hi; t += 64) {
-    const char* buf = smem + which * BUF;
-    if (t + 64 < hi) fetch(t + 64);
-    if (t < hi_wave && t + 64 > lo_wave) {
-      f32x16 w[2];
+  // the keys of 32 tokens, half i of the step in buf, and their scores
+  u32x4 kx[KS];
+  auto read_keys = [&](const char* buf, int i) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int k = 0; k < KS; ++k) kx[k] = *(const u32x4*)(buf + (32 * i + c) * KLD + 32 * k + 16 * h);
+  };
+  auto dots = [&](f32x16& w) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[i][e] = 0.0f;
+    for (int e = 0; e < 16; ++e) w[e] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+    for (int k = 0; k < KS; ++k) w = mfma32<DT>(kx[k], qf[k], w);
+  };
+  // masks them, and moves the running maximum where one exceeds it
+  auto limit = [&](int t, f32x2_t ks, f32x2_t lv, f32x16& w) {
+    if (t < lo_all || t + 32 > hi_all) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          w[i] = mfma32<DT>(*(const u32x4*)(buf + (32 * i + c) * KLD + 32 * k + 16 * h), qf[k], w[i]);
-      const f32x4 ks = *(const f32x4*)(buf + KB + VB), lv = *(const f32x4*)(buf + KB + VB + 16),
-                  iv = *(const f32x4*)(buf + KB + VB + 32);
-      if (t < lo_all || t + 64 > hi_all) {
-        asm volatile("");  // (kept a branch: most steps have nothing to mask)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int token = t + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (token < from || token >= to) w[i][e] = -__builtin_inff();
-          }
+      for (int e = 0; e < 16; ++e) {
+        const int token = t + 8 * (e >> 2) + 4 * h + (e & 3);
+        if (token < from || token >= to) w[e] = -__builtin_inff();
       }
-      // a 16-token tile's scale is positive, so its largest score is its largest dot product's
-      float m = -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float x = w[i][8 * g];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) x = fmaxf(x, w[i][8 * g + e]);
-          m = fmaxf(m, fmaf(x, ks[2 * i + g], lv[2 * i + g]));
-        }
-      const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-      m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-      if (__ballot(m > top) != 0) {
-        m = fmaxf(m, top);
-        const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
-        sum *= keep;
-#pragma unroll
-        for (int j = 0; j < OT; ++j) o[j] *= keep;
-        top = m;
-      }
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-      u32x4 p[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float scale = ks[2 * i + g], shift_v = lv[2 * i + g] - base;
-          float part_sum = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t pair = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[i][8 * g + 2 * e], scale, shift_v)),
-                                            __builtin_amdgcn_exp2f(fmaf(w[i][8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
-            p[2 * i + g][e] = pair;
-            part_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, part_sum, false);
-          }
-          sum = fmaf(part_sum, iv[2 * i + g], sum);
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < OT; ++j)
-          o[j] = mfma32<KQ_DTYPE_F16>(*(const u32x4*)(buf + KB + (32 * j + c) * VLD + 32 * k + 16 * h), p[k], o[j]);
     }
-    if (t + 64 < hi) put(smem + (which ^ 1) * BUF);
-    __syncthreads();
-    which ^= 1;
+    // a 16-token tile's scale is positive, so its largest score is its largest dot product's
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float x = w[8 * g];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) x = fmaxf(x, w[8 * g + e]);
+      m = fmaxf(m, fmaf(x, ks[g], lv[g]));
+    }
+    const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    if (__ballot(m > top) != 0) {
+      m = fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
+      sum *= keep;
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[j] *= keep;
+      top = m;
+    }
+  };
+  auto weights = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2]) {
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float scale = ks[g], shift_v = lv[g] - base;
+      float part_sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t pair = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e], scale, shift_v)),
+                                        __builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
+        p[g][e] = pair;
+        part_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, part_sum, false);
+      }
+      sum = fmaf(part_sum, iv[g], sum);
+    }
+  };
+  u32x4 vx[2][OT];
+  auto read_values = [&](const char* buf, int i, int k) {
+#pragma unroll
+    for (int j = 0; j < OT; ++j) vx[k][j] = *(const u32x4*)(buf + KB + (32 * j + c) * VLD + 64 * i + 32 * k + 16 * h);
+  };
+  auto add_values = [&](const u32x4 (&p)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[j] = mfma32<KQ_DTYPE_F16>(vx[k][j], p[k], o[j]);
+  };
+  auto pair_at = [&](const char* buf, int which, int i) { return *(const f32x2_t*)(buf + KB + VB + 16 * which + 8 * i); };
+
+  // The order of a half step's instructions: the first values are read while scores are
+  // multiplied, an MFMA for every few of the weights' operations, then the other half.
+  auto pace = [] {
+    __builtin_amdgcn_sched_group_barrier(0x100, OT, 0);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+      if (k >= KS / 2) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OT / KS, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * OT; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+    }
+  };
+
+  // Half steps of 32 tokens, each one's weights computed while the next one's scores are:
+  // the matrix cores have work from the wave itself, not from the other one on its SIMD
+  // alone.  The next step's keys reach LDS before its first half is needed, in the middle
+  // of this step, and its values at the end.
+  if (lo < hi) {
+    Place here = place_of(lo, page_at(lo));
+    fetch_k(here);
+    fetch_v(here);
+    put_k(smem);
+    put_v(smem);
+    here = place_of(lo + 64, page_at(lo + 64));
+    fetch_k(here);
+    fetch_v(here);
+    int next_page = page_at(lo + 128);
+    meet();
+    f32x16 x, y;
+    read_keys(smem, 0);
+    dots(x);
+    int which = 0;
+    for (int t = lo; t < hi; t += 64) {
+      const char* buf = smem + which * BUF;
+      char* next = smem + (which ^ 1) * BUF;
+      u32x4 p[2];
+      {
+        const f32x2_t ks = pair_at(buf, 0, 0), lv = pair_at(buf, 1, 0), iv = pair_at(buf, 2, 0);
+        read_keys(buf, 1);
+        limit(t, ks, lv, x);
+        read_values(buf, 0, 0);
+        dots(y);
+        weights(ks, lv, iv, x, p);
+        read_values(buf, 0, 1);
+        add_values(p);
+        put_k(next);
+        pace();
+        here = place_of(t + 128, next_page);
+        fetch_k(here);
+      }
+      meet();
+      {
+        const f32x2_t ks = pair_at(buf, 0, 1), lv = pair_at(buf, 1, 1), iv = pair_at(buf, 2, 1);
+        read_keys(next, 0);
+        limit(t + 32, ks, lv, y);
+        read_values(buf, 1, 0);
+        dots(x);
+        weights(ks, lv, iv, y, p);
+        read_values(buf, 1, 1);
+        add_values(p);
+        put_v(next);
+        pace();
+        fetch_v(here);
+        next_page = page_at(t + 192);
+      }
+      meet();
+      which ^= 1;
+    }
   }
   sum += __shfl_xor(sum, 32, 64);
 
   if (!real) return;
-  // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values
+  // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values.  Stores of
+  // neighbouring d: pairs of one tile where VW = 16, one element of every tile where VW = 32.
+  auto store = [&](auto put) {
+#pragma unroll
+    for (int e = 0; e < VW / 2; ++e) {
+      const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+      if constexpr (VW == 16) {
+#pragma unroll
+        for (int j = 0; j < OT; ++j) put(r * VY + 2 * j, o[j][e], o[j][8 + e]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < OT; j += 2) put(r * VY + j, o[j][e], o[j + 1][e]);
+      }
+    }
+  };
   if (a.splits > 1) {
-    float* dst = a.big_part + ((((int64_t)head * a.big_tiles + nth) * a.splits + part) * 128 + wave * 32 + c) * LD;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int j = 0; j < OT; ++j)
-        *(f32x2_t*)(dst + (8 * (e >> 2) + 4 * h + (e & 3)) * (D / 16) + 2 * j) = f32x2_t{o[j][e], o[j][8 + e]};
+    float* dst = a.big_part + ((((int64_t)head * a.big_tiles + nth) * a.splits + part) * ROWS + wave * 32 + c) * LD;
+    store([&](int d, float x, float y) { *(f32x2_t*)(dst + d) = f32x2_t{x, y}; });
     if (h == 0) *(f32x2_t*)(dst + D) = f32x2_t{top, sum};
     return;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees no token is zero)
   uint16_t* dst = a.out + ((int64_t)(q.row0 + row) * a.heads + head * group + qh) * D;
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-#pragma unroll
-    for (int j = 0; j < OT; ++j)
-      *(uint32_t*)(dst + (8 * (e >> 2) + 4 * h + (e & 3)) * (D / 16) + 2 * j) = pack_act2(o[j][e] * inv, o[j][8 + e] * inv, DT);
+  store([&](int d, float x, float y) { *(uint32_t*)(dst + d) = pack_act2(x * inv, y * inv, DT); });
 }
 
 // Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
 constexpr int rows_slots(int64_t dim) { return 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1); }
+
+// Waves of a large tile's workgroup: eight share what a step widens among twice the
+// rows, where their registers fit a CU together.
+constexpr int tile_waves(int64_t dim) { return dim == 128 ? 8 : 4; }
 
 // rows * group up to which a sequence goes to tiles of 16 rows, which stream its
 // tokens once per tile
@@ -741,7 +833,7 @@ constexpr int kFewItems = 32;
 
 struct Plan {
   bool rows, tiles;  // which kernels run
-  int few, shares, splits;
+  int few, shares, splits, big_rows;
   int64_t big_tiles;
   size_t part, big_part;  // bytes
 };
@@ -758,15 +850,16 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
     p.rows = seqs > 1;
     p.tiles = true;
     p.few = p.rows ? kFewItems : 0;
-    p.big_tiles = items / 128 + std::min<int64_t>(seqs, items / (p.few + 1));
+    p.big_rows = tile_waves(dim) * 32;
+    p.big_tiles = items / p.big_rows + std::min<int64_t>(seqs, items / (p.few + 1));
     // few tiles: cut their tokens until two workgroups a CU have some
     const int64_t most = std::max<int64_t>((tokens + 511) / 512, 1);
-    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, 512 / (p.big_tiles * kv_heads)));
+    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, (dim == 64 ? 768 : dim == 128 ? 256 : 256) / (p.big_tiles * kv_heads)));
   }
   p.splits = std::max(p.splits, 1);
   p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
   if (p.rows && tokens > 256) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
-  if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * 128 * (dim + 4));
+  if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * p.big_rows * (dim + 4));
   return p;
 }
 
@@ -789,7 +882,8 @@ static void launch(const AttendArgs& a, const Plan& p, const KvCache& c, const K
       launch_rows<D, DT, NT, 4>(a, c, b, st);
   }
   if (p.tiles)
-    hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)), dim3(256), 0, st,
+    hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT, tile_waves(D)>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)),
+                       dim3(64 * tile_waves(D)), 0, st,
                        a, c, b, b.table, c.k_scale, c.v_scale);
   if (a.part != nullptr || a.big_part != nullptr)
     hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0, st, a,
@@ -846,7 +940,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
     return KQ_EWORKSPACE;
   }
   // threads of one launch, and blocks of all tiles
-  if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 256 >= (1LL << 32) ||
+  if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 512 >= (1LL << 32) ||
       (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256) >= (1LL << 31)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
@@ -861,7 +955,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.scale = fmaxf(fabsf(scale) * 1.44269504088896340736f, 0x1p-60f);
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
-  a.shares = p.shares, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.splits = p.splits;
+  a.shares = p.shares, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.big_rows = p.big_rows, a.splits = p.splits;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
