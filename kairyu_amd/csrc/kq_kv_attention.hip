@@ -10,6 +10,7 @@
 #include "kq_kv.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace kq {
 
@@ -508,33 +509,34 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   const int wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int lane = lane_id(), c = lane & 31, h = lane >> 5, tid = (int)threadIdx.x;
-  const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
+  // (quotients come out of the vector unit: values of the whole wave go back to scalar registers)
+  auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
   // kv heads side by side, so that (for up to 8 of them) an XCD's workgroups share
   // theirs through its L2; the tiles with the most tokens first
-  const int head = (int)blockIdx.x % cache.kv_heads, rest = (int)blockIdx.x / cache.kv_heads;
-  const int part = rest % a.splits, nth = a.big_tiles - 1 - rest / a.splits;
+  const int rest = scalar((int)blockIdx.x / cache.kv_heads), head = (int)blockIdx.x - rest * cache.kv_heads;
+  const int above = scalar(rest / a.splits), part = rest - above * a.splits, nth = a.big_tiles - 1 - above;
   if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 64 * WAVES);  // (no other kernel does)
-  int tile;
-  const int s = kv_find(nth, batch.seqs, tile, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
+  int found;
+  const int s = scalar(
+      kv_find(nth, batch.seqs, found, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); }));
   if (s < 0) return;
+  const int tile = scalar(found);
   const KvSeq q = kv_seq_uniform(batch, s, shift);
   const int item = tile * ROWS + wave * 32 + c;
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
   const int pos = q.first + row;
-  // tokens [from, to) of this column, [lo_all, hi_all) of every row of the wave, [lo, hi) of the tile
+  // tokens [from, to) of this column, [lo_all, hi_all) of every row of the tile, [lo, hi) of any
   const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
   const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-  const int last_row = min(q.rows - 1, (tile * ROWS + ROWS - 1) / group);
+  const int first_row = scalar(tile * ROWS / group), last_row = min(q.rows - 1, scalar((tile * ROWS + ROWS - 1) / group));
   int hi = a.causal ? max(min(q.tokens, q.first + last_row + 1), 0) : q.tokens;
-  int lo = a.window > 0 ? max(q.first + tile * ROWS / group + 1 - a.window, 0) & ~63 : 0;
-  const int w_lo = (tile * ROWS + wave * 32) / group, w_hi = min(q.rows - 1, (tile * ROWS + wave * 32 + 31) / group);
-  const int hi_all = a.causal ? min(q.tokens, q.first + w_lo + 1) : q.tokens;
-  const int lo_all = a.window > 0 ? max(q.first + w_hi + 1 - a.window, 0) : 0;
-  const int lo_wave = a.window > 0 ? max(q.first + w_lo + 1 - a.window, 0) : 0;
-  const int hi_wave = a.causal ? min(q.tokens, q.first + w_hi + 1) : q.tokens;
+  int lo = a.window > 0 ? max(q.first + first_row + 1 - a.window, 0) & ~63 : 0;
+  const int hi_all = a.causal ? min(q.tokens, q.first + first_row + 1) : q.tokens;
+  const int lo_all = a.window > 0 ? max(q.first + last_row + 1 - a.window, 0) : 0;
   if (a.splits > 1) {
-    const int n = hi > lo ? (hi - lo + 63) >> 6 : 0, per = (n + a.splits - 1) / a.splits;
+    const int n = hi > lo ? (hi - lo + 63) >> 6 : 0, per = scalar((n + a.splits - 1) / a.splits);
     lo += part * per * 64;
     hi = min(hi, lo + per * 64);
   }
@@ -573,7 +575,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   };
   auto place_of = [&](int t, int page_) {
     const int page = __builtin_amdgcn_readfirstlane(page_), at = t + TOK * wave;
-    const bool there = page >= 0 && page < cache.pages && t + tile_at < hi;
+    const bool there = page >= 0 && page < (int)cache.pages && t + tile_at < hi;
     Place p;
     p.head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
     p.size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
@@ -659,15 +661,28 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 #pragma unroll
     for (int k = 0; k < KS; ++k) w = mfma32<DT>(kx[k], qf[k], w);
   };
-  // masks them, and moves the running maximum where one exceeds it
-  auto limit = [&](int t, f32x2_t ks, f32x2_t lv, f32x16& w) {
-    if (t < lo_all || t + 32 > hi_all) {
+  auto mask = [&](int t, f32x16& w) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int token = t + 8 * (e >> 2) + 4 * h + (e & 3);
-        if (token < from || token >= to) w[e] = -__builtin_inff();
-      }
+    for (int e = 0; e < 16; ++e) {
+      const int token = t + 8 * (e >> 2) + 4 * h + (e & 3);
+      if (token < from || token >= to) w[e] = -__builtin_inff();
     }
+  };
+  // Their weights by the running maximum as it is: it only has to keep them from
+  // overflowing, so it moves where one would exceed 2^8 (seldom after the first steps) and
+  // no weight waits for this step's maximum.
+  auto weights = [&](f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float scale = ks[g], shift_v = lv[g] - base;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        p[g][e] = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e], scale, shift_v)),
+                            __builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
+    }
+  };
+  auto largest = [&](f32x2_t ks, f32x2_t lv, const f32x16& w) {
     // a 16-token tile's scale is positive, so its largest score is its largest dot product's
     float m = -__builtin_inff();
 #pragma unroll
@@ -677,37 +692,37 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       for (int e = 1; e < 8; ++e) x = fmaxf(x, w[8 * g + e]);
       m = fmaxf(m, fmaf(x, ks[g], lv[g]));
     }
-    const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    if (__ballot(m > top) != 0) {
-      m = fmaxf(m, top);
-      const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
-      sum *= keep;
-#pragma unroll
-      for (int j = 0; j < OT; ++j) o[j] *= keep;
-      top = m;
-    }
+    return m;
   };
-  auto weights = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2]) {
-    const float base = top == -__builtin_inff() ? 0.0f : top;
+  auto limit = [&](float m, f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+    if (__ballot(m > top + 8.0f) == 0) return;
+    const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+    const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
+    sum *= keep;
+#pragma unroll
+    for (int j = 0; j < OT; ++j) o[j] *= keep;
+    top = m;
+    weights(ks, lv, w, p);
+  };
+  auto add_sum = [&](f32x2_t iv, const u32x4 (&p)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const float scale = ks[g], shift_v = lv[g] - base;
       float part_sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t pair = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e], scale, shift_v)),
-                                        __builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
-        p[g][e] = pair;
+        const uint32_t pair = p[g][e];
         part_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, part_sum, false);
       }
       sum = fmaf(part_sum, iv[g], sum);
     }
   };
   u32x4 vx[2][OT];
-  auto read_values = [&](const char* buf, int i, int k) {
+  auto read_values = [&](const char* buf, int i) {
 #pragma unroll
-    for (int j = 0; j < OT; ++j) vx[k][j] = *(const u32x4*)(buf + KB + (32 * j + c) * VLD + 64 * i + 32 * k + 16 * h);
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < OT; ++j) vx[k][j] = *(const u32x4*)(buf + KB + (32 * j + c) * VLD + 64 * i + 32 * k + 16 * h);
   };
   auto add_values = [&](const u32x4 (&p)[2]) {
 #pragma unroll
@@ -716,24 +731,6 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       for (int j = 0; j < OT; ++j) o[j] = mfma32<KQ_DTYPE_F16>(vx[k][j], p[k], o[j]);
   };
   auto pair_at = [&](const char* buf, int which, int i) { return *(const f32x2_t*)(buf + KB + VB + 16 * which + 8 * i); };
-
-  // The order of a half step's instructions: the first values are read while scores are
-  // multiplied, an MFMA for every few of the weights' operations, then the other half.
-  auto pace = [] {
-    __builtin_amdgcn_sched_group_barrier(0x100, OT, 0);
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
-      __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
-      if (k >= KS / 2) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OT / KS, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < 2 * OT; ++k) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
-    }
-  };
 
   // Half steps of 32 tokens, each one's weights computed while the next one's scores are:
   // the matrix cores have work from the wave itself, not from the other one on its SIMD
@@ -754,21 +751,22 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     read_keys(smem, 0);
     dots(x);
     int which = 0;
-    for (int t = lo; t < hi; t += 64) {
+    auto step = [&](int t, auto masked) {
       const char* buf = smem + which * BUF;
       char* next = smem + (which ^ 1) * BUF;
       u32x4 p[2];
       {
         const f32x2_t ks = pair_at(buf, 0, 0), lv = pair_at(buf, 1, 0), iv = pair_at(buf, 2, 0);
         read_keys(buf, 1);
-        limit(t, ks, lv, x);
-        read_values(buf, 0, 0);
+        if constexpr (masked) mask(t, x);
         dots(y);
-        weights(ks, lv, iv, x, p);
-        read_values(buf, 0, 1);
+        weights(ks, lv, x, p);
+        const float m = largest(ks, lv, x);
+        read_values(buf, 0);
+        limit(m, ks, lv, x, p);
         add_values(p);
+        add_sum(iv, p);
         put_k(next);
-        pace();
         here = place_of(t + 128, next_page);
         fetch_k(here);
       }
@@ -776,20 +774,26 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       {
         const f32x2_t ks = pair_at(buf, 0, 1), lv = pair_at(buf, 1, 1), iv = pair_at(buf, 2, 1);
         read_keys(next, 0);
-        limit(t + 32, ks, lv, y);
-        read_values(buf, 1, 0);
+        if constexpr (masked) mask(t + 32, y);
         dots(x);
-        weights(ks, lv, iv, y, p);
-        read_values(buf, 1, 1);
+        weights(ks, lv, y, p);
+        const float m = largest(ks, lv, y);
+        read_values(buf, 1);
+        limit(m, ks, lv, y, p);
         add_values(p);
+        add_sum(iv, p);
         put_v(next);
-        pace();
         fetch_v(here);
         next_page = page_at(t + 192);
       }
       meet();
       which ^= 1;
-    }
+    };
+    // steps that every row of the tile sees whole need no mask: those between
+    int t = lo;
+    for (; t < hi && t < lo_all; t += 64) step(t, std::true_type{});
+    for (; t + 64 <= min(hi, hi_all); t += 64) step(t, std::false_type{});
+    for (; t < hi; t += 64) step(t, std::true_type{});
   }
   sum += __shfl_xor(sum, 32, 64);
 
