@@ -671,28 +671,37 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   // Their weights by the running maximum as it is: it only has to keep them from
   // overflowing, so it moves where one would exceed 2^8 (seldom after the first steps) and
   // no weight waits for this step's maximum.
+  auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, const f32x16& w) {
+    const int g = i >> 2;
+    return pack_act2(__builtin_amdgcn_exp2f(fmaf(w[2 * i], ks[g], shift_v[g])),
+                     __builtin_amdgcn_exp2f(fmaf(w[2 * i + 1], ks[g], shift_v[g])), KQ_DTYPE_F16);
+  };
   auto weights = [&](f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
     const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float scale = ks[g], shift_v = lv[g] - base;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        p[g][e] = pack_act2(__builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e], scale, shift_v)),
-                            __builtin_amdgcn_exp2f(fmaf(w[8 * g + 2 * e + 1], scale, shift_v)), KQ_DTYPE_F16);
-    }
+    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, f32x2_t{lv[0] - base, lv[1] - base}, w);
   };
-  auto largest = [&](f32x2_t ks, f32x2_t lv, const f32x16& w) {
-    // a 16-token tile's scale is positive, so its largest score is its largest dot product's
-    float m = -__builtin_inff();
+  // Scores of the next 32 tokens with the weights of these (and their largest exponent)
+  // between the products, an MFMA to every pair or two: the order is pinned.
+  auto dots_under_weights = [&](f32x16& next, f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    const f32x2_t shift_v = {lv[0] - base, lv[1] - base};
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      float x = w[8 * g];
+    for (int e = 0; e < 16; ++e) next[e] = 0.0f;
+    float x[2] = {-__builtin_inff(), -__builtin_inff()};
 #pragma unroll
-      for (int e = 1; e < 8; ++e) x = fmaxf(x, w[8 * g + e]);
-      m = fmaxf(m, fmaf(x, ks[g], lv[g]));
+    for (int k = 0; k < KS; ++k) {
+      next = mfma32<DT>(kx[k], qf[k], next);
+#pragma unroll
+      for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) {
+        p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, w);
+        x[i >> 2] = fmaxf(fmaxf(x[i >> 2], w[2 * i]), w[2 * i + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    return m;
+    asm volatile("" : "+v"(p[0]), "+v"(p[1]));  // (not behind the branch that may compute them anew)
+    // a 16-token tile's scale is positive, so its largest score is its largest dot product's
+    return fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
   };
   auto limit = [&](float m, f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
     if (__ballot(m > top + 8.0f) == 0) return;
@@ -759,9 +768,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         const f32x2_t ks = pair_at(buf, 0, 0), lv = pair_at(buf, 1, 0), iv = pair_at(buf, 2, 0);
         read_keys(buf, 1);
         if constexpr (masked) mask(t, x);
-        dots(y);
-        weights(ks, lv, x, p);
-        const float m = largest(ks, lv, x);
+        const float m = dots_under_weights(y, ks, lv, x, p);
         read_values(buf, 0);
         limit(m, ks, lv, x, p);
         add_values(p);
@@ -775,9 +782,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         const f32x2_t ks = pair_at(buf, 0, 1), lv = pair_at(buf, 1, 1), iv = pair_at(buf, 2, 1);
         read_keys(next, 0);
         if constexpr (masked) mask(t + 32, y);
-        dots(x);
-        weights(ks, lv, y, p);
-        const float m = largest(ks, lv, y);
+        const float m = dots_under_weights(x, ks, lv, y, p);
         read_values(buf, 1);
         limit(m, ks, lv, y, p);
         add_values(p);
