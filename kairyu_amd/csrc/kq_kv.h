@@ -60,13 +60,6 @@ KQ_DEV KvSeq kv_seq_uniform(const KvBatch& b, int s, int page_shift) {
   return q;
 }
 
-// The page that holds `slot` of sequence s (slot < table_width), or -1 where the
-// entry names none.
-KQ_DEV int kv_page(const KvBatch& b, const KvCache& c, int s, int slot) {
-  const int p = b.table[(int64_t)s * b.table_ld + slot];
-  return p >= 0 && p < c.pages ? p : -1;
-}
-
 // Sum over lanes 0..l, in registers (DPP row shifts, then the rows' last lanes
 // broadcast to the rows behind them).
 template <int CTRL, int ROWS>
@@ -82,49 +75,83 @@ KQ_DEV int wave_scan(int v) {
   return dpp_add<0x143, 0xc>(v);  // row_bcast:31
 }
 
-// The sequence that unit `u` falls to when sequence s has count(s) units, found by
-// a wave together (64 sequences at a time: one load and a scan, where a binary
-// search would wait for a load at each of its steps), and its index there; -1 past
-// the last unit.  Uniform.
-template <typename F>
-KQ_DEV int kv_find(int64_t u, int seqs, int& local, F count) {
-  int64_t base = 0;
-  for (int s0 = 0; s0 < seqs; s0 += 64) {
-    const int s = s0 + lane_id();
-    const int c = s < seqs ? count(s) : 0;
-    const int incl = wave_scan(c);
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (u < base + total) {
-      const int at = (int)__builtin_ctzll(__ballot(base + incl > u));
-      local = (int)(u - base) - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
-      return s0 + at;
-    }
-    base += total;
-  }
-  local = 0;
-  return -1;
-}
+// The sequences of a batch, one a lane: up to 64 are loaded once and then looked at in
+// registers; more are read again, 64 at a time.
+struct KvLanes {
+  const KvBatch& b;
+  int shift;
+  KvSeq mine;
+  bool held;
 
-// The sequence of `row` and, in `units`, sum of count(s) over those before it; -1
-// for padding.
-template <typename F>
-KQ_DEV int kv_of_row(int row, const KvBatch& b, int page_shift, int64_t& units, F count) {
-  units = 0;
-  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
-    const int s = s0 + lane_id();
-    const KvSeq q = kv_seq(b, min(s, b.seqs - 1), page_shift);
-    const int c = s < b.seqs ? count(s) : 0;
-    const int incl = wave_scan(c);
-    const uint64_t here = __ballot(s < b.seqs && row >= q.row0 && row < q.row0 + q.rows);
-    if (here != 0) {
-      const int at = (int)__builtin_ctzll(here);
-      units += __builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at);
-      return s0 + at;
-    }
-    units += __builtin_amdgcn_readlane(incl, 63);
+  KQ_DEV KvLanes(const KvBatch& batch, int page_shift) : b(batch), shift(page_shift), mine{}, held(batch.seqs <= 64) {
+    if (held && lane_id() < b.seqs) mine = kv_seq(b, lane_id(), shift);
   }
-  return -1;
-}
+  // sequence s0 + lane (no rows past the last)
+  KQ_DEV KvSeq at_lane(int s0) const {
+    if (held) return mine;
+    KvSeq q{};
+    if (s0 + lane_id() < b.seqs) q = kv_seq(b, s0 + lane_id(), shift);
+    return q;
+  }
+  // sequence s, in scalar registers
+  KQ_DEV KvSeq operator[](int s) const {
+    if (!held) return kv_seq_uniform(b, s, shift);
+    KvSeq q;
+    q.row0 = __builtin_amdgcn_readlane(mine.row0, s);
+    q.rows = __builtin_amdgcn_readlane(mine.rows, s);
+    q.first = __builtin_amdgcn_readlane(mine.first, s);
+    q.tokens = __builtin_amdgcn_readlane(mine.tokens, s);
+    return q;
+  }
+  // Units of all sequences, count(q) of each (0 for one without rows).
+  template <typename F>
+  KQ_DEV int total(F count) const {
+    int sum = 0;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) sum += __builtin_amdgcn_readlane(wave_scan(count(at_lane(s0))), 63);
+    return sum;
+  }
+  // The sequence that unit `u` falls to, found by the wave together (one load and a scan
+  // per 64 sequences, where a binary search would wait for a load at each of its steps),
+  // and its index there; -1 past the last unit.
+  template <typename F>
+  KQ_DEV int find(int u, int& local, F count) const {
+    int base = 0;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+      const int c = count(at_lane(s0));
+      const int incl = wave_scan(c);
+      const int all = __builtin_amdgcn_readlane(incl, 63);
+      if (u < base + all) {
+        const int at = (int)__builtin_ctzll(__ballot(base + incl > u));
+        local = u - base - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
+        return s0 + at;
+      }
+      base += all;
+    }
+    local = 0;
+    return -1;
+  }
+  // The sequence of `row` and, in `units`, the units of those before it; -1 for padding.
+  template <typename F>
+  KQ_DEV int of_row(int row, int& units, F count) const {
+    units = 0;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+      const KvSeq q = at_lane(s0);
+      const int c = count(q);
+      const int incl = wave_scan(c);
+      const uint64_t here = __ballot(row >= q.row0 && row < q.row0 + q.rows);
+      if (here != 0) {
+        const int at = (int)__builtin_ctzll(here);
+        units += __builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at);
+        return s0 + at;
+      }
+      units += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return -1;
+  }
+};
+
+// A value of the whole wave in a scalar register (quotients come out of the vector unit).
+KQ_DEV int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Host checks that append and attention share; set_error and a status on failure.
 int kv_check(const char* what, int dtype, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,

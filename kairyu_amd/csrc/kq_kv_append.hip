@@ -182,18 +182,18 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
 
   __shared__ uint32_t red[2][THREADS / 64];
   const int shift = cache.page_shift, page_size = 1 << shift;
-  const int head = (int)blockIdx.x % cache.kv_heads;
+  const KvLanes lanes(batch, shift);
+  const int unit = scalar((int)blockIdx.x / cache.kv_heads), head = (int)blockIdx.x - unit * cache.kv_heads;
   int nth;
-  const int s = kv_find((int)blockIdx.x / cache.kv_heads, batch.seqs, nth, [&](int i) {
-    const KvSeq q = kv_seq(batch, i, shift);
+  const int s = lanes.find(unit, nth, [&](const KvSeq& q) {
     const int lo = max(q.first, 0);
     return q.rows > 0 && lo < q.tokens ? ((q.tokens - 1) >> shift) - (lo >> shift) + 1 : 0;
   });
   if (s < 0) return;
-  const KvSeq q = kv_seq(batch, s, shift);
+  const KvSeq q = lanes[s];
   const int slot = (max(q.first, 0) >> shift) + nth;
-  const int page = kv_page(batch, cache, s, slot);
-  if (page < 0) return;
+  const int page = scalar(batch.table[(int64_t)s * batch.table_ld + slot]);
+  if (page < 0 || page >= cache.pages) return;
   const int lo = max(max(q.first, 0), slot << shift), hi = min(q.tokens, (slot + 1) << shift);  // positions stored here
   const int kept = lo & (page_size - 1);                                                        // earlier tokens
 

@@ -82,47 +82,41 @@ KQ_DEV float column_sum(float v) {
 // A sequence's rows (new tokens x the group's query heads) go to tiles of 16, and the
 // tokens that they see to blocks of 256.  The blocks of all tiles, one after the
 // other, are dealt to `shares` workgroups per kv head in equal runs, so that every
-// workgroup streams the same number of bytes whatever the lengths are (units cut per
-// sequence left a third of the chip idle at the end of a ragged batch: 64 contexts of
-// up to 6000 tokens, XX us).  A run covers whole tiles, written at once, and
-// at most two parts of tiles: the end of one begun before it (part 0) and the
-// beginning of one that goes on behind it (part 1).
+// workgroup streams the same number of bytes whatever the lengths are.  A run covers
+// whole tiles, written at once, and at most two parts of tiles: the end of one begun
+// before it (part 0) and the beginning of one that goes on behind it (part 1).
 struct Deal {
-  int64_t run;  // blocks of a workgroup
+  const AttendArgs& a;
+  int group;
 
   // 64-token step of the first token that any row sees
-  KQ_DEV static int first(const AttendArgs& a, const KvSeq& q) {
-    return a.window > 0 ? max(q.first + 1 - a.window, 0) >> 6 : 0;
-  }
+  KQ_DEV int first(const KvSeq& q) const { return a.window > 0 ? max(q.first + 1 - a.window, 0) >> 6 : 0; }
   // at least one, so that rows that see nothing are written as well
-  KQ_DEV static int blocks(const AttendArgs& a, const KvSeq& q) {
-    return (max(((q.tokens + 63) >> 6) - first(a, q), 1) + 3) >> 2;
-  }
-  KQ_DEV static int tiles(const AttendArgs& a, const KvSeq& q, int group) {
+  KQ_DEV int blocks(const KvSeq& q) const { return (max(((q.tokens + 63) >> 6) - first(q), 1) + 3) >> 2; }
+  KQ_DEV int tiles(const KvSeq& q) const {
     const int items = q.rows * group;
     return items <= a.few ? (items + 15) >> 4 : 0;
   }
-};
-KQ_DEV int big_tiles(const AttendArgs& a, const KvSeq& q, int group) {
-  const int items = q.rows * group;
-  return items > a.few ? (items + a.big_rows - 1) / a.big_rows : 0;
-}
-
-// The same run in every workgroup.
-KQ_DEV Deal deal_of(const AttendArgs& a, const KvBatch& b, int shift, int group) {
-  int64_t total = 0;
-  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
-    const int s = s0 + lane_id();
-    int v = 0;
-    if (s < b.seqs) {
-      const KvSeq q = kv_seq(b, s, shift);
-      v = Deal::tiles(a, q, group) * Deal::blocks(a, q);
-    }
-    total += __builtin_amdgcn_readlane(wave_scan(v), 63);
+  KQ_DEV int operator()(const KvSeq& q) const { return tiles(q) * blocks(q); }
+  // blocks of a workgroup: the same in every one
+  KQ_DEV int run(const KvLanes& lanes) const {
+    return scalar((int)(((uint32_t)lanes.total(*this) + (uint32_t)a.shares - 1) / (uint32_t)a.shares));
   }
-  Deal r;
-  r.run = (total + a.shares - 1) / a.shares;
-  return r;
+};
+struct BigTiles {
+  const AttendArgs& a;
+  int group;
+  KQ_DEV int operator()(const KvSeq& q) const {
+    const int items = q.rows * group;
+    return items > a.few ? (items + a.big_rows - 1) / a.big_rows : 0;
+  }
+};
+
+// What waves have put in LDS is there for all of them; loads from memory stay in flight.
+KQ_DEV void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Rows of no sequence are zero: those of one kv head, dealt to `of` workgroups.
@@ -137,14 +131,6 @@ KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, in
     for (int j = (int)threadIdx.x; j < words; j += threads) dst[j] = 0;
   }
 }
-
-// Keys and values of one step of 16 * NT tokens in registers, and their scales.
-template <int D, int NT, int PP>
-struct Step {
-  u32x4 k[NT][D / 64];
-  uint32_t v[NT * 4][D / 64];
-  float ks[PP], vs[PP];  // scale times log2 e; value scale (0: no tokens here)
-};
 
 // One workgroup: its run of blocks of one kv head, tile by tile; its four waves take
 // a tile's steps of 16 * NT tokens in turn.
@@ -161,7 +147,7 @@ struct Step {
 // sequence's last token: slots past it, pages that are none and steps past the run
 // read as zero without a branch.
 template <int D, int DT, int NT, int PP>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 3)
 kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
                       const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
   constexpr int KS = D / 32;   // MFMA steps along a key
@@ -170,107 +156,123 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   constexpr int ST = 16 * NT;  // tokens of a step
   constexpr int LD = D + 4;
   __shared__ __attribute__((aligned(16))) float lds[4 * 16 * LD];
-  const int lane = lane_id(), wave = wave_id(), c = lane & 15, b = lane >> 4;
-  const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
+  const int lane = lane_id(), wave = scalar(wave_id()), c = lane & 15, b = lane >> 4;
+  const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
   const int head = (int)blockIdx.y;
 
   zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 256);
-  const Deal deal = deal_of(a, batch, shift, group);
-  const int64_t run_end = ((int64_t)blockIdx.x + 1) * deal.run;
-  int64_t block = (int64_t)blockIdx.x * deal.run;
-  int within = 0;  // blocks of the sequence before `block`
-  int s = kv_find(block, batch.seqs, within, [&](int i) {
-    const KvSeq q = kv_seq(batch, i, shift);
-    return Deal::tiles(a, q, group) * Deal::blocks(a, q);
-  });
+  const KvLanes lanes(batch, shift);
+  const Deal deal{a, group};
+  const int run = deal.run(lanes), run_end = ((int)blockIdx.x + 1) * run;
+  int block = (int)blockIdx.x * run;
+  int within = 0;  // blocks of the sequence, then of the tile, before `block`
+  int s = lanes.find(block, within, deal);
   if (s < 0) return;
-  KvSeq q = kv_seq_uniform(batch, s, shift);
-  int blocks = Deal::blocks(a, q), tile = within / blocks;
+  KvSeq q = lanes[s];
+  int blocks = deal.blocks(q), tile = scalar(within / blocks);
   within -= tile * blocks;
   const int64_t tile_bytes = (int64_t)D << shift;
   const int in_page = (1 << shift) - 1;
   const int k_lane = c * D + 16 * b, v_lane = 4 * b * D + c * (D / 16);
 
-  while (true) {
-  const int item = tile * 16 + c;  // this lane's column: row item / group, head item % group
-  const bool real = item < q.rows * group;
-  const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
-  const int pos = q.first + row;
-  // tokens [from, to) of this column; [lo, hi) of the tile; [lo_all, hi_all) of every row
-  const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
-  const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-  const int row_lo = (tile * 16) / group, row_hi = min(q.rows - 1, (tile * 16 + 15) / group);
-  int hi = a.causal ? min(q.tokens, q.first + row_hi + 1) : q.tokens;
-  int lo = a.window > 0 ? max(q.first + row_lo + 1 - a.window, 0) : 0;
-  const int hi_all = a.causal ? min(q.tokens, q.first + row_lo + 1) : q.tokens;
-  const int lo_all = a.window > 0 ? max(q.first + row_hi + 1 - a.window, 0) : 0;
-  const int part_blocks = (int)min((int64_t)(blocks - within), run_end - block);
-  const int begin = Deal::first(a, q) * 64 + within * 256;
-  hi = min((int64_t)hi, (int64_t)begin + (int64_t)part_blocks * 256);
-  lo = max(lo & ~63, begin);
-
+  // One part of a tile: its bounds, its rows of Q, and its loads on their way.
+  int from, to, lo, hi, lo_all, hi_all, part_blocks;
+  const int32_t* pages;
   u32x4 qf[KS];
+  int id[PP];
+  u32x4 kx[NT][D / 64];     // a step's keys and values, and their pages' scales (0: no tokens there)
+  uint32_t vx[NT * 4][VD];
+  float ks[PP], vs[PP];
+  // pages of the step at t
+  auto pages_of = [&](int t) {
 #pragma unroll
-  for (int i = 0; i < KS; ++i) qf[i] = u32x4{0, 0, 0, 0};
-  if (real) {
-    const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1)) ^ a.q_sign;
-  }
-
-  const int32_t* pages = table + (int64_t)s * batch.table_ld;
-  // pages of the step at t (-1 past the tile's last token)
-  auto pages_of = [&](int t, int (&id)[PP]) {
+    for (int p = 0; p < PP; ++p) id[p] = pages[min(t + p * (ST / PP), max(hi - 1, 0)) >> shift];
+  };
+  int64_t head_tile[PP];
+  uint32_t size[PP];
+  auto place = [&](int t) {
 #pragma unroll
     for (int p = 0; p < PP; ++p) {
-      const int at = t + p * (ST / PP);
-      const int got = pages[min(at, max(hi - 1, 0)) >> shift];
-      id[p] = at < hi ? got : -1;
+      const int at = t + p * (ST / PP), page = scalar(id[p]);
+      const bool there = page >= 0 && page < (int)cache.pages && at < hi;
+      head_tile[p] = (int64_t)(there ? page : 0) * cache.kv_heads + head;
+      size[p] = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
     }
   };
-  auto load = [&](int t, const int (&id)[PP], Step<D, NT, PP>& x) {
+  auto load_keys = [&](int t) {
 #pragma unroll
     for (int p = 0; p < PP; ++p) {
-      const int at = t + p * (ST / PP);
-      const int page = __builtin_amdgcn_readfirstlane(id[p]);
-      const bool there = page >= 0 && page < cache.pages;
-      const int64_t head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
-      const int left = min(q.tokens - (at & ~in_page), in_page + 1);
-      const uint32_t size = there ? (uint32_t)(left * D) : 0u;
-      const i32x4 kr = make_rsrc(cache.k + head_tile * tile_bytes, size);
-      const i32x4 vr = make_rsrc(cache.v + head_tile * tile_bytes, size);
-      const int off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
+      const i32x4 src = make_rsrc(cache.k + head_tile[p] * tile_bytes, size[p]);
+      const int off = ((t + p * (ST / PP)) & in_page) * D;
 #pragma unroll
-      for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i) {
-        const int so = off + (i - p * (NT / PP)) * 16 * D;
+      for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
 #pragma unroll
         for (int h = 0; h < D / 64; ++h)
-          x.k[i][h] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(kr, k_lane + 64 * h, so, 0));
+          kx[i][h] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(src, k_lane + 64 * h, off + (i - p * (NT / PP)) * 16 * D, 0));
+      ks[p] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + head_tile[p], size[p] != 0 ? 4 : 0), 0, 0, 0));
+      vs[p] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + head_tile[p], size[p] != 0 ? 4 : 0), 0, 0, 0));
+    }
+  };
+  auto load_values = [&](int t) {
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      const i32x4 src = make_rsrc(cache.v + head_tile[p] * tile_bytes, size[p]);
+      const int off = ((t + p * (ST / PP)) & in_page) * D;
+#pragma unroll
+      for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          const int so = off + (i - p * (NT / PP)) * 16 * D;
           if constexpr (VD == 1) {
-            x.v[4 * i + r][0] = (uint32_t)kq_rbl_i32(vr, v_lane + r * D, so, 0);
+            vx[4 * i + r][0] = (uint32_t)kq_rbl_i32(src, v_lane + r * D, so, 0);
           } else if constexpr (VD == 2) {
-            const i32x2 w = kq_rbl_v2i32(vr, v_lane + r * D, so, 0);
-            x.v[4 * i + r][0] = (uint32_t)w[0];
-            x.v[4 * i + r][1] = (uint32_t)w[1];
+            const i32x2 w = kq_rbl_v2i32(src, v_lane + r * D, so, 0);
+            vx[4 * i + r][0] = (uint32_t)w[0];
+            vx[4 * i + r][1] = (uint32_t)w[1];
           } else {
-            const i32x4 w = kq_rbl_v4i32(vr, v_lane + r * D, so, 0);
+            const i32x4 w = kq_rbl_v4i32(src, v_lane + r * D, so, 0);
 #pragma unroll
-            for (int d = 0; d < VD; ++d) x.v[4 * i + r][d] = (uint32_t)w[d];
+            for (int d = 0; d < VD; ++d) vx[4 * i + r][d] = (uint32_t)w[d];
           }
         }
-      }
-      x.ks[p] = there ? k_scale[head_tile] * a.scale : 0.0f;
-      x.vs[p] = there ? v_scale[head_tile] : 0.0f;
     }
+  };
+  auto begin_part = [&] {
+    const int item = tile * 16 + c;  // this lane's column: row item / group, head item % group
+    const bool real = item < q.rows * group;
+    const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
+    const int pos = q.first + row;
+    // tokens [from, to) of this column; [lo, hi) of the part; [lo_all, hi_all) of every row
+    to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
+    from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
+    const int row_lo = scalar(tile * 16 / group), row_hi = min(q.rows - 1, scalar((tile * 16 + 15) / group));
+    hi = a.causal ? min(q.tokens, q.first + row_hi + 1) : q.tokens;
+    lo = a.window > 0 ? max(q.first + row_lo + 1 - a.window, 0) : 0;
+    hi_all = a.causal ? min(q.tokens, q.first + row_lo + 1) : q.tokens;
+    lo_all = a.window > 0 ? max(q.first + row_hi + 1 - a.window, 0) : 0;
+    part_blocks = min(blocks - within, run_end - block);
+    const int begin = deal.first(q) * 64 + within * 256;
+    hi = (int)min((int64_t)hi, (int64_t)begin + (int64_t)part_blocks * 256);
+    lo = max(lo & ~63, begin);
+    pages = table + (int64_t)s * batch.table_ld;
+    const int t = lo + ST * wave;
+    pages_of(t);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qf[i] = u32x4{0, 0, 0, 0};
+    if (real) {
+      const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1)) ^ a.q_sign;
+    }
+    place(t);
+    load_keys(t);
+    load_values(t);
+    pages_of(t + 4 * ST);
   };
 
   f32x4 o[OT];
-#pragma unroll
-  for (int j = 0; j < OT; ++j) o[j] = f32x4{0, 0, 0, 0};
-  float top = -__builtin_inff(), sum = 0.0f;
-  auto compute = [&](int t, const Step<D, NT, PP>& x) {
+  float top, sum;
+  auto step = [&](int t) {
     f32x4 w[NT];
     float m = -__builtin_inff();
 #pragma unroll
@@ -278,14 +280,25 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int h = 0; h < KS / 2; ++h) {
-        acc = mfma16<DT>(widen_codes<DT>(x.k[i][h][0], x.k[i][h][1]), qf[2 * h], acc);
-        acc = mfma16<DT>(widen_codes<DT>(x.k[i][h][2], x.k[i][h][3]), qf[2 * h + 1], acc);
+        acc = mfma16<DT>(widen_codes<DT>(kx[i][h][0], kx[i][h][1]), qf[2 * h], acc);
+        acc = mfma16<DT>(widen_codes<DT>(kx[i][h][2], kx[i][h][3]), qf[2 * h + 1], acc);
       }
-      const int p = i / (NT / PP);
-      const float shift_v = __builtin_amdgcn_logf(x.vs[p]);  // (-inf where there are no tokens)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) w[i][r] = fmaf(acc[r], x.ks[p], shift_v);
+      w[i] = acc;
     }
+    float inv_v[PP];
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      const float shift_v = __builtin_amdgcn_logf(vs[p]), scale = ks[p] * a.scale;  // (-inf where there are no tokens)
+      inv_v[p] = vs[p] > 0.0f ? __builtin_amdgcn_rcpf(vs[p]) : 0.0f;
+#pragma unroll
+      for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[i][r] = fmaf(w[i][r], scale, shift_v);
+    }
+    // the keys' registers take the next step's while this one goes on, the values' then theirs
+    place(t + 4 * ST);
+    load_keys(t + 4 * ST);
+    pages_of(t + 8 * ST);
     if (t < lo_all || t + ST > hi_all) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
@@ -314,8 +327,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) w[i][r] = __builtin_amdgcn_exp2f(w[i][r] - base);
-      const float vs = x.vs[i / (NT / PP)];
-      sum += (w[i][0] + w[i][1] + w[i][2] + w[i][3]) * (vs > 0.0f ? 1.0f / vs : 0.0f);
+      sum = fmaf(w[i][0] + w[i][1] + w[i][2] + w[i][3], inv_v[i / (NT / PP)], sum);
       p[i >> 1][2 * (i & 1)] = pack_act2(w[i][0], w[i][1], KQ_DTYPE_F16);
       p[i >> 1][2 * (i & 1) + 1] = pack_act2(w[i][2], w[i][3], KQ_DTYPE_F16);
     }
@@ -327,132 +339,138 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) in[e][r] = x.v[8 * g + 4 * e + r][d];
+          for (int r = 0; r < 4; ++r) in[e][r] = vx[8 * g + 4 * e + r][d];
           transpose4(in[e], out[e]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           o[4 * d + j] = mfma16<KQ_DTYPE_F16>(widen_codes<KQ_DTYPE_F16>(out[0][j], out[1][j]), p[g], o[4 * d + j]);
       }
+    load_values(t + 4 * ST);
   };
 
-  // one step in flight while another is computed, the pages of a third looked up
-  int t = lo + ST * wave;
-  if (t < hi) {
-    int id[PP];
-    Step<D, NT, PP> x, y;
-    pages_of(t, id);
-    load(t, id, x);
-    pages_of(t + 4 * ST, id);
-    while (true) {
-      load(t + 4 * ST, id, y);
-      pages_of(t + 8 * ST, id);
-      compute(t, x);
-      t += 4 * ST;
-      if (t >= hi) break;
-      load(t + 4 * ST, id, x);
-      pages_of(t + 8 * ST, id);
-      compute(t, y);
-      t += 4 * ST;
-      if (t >= hi) break;
-    }
-  }
-  sum = column_sum(sum);
+  begin_part();
+  while (true) {
+#pragma unroll
+    for (int j = 0; j < OT; ++j) o[j] = f32x4{0, 0, 0, 0};
+    top = -__builtin_inff();
+    sum = 0.0f;
+    for (int t = lo + ST * wave; t < hi; t += 4 * ST) step(t);
+    sum = column_sum(sum);
 
-  // the waves' parts meet in LDS, added in wave order
-  const bool whole = part_blocks == blocks;
-  __syncthreads();  // (the last tile's parts have been read)
-  float* mine = lds + (wave * 16 + c) * LD;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int j = 0; j < OT; j += 4)
-      *(f32x4*)(mine + (4 * b + r) * OT + j) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
-  if (b == 0) {
-    mine[D] = top;
-    mine[D + 1] = sum;
-  }
-  __syncthreads();
-  for (int i = (int)threadIdx.x; i < 16 * (D / 2); i += 256) {
-    const int col = i / (D / 2), d = 2 * (i - col * (D / 2));
-    const int it = tile * 16 + col;
-    if (it >= q.rows * group) break;
-    float m = -__builtin_inff();
-#pragma unroll
-    for (int v = 0; v < 4; ++v) m = fmaxf(m, lds[(v * 16 + col) * LD + D]);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    float x = 0.0f, y = 0.0f, l = 0.0f;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float* part = lds + (v * 16 + col) * LD;
-      const float f = __builtin_amdgcn_exp2f(part[D] - base);
-      x += part[d] * f;
-      y += part[d + 1] * f;
-      l += part[D + 1] * f;
+    // the next part's loads travel while this one's waves meet
+    const KvSeq old = q;
+    const int old_tile = tile, old_within = within;
+    const bool whole = part_blocks == blocks;
+    block += part_blocks;
+    within = 0;
+    bool more = block < run_end;
+    if (more && ++tile >= deal.tiles(q)) {
+      tile = 0;
+      do {
+        more = ++s < batch.seqs;
+        if (!more) break;
+        q = lanes[s];
+      } while (deal.tiles(q) == 0);
+      blocks = deal.blocks(q);
     }
-    if (!whole) {
-      float* dst = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (within == 0)) * 16 + col) * LD;
-      *(f32x2_t*)(dst + d) = f32x2_t{x, y};
-      if (d == 0) *(f32x2_t*)(dst + D) = f32x2_t{m, l};
-      continue;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees no token is zero)
-    const int rw = it / group;
-    uint32_t* dst = (uint32_t*)(a.out + ((int64_t)(q.row0 + rw) * a.heads + head * group + (it - rw * group)) * D + d);
-    *dst = pack_act2(x * inv, y * inv, DT);
-  }
+    if (more) begin_part();
 
-  block += part_blocks;
-  within = 0;
-  if (block >= run_end) return;
-  if (++tile >= Deal::tiles(a, q, group)) {
-    tile = 0;
-    do {
-      if (++s >= batch.seqs) return;
-      q = kv_seq_uniform(batch, s, shift);
-    } while (Deal::tiles(a, q, group) == 0);
-    blocks = Deal::blocks(a, q);
-  }
+    // the waves' parts meet in LDS, added in wave order
+    float* mine = lds + (wave * 16 + c) * LD;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < OT; j += 4)
+        *(f32x4*)(mine + (4 * b + r) * OT + j) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
+    if (b == 0) {
+      mine[D] = top;
+      mine[D + 1] = sum;
+    }
+    meet();
+    for (int i = (int)threadIdx.x; i < 16 * (D / 2); i += 256) {
+      const int col = i / (D / 2), d = 2 * (i - col * (D / 2));
+      const int it = old_tile * 16 + col;
+      if (it >= old.rows * group) break;
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int v = 0; v < 4; ++v) m = fmaxf(m, lds[(v * 16 + col) * LD + D]);
+      const float base = m == -__builtin_inff() ? 0.0f : m;
+      float ox = 0.0f, oy = 0.0f, l = 0.0f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float* part = lds + (v * 16 + col) * LD;
+        const float f = __builtin_amdgcn_exp2f(part[D] - base);
+        ox += part[d] * f;
+        oy += part[d + 1] * f;
+        l += part[D + 1] * f;
+      }
+      if (!whole) {
+        float* dst = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (old_within == 0)) * 16 + col) * LD;
+        *(f32x2_t*)(dst + d) = f32x2_t{ox, oy};
+        if (d == 0) *(f32x2_t*)(dst + D) = f32x2_t{m, l};
+        continue;
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees no token is zero)
+      const int rw = it / group;
+      uint32_t* dst = (uint32_t*)(a.out + ((int64_t)(old.row0 + rw) * a.heads + head * group + (it - rw * group)) * D + d);
+      *dst = pack_act2(ox * inv, oy * inv, DT);
+    }
+    if (!more) return;
+    meet();
   }
 }
 
-// The parts of split tiles joined in the order of their tokens: one wave per row and
-// query head.
+// The parts of split tiles joined in the order of their tokens, one wave per row and
+// query head: of every row, or of the 16-row tiles alone where no large tile is split.
 template <int D, int DT>
 __global__ void __launch_bounds__(256)
-kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch) {
+kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch, int small_tiles) {
   constexpr int LD = D + 4, PER = D / 64;
-  const int shift = cache.page_shift, group = a.heads / cache.kv_heads;
-  const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
-  if (at >= (int64_t)batch.rows * a.heads) return;
-  const int row = (int)(at / a.heads), qh = (int)(at - (int64_t)row * a.heads), head = qh / group;
-  int64_t before;  // large tiles, or blocks, of the sequences before the row's
-  int s = kv_of_row(row, batch, shift, before, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); });
-  if (s < 0) return;
-  const KvSeq q = kv_seq_uniform(batch, s, shift);
-  const int item = (row - q.row0) * group + (qh - head * group);
+  const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
+  const int at = (int)blockIdx.x * 4 + scalar(wave_id());
+  const KvLanes lanes(batch, shift);
+  const Deal deal{a, group};
+  int s, item, head, block = 0, above = 0;  // blocks, and large tiles, of the sequences before s
+  if (small_tiles > 0) {
+    const int column = scalar(at / cache.kv_heads);
+    head = at - column * cache.kv_heads;
+    int tile;
+    s = lanes.find(column >> 4, tile, [&](const KvSeq& q) { return deal.tiles(q); });
+    if (s < 0) return;
+    item = tile * 16 + (column & 15);
+    if (item >= lanes[s].rows * group) return;
+    lanes.of_row(lanes[s].row0, block, deal);
+  } else {
+    const int row = scalar(at / a.heads), qh = at - row * a.heads;
+    if (row >= batch.rows) return;
+    head = scalar(qh / group);
+    s = lanes.of_row(row, block, deal);
+    if (s < 0) return;
+    item = (row - lanes[s].row0) * group + (qh - head * group);
+    if (a.splits > 1) lanes.of_row(row, above, BigTiles{a, group});
+  }
+  const KvSeq q = lanes[s];
   const float* src;
   int chunks;
   const bool big = q.rows * group > a.few;
   if (big) {
     if (a.splits == 1) return;
     chunks = a.splits;
-    src = a.big_part + ((((int64_t)head * a.big_tiles + before + item / a.big_rows) * a.splits) * a.big_rows + item % a.big_rows) * LD;
+    const int tile = scalar(item / a.big_rows);
+    src = a.big_part + ((((int64_t)head * a.big_tiles + above + tile) * a.splits) * a.big_rows + item - tile * a.big_rows) * LD;
   } else {
-    const Deal deal = deal_of(a, batch, shift, group);
-    kv_of_row(row, batch, shift, before, [&](int i) {
-      const KvSeq q = kv_seq(batch, i, shift);
-      return Deal::tiles(a, q, group) * Deal::blocks(a, q);
-    });
-    const int blocks = Deal::blocks(a, q);
-    const int64_t block = before + (int64_t)(item >> 4) * blocks;
-    const int x0 = (int)(block / deal.run);
-    chunks = (int)((block + blocks - 1) / deal.run) - x0 + 1;
+    if (a.part == nullptr) return;  // (one block each)
+    const int run = deal.run(lanes), blocks = deal.blocks(q);
+    block += (item >> 4) * blocks;
+    const int x0 = scalar(block / run);
+    chunks = scalar((block + blocks - 1) / run) - x0 + 1;
     if (chunks == 1) return;  // written already
     // part 1 of the run it begins in, then part 0 of those behind
     src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
   }
   auto at_part = [&](int i) { return src + (big ? (int64_t)i * a.big_rows : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
+  const int row = q.row0 + scalar(item / group), qh = head * group + item % group;
   float m = -__builtin_inff();
   for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
   m = wave_max(m);
@@ -509,20 +527,17 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   const int wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int lane = lane_id(), c = lane & 31, h = lane >> 5, tid = (int)threadIdx.x;
-  // (quotients come out of the vector unit: values of the whole wave go back to scalar registers)
-  auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
   // kv heads side by side, so that (for up to 8 of them) an XCD's workgroups share
   // theirs through its L2; the tiles with the most tokens first
   const int rest = scalar((int)blockIdx.x / cache.kv_heads), head = (int)blockIdx.x - rest * cache.kv_heads;
   const int above = scalar(rest / a.splits), part = rest - above * a.splits, nth = a.big_tiles - 1 - above;
   if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 64 * WAVES);  // (no other kernel does)
-  int found;
-  const int s = scalar(
-      kv_find(nth, batch.seqs, found, [&](int i) { return big_tiles(a, kv_seq(batch, i, shift), group); }));
+  const KvLanes lanes(batch, shift);
+  int tile;
+  const int s = lanes.find(nth, tile, BigTiles{a, group});
   if (s < 0) return;
-  const int tile = scalar(found);
-  const KvSeq q = kv_seq_uniform(batch, s, shift);
+  const KvSeq q = lanes[s];
   const int item = tile * ROWS + wave * 32 + c;
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
@@ -635,13 +650,6 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       dst[4] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
   };
-  // LDS is complete for every wave; loads from memory stay in flight
-  auto meet = [] {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-
   f32x16 o[OT];
 #pragma unroll
   for (int j = 0; j < OT; ++j)
@@ -830,7 +838,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 }
 
 // Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
-constexpr int rows_slots(int64_t dim) { return 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1); }
+constexpr int rows_slots(int64_t dim) { return 256 * (dim == 256 ? 2 : 3); }
 
 // Waves of a large tile's workgroup: eight share what a step widens among twice the
 // rows, where their registers fit a CU together.
@@ -843,7 +851,7 @@ constexpr int kFewItems = 32;
 struct Plan {
   bool rows, tiles;  // which kernels run
   int few, shares, splits, big_rows;
-  int64_t big_tiles;
+  int64_t big_tiles, small_tiles;  // small_tiles: 16-row tiles that may need joining (0: look at every row)
   size_t part, big_part;  // bytes
 };
 
@@ -866,6 +874,7 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
     p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, (dim == 64 ? 768 : dim == 128 ? 256 : 256) / (p.big_tiles * kv_heads)));
   }
   p.splits = std::max(p.splits, 1);
+  if (p.tiles && p.splits == 1) p.small_tiles = std::min<int64_t>(rows * group, seqs * (kFewItems / 16));
   p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
   if (p.rows && tokens > 256) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
   if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * p.big_rows * (dim + 4));
@@ -894,9 +903,11 @@ static void launch(const AttendArgs& a, const Plan& p, const KvCache& c, const K
     hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT, tile_waves(D)>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)),
                        dim3(64 * tile_waves(D)), 0, st,
                        a, c, b, b.table, c.k_scale, c.v_scale);
-  if (a.part != nullptr || a.big_part != nullptr)
-    hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0, st, a,
-                       c, b);
+  if (a.part != nullptr || a.big_part != nullptr) {
+    const int64_t waves = p.small_tiles > 0 ? (int64_t)p.small_tiles * 16 * c.kv_heads : (int64_t)b.rows * a.heads;
+    hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, c, b,
+                       (int)p.small_tiles);
+  }
 }
 
 template <int D>
