@@ -31,6 +31,8 @@ from typing import NamedTuple
 
 import torch
 
+from kairyu_amd.kernels import kv_cache_hip as hip
+
 __all__ = ["PagedKvCache", "paged_attention", "rotary_table", "rotate_append"]
 
 E4M3 = torch.float8_e4m3fn
@@ -81,54 +83,65 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0,
 
 
 # ------------------------------------------------------------------ checks
-def _check_cache(cache: PagedKvCache) -> None:
+# (a decode step's call is bound by this host path: each property is read once)
+def _check_cache(cache: PagedKvCache) -> torch.Size:
     k, v, ks, vs = cache
-    if k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"cache keys {tuple(k.shape)} and values {tuple(v.shape)} must be alike, "
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
+        raise ValueError(f"cache keys {tuple(shape)} and values {tuple(v.shape)} must be alike, "
                          "[pages, kv_heads, page_size, head_dim]")
-    if k.dtype != E4M3 or v.dtype != E4M3:
+    if k.dtype is not E4M3 or v.dtype is not E4M3:
         raise ValueError(f"cache codes must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
-    if ks.shape != k.shape[:2] or vs.shape != k.shape[:2] or ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise ValueError(f"cache scales must be float32 {tuple(k.shape[:2])}")
-    if k.shape[3] not in HEAD_DIMS:
-        raise ValueError(f"head dim must be one of {HEAD_DIMS}, got {k.shape[3]}")
-    if k.shape[2] not in PAGE_SIZES:
-        raise ValueError(f"page size must be one of {PAGE_SIZES}, got {k.shape[2]}")
+    scales = shape[:2]
+    if ks.shape != scales or vs.shape != scales or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+        raise ValueError(f"cache scales must be float32 {tuple(scales)}")
+    if shape[3] not in HEAD_DIMS:
+        raise ValueError(f"head dim must be one of {HEAD_DIMS}, got {shape[3]}")
+    if shape[2] not in PAGE_SIZES:
+        raise ValueError(f"page size must be one of {PAGE_SIZES}, got {shape[2]}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache tensors must be contiguous")
-    if k.data_ptr() % 16 or v.data_ptr() % 16:
+    if (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("cache codes must be 16-byte aligned")
+    return shape
 
 
-def _check_batch(device: torch.device, cache: PagedKvCache, table, cu_rows, lengths) -> None:
-    if table.dim() != 2 or lengths.dim() != 1 or cu_rows.dim() != 1:
+def _check_batch(q: torch.Tensor, cache: PagedKvCache, cache_shape: torch.Size, table, cu_rows, lengths) -> torch.Size:
+    """The queries, the cache and the batch; the queries' shape."""
+
+    shape, device = q.shape, q.device
+    if len(shape) != 3 or shape[2] != cache_shape[3]:
+        raise ValueError(f"q must be [rows, heads, {cache_shape[3]}], got {tuple(shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if shape[1] < 1 or cache_shape[1] < 1 or shape[1] % cache_shape[1]:
+        raise ValueError(f"{shape[1]} query heads are not a multiple of {cache_shape[1]} kv heads")
+    table_shape, cu_shape, seqs = table.shape, cu_rows.shape, lengths.shape
+    if len(table_shape) != 2 or len(seqs) != 1 or len(cu_shape) != 1:
         raise ValueError("block_table must be [S, W], cu_rows [S + 1] and lengths [S]")
-    seqs = lengths.shape[0]
-    if table.shape[0] != seqs or cu_rows.shape[0] != seqs + 1:
-        raise ValueError(f"block_table {tuple(table.shape)} and cu_rows {tuple(cu_rows.shape)} do not match {seqs} lengths")
-    for t in (table, cu_rows, lengths):
-        if t.dtype != torch.int32:
-            raise ValueError(f"block_table, cu_rows and lengths must be int32, got {t.dtype}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError("block_table, cu_rows and lengths need unit stride in their last dimension")
-    if seqs > 1 and table.stride(0) < table.shape[1]:
-        raise ValueError("rows of block_table must not overlap")
-    for t in (*cache, table, cu_rows, lengths):
+    if table_shape[0] != seqs[0] or cu_shape[0] != seqs[0] + 1:
+        raise ValueError(f"block_table {tuple(table_shape)} and cu_rows {tuple(cu_shape)} do not match {seqs[0]} lengths")
+    if table.dtype is not torch.int32 or cu_rows.dtype is not torch.int32 or lengths.dtype is not torch.int32:
+        raise ValueError(f"block_table, cu_rows and lengths must be int32, got {table.dtype}, {cu_rows.dtype}, {lengths.dtype}")
+    if not (cu_rows.is_contiguous() and lengths.is_contiguous() and (table.is_contiguous() or _rows_apart(table))):
+        raise ValueError("cu_rows, lengths and the rows of block_table must be contiguous, and its rows not overlap")
+    for t in (cache[0], cache[1], cache[2], cache[3], table, cu_rows, lengths):
         if t.device != device:
             raise RuntimeError(f"cache and batch tensors must be on {device}; found {t.device}")
+    return shape
 
 
-def _check_heads(x: torch.Tensor, name: str, like: torch.Tensor, kv: bool, cache: PagedKvCache) -> None:
-    if x.dim() != 3 or x.shape[2] != cache.k.shape[3]:
-        raise ValueError(f"{name} must be [rows, heads, {cache.k.shape[3]}], got {tuple(x.shape)}")
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError(f"{name} must be float16 or bfloat16, got {x.dtype}")
-    if x.dtype != like.dtype or x.device != like.device or x.shape[0] != like.shape[0]:
-        raise ValueError(f"{name} must match the queries' rows, dtype and device")
-    if kv and x.shape[1] != cache.k.shape[1]:
-        raise ValueError(f"{name} has {x.shape[1]} heads, the cache {cache.k.shape[1]}")
-    if not kv and x.shape[1] % cache.k.shape[1]:
-        raise ValueError(f"{x.shape[1]} query heads are not a multiple of {cache.k.shape[1]} kv heads")
+def _rows_apart(table: torch.Tensor) -> bool:
+    (rows, width), (pitch, unit) = table.shape, table.stride()
+    return (unit == 1 or width <= 1) and (pitch >= width or rows <= 1)
+
+
+def _check_keys(x: torch.Tensor, name: str, q: torch.Tensor, q_shape: torch.Size, cache_shape: torch.Size) -> None:
+    if x.shape != (q_shape[0], cache_shape[1], q_shape[2]):
+        raise ValueError(f"{name} must be [{q_shape[0]}, {cache_shape[1]}, {q_shape[2]}] as the queries' rows and the "
+                         f"cache's heads, got {tuple(x.shape)}")
+    if x.dtype is not q.dtype or x.device != q.device:
+        raise ValueError(f"{name} must have the queries' dtype and device")
 
 
 def _refuse_grad(*tensors) -> None:
@@ -162,17 +175,17 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     Heads may be strided views (``q``, ``k`` and ``v`` of one packed projection);
     rows that are not 16-byte aligned are copied first."""
 
-    _check_cache(cache)
-    _check_heads(q, "q", q, False, cache)
-    _check_heads(k, "k", q, True, cache)
-    _check_heads(v, "v", q, True, cache)
-    _check_batch(q.device, cache, block_table, cu_rows, lengths)
-    dim = q.shape[2]
+    cache_shape = _check_cache(cache)
+    shape = _check_batch(q, cache, cache_shape, block_table, cu_rows, lengths)
+    _check_keys(k, "k", q, shape, cache_shape)
+    _check_keys(v, "v", q, shape, cache_shape)
+    dim = shape[2]
     if cos_sin is not None:
-        if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.device != q.device or not cos_sin.is_contiguous():
+        angles = cos_sin.shape
+        if len(angles) != 2 or cos_sin.dtype is not torch.float32 or cos_sin.device != q.device or not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be a contiguous float32 [positions, rotary] table on the queries' device")
-        if cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= dim:
-            raise ValueError(f"rotary width must be a multiple of 16 up to {dim}, got {cos_sin.shape[1]}")
+        if angles[1] % 16 or not 16 <= angles[1] <= dim:
+            raise ValueError(f"rotary width must be a multiple of 16 up to {dim}, got {angles[1]}")
         if cos_sin.data_ptr() % 16:
             raise ValueError("cos_sin must be 16-byte aligned")
     for norm in (q_norm, k_norm):
@@ -181,11 +194,10 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     _refuse_grad(q, k, v, q_norm, k_norm)
     if not q.is_cuda:
         return _rotate_append_plain(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps)
-    from kairyu_amd.kernels import kv_cache_hip as hip
-
     q_norm = None if q_norm is None else hip.aligned(q_norm)
     k_norm = None if k_norm is None else hip.aligned(k_norm)
-    return hip.rotate_append(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps)
+    return hip.rotate_append(q, k, v, shape, cache, cache_shape, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm,
+                             k_norm, eps)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Tensor, cu_rows: torch.Tensor,
@@ -197,18 +209,15 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Ten
     ``window`` of them if that is positive; otherwise every token of the sequence.
     Returns ``[R, Hq, D]``; a row that sees no token is zero."""
 
-    _check_cache(cache)
-    _check_heads(q, "q", q, False, cache)
-    _check_batch(q.device, cache, block_table, cu_rows, lengths)
+    cache_shape = _check_cache(cache)
+    shape = _check_batch(q, cache, cache_shape, block_table, cu_rows, lengths)
     if window < 0 or window > 1 << 30 or (window and not causal):
         raise ValueError(f"window must be 0, or a positive number of tokens of causal attention, got {window}")
     _refuse_grad(q)
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    scale = shape[2] ** -0.5 if scale is None else float(scale)
     if not q.is_cuda:
         return _paged_attention_plain(q, cache, block_table, cu_rows, lengths, scale, causal, window)
-    from kairyu_amd.kernels import kv_cache_hip as hip
-
-    return hip.attention(q, cache, block_table, cu_rows, lengths, scale, causal, window)
+    return hip.attention(q, shape, cache, cache_shape, block_table, cu_rows, lengths, scale, causal, window)
 
 
 # ------------------------------------------------------------- plain forms

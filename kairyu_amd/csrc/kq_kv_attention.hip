@@ -25,6 +25,7 @@ struct AttendArgs {
   uint32_t q_sign;  // the softmax scale's sign, for two 16-bit elements
   int heads, causal, window;
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
+  int block_shift;  // log2 of the 64-token steps of a block
   float* big_part;  // partial outputs of the large tiles, null: their tokens are not split
   int big_rows;     // rows of such a tile
   int few;          // rows * group up to which a sequence goes to tiles of 16 rows
@@ -80,7 +81,8 @@ KQ_DEV float column_sum(float v) {
 }
 
 // A sequence's rows (new tokens x the group's query heads) go to tiles of 16, and the
-// tokens that they see to blocks of 256.  The blocks of all tiles, one after the
+// tokens that they see to blocks (of 256, or of 1024 where no sequence can be longer: one
+// block a tile then, and nothing to join).  The blocks of all tiles, one after the
 // other, are dealt to `shares` workgroups per kv head in equal runs, so that every
 // workgroup streams the same number of bytes whatever the lengths are.  A run covers
 // whole tiles, written at once, and at most two parts of tiles: the end of one begun
@@ -92,7 +94,7 @@ struct Deal {
   // 64-token step of the first token that any row sees
   KQ_DEV int first(const KvSeq& q) const { return a.window > 0 ? max(q.first + 1 - a.window, 0) >> 6 : 0; }
   // at least one, so that rows that see nothing are written as well
-  KQ_DEV int blocks(const KvSeq& q) const { return (max(((q.tokens + 63) >> 6) - first(q), 1) + 3) >> 2; }
+  KQ_DEV int blocks(const KvSeq& q) const { return (max(((q.tokens + 63) >> 6) - first(q), 1) + (1 << a.block_shift) - 1) >> a.block_shift; }
   KQ_DEV int tiles(const KvSeq& q) const {
     const int items = q.rows * group;
     return items <= a.few ? (items + 15) >> 4 : 0;
@@ -253,8 +255,8 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     hi_all = a.causal ? min(q.tokens, q.first + row_lo + 1) : q.tokens;
     lo_all = a.window > 0 ? max(q.first + row_hi + 1 - a.window, 0) : 0;
     part_blocks = min(blocks - within, run_end - block);
-    const int begin = deal.first(q) * 64 + within * 256;
-    hi = (int)min((int64_t)hi, (int64_t)begin + (int64_t)part_blocks * 256);
+    const int begin = deal.first(q) * 64 + (within << (6 + a.block_shift));
+    hi = (int)min((int64_t)hi, (int64_t)begin + ((int64_t)part_blocks << (6 + a.block_shift)));
     lo = max(lo & ~63, begin);
     pages = table + (int64_t)s * batch.table_ld;
     const int t = lo + ST * wave;
@@ -852,7 +854,7 @@ constexpr int kFewItems = 32;
 
 struct Plan {
   bool rows, tiles;  // which kernels run
-  int few, shares, splits, big_rows;
+  int few, shares, splits, big_rows, block_shift;
   int64_t big_tiles, small_tiles;  // small_tiles: 16-row tiles that may need joining (0: look at every row)
   size_t part, big_part;  // bytes
 };
@@ -878,7 +880,9 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
   p.splits = std::max(p.splits, 1);
   if (p.tiles && p.splits == 1) p.small_tiles = std::min<int64_t>(rows * group, seqs * (kFewItems / 16));
   p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
-  if (p.rows && tokens > 256) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
+  // (a block more costs a wave about 1.5 us, the second launch and its host time 7)
+  p.block_shift = tokens <= 1024 ? 4 : 2;
+  if (p.rows && tokens > 1024) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
   if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * p.big_rows * (dim + 4));
   return p;
 }
@@ -977,7 +981,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.scale = fmaxf(fabsf(scale) * 1.44269504088896340736f, 0x1p-60f);
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
-  a.shares = p.shares, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.big_rows = p.big_rows, a.splits = p.splits;
+  a.shares = p.shares, a.block_shift = p.block_shift, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.big_rows = p.big_rows, a.splits = p.splits;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};

@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from kairyu_amd import _native
+from kairyu_amd.kernels import kv_cache_hip as hip
 
 __all__ = ["block_norm"]
 
@@ -39,67 +40,71 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
     quantizers lay them out: ``"fp8"`` / ``"int8"`` per row (scales ``[..., 1]``),
     ``"fp8_block"`` per 128 elements (scales ``[..., ceil(H / 128)]``)."""
 
-    if quantize not in MODES:
+    mode = MODES.get(quantize)
+    if mode is None:
         raise ValueError(f"quantize must be one of {tuple(MODES)}, got {quantize!r}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_HIDDEN:
-        raise ValueError(f"rows must have 1 to {MAX_HIDDEN} elements, got {tuple(x.shape)}")
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError(f"block_norm supports float16/bfloat16 rows, got {x.dtype}")
-    hidden = x.shape[-1]
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) < 1 or not 1 <= shape[-1] <= MAX_HIDDEN:
+        raise ValueError(f"rows must have 1 to {MAX_HIDDEN} elements, got {tuple(shape)}")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"block_norm supports float16/bfloat16 rows, got {dtype}")
+    hidden = shape[-1]
     for name, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
         if t is None:
             continue
-        if t.dtype != x.dtype or t.device != x.device:
+        if t.dtype is not dtype or t.device != device:
             raise ValueError(f"{name} must have the rows' dtype and device, got {t.dtype} on {t.device}")
-        if t.shape != (hidden,) and not (name == "gate" and t.shape == x.shape):
-            raise ValueError(f"{name} {tuple(t.shape)} does not match rows {tuple(x.shape)}")
+        if t.shape != (hidden,) and not (name == "gate" and t.shape == shape):
+            raise ValueError(f"{name} {tuple(t.shape)} does not match rows {tuple(shape)}")
+    r_dtype = dtype
     if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device:
+        r_dtype = residual.dtype
+        if residual.shape != shape or residual.device != device:
             raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match rows "
-                             f"{tuple(x.shape)} on {x.device}")
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"residual must be {x.dtype} or float32, got {residual.dtype}")
+                             f"{tuple(shape)} on {device}")
+        if r_dtype is not dtype and r_dtype is not torch.float32:
+            raise ValueError(f"residual must be {dtype} or float32, got {r_dtype}")
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
         raise RuntimeError("block_norm is for inference: an input requires a gradient")
     if not x.is_cuda:
         return _plain(x, residual, weight, post_weight, gate, residual_scale, eps, unit_offset, quantize)
-    from kairyu_amd.kernels import kv_cache_hip as hip
-
-    hip.require_device(x.device, "block_norm")
-    flat = _rows(x, hidden)
-    res = None if residual is None else _rows(residual, hidden)
-    per_row = gate is not None and (gate.dim() > 1 or x.dim() == 1)
-    gates = None if gate is None else _rows(gate, hidden) if per_row else gate.contiguous()
-    rows = flat.shape[0]
-    dtype = x.dtype if residual is None else residual.dtype
-    r = torch.empty(x.shape, device=x.device, dtype=dtype)
-    form = {None: x.dtype, "int8": torch.int8}.get(quantize, torch.float8_e4m3fn)
-    y = torch.empty(x.shape, device=x.device, dtype=form)
+    hip.require_device(device, "block_norm")
+    flat, pitch, rows = _rows(x, hidden)
+    res, res_pitch, _ = (None, 0, 0) if residual is None else _rows(residual, hidden)
+    gates, gate_pitch = gate, 0
+    if gate is not None:
+        if len(shape) == 1 or gate.dim() > 1:
+            gates, gate_pitch, _ = _rows(gate, hidden)
+        else:
+            gates = gate.contiguous()
+    r = torch.empty(shape, device=device, dtype=r_dtype)
+    y = torch.empty(shape, device=device, dtype=dtype if mode == 0 else torch.int8 if mode == 2 else torch.float8_e4m3fn)
     scales = None
-    if quantize is not None:
-        wide = -(-hidden // 128) if quantize == "fp8_block" else 1
-        scales = torch.empty((*x.shape[:-1], wide), device=x.device, dtype=torch.float32)
+    if mode:
+        scales = torch.empty((*shape[:-1], -(-hidden // 128) if mode == 3 else 1), device=device, dtype=torch.float32)
     weight = weight.contiguous()
     post_weight = None if post_weight is None else post_weight.contiguous()
     hip.call_on(
-        x.device, "kq_block_norm", flat.data_ptr(), _native.dtype_code(x.dtype), rows, hidden, flat.stride(0),
-        _native.ptr(res), _native.dtype_code(dtype), 0 if res is None else res.stride(0), _native.ptr(post_weight),
-        _native.ptr(gates), gates.stride(0) if per_row else 0, residual_scale, weight.data_ptr(),
-        1.0 if unit_offset else 0.0, eps, MODES[quantize], r.data_ptr(), y.data_ptr(), _native.ptr(scales),
+        device, "kq_block_norm", flat.data_ptr(), _native.dtype_code(dtype), rows, hidden, pitch, _native.ptr(res),
+        _native.dtype_code(r_dtype), res_pitch, _native.ptr(post_weight), _native.ptr(gates), gate_pitch, residual_scale,
+        weight.data_ptr(), 1.0 if unit_offset else 0.0, eps, mode, r.data_ptr(), y.data_ptr(), _native.ptr(scales),
     )
     return (r, y) if scales is None else (r, y, scales)
 
 
-def _rows(x: torch.Tensor, hidden: int) -> torch.Tensor:
-    """``[rows, hidden]`` with unit stride along the row and a pitch of at least its
-    width: a view where ``x`` has one, else a copy."""
+def _rows(x: torch.Tensor, hidden: int) -> tuple[torch.Tensor, int, int]:
+    """``x`` as rows of unit stride (a view where it has them, else a copy), the pitch
+    from one to the next, at least their width, and their number."""
 
+    if x.is_contiguous():
+        return x, hidden, x.numel() // hidden
     if x.dim() != 2:
         x = x.reshape(-1, hidden)
-    if x.stride(1) == 1 and (x.stride(0) >= hidden or x.shape[0] <= 1):
-        return x if x.stride(0) >= hidden else x.as_strided(x.shape, (hidden, 1))
-    return x.contiguous()
+    rows, (pitch, unit) = x.shape[0], x.stride()
+    if unit == 1 and pitch >= hidden:
+        return x, pitch, rows
+    return x.contiguous(), hidden, rows
 
 
 def _rms(x, weight, offset, eps):
