@@ -44,58 +44,91 @@ KQ_DEV void widen(u32x4 raw, int dtype, float v[8]) {
   }
 }
 
-// 8 elements [8c, 8c + 8) of one head's row, normed and rotated.  `row` points at
-// the row; D / 8 neighbouring lanes hold one row (all of them active), so the norm's
-// sum goes over lanes.  Half-split pairs lie rotary / 2 apart: the partner chunk is
-// read again (from L1) instead of exchanged, which keeps any rotary width.
+// What one thread holds of a head's row: two chunks of 8 elements whose rotation needs
+// no other thread's, i.e. chunks c and c + rotary / 16 of half-split pairs; what does not
+// rotate goes in neighbouring chunks.  D / 16 neighbouring lanes hold a row.
+struct Pairing {
+  int c0, c1;   // chunks
+  int angle;    // first of this thread's angles (half-split: 8 for both; interleaved: 4 each)
+  bool turned;
+};
+
 template <int D>
-KQ_DEV void turn(const uint16_t* row, int c, int pos, const AppendArgs& a, const uint16_t* norm, int dtype, float x[8]) {
-  widen(*(const u32x4*)(row + 8 * c), dtype, x);
+KQ_DEV Pairing pairing(int u, const AppendArgs& a) {
+  Pairing p;
+  const int turning = a.rotary >> 4;  // pairs of chunks that rotate
+  p.turned = u < turning;
+  if (p.turned && !a.interleaved) {
+    p.c0 = u;
+    p.c1 = u + turning;
+    p.angle = 8 * u;
+  } else {
+    p.c0 = 2 * u;
+    p.c1 = 2 * u + 1;
+    p.angle = 8 * u;
+  }
+  return p;
+}
+
+// cos and sin of the thread's 8 angles at a position; NaN past the table
+struct Angles {
+  float co[8], si[8];
+};
+KQ_DEV Angles angles_at(const Pairing& p, int pos, const AppendArgs& a) {
+  Angles g;
+  const bool there = pos < a.positions;
+  const float* at = a.cos_sin + (int64_t)(there ? pos : 0) * a.rotary + p.angle;
   const int half = a.rotary >> 1;
-  const bool turned = a.cos_sin != nullptr && 8 * c < a.rotary;
-  float y[8];
-  const int pc = 8 * c < half ? 8 * c + half : 8 * c - half;  // partner chunk's first element
-  const bool split = turned && !a.interleaved;
-  if (split) widen(*(const u32x4*)(row + pc), dtype, y);
-  if (norm != nullptr) {
-    float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
-#pragma unroll
-    for (int off = 1; off < D / 8; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
-    float w[8];
-    widen(*(const u32x4*)(norm + 8 * c), dtype, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-    if (split) {
-      widen(*(const u32x4*)(norm + pc), dtype, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * w[e];
-    }
-  }
-  if (!turned) return;
-  if (pos >= a.positions) {  // no angle for it
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
-    return;
-  }
-  const float* cs = a.cos_sin + (int64_t)pos * a.rotary;
-  if (a.interleaved) {
-    const f32x4 co = *(const f32x4*)(cs + 4 * c), si = *(const f32x4*)(cs + half + 4 * c);
+  for (int h = 0; h < 2; ++h) {
+    const f32x4 co = there ? *(const f32x4*)(at + 4 * h) : f32x4{0, 0, 0, 0};
+    const f32x4 si = there ? *(const f32x4*)(at + half + 4 * h) : f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float p = x[2 * e], r = x[2 * e + 1];
-      x[2 * e] = p * co[e] - r * si[e];
-      x[2 * e + 1] = r * co[e] + p * si[e];
+      g.co[4 * h + e] = there ? co[e] : __builtin_nanf("");
+      g.si[4 * h + e] = si[e];
     }
+  }
+  return g;
+}
+
+// Norm over the row's lanes (all of them active).
+template <int D>
+KQ_DEV void head_norm(const Pairing& p, const uint16_t* norm, float eps, int dtype, float x[2][8]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += x[0][e] * x[0][e];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += x[1][e] * x[1][e];
+#pragma unroll
+  for (int off = 1; off < D / 16; off <<= 1) sum += __shfl_xor(sum, off, 64);
+  const float inv = 1.0f / sqrtf(sum * (1.0f / D) + eps);
+  float w[8];
+  widen(*(const u32x4*)(norm + 8 * p.c0), dtype, w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[0][e] = x[0][e] * inv * w[e];
+  widen(*(const u32x4*)(norm + 8 * p.c1), dtype, w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[1][e] = x[1][e] * inv * w[e];
+}
+
+KQ_DEV void turn(const Pairing& p, const Angles& g, bool interleaved, float x[2][8]) {
+  if (!p.turned) return;
+  if (interleaved) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float co = g.co[4 * h + e], si = g.si[4 * h + e], y = x[h][2 * e], z = x[h][2 * e + 1];
+        x[h][2 * e] = y * co - z * si;
+        x[h][2 * e + 1] = z * co + y * si;
+      }
   } else {
-    const bool low = 8 * c < half;
-    const float* at = cs + (low ? 8 * c : 8 * c - half);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float co = at[e], si = at[half + e];
-      x[e] = low ? x[e] * co - y[e] * si : x[e] * co + y[e] * si;
+      const float y = x[0][e], z = x[1][e];
+      x[0][e] = y * g.co[e] - z * g.si[e];
+      x[1][e] = z * g.co[e] + y * g.si[e];
     }
   }
 }
@@ -143,46 +176,70 @@ KQ_DEV uint32_t move4(uint32_t w, float ratio) {
   return (pack4_e4m3(t[0], t[1], t[2], t[3]) & ~nan) | (w & nan);
 }
 
-// Workgroups [0, page_units) : one page of one sequence and one kv head each, its
-// new tokens in registers (NCH chunks of 8 elements a thread, keys and values).
-// The others: query rows, 2048 / D heads each.
-template <int D, int NCH, int THREADS>
+// Workgroups [0, page_units): one page of one sequence and one kv head each, its new
+// tokens in registers (NCH pairs of chunks a thread, keys and values).  The others:
+// query rows, HPT heads of one row a thread, which share their angles.
+template <int D, int NCH, int THREADS, int HPT>
 __global__ void __launch_bounds__(THREADS)
 kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
-  constexpr int CPR = D / 8;             // chunks (threads) of a head's row
-  constexpr int ROWS = THREADS / CPR;    // rows a workgroup holds at once
-  const int tid = (int)threadIdx.x, c = tid % CPR, rr = tid / CPR;
+  constexpr int TPR = D / 16;          // threads of a head's row
+  constexpr int ROWS = THREADS / TPR;  // rows a workgroup holds at once
+  const int tid = (int)threadIdx.x, rr = tid / TPR;
+  const Pairing p = pairing<D>(tid % TPR, a);
+  const int shift = cache.page_shift, page_size = 1 << shift;
+  const KvLanes lanes(batch, shift);
   if ((int)blockIdx.x >= a.page_units) {
+    const int per_row = (a.heads + HPT - 1) / HPT;  // threads (times TPR) of a query row
     const int64_t unit = (int64_t)(blockIdx.x - a.page_units) * ROWS + rr;
-    const int64_t row_ = unit / a.heads;
-    const int head = (int)(unit - row_ * a.heads);
+    const int64_t row_ = unit / per_row;
+    const int head0 = (int)(unit - row_ * per_row) * HPT;
     const int row = (int)(row_ < batch.rows ? row_ : batch.rows - 1);
-    // the sequence of the wave's first row, then a few steps from it
-    const int row0 = __builtin_amdgcn_readfirstlane(row);
-    int s = 0;
-    for (int s0 = 0; s0 < batch.seqs; s0 += 64) {
-      const bool past = s0 + lane_id() < batch.seqs && batch.cu[s0 + lane_id() + 1] <= row0;
-      s += (int)__popcll(__ballot(past));
+    // the sequence of the wave's first row, and from there for rows of another
+    int unused;
+    const int row0 = scalar(row);
+    const int s0 = lanes.of_row(row0, unused, [](const KvSeq&) { return 0; });
+    int pos = -1;  // (padding)
+    KvSeq q{};
+    if (s0 >= 0) q = lanes[s0];
+    if (__ballot(row < q.row0 || row >= q.row0 + q.rows) == 0) {
+      pos = q.first + row - q.row0;
+    } else {
+      for (int s = max(s0, 0); s < batch.seqs && batch.cu[s] <= row; ++s)
+        if (row < batch.cu[s + 1]) pos = batch.lengths[s] - (batch.cu[s + 1] - row);
     }
-    while (s < batch.seqs && batch.cu[s + 1] <= row) ++s;
-    const bool padding = s >= batch.seqs || row < batch.cu[s];
-    const int pos = padding ? -1 : batch.lengths[s] - (batch.cu[s + 1] - row);
-    float x[8];
-    turn<D>(a.q + (int64_t)row * a.q_ld + (int64_t)head * a.q_hs, c, max(pos, 0), a, a.q_norm, dtype, x);
-    if (row_ < batch.rows) {
-      u32x4 w = {0, 0, 0, 0};
-      if (pos >= 0) {
+    const uint16_t* src = a.q + (int64_t)row * a.q_ld;
+    u32x4 raw[HPT][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack_act2(x[2 * j], x[2 * j + 1], dtype);
+    for (int i = 0; i < HPT; ++i) {
+      const uint16_t* at = src + (int64_t)min(head0 + i, a.heads - 1) * a.q_hs;
+      raw[i][0] = *(const u32x4*)(at + 8 * p.c0);
+      raw[i][1] = *(const u32x4*)(at + 8 * p.c1);
+    }
+    Angles g;
+    if (p.turned) g = angles_at(p, max(pos, 0), a);
+#pragma unroll
+    for (int i = 0; i < HPT; ++i) {
+      float x[2][8];
+      widen(raw[i][0], dtype, x[0]);
+      widen(raw[i][1], dtype, x[1]);
+      if (a.q_norm != nullptr) head_norm<D>(p, a.q_norm, a.eps, dtype, x);
+      turn(p, g, a.interleaved, x);
+      if (row_ >= batch.rows || head0 + i >= a.heads) continue;
+      uint16_t* dst = a.q_out + ((int64_t)row * a.heads + head0 + i) * D;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 w = {0, 0, 0, 0};
+        if (pos >= 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = pack_act2(x[h][2 * j], x[h][2 * j + 1], dtype);
+        }
+        *(u32x4*)(dst + 8 * (h == 0 ? p.c0 : p.c1)) = w;
       }
-      *(u32x4*)(a.q_out + ((int64_t)row * a.heads + head) * D + 8 * c) = w;
     }
     return;
   }
 
   __shared__ uint32_t red[2][THREADS / 64];
-  const int shift = cache.page_shift, page_size = 1 << shift;
-  const KvLanes lanes(batch, shift);
   const int unit = scalar((int)blockIdx.x / cache.kv_heads), head = (int)blockIdx.x - unit * cache.kv_heads;
   int nth;
   const int s = lanes.find(unit, nth, [&](const KvSeq& q) {
@@ -197,7 +254,7 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
   const int lo = max(max(q.first, 0), slot << shift), hi = min(q.tokens, (slot + 1) << shift);  // positions stored here
   const int kept = lo & (page_size - 1);                                                        // earlier tokens
 
-  float k[NCH][8], v[NCH][8];
+  float k[NCH][2][8], v[NCH][2][8];
   uint32_t bad = 0;
   float ka = 0.0f, va = 0.0f;
 #pragma unroll
@@ -205,18 +262,28 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     const int pos = lo + i * ROWS + rr;
     if (pos >= hi) continue;  // (whole rows: a row's lanes stay together)
     const int64_t row = q.row0 + (pos - q.first);
-    turn<D>(a.k + row * a.k_ld + (int64_t)head * a.k_hs, c, pos, a, a.k_norm, dtype, k[i]);
-    widen(*(const u32x4*)(a.v + row * a.v_ld + (int64_t)head * a.v_hs + 8 * c), dtype, v[i]);
-    int ok = finite8(k[i]) && finite8(v[i]);
+    const uint16_t* ks = a.k + row * a.k_ld + (int64_t)head * a.k_hs;
+    const uint16_t* vs = a.v + row * a.v_ld + (int64_t)head * a.v_hs;
+    widen(*(const u32x4*)(ks + 8 * p.c0), dtype, k[i][0]);
+    widen(*(const u32x4*)(ks + 8 * p.c1), dtype, k[i][1]);
+    widen(*(const u32x4*)(vs + 8 * p.c0), dtype, v[i][0]);
+    widen(*(const u32x4*)(vs + 8 * p.c1), dtype, v[i][1]);
+    Angles g;
+    if (p.turned) g = angles_at(p, pos, a);
+    if (a.k_norm != nullptr) head_norm<D>(p, a.k_norm, a.eps, dtype, k[i]);
+    turn(p, g, a.interleaved, k[i]);
+    int ok = finite8(k[i][0]) && finite8(k[i][1]) && finite8(v[i][0]) && finite8(v[i][1]);
 #pragma unroll
-    for (int off = 1; off < CPR; off <<= 1) ok &= __shfl_xor(ok, off, 64);
+    for (int off = 1; off < TPR; off <<= 1) ok &= __shfl_xor(ok, off, 64);
     if (!ok) bad |= 1u << i;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (!(fabsf(v[i][e]) <= 3.402823466e38f)) v[i][e] = 0.0f;
-      if (ok) ka = fmaxf(ka, fabsf(k[i][e]));
-      va = fmaxf(va, fabsf(v[i][e]));
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!(fabsf(v[i][h][e]) <= 3.402823466e38f)) v[i][h][e] = 0.0f;
+        if (ok) ka = fmaxf(ka, fabsf(k[i][h][e]));
+        va = fmaxf(va, fabsf(v[i][h][e]));
+      }
   }
   const uint32_t kb = wave_max_u32_dpp(__float_as_uint(ka)), vb = wave_max_u32_dpp(__float_as_uint(va));
   if (lane_id() == 0) {
@@ -240,14 +307,14 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     __syncthreads();
     const float kn = fmaxf(ks, ko), vn = fmaxf(vs, vo);
     if (kn != ko)
-      for (int i = tid; i < kept * CPR; i += THREADS) {
+      for (int i = tid; i < kept * (D / 8); i += THREADS) {
         u32x2 w = *(const u32x2*)(kc + 8 * i);
         w[0] = move4(w[0], ko / kn);
         w[1] = move4(w[1], ko / kn);
         *(u32x2*)(kc + 8 * i) = w;
       }
     if (vn != vo)
-      for (int i = tid; i < kept * CPR; i += THREADS) {
+      for (int i = tid; i < kept * (D / 8); i += THREADS) {
         u32x2 w = *(const u32x2*)(vc + 8 * i);
         w[0] = move4(w[0], vo / vn);
         w[1] = move4(w[1], vo / vn);
@@ -265,9 +332,13 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
   for (int i = 0; i < NCH; ++i) {
     const int pos = lo + i * ROWS + rr;
     if (pos >= hi) continue;
-    const int at = (pos & (page_size - 1)) * D + 8 * c;
-    *(u32x2*)(kc + at) = (bad >> i) & 1 ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : encode8(k[i], ki);
-    *(u32x2*)(vc + at) = encode8(v[i], vi);
+    const int at = (pos & (page_size - 1)) * D;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 8 * (h == 0 ? p.c0 : p.c1);
+      *(u32x2*)(kc + at + c) = (bad >> i) & 1 ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : encode8(k[i][h], ki);
+      *(u32x2*)(vc + at + c) = encode8(v[i][h], vi);
+    }
   }
 }
 
@@ -301,29 +372,36 @@ int kv_check(const char* what, int dtype, int64_t rows, int64_t heads, int64_t k
   return KQ_OK;
 }
 
-template <int D, int NCH, int THREADS>
+template <int D, int NCH, int THREADS, int HPT>
 static void launch_append(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
-  const int rows = THREADS / (D / 8);
-  const int64_t query = ((int64_t)b.rows * a.heads + rows - 1) / rows;
-  hipLaunchKernelGGL((kv_append_kernel<D, NCH, THREADS>), dim3((unsigned)(a.page_units + query)), dim3(THREADS), 0, st, a, c, b,
+  const int rows = THREADS / (D / 16);
+  const int64_t query = ((int64_t)b.rows * ((a.heads + HPT - 1) / HPT) + rows - 1) / rows;
+  hipLaunchKernelGGL((kv_append_kernel<D, NCH, THREADS, HPT>), dim3((unsigned)(a.page_units + query)), dim3(THREADS), 0, st, a, c, b,
                      dtype);
 }
 
-// A page's tokens in registers: 256 threads hold 2048 elements a chunk; pages of 8
-// chunks and more go to 1024 threads instead of more registers.
-template <int D>
+// A page's tokens in registers: 256 threads hold 4096 elements a pair of chunks; pages
+// past 8192 elements go to 1024 threads instead of more registers.
+template <int D, int HPT>
 static void pick_append(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
-  const int chunks = (D << c.page_shift) / 2048;
-  if (chunks <= 1)
-    launch_append<D, 1, 256>(a, c, b, dtype, st);
-  else if (chunks == 2)
-    launch_append<D, 2, 256>(a, c, b, dtype, st);
-  else if (chunks <= 4)
-    launch_append<D, 4, 256>(a, c, b, dtype, st);
-  else if (chunks <= 8)
-    launch_append<D, 2, 1024>(a, c, b, dtype, st);
+  const int elements = D << c.page_shift;
+  if (elements <= 4096)
+    launch_append<D, 1, 256, HPT>(a, c, b, dtype, st);
+  else if (elements <= 8192)
+    launch_append<D, 2, 256, HPT>(a, c, b, dtype, st);
+  else if (elements <= 16384)
+    launch_append<D, 1, 1024, HPT>(a, c, b, dtype, st);
   else
-    launch_append<D, 4, 1024>(a, c, b, dtype, st);
+    launch_append<D, 2, 1024, HPT>(a, c, b, dtype, st);
+}
+
+// Four heads a thread once that still fills the chip; one where the rows are few.
+template <int D>
+static void pick_heads(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
+  if ((int64_t)b.rows * a.heads * D >= 4 * 256 * 4096)
+    pick_append<D, 4>(a, c, b, dtype, st);
+  else
+    pick_append<D, 1>(a, c, b, dtype, st);
 }
 
 }  // namespace kq
@@ -369,7 +447,7 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   while ((1 << shift) < page_size) ++shift;
   // a sequence of n rows touches at most 1 + ceil((n - 1) / page) pages, and a row at most one
   const int64_t units = seqs == 0 || pages == 0 ? 0 : std::min<int64_t>(rows, 2 * seqs + rows / page_size);
-  if ((units * kv_heads + rows * heads * dim / 2048 + 1) * 1024 >= (1LL << 32)) {  // threads of one launch
+  if ((units * kv_heads + rows * heads * dim / 4096 + 1) * 1024 >= (1LL << 32)) {  // threads of one launch
     set_error("%s: %lld rows of %lld heads are past the supported range", what, (long long)rows, (long long)heads);
     return KQ_EINVAL;
   }
@@ -378,10 +456,10 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   const KvBatch b{table, cu, lengths, table_ld, (int)seqs, (int)table_width, (int)rows};
   hipStream_t st = (hipStream_t)stream;
   if (dim == 64)
-    pick_append<64>(a, c, b, dtype, st);
+    pick_heads<64>(a, c, b, dtype, st);
   else if (dim == 128)
-    pick_append<128>(a, c, b, dtype, st);
+    pick_heads<128>(a, c, b, dtype, st);
   else
-    pick_append<256>(a, c, b, dtype, st);
+    pick_heads<256>(a, c, b, dtype, st);
   return check_launch(what);
 }
