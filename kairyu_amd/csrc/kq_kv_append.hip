@@ -159,22 +159,17 @@ KQ_DEV u32x2 encode8(const float v[8], float inv) {
   return w;
 }
 
-// Four codes of earlier tokens on a new scale: code * ratio, rounded again.
+// Four codes of earlier tokens on a coarser scale: code * ratio (below 1), rounded again;
+// NaN codes stay.
 KQ_DEV uint32_t move4(uint32_t w, float ratio) {
-  float t[4];
   uint32_t nan = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t b = (w >> (8 * e)) & 0xffu;
-    t[e] = e4m3_to_f32(b);
-    if ((b & 0x7fu) == 0x7fu) {
-      nan |= 0xffu << (8 * e);
-      t[e] = 0.0f;
-    }
-    t[e] = fminf(fmaxf(t[e] * ratio, -448.0f), 448.0f);
-  }
-  return (pack4_e4m3(t[0], t[1], t[2], t[3]) & ~nan) | (w & nan);
+  for (int e = 0; e < 4; ++e)
+    if ((w >> (8 * e) & 0x7fu) == 0x7fu) nan |= 0xffu << (8 * e);
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), true);
+  return (pack4_e4m3(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio) & ~nan) | (w & nan);
 }
+KQ_DEV u32x4 move16(u32x4 w, float ratio) { return u32x4{move4(w[0], ratio), move4(w[1], ratio), move4(w[2], ratio), move4(w[3], ratio)}; }
 
 // Workgroups [0, page_units): one page of one sequence and one kv head each, its new
 // tokens in registers (NCH pairs of chunks a thread, keys and values).  The others:
@@ -249,10 +244,25 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
   if (s < 0) return;
   const KvSeq q = lanes[s];
   const int slot = (max(q.first, 0) >> shift) + nth;
-  const int page = scalar(batch.table[(int64_t)s * batch.table_ld + slot]);
-  if (page < 0 || page >= cache.pages) return;
   const int lo = max(max(q.first, 0), slot << shift), hi = min(q.tokens, (slot + 1) << shift);  // positions stored here
   const int kept = lo & (page_size - 1);                                                        // earlier tokens
+
+  // the rows are on their way while the page is looked up and then its scales
+  u32x4 raw[NCH][4];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int64_t row = q.row0 + (min(lo + i * ROWS + rr, hi - 1) - q.first);
+    const uint16_t* ks = a.k + row * a.k_ld + (int64_t)head * a.k_hs;
+    const uint16_t* vs = a.v + row * a.v_ld + (int64_t)head * a.v_hs;
+    raw[i][0] = *(const u32x4*)(ks + 8 * p.c0);
+    raw[i][1] = *(const u32x4*)(ks + 8 * p.c1);
+    raw[i][2] = *(const u32x4*)(vs + 8 * p.c0);
+    raw[i][3] = *(const u32x4*)(vs + 8 * p.c1);
+  }
+  const int page = scalar(batch.table[(int64_t)s * batch.table_ld + slot]);
+  if (page < 0 || page >= cache.pages) return;
+  const int64_t tile = (int64_t)page * cache.kv_heads + head;
+  const float ko = cache.k_scale[tile], vo = cache.v_scale[tile];  // (needed where kept > 0)
 
   float k[NCH][2][8], v[NCH][2][8];
   uint32_t bad = 0;
@@ -261,13 +271,10 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
   for (int i = 0; i < NCH; ++i) {
     const int pos = lo + i * ROWS + rr;
     if (pos >= hi) continue;  // (whole rows: a row's lanes stay together)
-    const int64_t row = q.row0 + (pos - q.first);
-    const uint16_t* ks = a.k + row * a.k_ld + (int64_t)head * a.k_hs;
-    const uint16_t* vs = a.v + row * a.v_ld + (int64_t)head * a.v_hs;
-    widen(*(const u32x4*)(ks + 8 * p.c0), dtype, k[i][0]);
-    widen(*(const u32x4*)(ks + 8 * p.c1), dtype, k[i][1]);
-    widen(*(const u32x4*)(vs + 8 * p.c0), dtype, v[i][0]);
-    widen(*(const u32x4*)(vs + 8 * p.c1), dtype, v[i][1]);
+    widen(raw[i][0], dtype, k[i][0]);
+    widen(raw[i][1], dtype, k[i][1]);
+    widen(raw[i][2], dtype, v[i][0]);
+    widen(raw[i][3], dtype, v[i][1]);
     Angles g;
     if (p.turned) g = angles_at(p, pos, a);
     if (a.k_norm != nullptr) head_norm<D>(p, a.k_norm, a.eps, dtype, k[i]);
@@ -290,6 +297,7 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     red[0][wave_id()] = kb;
     red[1][wave_id()] = vb;
   }
+  asm volatile("" ::"v"(ko), "v"(vo));  // (every thread has read the scales before one writes them)
   __syncthreads();
   uint32_t kt = 0, vt = 0;
 #pragma unroll
@@ -297,29 +305,29 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     kt = max(kt, red[0][w]);
     vt = max(vt, red[1][w]);
   }
-  const int64_t tile = (int64_t)page * cache.kv_heads + head;
   uint8_t* kc = cache.k + (tile << shift) * D;
   uint8_t* vc = cache.v + (tile << shift) * D;
   float ks = kv_scale_for(__uint_as_float(kt)), vs = kv_scale_for(__uint_as_float(vt));
   if (kept > 0) {
-    const float ko = cache.k_scale[tile], vo = cache.v_scale[tile];
-    // (every thread has read the scales before one writes them)
-    __syncthreads();
     const float kn = fmaxf(ks, ko), vn = fmaxf(vs, vo);
-    if (kn != ko)
-      for (int i = tid; i < kept * (D / 8); i += THREADS) {
-        u32x2 w = *(const u32x2*)(kc + 8 * i);
-        w[0] = move4(w[0], ko / kn);
-        w[1] = move4(w[1], ko / kn);
-        *(u32x2*)(kc + 8 * i) = w;
+    const float kr = ko / kn, vr = vo / vn;
+    if (kr < 1.0f || vr < 1.0f) {  // keys and values together: their loads are in flight at once
+      const int n = kept * (D / 16);
+      for (int i = tid; i < n; i += 2 * THREADS) {
+        u32x4 w[4];
+        const int j = min(i + THREADS, n - 1);  // (past the end: the last chunk, not stored)
+        w[0] = *(const u32x4*)(kc + 16 * i);
+        w[1] = *(const u32x4*)(vc + 16 * i);
+        w[2] = *(const u32x4*)(kc + 16 * j);
+        w[3] = *(const u32x4*)(vc + 16 * j);
+        if (kr < 1.0f) *(u32x4*)(kc + 16 * i) = move16(w[0], kr);
+        if (vr < 1.0f) *(u32x4*)(vc + 16 * i) = move16(w[1], vr);
+        if (i + THREADS < n) {
+          if (kr < 1.0f) *(u32x4*)(kc + 16 * j) = move16(w[2], kr);
+          if (vr < 1.0f) *(u32x4*)(vc + 16 * j) = move16(w[3], vr);
+        }
       }
-    if (vn != vo)
-      for (int i = tid; i < kept * (D / 8); i += THREADS) {
-        u32x2 w = *(const u32x2*)(vc + 8 * i);
-        w[0] = move4(w[0], vo / vn);
-        w[1] = move4(w[1], vo / vn);
-        *(u32x2*)(vc + 8 * i) = w;
-      }
+    }
     ks = kn;
     vs = vn;
   }
