@@ -36,17 +36,22 @@ struct NormArgs {
   float eps, residual_scale, offset;
 };
 
-KQ_DEV void norm_load(const uint16_t* p, int64_t i, int64_t n, bool vec, int dtype, float v[8]) {
-  if (vec && i + 8 <= n) {
-    const u32x4 raw = *(const u32x4*)(p + i);
+// Elements [i, i + 8) of a 16-bit row, packed as they are; 0 past its end.
+KQ_DEV u32x4 norm_raw(const uint16_t* p, int64_t i, int64_t n, bool vec) {
+  if (vec && i + 8 <= n) return *(const u32x4*)(p + i);
+  uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = act_lo(raw[j], dtype);
-      v[2 * j + 1] = act_hi(raw[j], dtype);
-    }
-  } else {
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = i + 2 * j < n ? p[i + 2 * j] : 0u, hi = i + 2 * j + 1 < n ? p[i + 2 * j + 1] : 0u;
+    w[j] = lo | hi << 16;
+  }
+  return u32x4{w[0], w[1], w[2], w[3]};
+}
+KQ_DEV void norm_widen(u32x4 raw, int dtype, float v[8]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = i + j < n ? load_as_f32(p, dtype, i + j) : 0.0f;
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = act_lo(raw[j], dtype);
+    v[2 * j + 1] = act_hi(raw[j], dtype);
   }
 }
 
@@ -68,17 +73,30 @@ KQ_DEV void block_sum(float& sum, uint32_t& most, float* red, uint32_t* redm) {
   }
 }
 
-KQ_DEV uint32_t quant4_i8(const float v[4]) {
+// Four quantized elements y / s.  Finite rows take the correctly rounded quotient from
+// one reciprocal a row (div_by_recip: s is at least 1e-12 / 448) and the hardware's
+// conversions; rows that hold inf or NaN keep IEEE division and NaN codes.
+template <bool INT8>
+KQ_DEV uint32_t quant4(const float y[4], float s, float rs, bool fast) {
+  float t[4];
   uint32_t w = 0;
+  if (fast) {
+    constexpr float most = INT8 ? 127.0f : 448.0f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    w |= ((uint32_t)(int32_t)__builtin_rintf(clamp_keep_nan(v[e], 127.0f)) & 0xffu) << (8 * e);
-  return w;
-}
-KQ_DEV uint32_t quant4_fp8(const float v[4]) {
-  uint32_t w = 0;
+    for (int e = 0; e < 4; ++e) t[e] = fminf(fmaxf(div_by_recip(y[e], s, rs), -most), most);
+    if (!INT8) return pack4_e4m3(t[0], t[1], t[2], t[3]);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w |= f32_to_e4m3(clamp_keep_nan(v[e], 448.0f)) << (8 * e);
+    for (int e = 0; e < 4; ++e) w |= ((uint32_t)(int32_t)__builtin_rintf(t[e]) & 0xffu) << (8 * e);
+    return w;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float q = __fdiv_rn(y[e], s);
+    if (INT8)
+      w |= ((uint32_t)(int32_t)__builtin_rintf(clamp_keep_nan(q, 127.0f)) & 0xffu) << (8 * e);
+    else
+      w |= f32_to_e4m3(clamp_keep_nan(q, 448.0f)) << (8 * e);
+  }
   return w;
 }
 
@@ -92,17 +110,12 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
   float v[NCH][8], r[NCH][8];
   const uint16_t* x = a.x + row * a.x_ld;
   float sum = 0.0f;
+  // every operand is on its way before the first sum goes round
+  u32x4 xr[NCH], wr[NCH], pr[NCH], gr[NCH];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int64_t i = ((int64_t)tid + (int64_t)threads * c) * 8;
-    norm_load(x, i, n, vec, dtype, v[c]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[c][e] * v[c][e];
-  }
-  // (the residual is on its way while the first sum goes round)
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int64_t i = ((int64_t)tid + (int64_t)threads * c) * 8;
+    xr[c] = norm_raw(x, i, n, vec);
     if (a.residual == nullptr) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[c][e] = 0.0f;
@@ -120,8 +133,17 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
         for (int e = 0; e < 8; ++e) r[c][e] = i + e < n ? p[i + e] : 0.0f;
       }
     } else {
-      norm_load((const uint16_t*)a.residual + row * a.residual_ld, i, n, vec, dtype, r[c]);
+      norm_widen(norm_raw((const uint16_t*)a.residual + row * a.residual_ld, i, n, vec), dtype, r[c]);
     }
+    if (a.gate != nullptr) gr[c] = norm_raw(a.gate + row * a.gate_ld, i, n, vec);
+    if (a.post != nullptr) pr[c] = norm_raw(a.post, i, n, vec);
+    wr[c] = norm_raw(a.weight, i, n, vec);
+  }
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    norm_widen(xr[c], dtype, v[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[c][e] * v[c][e];
   }
   float inv = 1.0f;
   uint32_t none = 0;
@@ -137,18 +159,18 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
     if (i < n) {
       if (a.post != nullptr) {
         float w[8];
-        norm_load(a.post, i, n, vec, dtype, w);
+        norm_widen(pr[c], dtype, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * inv * (w[e] + a.offset);
       }
       if (a.gate != nullptr) {
         float g[8];
-        norm_load(a.gate + row * a.gate_ld, i, n, vec, dtype, g);
+        norm_widen(gr[c], dtype, g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[c][e] *= g[e];
       }
       float w[8];
-      norm_load(a.weight, i, n, vec, dtype, w);
+      norm_widen(wr[c], dtype, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float z = i + e < n ? r[c][e] + a.residual_scale * v[c][e] : 0.0f;
@@ -180,7 +202,9 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
   block_sum(sum2, most, red[1], redm[1]);
   inv = 1.0f / sqrtf(sum2 / (float)n + a.eps);
   float s = 0.0f;
+  bool fast = true;
   if (MODE == kNormFp8 || MODE == kNormInt8) {
+    fast = most < 0x7f800000u && inv <= 3.402823466e38f;
     s = __fdiv_rn(max_keep_nan(__uint_as_float(most) * inv, 1e-12f), MODE == kNormFp8 ? 448.0f : 127.0f);
     if (tid == 0) a.scales[row] = s;
   }
@@ -200,6 +224,7 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
       top = dpp_max_u32<0x141>(top);
       top = dpp_max_u32<0x140>(top);
       s = __fdiv_rn(max_keep_nan(__uint_as_float(top), 1e-12f), 448.0f);
+      fast = __ballot(top >= 0x7f800000u) == 0;
       if (i < n && (tid & 15) == 0) a.scales[row * ((n + 127) / 128) + i / 128] = s;
     } else {
 #pragma unroll
@@ -216,14 +241,10 @@ block_norm_kernel(NormArgs a, int dtype, int res_dtype, bool vec) {
       }
       continue;
     }
+    const float rs = __fdiv_rn(1.0f, s);
     uint32_t w[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float t[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = __fdiv_rn(y[4 * h + e], s);
-      w[h] = MODE == kNormInt8 ? quant4_i8(t) : quant4_fp8(t);
-    }
+    for (int h = 0; h < 2; ++h) w[h] = quant4<MODE == kNormInt8>(y + 4 * h, s, rs, fast);
     uint8_t* p = (uint8_t*)a.y_out + row * n;
     if (vec && i + 8 <= n) {
       *(u32x2*)(p + i) = u32x2{w[0], w[1]};
@@ -281,11 +302,11 @@ extern "C" int kq_block_norm(const void* x, int dtype, int64_t rows, int64_t hid
   const uintptr_t at = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)weight |
                        (uintptr_t)r_out | (uintptr_t)y_out;
   const bool vec = at % 16 == 0 && (x_ld | residual_ld | gate_ld | hidden) % 8 == 0;
-  // rows that fill the chip keep 256 threads each, so that several are in flight on a
-  // CU; fewer spread a row over up to 1024
+  // rows that fill the chip keep up to 512 threads each, so that several are in flight on
+  // a CU (4096 rows of 8192: 54.6 us, with 256 threads 58.5); fewer spread a row over 1024
   const int64_t chunks = (hidden + 7) / 8;
-  const int64_t wide = rows < 256 ? 1024 : 256;
-  const int nch = chunks <= wide ? 1 : chunks <= 2 * wide ? 2 : 4;
+  const int64_t wide = rows < 256 ? 1024 : 512;
+  const int nch = chunks <= wide ? 1 : chunks <= 2 * 1024 ? 2 : 4;
   const int64_t per = (chunks + nch - 1) / nch;
   const int threads = (int)std::min<int64_t>(1024, std::max<int64_t>(64, (per + 63) / 64 * 64));
   hipStream_t st = (hipStream_t)stream;
