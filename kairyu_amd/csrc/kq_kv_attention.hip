@@ -872,10 +872,14 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
     p.tiles = true;
     p.few = p.rows ? kFewItems : 0;
     p.big_rows = tile_waves(dim) * 32;
-    p.big_tiles = items / p.big_rows + std::min<int64_t>(seqs, items / (p.few + 1));
-    // few tiles: cut their tokens until two workgroups a CU have some
-    const int64_t most = std::max<int64_t>((tokens + 511) / 512, 1);
-    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, (dim == 64 ? 768 : dim == 128 ? 256 : 256) / (p.big_tiles * kv_heads)));
+    // (no sequence of more than `few` items ends more than one tile short)
+    const int64_t ends = std::min<int64_t>(seqs, items / (p.few + 1));
+    p.big_tiles = (items + ends * (p.big_rows - 1)) / p.big_rows;
+    // few tiles: cut their tokens until every workgroup slot has some, but not below 1024 each: a cut costs the
+    // second launch and the partial sums' way through memory (32 heads over 8 of 128 channels, one sequence: 512 rows
+    // behind 4096 tokens 130 us whole, 70 cut; 1024 rows behind 8192 on 4 heads 250 and 166; 1024 rows of 1024 42 and 52)
+    const int64_t most = std::max<int64_t>(tokens / 1024, 1), slots = dim == 64 ? 768 : 256;
+    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, slots / std::max<int64_t>(1, p.big_tiles * kv_heads)));
   }
   p.splits = std::max(p.splits, 1);
   if (p.tiles && p.splits == 1) p.small_tiles = std::min<int64_t>(rows * group, seqs * (kFewItems / 16));
