@@ -682,20 +682,24 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   };
   // Their weights by the running maximum as it is: it only has to keep them from
   // overflowing, so it moves where one would exceed 2^8 (seldom after the first steps) and
-  // no weight waits for this step's maximum.
-  auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, const f32x16& w) {
+  // no weight waits for this step's maximum.  l adds the denominator's share from the
+  // weights before their rounding to fp16, in fp32: a page of small values has a small
+  // value scale, and weights that are 0 in fp16 may be what the denominator consists of.
+  auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, f32x2_t iv, const f32x16& w, float& l) {
     const int g = i >> 2;
-    return pack_act2(__builtin_amdgcn_exp2f(fmaf(w[2 * i], ks[g], shift_v[g])),
-                     __builtin_amdgcn_exp2f(fmaf(w[2 * i + 1], ks[g], shift_v[g])), KQ_DTYPE_F16);
+    const float x = __builtin_amdgcn_exp2f(fmaf(w[2 * i], ks[g], shift_v[g]));
+    const float y = __builtin_amdgcn_exp2f(fmaf(w[2 * i + 1], ks[g], shift_v[g]));
+    l = i == 0 ? (x + y) * iv[g] : fmaf(x + y, iv[g], l);
+    return pack_act2(x, y, KQ_DTYPE_F16);
   };
-  auto weights = [&](f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+  auto weights = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
     const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, f32x2_t{lv[0] - base, lv[1] - base}, w);
+    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, f32x2_t{lv[0] - base, lv[1] - base}, iv, w, l);
   };
   // Scores of the next 32 tokens with the weights of these (and their largest exponent)
   // between the products, an MFMA to every pair or two: the order is pinned.
-  auto dots_under_weights = [&](f32x16& next, f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+  auto dots_under_weights = [&](f32x16& next, f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
     const float base = top == -__builtin_inff() ? 0.0f : top;
     const f32x2_t shift_v = {lv[0] - base, lv[1] - base};
 #pragma unroll
@@ -706,16 +710,16 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       next = mfma32<DT>(kx[k], qf[k], next);
 #pragma unroll
       for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) {
-        p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, w);
+        p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, w, l);
         x[i >> 2] = fmaxf(fmaxf(x[i >> 2], w[2 * i]), w[2 * i + 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("" : "+v"(p[0]), "+v"(p[1]));  // (not behind the branch that may compute them anew)
+    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));  // (not behind the branch that may compute them anew)
     // a 16-token tile's scale is positive, so its largest score is its largest dot product's
     return fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
   };
-  auto limit = [&](float m, f32x2_t ks, f32x2_t lv, const f32x16& w, u32x4 (&p)[2]) {
+  auto limit = [&](float m, f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
     if (__ballot(m > top + 8.0f) == 0) return;
     const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
@@ -724,19 +728,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 #pragma unroll
     for (int j = 0; j < OT; ++j) o[j] *= keep;
     top = m;
-    weights(ks, lv, w, p);
-  };
-  auto add_sum = [&](f32x2_t iv, const u32x4 (&p)[2]) {
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      float part_sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t pair = p[g][e];
-        part_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, part_sum, false);
-      }
-      sum = fmaf(part_sum, iv[g], sum);
-    }
+    weights(ks, lv, iv, w, p, l);
   };
   u32x4 vx[2][OT];
   auto read_values = [&](const char* buf, int i) {
@@ -776,15 +768,16 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       const char* buf = smem + which * BUF;
       char* next = smem + (which ^ 1) * BUF;
       u32x4 p[2];
+      float l;
       {
         const f32x2_t ks = pair_at(buf, 0, 0), lv = pair_at(buf, 1, 0), iv = pair_at(buf, 2, 0);
         read_keys(buf, 1);
         if constexpr (masked) mask(t, x);
-        const float m = dots_under_weights(y, ks, lv, x, p);
+        const float m = dots_under_weights(y, ks, lv, iv, x, p, l);
         read_values(buf, 0);
-        limit(m, ks, lv, x, p);
+        limit(m, ks, lv, iv, x, p, l);
         add_values(p);
-        add_sum(iv, p);
+        sum += l;
         put_k(next);
         here = place_of(t + 128, next_page);
         fetch_k(here);
@@ -794,11 +787,11 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         const f32x2_t ks = pair_at(buf, 0, 1), lv = pair_at(buf, 1, 1), iv = pair_at(buf, 2, 1);
         read_keys(next, 0);
         if constexpr (masked) mask(t + 32, y);
-        const float m = dots_under_weights(x, ks, lv, y, p);
+        const float m = dots_under_weights(x, ks, lv, iv, y, p, l);
         read_values(buf, 1);
-        limit(m, ks, lv, y, p);
+        limit(m, ks, lv, iv, y, p, l);
         add_values(p);
-        add_sum(iv, p);
+        sum += l;
         put_v(next);
         fetch_v(here);
         next_page = page_at(t + 192);

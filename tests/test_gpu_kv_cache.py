@@ -408,3 +408,20 @@ def test_no_pages_or_sequences(cuda):
     assert not paged_attention(q, pool, empty, bounds, seq).any()
     torch.cuda.synchronize()
     assert not pool.k.view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("heads", ["8 of 2, 64", "7 of 1, 128", "3 of 1, 256"])
+@pytest.mark.parametrize("new,total", [([1, 1], [200, 1300]), ([120, 200], [200, 900]), ([300], [4200])])
+def test_attention_over_pages_of_small_values(cuda, heads, new, total):
+    """Pages whose values are zero or far smaller than the others' count in the
+    denominator as much as any."""
+    banner(f"kv attention small values {heads} {new} {total}")
+    q, _, _, pool, table, cu, lengths = _case(cuda, (new, total), heads, 32, torch.bfloat16, seed=41)
+    g = kv.gen(42)
+    pick = torch.randint(0, 4, (pool.k.shape[0],), generator=g).to(cuda)
+    pool.v.view(torch.uint8)[pick == 0] = 0
+    pool.v_scale[pick == 0] = 2.0**-48
+    pool.v_scale[pick == 1] *= 2.0**-18
+    out = paged_attention(q * 0.25, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q * 0.25, pool, table, cu, lengths)
