@@ -215,6 +215,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Ten
         raise ValueError(f"window must be 0, or a positive number of tokens of causal attention, got {window}")
     _refuse_grad(q)
     scale = shape[2] ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= 2.0**100:
+        raise ValueError(f"scale must be finite and at most 2^100, got {scale}")
     if not q.is_cuda:
         return _paged_attention_plain(q, cache, block_table, cu_rows, lengths, scale, causal, window)
     return hip.attention(q, shape, cache, cache_shape, block_table, cu_rows, lengths, scale, causal, window)

@@ -41,7 +41,7 @@ KQ_DEV KvSeq kv_seq(const KvBatch& b, int s, int page_shift) {
   KvSeq q;
   // row bounds held within the tensor whatever cu says
   const int lo = min(max(b.cu[s], 0), b.rows), hi = min(max(b.cu[s + 1], lo), b.rows);
-  const int len = max(b.lengths[s], 0);
+  const int len = min(max(b.lengths[s], 0), 0x7fff0000);  // (positions a few steps on stay within 32 bits)
   q.row0 = lo;
   q.rows = hi - lo;
   q.first = len - q.rows;

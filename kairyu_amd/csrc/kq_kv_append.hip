@@ -199,8 +199,12 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     if (__ballot(row < q.row0 || row >= q.row0 + q.rows) == 0) {
       pos = q.first + row - q.row0;
     } else {
-      for (int s = max(s0, 0); s < batch.seqs && batch.cu[s] <= row; ++s)
-        if (row < batch.cu[s + 1]) pos = batch.lengths[s] - (batch.cu[s + 1] - row);
+      // (padding does not look through the sequences)
+      const int last = batch.seqs > 0 ? batch.cu[batch.seqs] : 0;
+      for (int s = max(s0, 0); row < last && s < batch.seqs && batch.cu[s] <= row; ++s) {
+        q = kv_seq(batch, s, shift);
+        if (row >= q.row0 && row < q.row0 + q.rows) pos = q.first + row - q.row0;
+      }
     }
     const uint16_t* src = a.q + (int64_t)row * a.q_ld;
     u32x4 raw[HPT][2];

@@ -24,6 +24,7 @@ struct AttendArgs {
   float scale;    // magnitude times log2 e, at least 2^-60: times a page's scale it stays positive
   uint32_t q_sign;  // the softmax scale's sign, for two 16-bit elements
   int heads, causal, window;
+  int most_blocks;  // no batch has more
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
   int block_shift;  // log2 of the 64-token steps of a block
   float* big_part;  // partial outputs of the large tiles, null: their tokens are not split
@@ -102,7 +103,9 @@ struct Deal {
   KQ_DEV int operator()(const KvSeq& q) const { return tiles(q) * blocks(q); }
   // blocks of a workgroup: the same in every one
   KQ_DEV int run(const KvLanes& lanes) const {
-    return scalar((int)(((uint32_t)lanes.total(*this) + (uint32_t)a.shares - 1) / (uint32_t)a.shares));
+    // (held to what a batch can have, whatever the row bounds say)
+    const uint32_t all = min((uint32_t)lanes.total(*this), (uint32_t)a.most_blocks);
+    return scalar((int)((all + (uint32_t)a.shares - 1) / (uint32_t)a.shares));
   }
 };
 struct BigTiles {
@@ -462,13 +465,15 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch, int small_tile
     if (a.splits == 1) return;
     chunks = a.splits;
     const int tile = scalar(item / a.big_rows);
+    if (above + tile >= a.big_tiles) return;  // (row bounds that go back: past the grid)
     src = a.big_part + ((((int64_t)head * a.big_tiles + above + tile) * a.splits) * a.big_rows + item - tile * a.big_rows) * LD;
   } else {
     if (a.part == nullptr) return;  // (one block each)
-    const int run = deal.run(lanes), blocks = deal.blocks(q);
+    const int run = max(deal.run(lanes), 1), blocks = deal.blocks(q);
     block += (item >> 4) * blocks;
-    const int x0 = scalar(block / run);
-    chunks = scalar((block + blocks - 1) / run) - x0 + 1;
+    // (within the shares also where row bounds that go back make counts wrap)
+    const int x0 = min(max(scalar(block / run), 0), a.shares - 1);
+    chunks = min(max(scalar((block + blocks - 1) / run), x0), a.shares - 1) - x0 + 1;
     if (chunks == 1) return;  // written already
     // part 1 of the run it begins in, then part 0 of those behind
     src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
@@ -941,6 +946,10 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   const char* what = "kq_kv_attention";
   int rc = kv_check(what, dtype, rows, heads, kv_heads, dim, page_size, pages, seqs, table_width, table_ld);
   if (rc) return rc;
+  if (!(fabsf(scale) <= 0x1p100f)) {
+    set_error("%s: scale %g", what, (double)scale);
+    return KQ_EINVAL;
+  }
   if (window < 0 || window > (1 << 30) || (window > 0 && !causal)) {
     set_error("%s: window %lld (a window is of causal attention)", what, (long long)window);
     return KQ_EINVAL;
@@ -963,8 +972,8 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
     return KQ_EWORKSPACE;
   }
   // threads of one launch, and blocks of all tiles
-  if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 512 >= (1LL << 32) ||
-      (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256) >= (1LL << 31)) {
+  const int64_t blocks = (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256);
+  if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 512 >= (1LL << 32) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
     return KQ_EINVAL;
@@ -978,6 +987,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.scale = fmaxf(fabsf(scale) * 1.44269504088896340736f, 0x1p-60f);
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
+  a.most_blocks = (int)blocks;
   a.shares = p.shares, a.block_shift = p.block_shift, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.big_rows = p.big_rows, a.splits = p.splits;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;

@@ -425,3 +425,81 @@ def test_attention_over_pages_of_small_values(cuda, heads, new, total):
     out = paged_attention(q * 0.25, pool, table, cu, lengths)
     torch.cuda.synchronize()
     kv.check_attention(out, q * 0.25, pool, table, cu, lengths)
+
+
+MANY = {  # more sequences than a wave has lanes
+    "decode": ([1] * 131, [1 + 37 * s % 211 for s in range(131)]),
+    "padded decode": ([1] * 70 + [0] * 60, [40 + s for s in range(70)] + [0] * 60),
+    "mixed": ([1, 40, 0, 3, 17] * 14, [90, 60, 33, 3, 200] * 14),
+}
+
+
+@pytest.mark.parametrize("heads", ["8 of 2, 64", "7 of 1, 128"])
+@pytest.mark.parametrize("batch", MANY)
+def test_many_sequences(cuda, batch, heads):
+    banner(f"kv many sequences {batch} {heads}")
+    q, k, v, pool, table, cu, lengths = _case(cuda, MANY[batch], heads, 16, torch.bfloat16, seed=43, pad=5)
+    before = kv.values(pool)
+    cos_sin = rotary_table(250, q.shape[2], device=cuda)
+    turned = rotate_append(q, k, v, pool, table, cu, lengths, cos_sin)
+    torch.cuda.synchronize()
+    kv.check_append(turned, pool, before, q, k, v, table.cpu(), cu.cpu(), lengths.cpu(), batch, cos_sin=cos_sin.cpu())
+    out = paged_attention(turned, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_attention(out, turned, pool, table, cu, lengths, batch)
+
+
+@pytest.mark.parametrize("slots", [64, 65])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 70]])
+def test_attention_around_one_block_of_tokens(cuda, slots, new):
+    """Tables of 1024 tokens, where no sequence's tokens are split, and one page more."""
+    banner(f"kv attention {slots} pages, new {new}")
+    q, _, _, pool, table, cu, lengths = _case(cuda, (new, [slots * 16, 1017, 100]), "8 of 2, 64", 16, torch.float16, seed=44)
+    assert table.shape[1] == slots
+    out = paged_attention(q, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths)
+
+
+@pytest.mark.parametrize("heads", ["8 of 2, 64", "4 of 4, 128", "3 of 1, 256"])
+@pytest.mark.parametrize("how", [dict(), dict(causal=False), dict(window=1500)], ids=str)
+def test_attention_of_few_rows_over_many_tokens(cuda, heads, how):
+    """Tiles whose tokens are cut into parts."""
+    banner(f"kv attention cut tokens {heads} {how}")
+    q, _, _, pool, table, cu, lengths = _case(cuda, ([90, 1], [5000, 4000]), heads, 64, torch.bfloat16, seed=45, pad=1)
+    out = paged_attention(q, pool, table, cu, lengths, **how)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths, **how)
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("how", [dict(), dict(window=40), dict(causal=False)], ids=str)
+@pytest.mark.parametrize("past", [30, 100_000, 2**31 - 1])
+def test_lengths_past_the_table(cuda, past, how, new):
+    """Only the tokens that the table has room for are there."""
+    banner(f"kv lengths past the table {past} {how} new {new}")
+    q, k, v, pool, table, cu, lengths = _case(cuda, ([new, new], [96, 60]), "8 of 2, 64", 16, torch.bfloat16, seed=46)
+    lengths[0] = min(96 + past, 2**31 - 1)
+    before = kv.values(pool)
+    turned = rotate_append(q, k, v, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_append(turned, pool, before, q, k, v, table.cpu(), cu.cpu(), lengths.cpu())
+    out = paged_attention(q, pool, table, cu, lengths, **how)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths, **how)
+
+
+def test_row_bounds_outside_the_rows(cuda):
+    """Rows before the first bound are padding, bounds past the rows end with them."""
+    banner("kv row bounds")
+    q, k, v, pool, table, _, lengths = _case(cuda, ([4, 1, 30], [40, 33, 70]), "8 of 2, 64", 32, torch.float16, seed=47)
+    cu = torch.tensor([2, 6, 7, 500], dtype=torch.int32, device=cuda)
+    within = cu.clamp(max=35)
+    before = kv.values(pool)
+    turned = rotate_append(q, k, v, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_append(turned, pool, before, q, k, v, table.cpu(), within.cpu(), lengths.cpu())
+    out = paged_attention(q, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, within, lengths)
+    assert not out[:2].any() and not turned[:2].any()

@@ -160,6 +160,18 @@ def test_attention_refuses(how):
         paged_attention(torch.zeros(rows, 2, 64, dtype=torch.bfloat16), kv.cache(pages, 2, 16, 64), table, cu, lengths, **how)
 
 
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e40])
+def test_attention_refuses_scales(scale):
+    from kairyu_amd import _native
+
+    table, cu, lengths, rows, pages = kv.batch([2], [20], 16)
+    with pytest.raises(ValueError, match="scale"):
+        paged_attention(torch.zeros(rows, 2, 64, dtype=torch.bfloat16), kv.cache(pages, 2, 16, 64), table, cu, lengths, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        _native.call("kq_kv_attention", None, 256, 64, 1, 1, 4, 2, 64, None, None, None, None, 1, 16, None, 1, 1, None, None, 1,
+                     scale, 1, 0, None, None, 0, None)
+
+
 def test_create():
     pool = PagedKvCache.create(5, 2, 64, 32, device="cpu")
     assert pool.k.shape == pool.v.shape == (5, 2, 32, 64) and pool.page_size == 32
