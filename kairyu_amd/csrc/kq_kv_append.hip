@@ -376,7 +376,7 @@ int kv_check(const char* what, int dtype, int64_t rows, int64_t heads, int64_t k
     return KQ_EINVAL;
   }
   // 32-bit row, page and unit counts inside the kernels
-  if (rows > (1 << 24) || heads > 1024 || pages > 0x7fffffffLL || seqs > (1 << 24) || table_width > (1 << 24) / page_size * 64) {
+  if (rows > (1 << 24) || heads > 1024 || pages * kv_heads >= (1LL << 29) || seqs > (1 << 24) || table_width > (1 << 24) / page_size * 64) {
     set_error("%s: rows=%lld, heads=%lld, pages=%lld, seqs=%lld or table width %lld past the supported range", what,
               (long long)rows, (long long)heads, (long long)pages, (long long)seqs, (long long)table_width);
     return KQ_EINVAL;

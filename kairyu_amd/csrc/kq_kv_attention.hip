@@ -186,44 +186,44 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
   int from, to, lo, hi, lo_all, hi_all, part_blocks;
   const int32_t* pages;
   u32x4 qf[KS];
-  int id[PP];
+  int id;                   // lane l: the page that holds the step's tokens from l % PP * (ST / PP) on
   u32x4 kx[NT][D / 64];     // a step's keys and values, and their pages' scales (0: no tokens there)
   uint32_t vx[NT * 4][VD];
-  float ks[PP], vs[PP];
+  float ks, vs;
   // pages of the step at t
-  auto pages_of = [&](int t) {
-#pragma unroll
-    for (int p = 0; p < PP; ++p) id[p] = pages[min(t + p * (ST / PP), max(hi - 1, 0)) >> shift];
-  };
-  int64_t head_tile[PP];
-  uint32_t size[PP];
+  const int nth_page = PP == 1 ? 0 : (lane & (PP - 1)) * (ST / PP);
+  auto pages_of = [&](int t) { id = pages[min(t + nth_page, max(hi - 1, 0)) >> shift]; };
+  int head_tile, size;
   auto place = [&](int t) {
-#pragma unroll
-    for (int p = 0; p < PP; ++p) {
-      const int at = t + p * (ST / PP), page = scalar(id[p]);
-      const bool there = page >= 0 && page < (int)cache.pages && at < hi;
-      head_tile[p] = (int64_t)(there ? page : 0) * cache.kv_heads + head;
-      size[p] = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
-    }
+    const int at = t + nth_page, page = PP == 1 ? scalar(id) : id;
+    const bool there = page >= 0 && page < (int)cache.pages && at < hi;
+    head_tile = (there ? page : 0) * cache.kv_heads + head;
+    size = there ? min(q.tokens - (at & ~in_page), in_page + 1) * D : 0;
+  };
+  auto of_page = [&](int v, int p) { return PP == 1 ? v : __builtin_amdgcn_readlane(v, p); };
+  auto scale_of = [&](const float* scales) {
+    if constexpr (PP == 1) return __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(scales + head_tile, size != 0 ? 4 : 0), 0, 0, 0));
+    const int end = (int)cache.pages * cache.kv_heads * 4;  // (an offset there reads 0)
+    return __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(scales, end), size != 0 ? 4 * head_tile : end, 0, 0));
   };
   auto load_keys = [&](int t) {
 #pragma unroll
     for (int p = 0; p < PP; ++p) {
-      const i32x4 src = make_rsrc(cache.k + head_tile[p] * tile_bytes, size[p]);
+      const i32x4 src = make_rsrc(cache.k + of_page(head_tile, p) * tile_bytes, of_page(size, p));
       const int off = ((t + p * (ST / PP)) & in_page) * D;
 #pragma unroll
       for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
 #pragma unroll
         for (int h = 0; h < D / 64; ++h)
           kx[i][h] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(src, k_lane + 64 * h, off + (i - p * (NT / PP)) * 16 * D, kAuxNT));
-      ks[p] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + head_tile[p], size[p] != 0 ? 4 : 0), 0, 0, 0));
-      vs[p] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + head_tile[p], size[p] != 0 ? 4 : 0), 0, 0, 0));
     }
+    ks = scale_of(k_scale);
+    vs = scale_of(v_scale);
   };
   auto load_values = [&](int t) {
 #pragma unroll
     for (int p = 0; p < PP; ++p) {
-      const i32x4 src = make_rsrc(cache.v + head_tile[p] * tile_bytes, size[p]);
+      const i32x4 src = make_rsrc(cache.v + of_page(head_tile, p) * tile_bytes, of_page(size, p));
       const int off = ((t + p * (ST / PP)) & in_page) * D;
 #pragma unroll
       for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
@@ -293,10 +293,13 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
       w[i] = acc;
     }
     float inv_v[PP];
+    const float lane_shift = __builtin_amdgcn_logf(vs), lane_scale = ks * a.scale;  // (-inf where there are no tokens)
+    const float lane_inv = vs > 0.0f ? __builtin_amdgcn_rcpf(vs) : 0.0f;
 #pragma unroll
     for (int p = 0; p < PP; ++p) {
-      const float shift_v = __builtin_amdgcn_logf(vs[p]), scale = ks[p] * a.scale;  // (-inf where there are no tokens)
-      inv_v[p] = vs[p] > 0.0f ? __builtin_amdgcn_rcpf(vs[p]) : 0.0f;
+      auto of = [&](float v) { return __uint_as_float((uint32_t)of_page((int)__float_as_uint(v), p)); };
+      const float shift_v = of(lane_shift), scale = of(lane_scale);
+      inv_v[p] = of(lane_inv);
 #pragma unroll
       for (int i = p * (NT / PP); i < (p + 1) * (NT / PP); ++i)
 #pragma unroll
