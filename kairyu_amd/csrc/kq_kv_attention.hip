@@ -82,12 +82,13 @@ KQ_DEV float column_sum(float v) {
 }
 
 // A sequence's rows (new tokens x the group's query heads) go to tiles of 16, and the
-// tokens that they see to blocks (of 256, or of 1024 where no sequence can be longer: one
-// block a tile then, and nothing to join).  The blocks of all tiles, one after the
-// other, are dealt to `shares` workgroups per kv head in equal runs, so that every
-// workgroup streams the same number of bytes whatever the lengths are.  A run covers
-// whole tiles, written at once, and at most two parts of tiles: the end of one begun
-// before it (part 0) and the beginning of one that goes on behind it (part 1).
+// tokens that they see to blocks (of 256; or so long that a tile is one block, and nothing
+// is to be joined, where no sequence can look at more than kWhole or kWholeMany tokens).
+// The blocks of all tiles, one after the other, are dealt to `shares` workgroups per kv
+// head in equal runs, so that every workgroup streams the same number of bytes whatever
+// the lengths are.  A run covers whole tiles, written at once, and at most two parts of
+// tiles: the end of one begun before it (part 0) and the beginning of one that goes on
+// behind it (part 1).
 struct Deal {
   const AttendArgs& a;
   int group;
@@ -853,6 +854,12 @@ constexpr int tile_waves(int64_t dim) { return dim == 128 ? 8 : 4; }
 // tokens once per tile
 constexpr int kFewItems = 32;
 
+constexpr int64_t kWhole = 1024;
+// ... and where a window makes the tiles alike and they fill the chip by themselves (64 single
+// tokens on 4 kv heads of 128, windows of 900, 1400 and 1900: 16.7, 21.5 and 25.7 us whole,
+// 25.4, 31.7 and 37.9 shared out; 4 on 8 kv heads, 1400: 17.1 and 13.4)
+constexpr int64_t kWholeMany = 2048;
+
 struct Plan {
   bool rows, tiles;  // which kernels run
   int few, shares, splits, big_rows, block_shift;
@@ -862,7 +869,7 @@ struct Plan {
 
 // From what the host knows: rows and sequences, not their lengths.
 static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
-                    int64_t seqs) {
+                    int64_t seqs, int64_t window) {
   Plan p{};
   const int64_t group = heads / kv_heads, items = rows * group, tokens = width * page_size;
   if (rows <= seqs || items <= kFewItems) {  // single tokens (no more rows than sequences)
@@ -885,9 +892,12 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
   p.splits = std::max(p.splits, 1);
   if (p.tiles && p.splits == 1) p.small_tiles = std::min<int64_t>(rows * group, seqs * (kFewItems / 16));
   p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
-  // (a block more costs a wave about 1.5 us, the second launch and its host time 7)
-  p.block_shift = tokens <= 1024 ? 4 : 2;
-  if (p.rows && tokens > 1024) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
+  // tokens that a sequence in 16-row tiles can look at, from its first step on
+  const int64_t most_rows = p.tiles ? std::max<int64_t>(kFewItems / group, 1) : rows;
+  const int64_t span = window > 0 ? std::min(tokens, window + most_rows + 64) : tokens;
+  const bool whole = span <= (window > 0 && seqs * kv_heads >= 256 ? kWholeMany : kWhole);
+  p.block_shift = !whole ? 2 : span > kWhole ? 5 : 4;
+  if (p.rows && !whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
   if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * p.big_rows * (dim + 4));
   return p;
 }
@@ -936,7 +946,7 @@ using namespace kq;
 extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                                  int64_t page_size, int64_t table_width, int64_t seqs) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
-  const Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs);
+  const Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs, 0);  // (a window needs no more)
   return p.part + p.big_part;
 }
 
@@ -964,7 +974,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   }
   if (rows == 0) return KQ_OK;
   const bool empty = seqs == 0 || pages == 0 || table_width == 0;  // every row is zero
-  Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs);
+  Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs, window);
   if (empty) {
     p = Plan{};
     p.rows = true;

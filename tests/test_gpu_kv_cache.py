@@ -503,3 +503,15 @@ def test_row_bounds_outside_the_rows(cuda):
     torch.cuda.synchronize()
     kv.check_attention(out, q, pool, table, within, lengths)
     assert not out[:2].any() and not turned[:2].any()
+
+
+@pytest.mark.parametrize("window", [900, 1024, 1700, 2100])
+@pytest.mark.parametrize("new", [[1] * 33, [2, 1, 60] * 11])
+def test_windows_of_many_sequences(cuda, new, window):
+    """Windows that one workgroup reads whole, and larger ones."""
+    banner(f"kv attention many windows {window} new {max(new)}")
+    total = [60 + 97 * s * s % 2600 for s in range(33)]
+    q, _, _, pool, table, cu, lengths = _case(cuda, (new, total), (8, 8, 64), 32, torch.float16, seed=48, pad=1)
+    out = paged_attention(q, pool, table, cu, lengths, window=window)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths, window=window)
