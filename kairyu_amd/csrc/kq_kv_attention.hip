@@ -118,6 +118,42 @@ struct BigTiles {
   }
 };
 
+// Large tiles by the tokens that they see, most first, so that the last workgroups to start
+// are the shortest.  Tile k of a sequence sees min(tokens, first + ((k + 1) * big_rows - 1) /
+// group + 1) of them (or all), which grows with k: how many of its tiles see at least 64 T
+// is a matter of a product and a shift.
+struct LongestFirst {
+  const AttendArgs& a;
+  const KvLanes& lanes;
+  int group, log_rows;
+
+  KQ_DEV int at_least(const KvSeq& q, int t) const {
+    const int tiles = BigTiles{a, group}(q);
+    if (t <= 0) return tiles;
+    if (tiles == 0 || q.tokens >> 6 < t) return 0;
+    const int row = 64 * t - 1 - q.first;  // the first that sees 64 t
+    if (!a.causal || row <= 0) return tiles;
+    return row < q.rows ? tiles - (row * group >> log_rows) : 0;
+  }
+  // The tile of a rank: its sequence (-1 past the last) and its index there.
+  KQ_DEV int find(int rank, int& tile) const {
+    if (rank >= lanes.total(BigTiles{a, group})) return -1;
+    int t = 0, end = (int)wave_max_u32_dpp((uint32_t)(lanes.at_lane(0).tokens >> 6)) + 1;
+    while (end - t > 1) {  // (at most 25 times)
+      const int mid = (t + end) >> 1;
+      if (lanes.total([&](const KvSeq& q) { return at_least(q, mid); }) > rank)
+        t = mid;
+      else
+        end = mid;
+    }
+    rank -= lanes.total([&](const KvSeq& q) { return at_least(q, t + 1); });
+    const int s = lanes.find(rank, tile, [&](const KvSeq& q) { return at_least(q, t) - at_least(q, t + 1); });
+    const KvSeq q = lanes[s];
+    tile += BigTiles{a, group}(q) - at_least(q, t);
+    return s;
+  }
+};
+
 // What waves have put in LDS is there for all of them; loads from memory stay in flight.
 KQ_DEV void meet() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -548,7 +584,9 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 64 * WAVES);  // (no other kernel does)
   const KvLanes lanes(batch, shift);
   int tile;
-  const int s = lanes.find(nth, tile, BigTiles{a, group});
+  const int s = a.splits == 1 && a.window == 0 && batch.seqs > 1 && lanes.held
+                    ? LongestFirst{a, lanes, group, ROWS == 256 ? 8 : 7}.find(above, tile)
+                    : lanes.find(nth, tile, BigTiles{a, group});
   if (s < 0) return;
   const KvSeq q = lanes[s];
   const int item = tile * ROWS + wave * 32 + c;
