@@ -28,11 +28,12 @@ struct AttendArgs {
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
   int block_shift;  // log2 of the 64-token steps of a block
   float* big_part;  // partial outputs of the large tiles, null: their tokens are not split
-  int big_rows;     // rows of such a tile
   int few;          // rows * group up to which a sequence goes to tiles of 16 rows
   int big_tiles;    // large tiles per kv head that the grid has room for
   int splits;       // parts that a large tile's tokens are cut into
 };
+
+constexpr int kBigRows = 128;  // rows of a large tile, 32 a wave
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
 template <int DT>
@@ -114,18 +115,18 @@ struct BigTiles {
   int group;
   KQ_DEV int operator()(const KvSeq& q) const {
     const int items = q.rows * group;
-    return items > a.few ? (items + a.big_rows - 1) / a.big_rows : 0;
+    return items > a.few ? (items + kBigRows - 1) / kBigRows : 0;
   }
 };
 
 // Large tiles by the tokens that they see, most first, so that the last workgroups to start
-// are the shortest.  Tile k of a sequence sees min(tokens, first + ((k + 1) * big_rows - 1) /
+// are the shortest.  Tile k of a sequence sees min(tokens, first + ((k + 1) * kBigRows - 1) /
 // group + 1) of them (or all), which grows with k: how many of its tiles see at least 64 T
 // is a matter of a product and a shift.
 struct LongestFirst {
   const AttendArgs& a;
   const KvLanes& lanes;
-  int group, log_rows;
+  int group;
 
   KQ_DEV int at_least(const KvSeq& q, int t) const {
     const int tiles = BigTiles{a, group}(q);
@@ -133,7 +134,7 @@ struct LongestFirst {
     if (tiles == 0 || q.tokens >> 6 < t) return 0;
     const int row = 64 * t - 1 - q.first;  // the first that sees 64 t
     if (!a.causal || row <= 0) return tiles;
-    return row < q.rows ? tiles - (row * group >> log_rows) : 0;
+    return row < q.rows ? tiles - row * group / kBigRows : 0;
   }
   // The tile of a rank: its sequence (-1 past the last) and its index there.
   KQ_DEV int find(int rank, int& tile) const {
@@ -504,9 +505,9 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch, int small_tile
   if (big) {
     if (a.splits == 1) return;
     chunks = a.splits;
-    const int tile = scalar(item / a.big_rows);
+    const int tile = item / kBigRows;
     if (above + tile >= a.big_tiles) return;  // (row bounds that go back: past the grid)
-    src = a.big_part + ((((int64_t)head * a.big_tiles + above + tile) * a.splits) * a.big_rows + item - tile * a.big_rows) * LD;
+    src = a.big_part + ((((int64_t)head * a.big_tiles + above + tile) * a.splits) * kBigRows + item - tile * kBigRows) * LD;
   } else {
     if (a.part == nullptr) return;  // (one block each)
     const int run = max(deal.run(lanes), 1), blocks = deal.blocks(q);
@@ -518,7 +519,7 @@ kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch, int small_tile
     // part 1 of the run it begins in, then part 0 of those behind
     src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * 16 + (item & 15)) * LD;
   }
-  auto at_part = [&](int i) { return src + (big ? (int64_t)i * a.big_rows : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
+  auto at_part = [&](int i) { return src + (big ? (int64_t)i * kBigRows : i == 0 ? 0 : (int64_t)(2 * i - 1) * 16) * LD; };
   const int row = q.row0 + scalar(item / group), qh = head * group + item % group;
   float m = -__builtin_inff();
   for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
@@ -551,7 +552,9 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // One workgroup: a tile of 32 rows a wave of one sequence and kv head, over the tokens
-// that it sees or one of `splits` parts of them, 64 at a step.
+// that it sees or one of `splits` parts of them, 64 at a step.  (With eight waves, which
+// share what a step widens, 8192 rows behind 12288 tokens took 1087 us and with four 1100,
+// but 1024 of 1024 42.7 and 31.6: fewer tiles fill the chip unevenly.)
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
 // are shared by the waves: they are widened once, keys to Q's type in rows of one
@@ -559,19 +562,17 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // lanes of S^T hold them (for each 16: 0-3, 8-11, then 4-7, 12-15), so that both are
 // read as 16-byte MFMA operands; rows are padded by 16 bytes, which spreads eight
 // lanes' reads over all banks.
-template <int D, int DT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2)
+template <int D, int DT>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
                        const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
   constexpr int KS = D / 16;            // MFMA steps along a key
   constexpr int OT = D / 32;            // output tiles
-  constexpr int ROWS = 32 * WAVES;
   constexpr int KLD = 2 * D + 16;       // bytes of a key's row
   constexpr int VLD = 2 * 64 + 16;      // bytes of a d's row of values
   constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale, its inverse)
-  constexpr int KC = D / WAVES / 16;    // 16-byte chunks of one token's key a thread moves
-  constexpr int VW = 4 * WAVES;         // threads that move four tokens' values
-  constexpr int VY = D / VW, VC = VY / 4;  // bytes and dwords of each token's a thread moves
+  constexpr int KC = D / 64;            // 16-byte chunks of one token's key a thread moves
+  constexpr int VY = D / 16, VC = VY / 4;  // bytes and dwords of each of four tokens' values a thread moves
   constexpr int LD = D + 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   const int wave = __builtin_amdgcn_readfirstlane(wave_id());
@@ -581,22 +582,23 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   // theirs through its L2; the tiles with the most tokens first
   const int rest = scalar((int)blockIdx.x / cache.kv_heads), head = (int)blockIdx.x - rest * cache.kv_heads;
   const int above = scalar(rest / a.splits), part = rest - above * a.splits, nth = a.big_tiles - 1 - above;
-  if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 64 * WAVES);  // (no other kernel does)
+  if (a.few == 0) zero_padding<D>(a, batch, head, group, rest, a.big_tiles * a.splits, 256);  // (no other kernel does)
   const KvLanes lanes(batch, shift);
   int tile;
   const int s = a.splits == 1 && a.window == 0 && batch.seqs > 1 && lanes.held
-                    ? LongestFirst{a, lanes, group, ROWS == 256 ? 8 : 7}.find(above, tile)
+                    ? LongestFirst{a, lanes, group}.find(above, tile)
                     : lanes.find(nth, tile, BigTiles{a, group});
   if (s < 0) return;
   const KvSeq q = lanes[s];
-  const int item = tile * ROWS + wave * 32 + c;
+  const int item = tile * kBigRows + wave * 32 + c;
   const bool real = item < q.rows * group;
   const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
   const int pos = q.first + row;
   // tokens [from, to) of this column, [lo_all, hi_all) of every row of the tile, [lo, hi) of any
   const int to = a.causal ? min(q.tokens, pos + 1) : q.tokens;
   const int from = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-  const int first_row = scalar(tile * ROWS / group), last_row = min(q.rows - 1, scalar((tile * ROWS + ROWS - 1) / group));
+  const int first_row = scalar(tile * kBigRows / group);
+  const int last_row = min(q.rows - 1, scalar((tile * kBigRows + kBigRows - 1) / group));
   int hi = a.causal ? max(min(q.tokens, q.first + last_row + 1), 0) : q.tokens;
   int lo = a.window > 0 ? max(q.first + first_row + 1 - a.window, 0) & ~63 : 0;
   const int hi_all = a.causal ? min(q.tokens, q.first + first_row + 1) : q.tokens;
@@ -616,19 +618,17 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h) ^ a.q_sign;
   }
 
-  // what this thread moves: D / WAVES bytes of one token's key, VY of four tokens' values;
-  // a wave moves part of one 16-token tile, which lies in one page.  Row R of the values
-  // is d = R % VW * VY + R / VW: any order of d does, and neighbouring lanes then write
+  // what this thread moves: D / 4 bytes of one token's key, D / 16 of four tokens' values;
+  // a wave moves one 16-token tile, which lies in one page.  Row R of the values is
+  // d = R % 16 * VY + R / 16: any order of d does, and neighbouring lanes then write
   // neighbouring rows.
-  constexpr int TOK = 64 / WAVES;  // tokens a wave moves
-  const int k_tok = tid / WAVES, v_grp = tid / VW, v_c = tid % VW;
-  const int k_lane = (k_tok % TOK) * D + (tid % WAVES) * (D / WAVES), v_lane = 4 * (v_grp % (TOK / 4)) * D + v_c * VY;
+  const int k_tok = tid / 4, v_grp = tid / 16, v_c = tid % 16;
+  const int k_lane = (k_tok % 16) * D + (tid % 4) * (D / 4), v_lane = 4 * (v_grp % 4) * D + v_c * VY;
   const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
   const int64_t tile_bytes = (int64_t)D << shift;
   const int in_page = (1 << shift) - 1;
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
-  const int tile_at = TOK * wave & ~15;  // (the waves that share a 16-token tile agree on its page)
-  auto page_at = [&](int t) { return pages[min(t + tile_at, max(hi - 1, 0)) >> shift]; };
+  auto page_at = [&](int t) { return pages[min(t + 16 * wave, max(hi - 1, 0)) >> shift]; };
   u32x4 kr[KC];
   uint32_t vr[4][VC];
   float sc_k = 0.0f, sc_v = 0.0f;
@@ -640,8 +640,8 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     int off;
   };
   auto place_of = [&](int t, int page_) {
-    const int page = __builtin_amdgcn_readfirstlane(page_), at = t + TOK * wave;
-    const bool there = page >= 0 && page < (int)cache.pages && t + tile_at < hi;
+    const int page = __builtin_amdgcn_readfirstlane(page_), at = t + 16 * wave;
+    const bool there = page >= 0 && page < (int)cache.pages && at < hi;
     Place p;
     p.head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
     p.size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
@@ -676,11 +676,11 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   auto put_k = [&](char* buf) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
-      char* dst = buf + k_tok * KLD + 2 * ((tid % WAVES) * (D / WAVES) + 16 * i);
+      char* dst = buf + k_tok * KLD + 2 * ((tid % 4) * (D / 4) + 16 * i);
       *(u32x4*)dst = widen_codes<DT>(kr[i][0], kr[i][1]);
       *(u32x4*)(dst + 16) = widen_codes<DT>(kr[i][2], kr[i][3]);
     }
-    if (lane == 0) ((float*)(buf + KB + VB))[wave * TOK / 16] = sc_k > 0.0f ? sc_k * a.scale : 1.0f;  // (waves of one tile write the same)
+    if (lane == 0) ((float*)(buf + KB + VB))[wave] = sc_k > 0.0f ? sc_k * a.scale : 1.0f;
   };
   auto put_v = [&](char* buf) {
 #pragma unroll
@@ -692,11 +692,11 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       for (int j = 0; j < 4; ++j) {
         const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, false)),
                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, true))};
-        *(u32x2*)(buf + KB + ((4 * i + j) * VW + v_c) * VLD + 2 * v_pos) = w;
+        *(u32x2*)(buf + KB + ((4 * i + j) * 16 + v_c) * VLD + 2 * v_pos) = w;
       }
     }
     if (lane == 0) {
-      float* dst = (float*)(buf + KB + VB) + 4 + wave * TOK / 16;
+      float* dst = (float*)(buf + KB + VB) + 4 + wave;
       dst[0] = __builtin_amdgcn_logf(sc_v);
       dst[4] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
@@ -855,23 +855,16 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   sum += __shfl_xor(sum, 32, 64);
 
   if (!real) return;
-  // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values.  Stores of
-  // neighbouring d: pairs of one tile where VW = 16, one element of every tile where VW = 32.
+  // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values, so that
+  // elements e and e + 8 are neighbouring d
   auto store = [&](auto put) {
 #pragma unroll
-    for (int e = 0; e < VW / 2; ++e) {
-      const int r = 8 * (e >> 2) + 4 * h + (e & 3);
-      if constexpr (VW == 16) {
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int j = 0; j < OT; ++j) put(r * VY + 2 * j, o[j][e], o[j][8 + e]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < OT; j += 2) put(r * VY + j, o[j][e], o[j + 1][e]);
-      }
-    }
+      for (int j = 0; j < OT; ++j) put((8 * (e >> 2) + 4 * h + (e & 3)) * VY + 2 * j, o[j][e], o[j][8 + e]);
   };
   if (a.splits > 1) {
-    float* dst = a.big_part + ((((int64_t)head * a.big_tiles + nth) * a.splits + part) * ROWS + wave * 32 + c) * LD;
+    float* dst = a.big_part + ((((int64_t)head * a.big_tiles + nth) * a.splits + part) * kBigRows + wave * 32 + c) * LD;
     store([&](int d, float x, float y) { *(f32x2_t*)(dst + d) = f32x2_t{x, y}; });
     if (h == 0) *(f32x2_t*)(dst + D) = f32x2_t{top, sum};
     return;
@@ -883,10 +876,6 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 
 // Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
 constexpr int rows_slots(int64_t dim) { return 256 * (dim == 256 ? 2 : 3); }
-
-// Waves of a large tile's workgroup: eight share what a step widens among twice the
-// rows, where their registers fit a CU together.
-constexpr int tile_waves(int64_t dim) { return dim == 128 ? 8 : 4; }
 
 // rows * group up to which a sequence goes to tiles of 16 rows, which stream its
 // tokens once per tile
@@ -900,7 +889,7 @@ constexpr int64_t kWholeMany = 2048;
 
 struct Plan {
   bool rows, tiles;  // which kernels run
-  int few, shares, splits, big_rows, block_shift;
+  int few, shares, splits, block_shift;
   int64_t big_tiles, small_tiles;  // small_tiles: 16-row tiles that may need joining (0: look at every row)
   size_t part, big_part;  // bytes
 };
@@ -917,14 +906,13 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
     p.rows = seqs > 1;
     p.tiles = true;
     p.few = p.rows ? kFewItems : 0;
-    p.big_rows = tile_waves(dim) * 32;
     // (no sequence of more than `few` items ends more than one tile short)
     const int64_t ends = std::min<int64_t>(seqs, items / (p.few + 1));
-    p.big_tiles = (items + ends * (p.big_rows - 1)) / p.big_rows;
+    p.big_tiles = (items + ends * (kBigRows - 1)) / kBigRows;
     // few tiles: cut their tokens until every workgroup slot has some, but not below 1024 each: a cut costs the
     // second launch and the partial sums' way through memory (32 heads over 8 of 128 channels, one sequence: 512 rows
     // behind 4096 tokens 130 us whole, 70 cut; 1024 rows behind 8192 on 4 heads 250 and 166; 1024 rows of 1024 42 and 52)
-    const int64_t most = std::max<int64_t>(tokens / 1024, 1), slots = dim == 64 ? 768 : 256;
+    const int64_t most = std::max<int64_t>(tokens / 1024, 1), slots = 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1);
     p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, slots / std::max<int64_t>(1, p.big_tiles * kv_heads)));
   }
   p.splits = std::max(p.splits, 1);
@@ -936,7 +924,7 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
   const bool whole = span <= (window > 0 && seqs * kv_heads >= 256 ? kWholeMany : kWhole);
   p.block_shift = !whole ? 2 : span > kWhole ? 5 : 4;
   if (p.rows && !whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
-  if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * p.big_rows * (dim + 4));
+  if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * kBigRows * (dim + 4));
   return p;
 }
 
@@ -959,9 +947,8 @@ static void launch(const AttendArgs& a, const Plan& p, const KvCache& c, const K
       launch_rows<D, DT, NT, 4>(a, c, b, st);
   }
   if (p.tiles)
-    hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT, tile_waves(D)>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)),
-                       dim3(64 * tile_waves(D)), 0, st,
-                       a, c, b, b.table, c.k_scale, c.v_scale);
+    hipLaunchKernelGGL((kv_attend_tiles_kernel<D, DT>), dim3((unsigned)(p.big_tiles * p.splits * c.kv_heads)), dim3(256), 0,
+                       st, a, c, b, b.table, c.k_scale, c.v_scale);
   if (a.part != nullptr || a.big_part != nullptr) {
     const int64_t waves = p.small_tiles > 0 ? (int64_t)p.small_tiles * 16 * c.kv_heads : (int64_t)b.rows * a.heads;
     hipLaunchKernelGGL((kv_attend_join_kernel<D, DT>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, c, b,
@@ -1039,7 +1026,7 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.causal = causal != 0, a.window = (int)window;
   a.most_blocks = (int)blocks;
-  a.shares = p.shares, a.block_shift = p.block_shift, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.big_rows = p.big_rows, a.splits = p.splits;
+  a.shares = p.shares, a.block_shift = p.block_shift, a.few = p.few, a.big_tiles = (int)p.big_tiles, a.splits = p.splits;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
