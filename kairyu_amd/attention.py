@@ -125,7 +125,7 @@ def _check_batch(q: torch.Tensor, cache: PagedKvCache, cache_shape: torch.Size, 
         raise ValueError(f"block_table, cu_rows and lengths must be int32, got {table.dtype}, {cu_rows.dtype}, {lengths.dtype}")
     if not (cu_rows.is_contiguous() and lengths.is_contiguous() and (table.is_contiguous() or _rows_apart(table))):
         raise ValueError("cu_rows, lengths and the rows of block_table must be contiguous, and its rows not overlap")
-    for t in (cache[0], cache[1], cache[2], cache[3], table, cu_rows, lengths):
+    for t in (*cache, table, cu_rows, lengths):
         if t.device != device:
             raise RuntimeError(f"cache and batch tensors must be on {device}; found {t.device}")
     return shape
@@ -145,8 +145,10 @@ def _check_keys(x: torch.Tensor, name: str, q: torch.Tensor, q_shape: torch.Size
 
 
 def _refuse_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the key/value cache is for inference: an input requires a gradient")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the key/value cache is for inference: an input requires a gradient")
 
 
 # ------------------------------------------------------------- public calls
@@ -194,8 +196,6 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     _refuse_grad(q, k, v, q_norm, k_norm)
     if not q.is_cuda:
         return _rotate_append_plain(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps)
-    q_norm = None if q_norm is None else hip.aligned(q_norm)
-    k_norm = None if k_norm is None else hip.aligned(k_norm)
     return hip.rotate_append(q, k, v, shape, cache, cache_shape, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm,
                              k_norm, eps)
 

@@ -41,28 +41,42 @@ def call_on(device: torch.device, entry: str, *args) -> None:
         _native.call(entry, *args, _native.stream_handle(device))
 
 
-def aligned(x: torch.Tensor) -> torch.Tensor:
-    """fp16 / bf16 ``x`` with unit stride in its last dimension and every row 16-byte
-    aligned: itself where it is so, else a contiguous copy."""
+def _heads(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """fp16 / bf16 ``x [rows, heads, dim]`` with unit stride in its last dimension and
+    every head 16-byte aligned (itself where it is so, else a contiguous copy), its
+    address and its pitches from row to row and head to head."""
 
-    *outer, unit = x.stride()
-    if unit == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    row, head, unit = x.stride()
+    at = x.data_ptr()
+    if unit != 1 or at & 15 or (row | head) & 7:
+        x = x.clone(memory_format=torch.contiguous_format)
+        row, head, unit = x.stride()
+        at = x.data_ptr()
+    return x, at, row, head
+
+
+def _weight(w: torch.Tensor | None) -> torch.Tensor | None:
+    """Norm weights, contiguous and 16-byte aligned."""
+
+    if w is None or (w.is_contiguous() and not w.data_ptr() & 15):
+        return w
+    return w.clone(memory_format=torch.contiguous_format)
 
 
 def rotate_append(q, k, v, shape, cache, cache_shape, table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps):
     device = q.device
     require_device(device, "the key/value append")
-    q, k, v = aligned(q), aligned(k), aligned(v)
+    q, q_at, q_row, q_head = _heads(q)
+    k, k_at, k_row, k_head = _heads(k)
+    v, v_at, v_row, v_head = _heads(v)
+    q_norm, k_norm = _weight(q_norm), _weight(k_norm)
     rows, heads, dim = shape
     pages, kv_heads, page, _ = cache_shape
-    out = torch.empty(shape, device=device, dtype=q.dtype)
-    (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     angles = (0, 0) if cos_sin is None else cos_sin.shape
     seqs, width = table.shape
     call_on(
-        device, "kq_kv_rotate_append", q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+        device, "kq_kv_rotate_append", q_at, q_row, q_head, k_at, k_row, k_head, v_at, v_row, v_head,
         _native.dtype_code(q.dtype), rows, heads, kv_heads, dim, cache[0].data_ptr(), cache[1].data_ptr(),
         cache[2].data_ptr(), cache[3].data_ptr(), pages, page, table.data_ptr(), _pitch(table, seqs, width), width,
         cu_rows.data_ptr(), lengths.data_ptr(), seqs, _native.ptr(cos_sin), angles[0], angles[1], interleaved,
@@ -83,18 +97,17 @@ def _attention_bytes(*shape: int) -> int:
 def attention(q, shape, cache, cache_shape, table, cu_rows, lengths, scale, causal, window):
     device = q.device
     require_device(device, "attention over a key/value cache")
-    q = aligned(q)
+    q, q_at, q_row, q_head = _heads(q)
     rows, heads, dim = shape
     pages, kv_heads, page, _ = cache_shape
     seqs, width = table.shape
-    out = torch.empty(shape, device=device, dtype=q.dtype)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     # partial results of split sequences, of the call's own: torch's allocator keeps
     # them to the calling stream and, under capture, to the graph
     need = _attention_bytes(rows, heads, kv_heads, dim, page, width, seqs)
     scratch = torch.empty(need, device=device, dtype=torch.uint8) if need else None
-    q_row, q_head, _ = q.stride()
     call_on(
-        device, "kq_kv_attention", q.data_ptr(), q_row, q_head, _native.dtype_code(q.dtype), rows, heads, kv_heads, dim,
+        device, "kq_kv_attention", q_at, q_row, q_head, _native.dtype_code(q.dtype), rows, heads, kv_heads, dim,
         cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(), pages, page, table.data_ptr(),
         _pitch(table, seqs, width), width, cu_rows.data_ptr(), lengths.data_ptr(), seqs, scale, causal, window,
         out.data_ptr(), _native.ptr(scratch), need,

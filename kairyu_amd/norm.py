@@ -18,6 +18,7 @@ from kairyu_amd.kernels import kv_cache_hip as hip
 __all__ = ["block_norm"]
 
 MODES = {None: 0, "fp8": 1, "int8": 2, "fp8_block": 3}
+Y_DTYPES = (None, torch.float8_e4m3fn, torch.int8, torch.float8_e4m3fn)
 MAX_HIDDEN = 32768
 
 
@@ -64,9 +65,10 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
                              f"{tuple(shape)} on {device}")
         if r_dtype is not dtype and r_dtype is not torch.float32:
             raise ValueError(f"residual must be {dtype} or float32, got {r_dtype}")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
-        raise RuntimeError("block_norm is for inference: an input requires a gradient")
+    if torch.is_grad_enabled():
+        for t in (x, residual, weight, post_weight, gate):
+            if t is not None and t.requires_grad:
+                raise RuntimeError("block_norm is for inference: an input requires a gradient")
     if not x.is_cuda:
         return _plain(x, residual, weight, post_weight, gate, residual_scale, eps, unit_offset, quantize)
     hip.require_device(device, "block_norm")
@@ -78,8 +80,9 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
             gates, gate_pitch, _ = _rows(gate, hidden)
         else:
             gates = gate.contiguous()
-    r = torch.empty(shape, device=device, dtype=r_dtype)
-    y = torch.empty(shape, device=device, dtype=dtype if mode == 0 else torch.int8 if mode == 2 else torch.float8_e4m3fn)
+    r = torch.empty_like(x, dtype=r_dtype, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x, dtype=Y_DTYPES[mode], memory_format=torch.contiguous_format) if mode else torch.empty_like(
+        x, memory_format=torch.contiguous_format)
     scales = None
     if mode:
         scales = torch.empty((*shape[:-1], -(-hidden // 128) if mode == 3 else 1), device=device, dtype=torch.float32)
