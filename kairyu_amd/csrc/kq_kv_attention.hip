@@ -727,11 +727,13 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       if (token < from || token >= to) w[e] = -__builtin_inff();
     }
   };
-  // Their weights by the running maximum as it is: it only has to keep them from
-  // overflowing, so it moves where one would exceed 2^8 (seldom after the first steps) and
-  // no weight waits for this step's maximum.  l adds the denominator's share from the
-  // weights before their rounding to fp16, in fp32: a page of small values has a small
+  // Their weights by an earlier maximum: it only has to keep them from overflowing, so it
+  // moves where they may add up to more than 2^10 (seldom after the first steps), no weight
+  // waits for this step's maximum and none is computed.  l adds up the denominator's share
+  // before the weights are rounded to fp16, in fp32: a page of small values has a small
   // value scale, and weights that are 0 in fp16 may be what the denominator consists of.
+  // (l is the weights times 1 / value scale of either 16-token tile, so that none is above
+  // l / min(iv); a tile without a page has 0 there and only makes the maximum move early.)
   auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, f32x2_t iv, const f32x16& w, float& l) {
     const int g = i >> 2;
     const float x = __builtin_amdgcn_exp2f(fmaf(w[2 * i], ks[g], shift_v[g]));
@@ -739,43 +741,42 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     l = i == 0 ? (x + y) * iv[g] : fmaf(x + y, iv[g], l);
     return pack_act2(x, y, KQ_DTYPE_F16);
   };
-  auto weights = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, f32x2_t{lv[0] - base, lv[1] - base}, iv, w, l);
-  };
-  // Scores of the next 32 tokens with the weights of these (and their largest exponent)
-  // between the products, an MFMA to every pair or two: the order is pinned.
+  auto base_of = [](float m) { return m == -__builtin_inff() ? 0.0f : m; };
+  // Scores of the next 32 tokens with the weights of these between the products, an MFMA to
+  // every pair or two: the order is pinned.
   auto dots_under_weights = [&](f32x16& next, f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    const f32x2_t shift_v = {lv[0] - base, lv[1] - base};
+    const f32x2_t shift_v = {lv[0] - base_of(top), lv[1] - base_of(top)};
 #pragma unroll
     for (int e = 0; e < 16; ++e) next[e] = 0.0f;
-    float x[2] = {-__builtin_inff(), -__builtin_inff()};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       next = mfma32<DT>(kx[k], qf[k], next);
 #pragma unroll
-      for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) {
-        p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, w, l);
-        x[i >> 2] = fmaxf(fmaxf(x[i >> 2], w[2 * i]), w[2 * i + 1]);
-      }
+      for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, w, l);
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));  // (not behind the branch that may compute them anew)
-    // a 16-token tile's scale is positive, so its largest score is its largest dot product's
-    return fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
   };
-  auto limit = [&](float m, f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    if (__ballot(m > top + 8.0f) == 0) return;
+  auto limit = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
+    if (__ballot(l > 1024.0f * fminf(iv[0], iv[1]) || top == -__builtin_inff()) == 0) return;
+    // a 16-token tile's scale is positive, so its largest score is its largest dot product's
+    float x[2] = {w[0], w[8]};
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      x[0] = fmaxf(x[0], w[e]);
+      x[1] = fmaxf(x[1], w[8 + e]);
+    }
+    float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
     const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
-    const float keep = __builtin_amdgcn_exp2f(top - (m == -__builtin_inff() ? 0.0f : m));
+    const float keep = __builtin_amdgcn_exp2f(top - base_of(m));
     sum *= keep;
 #pragma unroll
     for (int j = 0; j < OT; ++j) o[j] *= keep;
     top = m;
-    weights(ks, lv, iv, w, p, l);
+    const f32x2_t shift_v = {lv[0] - base_of(top), lv[1] - base_of(top)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, w, l);
   };
   u32x4 vx[2][OT];
   auto read_values = [&](const char* buf, int i) {
@@ -820,9 +821,9 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         const f32x2_t ks = pair_at(buf, 0, 0), lv = pair_at(buf, 1, 0), iv = pair_at(buf, 2, 0);
         read_keys(buf, 1);
         if constexpr (masked) mask(t, x);
-        const float m = dots_under_weights(y, ks, lv, iv, x, p, l);
+        dots_under_weights(y, ks, lv, iv, x, p, l);
         read_values(buf, 0);
-        limit(m, ks, lv, iv, x, p, l);
+        limit(ks, lv, iv, x, p, l);
         add_values(p);
         sum += l;
         put_k(next);
@@ -834,9 +835,9 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
         const f32x2_t ks = pair_at(buf, 0, 1), lv = pair_at(buf, 1, 1), iv = pair_at(buf, 2, 1);
         read_keys(next, 0);
         if constexpr (masked) mask(t + 32, y);
-        const float m = dots_under_weights(x, ks, lv, iv, y, p, l);
+        dots_under_weights(x, ks, lv, iv, y, p, l);
         read_values(buf, 1);
-        limit(m, ks, lv, iv, y, p, l);
+        limit(ks, lv, iv, y, p, l);
         add_values(p);
         sum += l;
         put_v(next);
