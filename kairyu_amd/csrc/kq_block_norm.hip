@@ -12,8 +12,10 @@
 // one rounding fewer on each than the separate operations have.
 //
 // One workgroup per row, the row in registers, each operand read once.  HBM bound on
-// many rows; on few, by the chain load -> sum -> sum -> store, so the amax joins the
-// second sum (amax(y) = amax(r * weight) / rms(r)) instead of following it.
+// many rows (8192 of 4096, gate and fp32 residual, out in blocks: 437 MB in 76-87 us,
+// 5.0-5.7 TB/s, the rate of a copy); on few, by the chain load -> sum -> sum -> store
+// (48 of 3584: 4.2 us), so the amax joins the second sum (amax(y) = amax(r * weight) /
+// rms(r)) instead of following it.
 #include "kq_common.h"
 
 #include <algorithm>

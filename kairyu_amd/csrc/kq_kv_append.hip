@@ -172,8 +172,13 @@ KQ_DEV uint32_t move4(uint32_t w, float ratio) {
 KQ_DEV u32x4 move16(u32x4 w, float ratio) { return u32x4{move4(w[0], ratio), move4(w[1], ratio), move4(w[2], ratio), move4(w[3], ratio)}; }
 
 // Workgroups [0, page_units): one page of one sequence and one kv head each, its new
-// tokens in registers (NCH pairs of chunks a thread, keys and values).  The others:
-// query rows, HPT heads of one row a thread, which share their angles.
+// tokens in registers (NCH pairs of chunks a thread, keys and values), so that the scale
+// is known before a code is written and each row is read once.  The others: query rows,
+// HPT heads of one row a thread, which share their angles.
+//
+// Bound by HBM on prompts: 8 of up to 2048 rows, 32 + 8 + 8 heads of 128, 183 MB, 40 us
+// (4.6 TB/s; a copy's rate is 5.2).  64 single tokens take 6 us: a launch and the chain
+// bounds -> table entry -> page -> scales -> codes, whose rows' loads go first.
 template <int D, int NCH, int THREADS, int HPT>
 __global__ void __launch_bounds__(THREADS)
 kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
@@ -392,22 +397,27 @@ static void launch_append(const AppendArgs& a, const KvCache& c, const KvBatch& 
                      dtype);
 }
 
-// A page's tokens in registers: 256 threads hold 4096 elements a pair of chunks; pages
-// past 8192 elements go to 1024 threads instead of more registers.
+// A page's tokens in registers: 256 threads hold 4096 elements a pair of chunks.  Pages of
+// 8192 go to 512 threads where the rows are few and the chain is what takes the time (64
+// single tokens 6.1 us, with 256 threads 6.7; the prompts 43.3 and 41.6), pages of 16384
+// to 512 with two pairs (the prompts 42.2 us, with 1024 and one pair 47.9; 6.2 and 7.7), larger ones to 1024
+// with two (heads of 256: 49 us, with 512 and four 54).
 template <int D, int HPT>
 static void pick_append(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
   const int elements = D << c.page_shift;
   if (elements <= 4096)
     launch_append<D, 1, 256, HPT>(a, c, b, dtype, st);
   else if (elements <= 8192)
-    launch_append<D, 2, 256, HPT>(a, c, b, dtype, st);
+    launch_append<D, HPT == 4 ? 2 : 1, HPT == 4 ? 256 : 512, HPT>(a, c, b, dtype, st);
   else if (elements <= 16384)
-    launch_append<D, 1, 1024, HPT>(a, c, b, dtype, st);
+    launch_append<D, 2, 512, HPT>(a, c, b, dtype, st);
   else
     launch_append<D, 2, 1024, HPT>(a, c, b, dtype, st);
 }
 
-// Four heads a thread once that still fills the chip; one where the rows are few.
+// Four heads a thread, which share their angles' loads, once that still fills the chip;
+// one where the rows are few (the prompts above 41 us with four and 48 with one, the 64
+// single tokens with it 8.7 and 6.8).
 template <int D>
 static void pick_heads(const AppendArgs& a, const KvCache& c, const KvBatch& b, int dtype, hipStream_t st) {
   if ((int64_t)b.rows * a.heads * D >= 4 * 256 * 4096)

@@ -191,6 +191,11 @@ KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, in
 // read as zero without a branch.  They are marked non-temporal: a token is read once by
 // a tile and most sequences have one (64 ragged contexts 51.2 -> 46.5 us, 3 x 131001
 // tokens 158 -> 139; two tiles a sequence, which then share less, 66 -> 69).
+//
+// Bound by HBM on long contexts: 3 x 131001 tokens on 8 kv heads of 128, 805 MB, take
+// 124 us (6.5 TB/s); 64 of up to 6000 on 4, 186 MB, 40 (4.6), where starting, the first
+// loads' latency and the last part's merge are 8 of them.  A single context of 700 tokens
+// takes 8 us, its three steps' latency.
 template <int D, int DT, int NT, int PP>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 3)
 kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -471,6 +476,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
 
 // The parts of split tiles joined in the order of their tokens, one wave per row and
 // query head: of every row, or of the 16-row tiles alone where no large tile is split.
+// Latency: 5 us for 64 contexts, most of it the launch and two dependent loads.
 template <int D, int DT>
 __global__ void __launch_bounds__(256)
 kv_attend_join_kernel(AttendArgs a, KvCache cache, KvBatch batch, int small_tiles) {
@@ -555,6 +561,11 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // that it sees or one of `splits` parts of them, 64 at a step.  (With eight waves, which
 // share what a step widens, 8192 rows behind 12288 tokens took 1087 us and with four 1100,
 // but 1024 of 1024 42.7 and 31.6: fewer tiles fill the chip unevenly.)
+//
+// 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1080-1140 us, 1.0
+// PFLOP/s.  The matrix cores are busy for 46% of that and the vector unit, with 16
+// exponentials and 95 other instructions a half step of 32 tokens, for about the rest: the
+// two overlap little on a SIMD, and time falls with the vector instructions.
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
 // are shared by the waves: they are widened once, keys to Q's type in rows of one
@@ -875,13 +886,17 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   store([&](int d, float x, float y) { *(uint32_t*)(dst + d) = pack_act2(x * inv, y * inv, DT); });
 }
 
-// Workgroups that fill the chip: 256 CUs times what the registers let a CU hold.
+// Workgroups that fill the chip: CUs times what the registers let a CU hold.
 constexpr int rows_slots(int64_t dim) { return 256 * (dim == 256 ? 2 : 3); }
 
 // rows * group up to which a sequence goes to tiles of 16 rows, which stream its
-// tokens once per tile
+// tokens once per tile (24 sequences behind 3000 tokens, 4 heads a kv head: 5 rows 65 us
+// either way; 15 rows 79 in large tiles, 113 in small ones)
 constexpr int kFewItems = 32;
 
+// Tokens up to which one workgroup reads a tile's whole: a second launch costs 4 us of host
+// time (16 contexts of up to 700 tokens on 8 kv heads 11.9 us whole, 13.1 shared out; 4 of
+// 1000 13.4 and 12.7)
 constexpr int64_t kWhole = 1024;
 // ... and where a window makes the tiles alike and they fill the chip by themselves (64 single
 // tokens on 4 kv heads of 128, windows of 900, 1400 and 1900: 16.7, 21.5 and 25.7 us whole,
@@ -923,7 +938,8 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
   const int64_t most_rows = p.tiles ? std::max<int64_t>(kFewItems / group, 1) : rows;
   const int64_t span = window > 0 ? std::min(tokens, window + most_rows + 64) : tokens;
   const bool whole = span <= (window > 0 && seqs * kv_heads >= 256 ? kWholeMany : kWhole);
-  p.block_shift = !whole ? 2 : span > kWhole ? 5 : 4;
+  p.block_shift = 2;
+  while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
   if (p.rows && !whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
   if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * kBigRows * (dim + 4));
   return p;
