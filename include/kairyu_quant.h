@@ -416,7 +416,8 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
  * does a position past the table.  Rows of no sequence are padding: their
  * outputs are zero and nothing is stored for them.  `*_ld` and `*_hs` are the
  * pitches in elements from row to row and from head to head (multiples of 8;
- * rows 16-byte aligned). */
+ * rows 16-byte aligned).  Up to 2^30 tokens a table, 2^29 pages times heads and
+ * 1024 heads; lengths past the table only move the positions. */
 
 /* Rotation of queries and keys by position and the append of keys and values.
  * cos_sin fp32 [positions, rotary] holds each position's rotary / 2 cosines,
@@ -446,7 +447,8 @@ int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k
  * where that is positive.  A row that sees none is zero.  Stored values must not
  * be NaN codes in slots that hold tokens (slots past a sequence's end may hold
  * anything); NaN keys make the rows that see them NaN and no other.  out
- * [rows, heads, dim].  Workspace: kq_kv_attention_workspace_size bytes.
+ * [rows, heads, dim].  |scale| at most 2^100.  Workspace:
+ * kq_kv_attention_workspace_size bytes, of the call's own.
  * Replaces the paged attention backends (kairyu/engine/core/attention/) for an
  * 8-bit cache. */
 int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
