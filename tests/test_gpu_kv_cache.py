@@ -515,3 +515,56 @@ def test_windows_of_many_sequences(cuda, new, window):
     out = paged_attention(q, pool, table, cu, lengths, window=window)
     torch.cuda.synchronize()
     kv.check_attention(out, q, pool, table, cu, lengths, window=window)
+
+
+@pytest.mark.parametrize("batch", [([1] * 5, [900, 20, 333, 64, 1]), ([20] + [0] * 23, [700] + [30] * 23), ([3, 40], [60, 500])])
+@pytest.mark.parametrize("heads", [(200, 1, 64), (48, 2, 128)])
+def test_attention_of_large_groups(cuda, batch, heads):
+    """More query heads to a kv head than a tile has rows; one sequence with all the rows."""
+    banner(f"kv attention large groups {batch} {heads}")
+    q, _, _, pool, table, cu, lengths = _case(cuda, batch, heads, 32, torch.bfloat16, seed=49, pad=1)
+    out = paged_attention(q, pool, table, cu, lengths)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths)
+
+
+def test_misaligned_head_norms(cuda):
+    banner("kv append misaligned head norms")
+    q, k, v, pool, table, cu, lengths = _case(cuda, "mixed", (6, 3, 64), 16, torch.bfloat16, seed=50)
+    g = kv.gen(51)
+    wide = (torch.randn(2 * 64 + 1, generator=g) * 0.1 + 1).to(q.dtype).to(cuda)
+    norms = [wide[1:65], wide[:128:2]]  # 2-byte aligned, and not contiguous
+    before = kv.values(pool)
+    out = rotate_append(q, k, v, pool, table, cu, lengths, q_norm=norms[0], k_norm=norms[1])
+    torch.cuda.synchronize()
+    kv.check_append(out, pool, before, q, k, v, table.cpu(), cu.cpu(), lengths.cpu(), q_norm=norms[0].cpu(), k_norm=norms[1].cpu())
+
+
+def test_captured_batches_replay_beside_each_other(cuda):
+    """Two graphs, prompts whose tokens are cut and ragged single tokens, replayed in turn on
+    two streams for changing lengths: each equals the eager call bit for bit."""
+    banner("kv captured prompts and decode")
+    parts = [_case(cuda, ([90, 1], [5000, 4000]), "4 of 4, 128", 64, torch.bfloat16, seed=52, pad=2),
+             _case(cuda, ([1] * 9, [3000 - 300 * s for s in range(9)]), "7 of 1, 128", 32, torch.float16, seed=53)]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in parts], [], []
+    for stream, (q, _, _, pool, table, cu, lengths) in zip(streams, parts):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            paged_attention(q, pool, table, cu, lengths)
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention(q, pool, table, cu, lengths))
+        graphs.append(graph)
+    full = [p[6].clone() for p in parts]
+    for less in (0, 700, 33, 1500, 0):
+        for part, most in zip(parts, full):
+            part[6].copy_((most - less).clamp(min=1))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for part, out in zip(parts, outs):
+            assert torch.equal(out, paged_attention(part[0], *part[3:])), less
+            torch.cuda.synchronize()
