@@ -889,6 +889,15 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 // Workgroups that fill the chip: CUs times what the registers let a CU hold.
 constexpr int rows_slots(int64_t dim) { return 256 * (dim == 256 ? 2 : 3); }
 
+constexpr int64_t tile_slots(int64_t dim) { return 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1); }
+
+// Tokens up to which sequences of few rows go to large tiles as well, a launch and a join
+// less, where there are no more than 64 tokens to a new row and the tiles are few (32 heads
+// over 8 of 128: 24 sequences of up to 300 rows behind 2000 tokens 103 -> 94 us, 12 of 64
+// behind 1000 45 -> 32; but a prompt of 512 rows beside one token behind 2000 37 -> 47, behind
+// 8000 42 -> 81, beside 100 tokens behind 1000 66 -> 81)
+constexpr int64_t kAlone = 2048, kAloneTokens = 64;
+
 // rows * group up to which a sequence goes to tiles of 16 rows, which stream its
 // tokens once per tile (24 sequences behind 3000 tokens, 4 heads a kv head: 5 rows 65 us
 // either way; 15 rows 79 in large tiles, 113 in small ones)
@@ -910,16 +919,20 @@ struct Plan {
   size_t part, big_part;  // bytes
 };
 
-// From what the host knows: rows and sequences, not their lengths.
-static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
-                    int64_t seqs, int64_t window) {
+// From what the host knows: rows and sequences, not their lengths.  `alone`: large tiles
+// take every sequence, however few its rows are.
+static Plan plan_with(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
+                      int64_t seqs, int64_t window, bool alone) {
   Plan p{};
   const int64_t group = heads / kv_heads, items = rows * group, tokens = width * page_size;
+  // tokens that some rows of a sequence can look at, from their first step on
+  auto span_of = [&](int64_t most_rows) { return window > 0 ? std::min(tokens, window + most_rows + 64) : tokens; };
+  int64_t span = span_of(rows);
   if (rows <= seqs || items <= kFewItems) {  // single tokens (no more rows than sequences)
     p.rows = true;
     p.few = 0x7fffffff;
   } else {
-    p.rows = seqs > 1;
+    p.rows = !alone && seqs > 1;
     p.tiles = true;
     p.few = p.rows ? kFewItems : 0;
     // (no sequence of more than `few` items ends more than one tile short)
@@ -928,21 +941,27 @@ static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, 
     // few tiles: cut their tokens until every workgroup slot has some, but not below 1024 each: a cut costs the
     // second launch and the partial sums' way through memory (32 heads over 8 of 128 channels, one sequence: 512 rows
     // behind 4096 tokens 130 us whole, 70 cut; 1024 rows behind 8192 on 4 heads 250 and 166; 1024 rows of 1024 42 and 52)
-    const int64_t most = std::max<int64_t>(tokens / 1024, 1), slots = 256 * (dim == 64 ? 3 : dim == 128 ? 2 : 1);
-    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, slots / std::max<int64_t>(1, p.big_tiles * kv_heads)));
+    const int64_t most = std::max<int64_t>(span_of(kBigRows) / 1024, 1);
+    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, tile_slots(dim) / std::max<int64_t>(1, p.big_tiles * kv_heads)));
+    span = span_of(std::max<int64_t>(kFewItems / group, 1));
   }
   p.splits = std::max(p.splits, 1);
-  if (p.tiles && p.splits == 1) p.small_tiles = std::min<int64_t>(rows * group, seqs * (kFewItems / 16));
+  if (p.rows && p.splits == 1) p.small_tiles = p.tiles ? std::min<int64_t>(rows * group, seqs * (kFewItems / 16)) : 0;
   p.shares = (int)std::max<int64_t>(rows_slots(dim) / kv_heads, 1);
-  // tokens that a sequence in 16-row tiles can look at, from its first step on
-  const int64_t most_rows = p.tiles ? std::max<int64_t>(kFewItems / group, 1) : rows;
-  const int64_t span = window > 0 ? std::min(tokens, window + most_rows + 64) : tokens;
   const bool whole = span <= (window > 0 && seqs * kv_heads >= 256 ? kWholeMany : kWhole);
   p.block_shift = 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
   if (p.rows && !whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * (dim + 4));
   if (p.splits > 1) p.big_part = sizeof(float) * (size_t)(p.big_tiles * kv_heads * p.splits * kBigRows * (dim + 4));
   return p;
+}
+
+static Plan plan_of(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
+                    int64_t seqs, int64_t window) {
+  const int64_t tokens = width * page_size, span = window > 0 ? std::min(tokens, window + kFewItems + 64) : tokens;
+  const int64_t tiles = rows * (heads / kv_heads) / kBigRows + seqs;
+  return plan_with(rows, heads, kv_heads, dim, page_size, width, seqs, window,
+                   span <= kAlone && kAloneTokens * rows >= seqs * span && tiles * kv_heads <= 2 * tile_slots(dim));
 }
 
 template <int D, int DT, int NT, int PP>
@@ -988,8 +1007,12 @@ using namespace kq;
 extern "C" size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                                  int64_t page_size, int64_t table_width, int64_t seqs) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
-  const Plan p = plan_of(rows, heads, kv_heads, dim, page_size, table_width, seqs, 0);  // (a window needs no more)
-  return p.part + p.big_part;
+  size_t most = 0;  // (a window needs no more than none)
+  for (const bool alone : {false, true}) {
+    const Plan p = plan_with(rows, heads, kv_heads, dim, page_size, table_width, seqs, 0, alone);
+    most = std::max(most, p.part + p.big_part);
+  }
+  return most;
 }
 
 extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,

@@ -568,3 +568,22 @@ def test_captured_batches_replay_beside_each_other(cuda):
         for part, out in zip(parts, outs):
             assert torch.equal(out, paged_attention(part[0], *part[3:])), less
             torch.cuda.synchronize()
+
+
+BESIDE = {  # mostly single tokens, so that they and the prompts' tiles are two launches
+    "short": ([1] * 40 + [45, 3, 9, 130], [30 + 19 * s for s in range(40)] + [300, 900, 9, 130]),
+    "joined": ([1] * 40 + [45, 3, 9, 130], [30 + 37 * s for s in range(40)] + [300, 1900, 9, 130]),
+    "long": ([1] * 5 + [50, 2, 70, 90], [2600, 1, 700, 2049, 64, 900, 2300, 70, 1700]),
+    "many": ([1, 1, 1, 1, 1, 1, 8, 36] * 10, [700, 33, 1500, 64, 65, 1024, 1100, 400] * 10),
+}
+
+
+@pytest.mark.parametrize("how", [dict(), dict(causal=False), dict(window=300)], ids=str)
+@pytest.mark.parametrize("heads", ["8 of 2, 64", "7 of 1, 128", "3 of 1, 256"])
+@pytest.mark.parametrize("batch", BESIDE)
+def test_single_tokens_beside_prompts(cuda, batch, heads, how):
+    banner(f"kv attention beside {batch} {heads} {how}")
+    q, _, _, pool, table, cu, lengths = _case(cuda, BESIDE[batch], heads, 32, torch.bfloat16, seed=54, pad=2)
+    out = paged_attention(q, pool, table, cu, lengths, **how)
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths, batch, **how)
