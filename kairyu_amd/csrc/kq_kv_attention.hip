@@ -636,7 +636,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   const int k_tok = tid / 4, v_grp = tid / 16, v_c = tid % 16;
   const int k_lane = (k_tok % 16) * D + (tid % 4) * (D / 4), v_lane = 4 * (v_grp % 4) * D + v_c * VY;
   const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
-  const int64_t tile_bytes = (int64_t)D << shift;
+  const int tile_shift = shift + (D == 64 ? 6 : D == 128 ? 7 : 8);  // log2 of a page's bytes
   const int in_page = (1 << shift) - 1;
   const int32_t* pages = table + (int64_t)s * batch.table_ld;
   auto page_at = [&](int t) { return pages[min(t + 16 * wave, max(hi - 1, 0)) >> shift]; };
@@ -646,28 +646,26 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   // a step's page of this wave: its tile, the bytes before the sequence's end (slots past
   // it hold whatever was there, NaN perhaps; the resources end before them) and the offset
   struct Place {
-    int64_t head_tile;
-    uint32_t size;
-    int off;
+    int head_tile, size, off;
   };
   auto place_of = [&](int t, int page_) {
     const int page = __builtin_amdgcn_readfirstlane(page_), at = t + 16 * wave;
     const bool there = page >= 0 && page < (int)cache.pages && at < hi;
     Place p;
-    p.head_tile = (int64_t)(there ? page : 0) * cache.kv_heads + head;
-    p.size = there ? (uint32_t)(min(q.tokens - (at & ~in_page), in_page + 1) * D) : 0u;
-    p.off = __builtin_amdgcn_readfirstlane((at & in_page) * D);
+    p.head_tile = (there ? page : 0) * cache.kv_heads + head;
+    p.size = there ? min(q.tokens - (at & ~in_page), in_page + 1) * D : 0;
+    p.off = (at & in_page) * D;
     return p;
   };
   auto fetch_k = [&](const Place& p) {
-    const i32x4 src = make_rsrc(cache.k + p.head_tile * tile_bytes, p.size);
+    const i32x4 src = make_rsrc(cache.k + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
 #pragma unroll
     for (int i = 0; i < KC; ++i) kr[i] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(src, k_lane + 16 * i, p.off, 0));
     // (a vector load, which the barriers do not wait for; 0 where there is no page)
     sc_k = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
   };
   auto fetch_v = [&](const Place& p) {
-    const i32x4 src = make_rsrc(cache.v + p.head_tile * tile_bytes, p.size);
+    const i32x4 src = make_rsrc(cache.v + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if constexpr (VC == 1) {
