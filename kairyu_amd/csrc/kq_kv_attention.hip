@@ -563,9 +563,10 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // but 1024 of 1024 42.7 and 31.6: fewer tiles fill the chip unevenly.)
 //
 // 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1080-1140 us, 1.0
-// PFLOP/s.  The matrix cores are busy for 48% of that and the vector unit, with about 95
-// instructions a half step of 32 tokens, 16 of them exponentials, for about the rest: the
-// two overlap little on a SIMD, and time falls with the vector instructions.
+// PFLOP/s.  No unit bounds it alone: the matrix cores are busy for 48% of that, LDS for 53%,
+// the vector unit, with about 95 instructions a half step of 32 tokens, 16 of them
+// exponentials, for about half.  Widening and staging account for 27% of the time, the
+// products with the values for 20%, exponentials for 8% (copies timed without them).
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
 // are shared by the waves: they are widened once, keys to Q's type in rows of one
