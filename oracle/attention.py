@@ -109,8 +109,10 @@ def attend(q, cache, table, cu, lengths, scale=None, causal=True, window=0):
       roundings of ``|w|``, the base-2 exponent.  A weight is thus off by
       ``d = ln 2 * (dim * 2^-24 * sum |q k| scale log2 e + 8 * 2^-24 * max |w|) + 2^-21``
       relative, the numerator and denominator alike: ``2 d A``.
-    * a weight enters the product with the values rounded to fp16, ``2^-11`` of it,
-      or ``2^-25`` of the largest where it is subnormal.
+    * a weight enters the product with the values rounded once, ``2^-11`` of it, and
+      one far below the largest by no more than ``2^-34`` of that: beside a token that
+      takes nearly all of the mass, a million others lose ``2^-14`` of a value together
+      at the very most.
     * numerator and denominator add ``n`` terms in fp32 and the parts of a split
       sequence are rescaled: ``(2 n + 64) * 2^-24 A``.
     """
@@ -154,7 +156,7 @@ def attend(q, cache, table, cu, lengths, scale=None, causal=True, window=0):
             d = math.log(2) * (dim * U32 * magnitude.amax(-1, keepdim=True) * log2e + 8 * U32 * spread) + 2.0**-21
             # the largest exp2(w) against the denominator, in units of sum p
             unit_p = torch.exp((high - torch.where(top == -math.inf, 0.0, top) * log2e) * math.log(2))
-            sub = 2.0**-25 * torch.where(total == 0, 0.0, unit_p / some) * (seen.double() @ code["v"].abs())
+            sub = 2.0**-34 * torch.where(total == 0, 0.0, unit_p / some) * (seen.double() @ code["v"].abs())
             err = a * (2 * d + 2.0**-11 + (2 * tokens + 64) * U32) + sub
             out[row: row + n, h * group: (h + 1) * group] = o.reshape(n, group, dim)
             bound[row: row + n, h * group: (h + 1) * group] = err.reshape(n, group, dim)

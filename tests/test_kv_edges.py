@@ -1,0 +1,32 @@
+"""The paged 8-bit key/value cache on the CPU where it is easily wrong: what the oracle
+allows beside a dominant token."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+import kv_helpers as kv
+from oracle import attention as oatt
+
+
+def test_the_oracles_bound_beside_a_sink():
+    """Where one token holds nearly all of the mass and has a value of zero, the output is
+    the others' tail, and the bound is far below it."""
+
+    n, dim = 32768, 64
+    table, cu, lengths, rows, pages = kv.batch([1], [n], 128, spare=0)
+    pool = kv.cache(pages, 1, 128, dim)
+    pool.k.view(torch.uint8).zero_()
+    pool.v.view(torch.uint8).fill_(0x38)  # 1.0
+    pool.k_scale.fill_(1.0)
+    pool.v_scale.fill_(1.0)
+    sink = int(table[0, 0])
+    pool.k[sink, 0, 0] = torch.tensor(2.0).to(kv.E4M3)
+    pool.v.view(torch.uint8)[sink, 0, 0] = 0
+    score = math.log(n * 999.0)
+    q = torch.full((1, 1, dim), score / (dim**0.5 * 2.0))
+    o, bound = oatt.attend(q, kv.values(pool), table, cu, lengths)
+    assert (o - 1e-3).abs().max() <= 1e-5
+    assert (bound <= 0.01 * o).all()
