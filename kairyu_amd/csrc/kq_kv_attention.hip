@@ -4,9 +4,16 @@
 // a row sees, in one pass with a running maximum.  Key codes enter the products as
 // they are and the page's scale multiplies the finished dot product; the value scale
 // joins the exponent instead, w_t = log2(e) scale k_scale (q . code_t) + log2 v_scale,
-// so that exp2(w_t - max w) <= 1 multiplies the value's codes whatever the scales of
-// the pages are and keeps 11 bits as fp16; the denominator adds exp2(w_t - max w) /
-// v_scale.  Maxima, denominators and outputs are held in fp32.
+// so that exp2(w_t - max w + lift) multiplies the value's codes whatever the scales of
+// the pages are; the denominator adds the same over v_scale.  Maxima, denominators and
+// outputs are held in fp32, and the lift, which a row's sums all have, cancels.
+//
+// Weights enter the products with the values as fp16: 11 bits, 8 with bf16, which fp16
+// rows would show.  fp16 ends 2^-14 (11 bits) or 2^-25 (anything) below one, and a token
+// that most of the mass goes to may have a value of nearly zero, so that the others' tail
+// is the answer: the lift takes the largest weights towards the top of fp16's range, and
+// a weight keeps its 11 bits down to 2^-23 of the largest and some down to 2^-34 (tiles of
+// 128; 2^-29 and 2^-40 in tiles of 16).
 #include "kq_kv.h"
 
 #include <algorithm>
@@ -34,6 +41,13 @@ struct AttendArgs {
 };
 
 constexpr int kBigRows = 128;  // rows of a large tile, 32 a wave
+
+// log2 of the largest weight.  Tiles of 16 have the exact maximum.  Tiles of 128 move theirs
+// when a lane's 16 weights of a half step may add up to more than fp16 holds, 128 of 2^9: a
+// larger lift leaves less room and moves it more often (8192 rows behind 12288 tokens and 24
+// windows of heads of 64 with lifts of 5, 8, 9, 10 and 11: 1120, 1127, 1133, 1135 and 1142 us,
+// 50.9, 52.3, 53.2, 53.5 and 55.0; none at all 1106 and 51.3, with weights that are lost).
+constexpr float kLift = 15.0f, kBigLift = 9.0f, kBigMost = 65504.0f;
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
 template <int DT>
@@ -374,7 +388,7 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
       for (int j = 0; j < OT; ++j) o[j] *= keep;
       top = m;
     }
-    const float base = top == -__builtin_inff() ? 0.0f : top;
+    const float base = top == -__builtin_inff() ? 0.0f : top - kLift;
     u32x4 p[NT / 2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -582,7 +596,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   constexpr int OT = D / 32;            // output tiles
   constexpr int KLD = 2 * D + 16;       // bytes of a key's row
   constexpr int VLD = 2 * 64 + 16;      // bytes of a d's row of values
-  constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale, its inverse)
+  constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale + kBigLift, its inverse)
   constexpr int KC = D / 64;            // 16-byte chunks of one token's key a thread moves
   constexpr int VY = D / 16, VC = VY / 4;  // bytes and dwords of each of four tokens' values a thread moves
   constexpr int LD = D + 4;
@@ -707,7 +721,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     }
     if (lane == 0) {
       float* dst = (float*)(buf + KB + VB) + 4 + wave;
-      dst[0] = __builtin_amdgcn_logf(sc_v);
+      dst[0] = __builtin_amdgcn_logf(sc_v) + kBigLift;
       dst[4] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
   };
@@ -738,7 +752,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     }
   };
   // Their weights by an earlier maximum: it only has to keep them from overflowing, so it
-  // moves where they may add up to more than 2^10 (seldom after the first steps), no weight
+  // moves where they may add up to more than kBigMost (seldom after the first steps), no weight
   // waits for this step's maximum and none is computed.  l adds up the denominator's share
   // before the weights are rounded to fp16, in fp32: a page of small values has a small
   // value scale, and weights that are 0 in fp16 may be what the denominator consists of.
@@ -768,7 +782,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));  // (not behind the branch that may compute them anew)
   };
   auto limit = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    if (__ballot(l > 1024.0f * fminf(iv[0], iv[1]) || top == -__builtin_inff()) == 0) return;
+    if (__ballot(l > kBigMost * fminf(iv[0], iv[1]) || top == -__builtin_inff()) == 0) return;
     // a 16-token tile's scale is positive, so its largest score is its largest dot product's
     float x[2] = {w[0], w[8]};
 #pragma unroll
@@ -776,7 +790,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       x[0] = fmaxf(x[0], w[e]);
       x[1] = fmaxf(x[1], w[8 + e]);
     }
-    float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
+    float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1])) - kBigLift;
     const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
     const float keep = __builtin_amdgcn_exp2f(top - base_of(m));
