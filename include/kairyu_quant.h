@@ -421,7 +421,8 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
 
 /* Rotation of queries and keys by position and the append of keys and values.
  * cos_sin fp32 [positions, rotary] holds each position's rotary / 2 cosines,
- * then its sines (null: no rotation; a position past the table becomes NaN);
+ * then its sines (null: no rotation, unless positions is 0 and rotary is not; a
+ * position past the table, any of one without positions, becomes NaN);
  * rotary a multiple of 16 up to dim, pairs rotary / 2 apart or (interleaved)
  * neighbouring; q_norm / k_norm [dim] of the activations' dtype, or null, are
  * weights of a per-head RMS norm before it.  q_out [rows, heads, dim] receives

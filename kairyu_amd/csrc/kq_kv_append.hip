@@ -27,12 +27,12 @@ struct AppendArgs {
   int64_t q_ld, k_ld, v_ld;  // elements from one row to the next
   int64_t q_hs, k_hs, v_hs;  // and from one head to the next
   uint16_t* q_out;           // [rows][heads][D]
-  const float* cos_sin;      // [positions][rotary]: cos, then sin; null: no rotation
+  const float* cos_sin;      // [positions][rotary]: cos, then sin
   int64_t positions;
   const uint16_t* q_norm;
   const uint16_t* k_norm;
   float eps;
-  int heads, rotary, interleaved;
+  int heads, rotary, interleaved;  // (rotary 0: no rotation)
   int page_units;  // workgroups of the append (the rest rotate queries)
 };
 
@@ -440,7 +440,9 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   const char* what = "kq_kv_rotate_append";
   int rc = kv_check(what, dtype, rows, heads, kv_heads, dim, page_size, pages, seqs, table_width, table_ld);
   if (rc) return rc;
-  if (cos_sin != nullptr && (rotary < 16 || rotary > dim || rotary % 16 != 0 || positions < 0)) {
+  // (a table without positions has no address, but turns: every position is past it)
+  const bool turns = cos_sin != nullptr || (rotary > 0 && positions == 0);
+  if (turns && (rotary < 16 || rotary > dim || rotary % 16 != 0 || positions < 0)) {
     set_error("%s: rotary width must be a multiple of 16 up to the head dim, got %lld", what, (long long)rotary);
     return KQ_EINVAL;
   }
@@ -459,7 +461,7 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   a.q_out = (uint16_t*)q_out;
   a.cos_sin = cos_sin;
   a.positions = positions;
-  a.rotary = cos_sin != nullptr ? (int)rotary : 0;
+  a.rotary = turns ? (int)rotary : 0;
   a.interleaved = interleaved;
   a.q_norm = (const uint16_t*)q_norm;
   a.k_norm = (const uint16_t*)k_norm;

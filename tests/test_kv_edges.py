@@ -1,5 +1,5 @@
 """The paged 8-bit key/value cache on the CPU where it is easily wrong: what the oracle
-allows beside a dominant token."""
+allows beside a dominant token, angles without positions."""
 
 from __future__ import annotations
 
@@ -8,6 +8,7 @@ import math
 import torch
 
 import kv_helpers as kv
+from kairyu_amd.attention import rotary_table, rotate_append
 from oracle import attention as oatt
 
 
@@ -30,3 +31,16 @@ def test_the_oracles_bound_beside_a_sink():
     o, bound = oatt.attend(q, kv.values(pool), table, cu, lengths)
     assert (o - 1e-3).abs().max() <= 1e-5
     assert (bound <= 0.01 * o).all()
+
+
+def test_angles_without_positions():
+    """Every position is past a table that has none: NaN where heads would turn."""
+
+    table, cu, lengths, rows, pages = kv.batch([3, 1], [20, 7], 16, pad=1)
+    pool = kv.cache(pages, 2, 16, 64)
+    q, k, v = (torch.randn(rows, h, 64, generator=kv.gen(h)).to(torch.bfloat16) for h in (4, 2, 2))
+    before = kv.values(pool)
+    cos_sin = rotary_table(0, 32, device="cpu")
+    out = rotate_append(q, k, v, pool, table, cu, lengths, cos_sin)
+    assert out[:4, :, :32].isnan().all() and not out[:4, :, 32:].isnan().any()
+    kv.check_append(out, pool, before, q, k, v, table, cu, lengths, cos_sin=cos_sin)
