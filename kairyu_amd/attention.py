@@ -303,7 +303,7 @@ def _paged_attention_plain(q, cache, table, cu_rows, lengths, scale, causal, win
     heads, kv_heads, pages, page = q.shape[1], cache.k.shape[1], cache.k.shape[0], cache.page_size
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     for s, row, n, first, tokens in _sequences(q.shape[0], cache, table, cu_rows, lengths):
-        if not n or not tokens:
+        if not n or not tokens or not pages:
             continue
         at = table[s, : -(-tokens // page)].long()
         there = ((at >= 0) & (at < pages)).repeat_interleave(page)[:tokens]

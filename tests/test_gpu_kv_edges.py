@@ -1,5 +1,5 @@
 """The paged 8-bit key/value cache on the GPU where it is easily wrong: angles without
-positions."""
+positions, caches without pages."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 
 import kv_helpers as kv
 from gpu_helpers import banner
-from kairyu_amd.attention import rotary_table, rotate_append
+from kairyu_amd.attention import PagedKvCache, paged_attention, rotary_table, rotate_append
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,20 @@ def test_angles_without_positions(cuda, rows, interleaved):
     torch.cuda.synchronize()
     assert out[: sum(rows), :, :64].isnan().all() and not out[: sum(rows), :, 64:].isnan().any()
     kv.check_append(out, on, before, q, k, v, table, cu, lengths, cos_sin=cos_sin.cpu(), interleaved=interleaved)
+
+
+def test_caches_without_pages(cuda):
+    """No token is there: zero outputs, turned queries."""
+    banner("kv no pages")
+    pool = PagedKvCache.create(0, 2, 64, 16, device=cuda)
+    table, cu, lengths, rows, _ = kv.batch([40, 1], [70, 7], 16, pad=1)
+    q, k = (torch.randn(rows, h, 64, generator=kv.gen(h)).to(torch.bfloat16).to(cuda) for h in (4, 2))
+    where = (table.to(cuda), cu.to(cuda), lengths.to(cuda))
+    out = paged_attention(q, pool, *where)
+    cos_sin = rotary_table(80, 64, device=cuda)
+    turned = rotate_append(q, k, k, pool, *where, cos_sin)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape and not out.any()
+    some = kv.to(kv.cache(9, 2, 16, 64), cuda)
+    assert torch.equal(turned, rotate_append(q, k, k, some, *where, cos_sin))
+    torch.cuda.synchronize()

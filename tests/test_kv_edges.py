@@ -1,5 +1,5 @@
 """The paged 8-bit key/value cache on the CPU where it is easily wrong: what the oracle
-allows beside a dominant token, angles without positions."""
+allows beside a dominant token, angles without positions, caches without pages."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import math
 import torch
 
 import kv_helpers as kv
-from kairyu_amd.attention import rotary_table, rotate_append
+from kairyu_amd.attention import PagedKvCache, paged_attention, rotary_table, rotate_append
 from oracle import attention as oatt
 
 
@@ -44,3 +44,16 @@ def test_angles_without_positions():
     out = rotate_append(q, k, v, pool, table, cu, lengths, cos_sin)
     assert out[:4, :, :32].isnan().all() and not out[:4, :, 32:].isnan().any()
     kv.check_append(out, pool, before, q, k, v, table, cu, lengths, cos_sin=cos_sin)
+
+
+def test_caches_without_pages():
+    """No token is there: zero outputs, turned queries."""
+
+    pool = PagedKvCache.create(0, 2, 64, 16, device="cpu")
+    table, cu, lengths, rows, _ = kv.batch([3, 1], [20, 7], 16, pad=1)
+    q, k = (torch.randn(rows, h, 64, generator=kv.gen(h)).to(torch.bfloat16) for h in (4, 2))
+    out = paged_attention(q, pool, table, cu, lengths)
+    assert out.shape == q.shape and not out.any()
+    some = kv.cache(9, 2, 16, 64)
+    where = (table, cu, lengths, rotary_table(32, 64, device="cpu"))
+    assert torch.equal(rotate_append(q, k, k, pool, *where), rotate_append(q, k, k, some, *where))
