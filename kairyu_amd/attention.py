@@ -144,6 +144,17 @@ def _check_keys(x: torch.Tensor, name: str, q: torch.Tensor, q_shape: torch.Size
         raise ValueError(f"{name} must have the queries' dtype and device")
 
 
+def check_scores(scale: float | None, causal: bool, window: int, dim: int) -> float:
+    """The factor of the scores; what attention refuses of its own arguments."""
+
+    if window < 0 or window > 1 << 30 or (window and not causal):
+        raise ValueError(f"window must be 0, or a positive number of tokens of causal attention, got {window}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= 2.0**100:
+        raise ValueError(f"scale must be finite and at most 2^100, got {scale}")
+    return scale
+
+
 def _refuse_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -211,12 +222,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Ten
 
     cache_shape = _check_cache(cache)
     shape = _check_batch(q, cache, cache_shape, block_table, cu_rows, lengths)
-    if window < 0 or window > 1 << 30 or (window and not causal):
-        raise ValueError(f"window must be 0, or a positive number of tokens of causal attention, got {window}")
+    scale = check_scores(scale, causal, window, shape[2])
     _refuse_grad(q)
-    scale = shape[2] ** -0.5 if scale is None else float(scale)
-    if not abs(scale) <= 2.0**100:
-        raise ValueError(f"scale must be finite and at most 2^100, got {scale}")
     if not q.is_cuda:
         return _paged_attention_plain(q, cache, block_table, cu_rows, lengths, scale, causal, window)
     return hip.attention(q, shape, cache, cache_shape, block_table, cu_rows, lengths, scale, causal, window)

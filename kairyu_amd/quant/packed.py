@@ -285,7 +285,7 @@ class QuantLinearPack:
         ``hidden [..., K]`` holds the batch's rows in order; returns ``[...,
         q_features]``."""
 
-        from kairyu_amd.attention import paged_attention, rotate_append
+        from kairyu_amd.attention import check_scores, paged_attention, rotate_append
 
         heads, dim = cache.k.shape[1], cache.k.shape[3]
         widths = self._out_features
@@ -294,6 +294,7 @@ class QuantLinearPack:
                              f"got widths {widths}")
         if torch.is_grad_enabled() and hidden.requires_grad:
             raise RuntimeError("attend is for inference: the hidden states require a gradient")
+        check_scores(scale, causal, window, dim)  # (before anything is stored)
         with torch.no_grad():
             q, k, v = (part.reshape(-1, part.shape[-1]).unflatten(-1, (-1, dim)) for part in self(hidden))
             q = rotate_append(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved=interleaved,

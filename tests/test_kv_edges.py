@@ -1,15 +1,19 @@
 """The paged 8-bit key/value cache on the CPU where it is easily wrong: what the oracle
-allows beside a dominant token, angles without positions, caches without pages."""
+allows beside a dominant token, angles without positions, caches without pages, calls
+that are refused."""
 
 from __future__ import annotations
 
 import math
 
+import pytest
 import torch
 
 import kv_helpers as kv
 from kairyu_amd.attention import PagedKvCache, paged_attention, rotary_table, rotate_append
+from kairyu_amd.quant.packed import QuantLinearPack
 from oracle import attention as oatt
+from test_packed import _int8
 
 
 def test_the_oracles_bound_beside_a_sink():
@@ -57,3 +61,16 @@ def test_caches_without_pages():
     some = kv.cache(9, 2, 16, 64)
     where = (table, cu, lengths, rotary_table(32, 64, device="cpu"))
     assert torch.equal(rotate_append(q, k, k, pool, *where), rotate_append(q, k, k, some, *where))
+
+
+@pytest.mark.parametrize("how", [dict(window=-1), dict(window=8, causal=False), dict(scale=math.nan)], ids=str)
+def test_attend_refuses_before_it_stores(how):
+    table, cu, lengths, rows, pages = kv.batch([2, 1], [20, 3], 16)
+    pack = QuantLinearPack.create([_int8(64, n, n) for n in (256, 128, 128)])
+    pool = kv.cache(pages, 2, 16, 64)
+    before = [t.clone() for t in pool]
+    hidden = torch.randn(rows, 64, generator=kv.gen(1)).to(torch.bfloat16)
+    with pytest.raises(ValueError):
+        pack.attend(hidden, pool, table, cu, lengths, **how)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pool, before))
+    assert pack.attend(hidden, pool, table, cu, lengths).shape == (rows, 256)
