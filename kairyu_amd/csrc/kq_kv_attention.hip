@@ -169,6 +169,15 @@ struct LongestFirst {
   }
 };
 
+// Whether any of tokens [from, to) is there.  Scores over a token of no page are 0 * q, NaN
+// where the query is not finite, though the row does not see it: a lane whose sum is NaN
+// looks at the pages again, and takes the sum for empty if there are none.
+KQ_DEV bool any_there(const int32_t* pages, int64_t count, int from, int to, int shift) {
+  for (int i = from >> shift; from < to && i <= (to - 1) >> shift; ++i)
+    if (pages[i] >= 0 && pages[i] < count) return true;
+  return false;
+}
+
 // What waves have put in LDS is there for all of them; loads from memory stay in flight.
 KQ_DEV void meet() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -424,6 +433,11 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
     sum = 0.0f;
     for (int t = lo + ST * wave; t < hi; t += 4 * ST) step(t);
     sum = column_sum(sum);
+    if (sum != sum && !any_there(pages, cache.pages, max(from, lo), min(to, hi), shift)) {
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[j] = f32x4{0, 0, 0, 0};
+    }
 
     // the next part's loads travel while this one's waves meet
     const KvSeq old = q;
@@ -878,6 +892,13 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     for (; t < hi; t += 64) step(t, std::true_type{});
   }
   sum += __shfl_xor(sum, 32, 64);
+  if (sum != sum && !any_there(pages, cache.pages, max(from, lo), min(to, hi), shift)) {
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < OT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
+  }
 
   if (!real) return;
   // element e of tile j: row R = 32 j + 8 (e / 4) + 4 h + e % 4 of the values, so that

@@ -1,7 +1,9 @@
 """The paged 8-bit key/value cache on the GPU where it is easily wrong: angles without
-positions, caches without pages."""
+positions, caches without pages, queries that are not finite."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -46,3 +48,31 @@ def test_caches_without_pages(cuda):
     some = kv.to(kv.cache(9, 2, 16, 64), cuda)
     assert torch.equal(turned, rotate_append(q, k, k, some, *where, cos_sin))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (7, 1, 128), (3, 1, 256)], ids=str)
+@pytest.mark.parametrize("new,total", [([1, 1, 1], [600, 300, 150]), ([1, 1, 1], [3000, 2000, 150]),
+                                       ([150, 150, 150], [600, 300, 150]), ([150, 150, 150], [5000, 2300, 150])], ids=str)
+def test_queries_that_are_not_finite_over_tokens_of_no_page(cuda, new, total, heads, value):
+    """A row that sees no token is zero whatever its query holds; one that sees a token
+    is NaN then; and no other row is touched."""
+    banner(f"kv attention queries {value} {new} {total} {heads}")
+    hq, hk, dim = heads
+    page = 32
+    holes = [(0, s) for s in range(-(-total[0] // page))] + [(1, 0)]
+    table, cu, lengths, n, pages = kv.batch(new, total, page, seed=74, holes=holes)
+    pool = kv.cache(pages, hk, page, dim, seed=75)
+    kv.stain(pool, table, lengths)
+    q = torch.randn(n, hq, dim, generator=kv.gen(76)).to(torch.bfloat16)
+    clean = q.clone()
+    rows = [0, new[0] - 1, new[0], n - 1]  # the first two in a sequence without pages
+    for r in rows:
+        q[r, 1, 5] = value
+    on, where = kv.to(pool, cuda), (table.to(cuda), cu.to(cuda), lengths.to(cuda))
+    out = paged_attention(q.to(cuda), on, *where).cpu()
+    assert not out[: new[0]].any()
+    assert out[new[0], 1].isnan().all() and out[n - 1, 1].isnan().all()
+    want, bound = kv.oatt.attend(clean, kv.values(pool), table, cu, lengths)
+    out[rows, 1], want[rows, 1] = 0, 0
+    kv.assert_within(out, want, bound, q.dtype, "the others")
