@@ -416,8 +416,11 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
  * does a position past the table.  Rows of no sequence are padding: their
  * outputs are zero and nothing is stored for them.  `*_ld` and `*_hs` are the
  * pitches in elements from row to row and from head to head (multiples of 8;
- * rows 16-byte aligned).  Up to 2^30 tokens a table, 2^29 pages times heads and
- * 1024 heads; lengths past the table only move the positions. */
+ * rows 16-byte aligned).  Up to 2^30 tokens a table, 2^29 pages times kv heads,
+ * 1024 heads, 2^24 rows and 2^24 sequences; attention of fewer than 2^26 rows
+ * times heads and, over the sequences of few rows, fewer than 2^30 blocks of 16
+ * rows (times the heads of a kv head) by 256 tokens of the table.  Lengths past
+ * the table only move the positions. */
 
 /* Rotation of queries and keys by position and the append of keys and values.
  * cos_sin fp32 [positions, rotary] holds each position's rotary / 2 cosines,

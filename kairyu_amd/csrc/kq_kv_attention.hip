@@ -1083,8 +1083,9 @@ extern "C" int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dt
     set_error("%s: workspace of %zu bytes is too small", what, workspace_bytes);
     return KQ_EWORKSPACE;
   }
-  // threads of one launch, and blocks of all tiles
-  const int64_t blocks = (rows * (heads / kv_heads) / 16 + seqs) * ((table_width * page_size + 255) / 256);
+  // threads of one launch, and blocks of all tiles of 16 (beside large ones: of few rows a sequence)
+  const int64_t few_tiles = empty || !p.rows ? 0 : p.tiles ? seqs * (kFewItems / 16) : rows * (heads / kv_heads) / 16 + seqs;
+  const int64_t blocks = few_tiles * ((table_width * page_size + 255) / 256);
   if (rows * heads * 64 >= (1LL << 32) || p.big_tiles * p.splits * kv_heads * 512 >= (1LL << 32) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));

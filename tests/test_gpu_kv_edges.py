@@ -1,5 +1,5 @@
 """The paged 8-bit key/value cache on the GPU where it is easily wrong: angles without
-positions, caches without pages, queries that are not finite."""
+positions, caches without pages, queries that are not finite, prompts in wide tables."""
 
 from __future__ import annotations
 
@@ -76,3 +76,26 @@ def test_queries_that_are_not_finite_over_tokens_of_no_page(cuda, new, total, he
     want, bound = kv.oatt.attend(clean, kv.values(pool), table, cu, lengths)
     out[rows, 1], want[rows, 1] = 0, 0
     kv.assert_within(out, want, bound, q.dtype, "the others")
+
+
+@pytest.mark.parametrize("seqs", [1, 2])
+def test_many_rows_in_a_wide_table(cuda, seqs):
+    """Prompts of many rows and heads in a table for a million tokens, whose pages repeat."""
+    banner(f"kv attention many rows in a wide table, {seqs}")
+    rows, heads, dim, page, window = 65536, 64, 64, 16, 40
+    pool = kv.to(kv.cache(40, 1, page, dim, seed=77), cuda)
+    slots = (1 << 20) // page
+    table = (torch.arange(slots, device=cuda) % 40).to(torch.int32).expand(seqs, -1).contiguous()
+    bounds = [0, rows - 30, rows] if seqs == 2 else [0, rows]
+    cu = torch.tensor(bounds, dtype=torch.int32, device=cuda)
+    lengths = torch.tensor([bounds[s + 1] - bounds[s] + 70 for s in range(seqs)], dtype=torch.int32, device=cuda)
+    row = torch.randn(1, heads, dim, generator=kv.gen(78)).to(torch.bfloat16).to(cuda)
+    out = paged_attention(row.expand(rows, -1, -1), pool, table, cu, lengths, window=window)
+    torch.cuda.synchronize()
+    # a row by itself, as a sequence of that length
+    for r in (0, 1000, rows - 31, rows - 30, rows - 1):
+        s = seqs - 1 if r >= rows - 30 else 0
+        length = int(lengths[s]) - (bounds[s + 1] - r) + 1
+        near = (length - 64) // page if length > 64 else 0  # pages that the window touches, and their tokens
+        kv.check_attention(out[r: r + 1], row, pool, table[:1, near: near + 8], torch.tensor([0, 1], dtype=torch.int32),
+                           torch.tensor([length - near * page], dtype=torch.int32), f"row {r}", window=window)
