@@ -450,7 +450,9 @@ int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k
  * them, or (causal) those up to its own position, at most the last `window`
  * where that is positive.  A row that sees none is zero.  Stored values must not
  * be NaN codes in slots that hold tokens (slots past a sequence's end may hold
- * anything); NaN keys make the rows that see them NaN and no other.  out
+ * anything); NaN keys make the rows that see them NaN and no other.  Tokens
+ * count in full where the value scales that a row sees lie up to 2^100 apart
+ * (an append's are at least 2^-48, so with values of up to 2^60).  out
  * [rows, heads, dim].  |scale| at most 2^100.  Workspace:
  * kq_kv_attention_workspace_size bytes, of the call's own.
  * Replaces the paged attention backends (kairyu/engine/core/attention/) for an

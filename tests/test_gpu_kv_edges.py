@@ -1,5 +1,6 @@
 """The paged 8-bit key/value cache on the GPU where it is easily wrong: angles without
-positions, caches without pages, queries that are not finite, prompts in wide tables."""
+positions, caches without pages, queries that are not finite, prompts in wide tables,
+pages that nobody holds, value scales far apart."""
 
 from __future__ import annotations
 
@@ -99,3 +100,39 @@ def test_many_rows_in_a_wide_table(cuda, seqs):
         near = (length - 64) // page if length > 64 else 0  # pages that the window touches, and their tokens
         kv.check_attention(out[r: r + 1], row, pool, table[:1, near: near + 8], torch.tensor([0, 1], dtype=torch.int32),
                            torch.tensor([length - near * page], dtype=torch.int32), f"row {r}", window=window)
+
+
+@pytest.mark.parametrize("page,heads", [(16, (8, 2, 64)), (32, (8, 2, 64)), (64, (8, 2, 64)), (16, (7, 1, 128)), (32, (4, 4, 128)),
+                                        (128, (7, 1, 128)), (16, (3, 1, 256)), (32, (3, 1, 256))], ids=str)
+@pytest.mark.parametrize("new,total", [([1, 1, 2], [600, 303, 1100]), ([150, 1, 70], [600, 303, 2100]), ([90, 9], [5000, 133])],
+                         ids=str)
+def test_a_first_page_that_nobody_holds(cuda, new, total, page, heads):
+    """Loads for tokens that are not there must not take the cache's first page, all NaN."""
+    banner(f"kv attention first page {page} {heads} {new}")
+    hq, hk, dim = heads
+    table, cu, lengths, n, pages = kv.batch(new, total, page, seed=79)
+    table = torch.where(table >= 0, table + 1, table)
+    table[0, 1], table[0, total[0] // page - 1], table[1, 0] = -1, pages + 1, -5
+    pool = kv.cache(pages + 1, hk, page, dim, seed=80)
+    kv.stain(pool, table, lengths)
+    for scales in pool[2:]:
+        scales[0] = math.nan
+    q = torch.randn(n, hq, dim, generator=kv.gen(81)).to(torch.bfloat16)
+    out = paged_attention(q.to(cuda), kv.to(pool, cuda), table.to(cuda), cu.to(cuda), lengths.to(cuda))
+    torch.cuda.synchronize()
+    pool.k_scale[0], pool.v_scale[0] = 1, 1
+    kv.check_attention(out, q, pool, table, cu, lengths)
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [600, 303]), ([1, 1], [3000, 1303]), ([150, 70], [600, 303]), ([90], [5000])], ids=str)
+def test_value_scales_far_apart(cuda, new, total):
+    """Pages whose value scales lie 2^98 apart: those of small values add nothing to the
+    output and count in its denominator."""
+    banner(f"kv attention value scales {new} {total}")
+    table, cu, lengths, n, pages = kv.batch(new, total, 32, seed=82)
+    pool = kv.cache(pages, 2, 32, 128, seed=83)
+    pool.v_scale.copy_(torch.where(torch.rand(pool.v_scale.shape, generator=kv.gen(84)) < 0.5, 2.0**-48, 2.0**50))
+    q = (0.25 * torch.randn(n, 8, 128, generator=kv.gen(85))).to(torch.bfloat16)
+    out = paged_attention(q.to(cuda), kv.to(pool, cuda), table.to(cuda), cu.to(cuda), lengths.to(cuda))
+    torch.cuda.synchronize()
+    kv.check_attention(out, q, pool, table, cu, lengths)
