@@ -3,9 +3,11 @@
 ``block_norm`` runs what lies between a block's output projection and the next
 block's first one: the norm after the block, its gate and residual scale, the
 residual sum, and the norm before the next block, whose rows come out in 16 bits
-or already quantized as that projection's kernels take them.  Counterpart of the
-reference's RMS norm kernels (kairyu/kernels/rms_norm_gpu.py) next to this
-package's activation quantizers.
+or quantized as this package's activation quantizers lay them out.  The library's
+W8A8 and block-FP8 GEMM entries (``include/kairyu_quant.h``) take quantized rows and
+their scales; the module classes and packs take 16-bit rows and quantize them
+themselves.  Counterpart of the reference's RMS norm kernels
+(kairyu/kernels/rms_norm_gpu.py).
 """
 
 from __future__ import annotations
