@@ -434,9 +434,9 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
  * scale it has where it holds earlier tokens, which move to the new scale.  A
  * token whose rotated key or whose value has a non-finite element in a head is
  * stored there as a key of NaN codes, and those elements of its value as 0.  No
- * page may be written for two sequences by one call.  Replaces the rotary and
- * paged-write kernels (kairyu/kernels/rope_gpu.py, paged_kv_write_gpu.py) for
- * an 8-bit cache. */
+ * page may be written for two sequences, or two slots of one, by one call.
+ * Replaces the rotary and paged-write kernels (kairyu/kernels/rope_gpu.py,
+ * paged_kv_write_gpu.py) for an 8-bit cache. */
 int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld, int64_t k_hs,
                         const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
                         int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,

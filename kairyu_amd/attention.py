@@ -183,7 +183,8 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     key or value is not finite in a head is stored as a key of NaN codes there (with
     zeros for such elements of the value): rows that attend to it become NaN, and
     only they.  Tokens whose table entry is no page, or whose position is past the
-    table, are not stored.  No two sequences of a call may append to one page.
+    table, are not stored.  No two sequences of a call, nor two slots of one, may
+    append to one page.
 
     Heads may be strided views (``q``, ``k`` and ``v`` of one packed projection);
     rows that are not 16-byte aligned are copied first."""

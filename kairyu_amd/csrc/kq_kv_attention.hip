@@ -218,7 +218,7 @@ KQ_DEV void zero_padding(const AttendArgs& a, const KvBatch& batch, int head, in
 // Bound by HBM on long contexts: 3 x 131001 tokens on 8 kv heads of 128, 805 MB, take
 // 124 us (6.5 TB/s); 64 of up to 6000 on 4, 186 MB, 40 (4.6), where starting, the first
 // loads' latency and the last part's merge are 8 of them.  A single context of 700 tokens
-// takes 8 us, its three steps' latency.
+// takes 8-10 us, its three steps' latency.
 template <int D, int DT, int NT, int PP>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 3)
 kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -590,11 +590,13 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // share what a step widens, 8192 rows behind 12288 tokens took 1087 us and with four 1100,
 // but 1024 of 1024 42.7 and 31.6: fewer tiles fill the chip unevenly.)
 //
-// 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1080-1140 us, 1.0
-// PFLOP/s.  No unit bounds it alone: the matrix cores are busy for 48% of that, LDS for 53%,
-// the vector unit, with about 95 instructions a half step of 32 tokens, 16 of them
+// 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1097-1145 us, 1.0
+// PFLOP/s.  No unit bounds it alone: the matrix cores are busy for 47% of that, LDS for 52%,
+// the vector unit, with about 100 instructions a half step of 32 tokens, 16 of them
 // exponentials, for about half.  Widening and staging account for 27% of the time, the
 // products with the values for 20%, exponentials for 8% (copies timed without them).
+// Waves past a sequence's rows compute like the others: where rows are few, as long as
+// the longest tile (24 windows of 1024 tokens, heads of 64: 50 us, 35% of the waves empty).
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
 // are shared by the waves: they are widened once, keys to Q's type in rows of one
@@ -934,12 +936,18 @@ constexpr int64_t kAlone = 2048, kAloneTokens = 64;
 
 // rows * group up to which a sequence goes to tiles of 16 rows, which stream its
 // tokens once per tile (24 sequences behind 3000 tokens, 4 heads a kv head: 5 rows 65 us
-// either way; 15 rows 79 in large tiles, 113 in small ones)
+// either way; 15 rows 79 in large tiles, 113 in small ones).  That is for sequences that
+// fill the chip.  Few of them fall off at this limit, since large tiles are cut no finer
+// than 1024 tokens: one behind 1000, 4096 and 16384, 32 heads over 8 of 128, 8 rows 15, 18
+// and 31 us and 9 rows 27, 31 and 35; heads of 256, 8 over 1, 4 rows 22, 16 and 23 and
+// 8 rows 52, 58 and 60; four behind 16384 do not (8 rows 65, 9 rows 60).
 constexpr int kFewItems = 32;
 
 // Tokens up to which one workgroup reads a tile's whole: a second launch costs 4 us of host
 // time (16 contexts of up to 700 tokens on 8 kv heads 11.9 us whole, 13.1 shared out; 4 of
-// 1000 13.4 and 12.7)
+// 1000 13.4 and 12.7).  By the table's width, which is all that the host knows: in a table
+// for 32768 tokens those 16 contexts take 14.5 us instead of 11.1, six prompts of kAlone's
+// kind 82 instead of 71.
 constexpr int64_t kWhole = 1024;
 // ... and where a window makes the tiles alike and they fill the chip by themselves (64 single
 // tokens on 4 kv heads of 128, windows of 900, 1400 and 1900: 16.7, 21.5 and 25.7 us whole,
@@ -974,7 +982,8 @@ static Plan plan_with(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim
     p.big_tiles = (items + ends * (kBigRows - 1)) / kBigRows;
     // few tiles: cut their tokens until every workgroup slot has some, but not below 1024 each: a cut costs the
     // second launch and the partial sums' way through memory (32 heads over 8 of 128 channels, one sequence: 512 rows
-    // behind 4096 tokens 130 us whole, 70 cut; 1024 rows behind 8192 on 4 heads 250 and 166; 1024 rows of 1024 42 and 52)
+    // behind 4096 tokens 130 us whole, 70 cut; 1024 rows behind 8192 on 4 heads 250 and 166; 1024 rows of 1024 42 and
+    // 52; fewer rows than these would want finer cuts, see kFewItems)
     const int64_t most = std::max<int64_t>(span_of(kBigRows) / 1024, 1);
     p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, tile_slots(dim) / std::max<int64_t>(1, p.big_tiles * kv_heads)));
     span = span_of(std::max<int64_t>(kFewItems / group, 1));
