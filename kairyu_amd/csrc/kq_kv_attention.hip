@@ -45,9 +45,12 @@ constexpr int kBigRows = 128;  // rows of a large tile, 32 a wave
 // log2 of the largest weight.  Tiles of 16 have the exact maximum.  Tiles of 128 move theirs
 // when a lane's 16 weights of a half step may add up to more than fp16 holds, 128 of 2^9: a
 // larger lift leaves less room and moves it more often (8192 rows behind 12288 tokens and 24
-// windows of heads of 64 with lifts of 5, 8, 9, 10 and 11: 1120, 1127, 1133, 1135 and 1142 us,
-// 50.9, 52.3, 53.2, 53.5 and 55.0; none at all 1106 and 51.3, with weights that are lost).
+// windows of heads of 64 with lifts of 5, 8, 9 and 11: 1092, 1101, 1107 and 1119 us, 52.5, 53.2,
+// 54.8 and 57.3; weights of at most one, which are lost, 1080 and 51.0).
 constexpr float kLift = 15.0f, kBigLift = 9.0f, kBigMost = 65504.0f;
+// Beyond this magnitude of the maximum, log2 of a value scale and the lift drown in a score's
+// last bits: tiles of 128 then form each exponent from the rounded score, as tiles of 16 do.
+constexpr float kCoarse = 0x1p20f;
 
 // e4m3 codes widened to the 16-bit type of a product (exact in both)
 template <int DT>
@@ -397,12 +400,12 @@ kv_attend_rows_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t*
       for (int j = 0; j < OT; ++j) o[j] *= keep;
       top = m;
     }
-    const float base = top == -__builtin_inff() ? 0.0f : top - kLift;
+    const float base = top == -__builtin_inff() ? 0.0f : top;
     u32x4 p[NT / 2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[i][r] = __builtin_amdgcn_exp2f(w[i][r] - base);
+      for (int r = 0; r < 4; ++r) w[i][r] = __builtin_amdgcn_exp2f((w[i][r] - base) + kLift);  // (the difference exact: at most kLift)
       sum = fmaf(w[i][0] + w[i][1] + w[i][2] + w[i][3], inv_v[i / (NT / PP)], sum);
       p[i >> 1][2 * (i & 1)] = pack_act2(w[i][0], w[i][1], KQ_DTYPE_F16);
       p[i >> 1][2 * (i & 1) + 1] = pack_act2(w[i][2], w[i][3], KQ_DTYPE_F16);
@@ -590,13 +593,13 @@ KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // share what a step widens, 8192 rows behind 12288 tokens took 1087 us and with four 1100,
 // but 1024 of 1024 42.7 and 31.6: fewer tiles fill the chip unevenly.)
 //
-// 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1097-1145 us, 1.0
+// 8192 rows behind 12288 tokens, 32 heads over 8 of 128, 1.1 TFLOP: 1105-1150 us, 1.0
 // PFLOP/s.  No unit bounds it alone: the matrix cores are busy for 47% of that, LDS for 52%,
 // the vector unit, with about 100 instructions a half step of 32 tokens, 16 of them
 // exponentials, for about half.  Widening and staging account for 27% of the time, the
 // products with the values for 20%, exponentials for 8% (copies timed without them).
 // Waves past a sequence's rows compute like the others: where rows are few, as long as
-// the longest tile (24 windows of 1024 tokens, heads of 64: 50 us, 35% of the waves empty).
+// the longest tile (24 windows of 1024 tokens, heads of 64: 53 us, 35% of the waves empty).
 //
 // The same transposed products as above on 32x32x16 MFMAs.  A step's keys and values
 // are shared by the waves: they are widened once, keys to Q's type in rows of one
@@ -612,7 +615,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   constexpr int OT = D / 32;            // output tiles
   constexpr int KLD = 2 * D + 16;       // bytes of a key's row
   constexpr int VLD = 2 * 64 + 16;      // bytes of a d's row of values
-  constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale + kBigLift, its inverse)
+  constexpr int KB = 64 * KLD, VB = D * VLD, BUF = KB + VB + 64;  // ... and 4 x (scale, log2 of the value scale, its inverse)
   constexpr int KC = D / 64;            // 16-byte chunks of one token's key a thread moves
   constexpr int VY = D / 16, VC = VY / 4;  // bytes and dwords of each of four tokens' values a thread moves
   constexpr int LD = D + 4;
@@ -737,7 +740,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     }
     if (lane == 0) {
       float* dst = (float*)(buf + KB + VB) + 4 + wave;
-      dst[0] = __builtin_amdgcn_logf(sc_v) + kBigLift;
+      dst[0] = __builtin_amdgcn_logf(sc_v);
       dst[4] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
     }
   };
@@ -747,6 +750,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
   float top = -__builtin_inff(), sum = 0.0f;
+  float ref = -kBigLift;  // what exponents are formed against: top (0 while there is none) - kBigLift
 
   // the keys of 32 tokens, half i of the step in buf, and their scores
   u32x4 kx[KS];
@@ -785,7 +789,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
   // Scores of the next 32 tokens with the weights of these between the products, an MFMA to
   // every pair or two: the order is pinned.
   auto dots_under_weights = [&](f32x16& next, f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    const f32x2_t shift_v = {lv[0] - base_of(top), lv[1] - base_of(top)};
+    const f32x2_t shift_v = {lv[0] - ref, lv[1] - ref};
 #pragma unroll
     for (int e = 0; e < 16; ++e) next[e] = 0.0f;
 #pragma unroll
@@ -798,7 +802,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
     asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l));  // (not behind the branch that may compute them anew)
   };
   auto limit = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
-    if (__ballot(l > kBigMost * fminf(iv[0], iv[1]) || top == -__builtin_inff()) == 0) return;
+    if (__ballot(l > kBigMost * fminf(iv[0], iv[1]) || !(fabsf(top) <= kCoarse)) == 0) return;
     // a 16-token tile's scale is positive, so its largest score is its largest dot product's
     float x[2] = {w[0], w[8]};
 #pragma unroll
@@ -806,7 +810,7 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
       x[0] = fmaxf(x[0], w[e]);
       x[1] = fmaxf(x[1], w[8 + e]);
     }
-    float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1])) - kBigLift;
+    float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
     const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
     const float keep = __builtin_amdgcn_exp2f(top - base_of(m));
@@ -814,9 +818,16 @@ kv_attend_tiles_kernel(AttendArgs a, KvCache cache, KvBatch batch, const int32_t
 #pragma unroll
     for (int j = 0; j < OT; ++j) o[j] *= keep;
     top = m;
-    const f32x2_t shift_v = {lv[0] - base_of(top), lv[1] - base_of(top)};
+    const float base = base_of(m);
+    ref = base - kBigLift;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, w, l);
+    for (int i = 0; i < 8; ++i) {  // (exact differences, of at most kBigLift with it)
+      const int g = i >> 2;
+      const float u = __builtin_amdgcn_exp2f((fmaf(w[2 * i], ks[g], lv[g]) - base) + kBigLift);
+      const float v = __builtin_amdgcn_exp2f((fmaf(w[2 * i + 1], ks[g], lv[g]) - base) + kBigLift);
+      l = i == 0 ? (u + v) * iv[g] : fmaf(u + v, iv[g], l);
+      p[i >> 2][i & 3] = pack_act2(u, v, KQ_DTYPE_F16);
+    }
   };
   u32x4 vx[2][OT];
   auto read_values = [&](const char* buf, int i) {

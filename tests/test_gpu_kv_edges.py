@@ -136,3 +136,37 @@ def test_value_scales_far_apart(cuda, new, total):
     out = paged_attention(q.to(cuda), kv.to(pool, cuda), table.to(cuda), cu.to(cuda), lengths.to(cuda))
     torch.cuda.synchronize()
     kv.check_attention(out, q, pool, table, cu, lengths)
+
+
+@pytest.mark.parametrize("size", [10, 20, 24, 25, 26, 27, 28, 40, 100])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (7, 1, 128), (3, 1, 256)], ids=str)
+@pytest.mark.parametrize("new,total", [([1, 1], [600, 303]), ([1, 1], [3000, 1303]), ([150, 70], [600, 303]), ([90], [5000])], ids=str)
+def test_scores_of_any_size(cuda, new, total, heads, size):
+    """Rows whose largest score, times 2^size, stands far above the others take its value,
+    or the mean of two in one page, however coarse fp32 is up there."""
+    banner(f"kv attention scores of 2^{size} {heads} {new}")
+    hq, hk, dim = heads
+    table, cu, lengths, n, pages = kv.batch(new, total, 32, seed=86)
+    pool = kv.cache(pages, hk, 32, dim, seed=87)
+    g = kv.gen(88)
+    pool.k.view(torch.uint8).zero_()
+    pool.k[..., 3] = (torch.rand(pool.k.shape[:3], generator=g) * 300 - 200).to(kv.E4M3)  # at most 104
+    pool.k_scale.fill_(1.0)
+    want = torch.zeros(n, hq, dim, dtype=torch.float64)
+    for s, (rows, length) in enumerate(zip(new, total)):
+        first = length - rows  # token 40 for the first row, then 72 and 73 of one page, alike
+        for token, code in ((40, 384.0), (72, 448.0), (73, 448.0)):
+            pool.k[int(table[s, token // 32]), :, token % 32, 3] = torch.tensor(code).to(kv.E4M3)
+        for r in range(rows):
+            at = [72, 73] if first + r >= 73 else [72] if first + r == 72 else [40] if first + r >= 40 else None
+            assert at is not None
+            value = torch.stack([pool.v[int(table[s, t // 32]), :, t % 32].double()
+                                 * pool.v_scale[int(table[s, t // 32])].double()[:, None] for t in at]).mean(0)
+            want[int(cu[s]) + r] = value.repeat_interleave(hq // hk, 0)
+    q = torch.zeros(n, hq, dim, dtype=torch.bfloat16)
+    q[..., 3] = 2.0 ** size
+    kv.stain(pool, table, lengths)
+    out = paged_attention(q.to(cuda), kv.to(pool, cuda), table.to(cuda), cu.to(cuda), lengths.to(cuda))
+    torch.cuda.synchronize()
+    # one weight or two alike, exact but for the weights' and the quotient's roundings
+    kv.assert_within(out, want, 2.0**-10 * want.abs(), q.dtype)
