@@ -42,7 +42,9 @@ PAGE_SIZES = (16, 32, 64, 128)
 
 class PagedKvCache(NamedTuple):
     """Codes ``[pages, kv_heads, page_size, head_dim]`` and fp32 scales
-    ``[pages, kv_heads]`` of keys and values; an element is ``code * scale``."""
+    ``[pages, kv_heads]`` of keys and values; an element is ``code * scale``.  The
+    append writes powers of two; scales of the caller's own must be positive and
+    finite (a page of zeros too), and values' codes not NaN."""
 
     k: torch.Tensor
     v: torch.Tensor
