@@ -406,7 +406,8 @@ int kq_moe_routed_block_fp8_experts(const void* logits, int logits_dtype, int no
 /* ------------------------------------------- paged e4m3 key/value cache
  * k_cache and v_cache are e4m3 [pages, kv_heads, page_size, dim] and their
  * scales fp32 [pages, kv_heads], positive and finite where tokens are held: a
- * stored element is code * scale.  Page size 16, 32, 64 or 128 tokens, dim 64, 128 or 256.  Rows [cu[s], cu[s + 1]) of the
+ * stored element is code * scale.  Page size 16, 32, 64 or 128 tokens, dim 64,
+ * 128 or 256.  Rows [cu[s], cu[s + 1]) of the
  * packed activations are sequence s's new tokens, the last ones of its
  * lengths[s] tokens (new ones included); token t lies in page
  * table[s][t / page_size].  cu int32 [seqs + 1], lengths int32 [seqs], table
