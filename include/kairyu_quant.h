@@ -446,6 +446,17 @@ int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k
                         const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
                         const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream);
 
+/* The same with the positions that rows turn by given: at int32 [rows] (drafted
+ * tokens that branch); one before or past the table turns to NaN.  Keys and values
+ * are stored in the slots all the same.  at null: kq_kv_rotate_append. */
+int kq_kv_rotate_append_at(const int32_t* at, const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld,
+                           int64_t k_hs, const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
+                           int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                           float* v_scale, int64_t pages, int64_t page_size, const int32_t* table, int64_t table_ld,
+                           int64_t table_width, const int32_t* cu, const int32_t* lengths, int64_t seqs,
+                           const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
+                           const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream);
+
 /* out[r, h] = sum_t softmax_t(scale * q[r, h] . k_t) v_t over the tokens t that
  * row r sees in its sequence's pages, kv head h / (heads / kv_heads): all of
  * them, or (causal) those up to its own position, at most the last `window`
@@ -466,6 +477,82 @@ int kq_kv_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_
                     void* workspace, size_t workspace_bytes, void* stream);
 size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size,
                                       int64_t table_width, int64_t seqs);
+
+/* Attention of drafted tokens, rows [cu[s], cu[s + 1]) and the last tokens of
+ * their sequence as above: row r sees the tokens before the sequence's new rows
+ * (with a positive window those past max(positions[r], first new slot) - window)
+ * and the new token j where bit j % 32 of word j / 32 of mask [rows, words] (int32,
+ * up to 32 words) is set.  A row whose position is negative sees nothing, and a row
+ * that sees nothing is zero.  What kq_kv_attention says of values, scales, NaN keys
+ * and ranges holds here (blocks: of all sequences, of 16, 32 or 64 rows).
+ * Workspace: kq_kv_tree_attention_workspace_size bytes, of the call's own. */
+int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
+                         int64_t kv_heads, int64_t dim, const uint8_t* k_cache, const uint8_t* v_cache,
+                         const float* k_scale, const float* v_scale, int64_t pages, int64_t page_size,
+                         const int32_t* table, int64_t table_ld, int64_t table_width, const int32_t* cu,
+                         const int32_t* lengths, int64_t seqs, const int32_t* mask, int64_t words,
+                         const int32_t* positions, float scale, int64_t window, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t kq_kv_tree_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size,
+                                           int64_t table_width, int64_t seqs);
+
+/* ------------------------------------------- drafted tokens that branch
+ * Rows are a batch's new tokens as above, at most `most` <= 1024 of a sequence.
+ * parents int32 [rows]: a row's parent, counted from its sequence's first row and
+ * before the row itself (anything else: a root, which follows the context). */
+
+/* mask int32 [rows, ceil(most / 32)]: a row's own bit and its ancestors', with a
+ * positive window those at most window - 1 above it; positions int32 [rows]: the
+ * context's length plus the depth.  Rows of no sequence, those at or past `most` and
+ * those before the first token: empty masks and position -1. */
+int kq_draft_tree(const int32_t* parents, int64_t rows, const int32_t* cu, const int32_t* lengths, int64_t seqs,
+                  int64_t most, int64_t window, int32_t* mask, int32_t* positions, void* stream);
+
+/* The greedy walk: from a sequence's first row to the lowest child whose token is
+ * the target of the row it is at.  tokens, targets [rows] int32, or int64 (wide);
+ * kept int32 [seqs, most] (the rows walked along, -1 behind them), counts int32
+ * [seqs], following [seqs] (of the tokens' type): the last one's target, or -1. */
+int kq_draft_accept(const void* tokens, const void* targets, int wide, const int32_t* parents, int64_t rows,
+                    const int32_t* cu, int64_t seqs, int64_t most, int32_t* kept, int32_t* counts, void* following,
+                    void* stream);
+
+/* ------------------------------------------- pages that sequences share
+ * `caches` is a host array of 4 device addresses a layer: k_cache, v_cache,
+ * k_scale, v_scale, of up to 4096 layers alike in shape (read during the call). */
+
+/* Kept new tokens move behind their context in every layer: new row kept[s, i] of
+ * sequence s to slot lengths[s] - rows of s + i, for i < counts[s]; new_lengths [seqs]
+ * are the lengths then.  kept int32 [seqs, most], most <= 1024.  A sequence's kept
+ * tokens end before the first that is not one of its (first 1024) rows, not above the
+ * one before it, or whose slot, old or new, is in no page; more rows than tokens: none
+ * are kept.  A page that tokens move into gets the largest scale that the page of any
+ * token it then holds had, and its codes are rounded to it once. */
+int kq_kv_keep_tokens(const uint64_t* caches, int64_t layers, int64_t pages, int64_t kv_heads, int64_t page_size,
+                      int64_t dim, const int32_t* table, int64_t table_ld, int64_t table_width, const int32_t* cu,
+                      const int32_t* lengths, int64_t seqs, const int32_t* kept, int64_t most, const int32_t* counts,
+                      int32_t* new_lengths, void* stream);
+
+/* Page targets[i] becomes a copy of page sources[i], codes and scales, in every
+ * layer, for i < count; pairs that name no page, or one twice, do nothing.  No page
+ * may be a target twice, or a target and a source. */
+int kq_kv_copy_pages(const uint64_t* caches, int64_t layers, int64_t pages, int64_t kv_heads, int64_t page_size,
+                     int64_t dim, const int32_t* sources, const int32_t* targets, int64_t count, void* stream);
+
+/* Rows go on as other rows.  holders int32 [pages] counts the table entries that
+ * name a page (0: free) and is brought up to date.  New row j of new_table [rows,
+ * table_width] continues row parents[j] (outside [0, seqs): an empty row) with its
+ * length: pages full of tokens are shared; those of the next `room` tokens are the
+ * parent's where no other entry names them and j is the first with that parent, else
+ * the lowest pages free before the call, in the order of rows and slots, and a
+ * half-filled page's tokens are copied in every layer; entries behind are -1 (room 0: a
+ * half-filled page is shared).  missing [1]: pages that there were too few; their
+ * entries are -1.  Workspace: kq_kv_fork_workspace_size bytes, of the call's own. */
+int kq_kv_fork_sequences(const uint64_t* caches, int64_t layers, int64_t pages, int64_t kv_heads, int64_t page_size,
+                         int64_t dim, int32_t* holders, const int32_t* table, int64_t table_ld, int64_t table_width,
+                         const int32_t* lengths, int64_t seqs, const int32_t* parents, int64_t rows, int64_t room,
+                         int32_t* new_table, int32_t* new_lengths, int32_t* missing, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t kq_kv_fork_workspace_size(int64_t seqs, int64_t rows, int64_t table_width, int64_t page_size, int64_t room);
 
 /* The norms around a decoder block, rows of `hidden` <= 32768 elements:
  * r = residual + residual_scale * gate * (x / rms(x) * (offset + post)) and

@@ -104,11 +104,30 @@ _SIGNATURES: dict[str, list] = {
         _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
         _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I, _P, _P, _F, _P, _P,
     ],
+    "kq_kv_rotate_append_at": [
+        _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
+        _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I, _P, _P, _F, _P, _P,
+    ],
     "kq_kv_attention": [
         _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
         _F, _I, _I64, _P, _P, _SZ, _P,
     ],
     "kq_kv_attention_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "kq_kv_tree_attention": [
+        _P, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
+        _P, _I64, _P, _F, _I64, _P, _P, _SZ, _P,
+    ],
+    "kq_kv_tree_attention_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "kq_draft_tree": [_P, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _P],
+    "kq_draft_accept": [_P, _P, _I, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P],
+    "kq_kv_keep_tokens": [
+        _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P,
+    ],
+    "kq_kv_copy_pages": [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P],
+    "kq_kv_fork_sequences": [
+        _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P,
+    ],
+    "kq_kv_fork_workspace_size": [_I64, _I64, _I64, _I64, _I64],
     "kq_block_norm": [
         _P, _I, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _I64, _F, _P, _F, _F, _I, _P, _P, _P, _P,
     ],
@@ -147,7 +166,9 @@ def _load() -> ctypes.CDLL:
                           "kq_w8a8_swiglu_workspace_size": ctypes.c_size_t,
                           "kq_block_fp8_workspace_size": ctypes.c_size_t,
                           "kq_moe_workspace_size": ctypes.c_size_t,
-                          "kq_kv_attention_workspace_size": ctypes.c_size_t}.get(name, ctypes.c_int)
+                          "kq_kv_attention_workspace_size": ctypes.c_size_t,
+                          "kq_kv_tree_attention_workspace_size": ctypes.c_size_t,
+                          "kq_kv_fork_workspace_size": ctypes.c_size_t}.get(name, ctypes.c_int)
         _lib = lib
         return lib
 

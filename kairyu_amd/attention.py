@@ -10,6 +10,8 @@ codes with one power-of-two scale per page and head:
   Qwen3's per-head norms, if given) and stores keys and values, one launch.
 * :func:`paged_attention` attends to the cache: single tokens, prompts, chunks
   of prompts and any mix of them in one ragged batch.
+* :func:`tree_attention` attends with drafted tokens that branch, each seeing the
+  tokens before all drafts and its own ancestors (``kairyu_amd/drafts.py``).
 
 :meth:`QuantLinearPack.attend` runs them behind a pack's projection.  A batch is
 given by ``cu_rows [S + 1]`` (sequence ``s`` has rows ``cu_rows[s]`` up to
@@ -33,11 +35,12 @@ import torch
 
 from kairyu_amd.kernels import kv_cache_hip as hip
 
-__all__ = ["PagedKvCache", "paged_attention", "rotary_table", "rotate_append"]
+__all__ = ["DraftTree", "PagedKvCache", "paged_attention", "rotary_table", "rotate_append", "tree_attention"]
 
 E4M3 = torch.float8_e4m3fn
 HEAD_DIMS = (64, 128, 256)
 PAGE_SIZES = (16, 32, 64, 128)
+MOST_NODES = 1024  # drafted tokens of one sequence
 
 
 class PagedKvCache(NamedTuple):
@@ -67,6 +70,17 @@ class PagedKvCache(NamedTuple):
     @property
     def page_size(self) -> int:
         return self.k.shape[2]
+
+
+class DraftTree(NamedTuple):
+    """Drafted tokens of a batch's rows (:func:`kairyu_amd.drafts.draft_tree`, or the
+    caller's own): ``mask [R, words]`` int32, whose bit ``j % 32`` of word ``j // 32``
+    says that the row sees its sequence's ``j``-th new token (itself among them), and
+    ``positions [R]`` int32, the place of each in its own continuation; a row whose
+    position is negative sees nothing."""
+
+    mask: torch.Tensor
+    positions: torch.Tensor
 
 
 def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0,
@@ -157,6 +171,27 @@ def check_scores(scale: float | None, causal: bool, window: int, dim: int) -> fl
     return scale
 
 
+def _check_positions(positions: torch.Tensor, rows: int, device: torch.device) -> None:
+    if positions.shape != (rows,) or positions.dtype is not torch.int32 or not positions.is_contiguous():
+        raise ValueError(f"positions must be contiguous int32 [{rows}], got {positions.dtype} {tuple(positions.shape)}")
+    if positions.device != device:
+        raise RuntimeError(f"positions must be on {device}; found {positions.device}")
+
+
+def check_tree(tree: DraftTree, rows: int, device: torch.device) -> int:
+    """Words of a row's mask; what attention refuses of a tree."""
+
+    mask, positions = tree
+    _check_positions(positions, rows, device)
+    if mask.dim() != 2 or mask.shape[0] != rows or mask.dtype is not torch.int32 or not mask.is_contiguous():
+        raise ValueError(f"mask must be contiguous int32 [{rows}, words], got {mask.dtype} {tuple(mask.shape)}")
+    if not 1 <= mask.shape[1] <= MOST_NODES // 32:
+        raise ValueError(f"mask must have 1 to {MOST_NODES // 32} words a row, got {mask.shape[1]}")
+    if mask.device != device:
+        raise RuntimeError(f"mask must be on {device}; found {mask.device}")
+    return mask.shape[1]
+
+
 def _refuse_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -168,7 +203,7 @@ def _refuse_grad(*tensors) -> None:
 def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKvCache, block_table: torch.Tensor,
                   cu_rows: torch.Tensor, lengths: torch.Tensor, cos_sin: torch.Tensor | None = None, *,
                   interleaved: bool = False, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
-                  eps: float = 1e-6) -> torch.Tensor:
+                  eps: float = 1e-6, positions: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate ``q [R, Hq, D]`` and ``k [R, Hkv, D]`` by their positions, store the
     keys and ``v [R, Hkv, D]`` in the cache, and return the rotated queries.
 
@@ -177,7 +212,10 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     lie half that width apart or, ``interleaved``, next to each other.  None
     rotates nothing.  ``q_norm`` / ``k_norm [D]``, if given, are the weights of an
     RMS norm of each head before the rotation.  A position past the table makes
-    its queries and keys NaN.
+    its queries and keys NaN.  ``positions [R]`` int32, if given, says where rows turn
+    instead of their slots (drafted tokens that branch, :class:`DraftTree`; a
+    negative one is past the table); keys and values are stored in the slots all the
+    same.
 
     A page's scale is the smallest power of two that holds what this call stores in
     it within e4m3's 448, and no smaller than the scale the page has if it holds
@@ -207,11 +245,14 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     for norm in (q_norm, k_norm):
         if norm is not None and (norm.shape != (dim,) or norm.dtype != q.dtype or norm.device != q.device):
             raise ValueError(f"head norm weights must be [{dim}] of the queries' dtype and device")
+    if positions is not None:
+        _check_positions(positions, shape[0], q.device)
     _refuse_grad(q, k, v, q_norm, k_norm)
     if not q.is_cuda:
-        return _rotate_append_plain(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps)
+        return _rotate_append_plain(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps,
+                                    positions)
     return hip.rotate_append(q, k, v, shape, cache, cache_shape, block_table, cu_rows, lengths, cos_sin, interleaved, q_norm,
-                             k_norm, eps)
+                             k_norm, eps, positions)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Tensor, cu_rows: torch.Tensor,
@@ -232,6 +273,24 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Ten
     return hip.attention(q, shape, cache, cache_shape, block_table, cu_rows, lengths, scale, causal, window)
 
 
+def tree_attention(q: torch.Tensor, cache: PagedKvCache, block_table: torch.Tensor, cu_rows: torch.Tensor,
+                   lengths: torch.Tensor, tree: DraftTree, *, scale: float | None = None, window: int = 0) -> torch.Tensor:
+    """Attention of drafted tokens ``q [R, Hq, D]``, stored as their sequences' last
+    ones: each sees the tokens before its sequence's new ones (from ``position -
+    window`` on, exclusive, where ``window`` is positive) and those new ones that its
+    mask names.  Heads, scores and the result are :func:`paged_attention`'s; a row that
+    sees no token is zero."""
+
+    cache_shape = _check_cache(cache)
+    shape = _check_batch(q, cache, cache_shape, block_table, cu_rows, lengths)
+    scale = check_scores(scale, True, window, shape[2])
+    words = check_tree(tree, shape[0], q.device)
+    _refuse_grad(q)
+    if not q.is_cuda:
+        return _paged_attention_plain(q, cache, block_table, cu_rows, lengths, scale, True, window, tree)
+    return hip.tree_attention(q, shape, cache, cache_shape, block_table, cu_rows, lengths, scale, tree, words, window)
+
+
 # ------------------------------------------------------------- plain forms
 def _sequences(rows: int, cache: PagedKvCache, table, cu_rows, lengths):
     """(sequence, first row, rows, position of the first row, tokens that the table
@@ -250,7 +309,7 @@ def _head_norm(x, weight, eps):
 
 def _rotated(x, cos_sin, positions, interleaved):
     r = cos_sin.shape[1]
-    inside = (positions < cos_sin.shape[0])[:, None, None]
+    inside = ((positions >= 0) & (positions < cos_sin.shape[0]))[:, None, None]
     angles = cos_sin[positions.clamp(0, max(cos_sin.shape[0] - 1, 0))][:, None] if cos_sin.shape[0] else x.new_zeros(1, 1, r)
     cos, sin = angles.chunk(2, -1)
     if interleaved:
@@ -267,14 +326,14 @@ def _power_of_two_scale(amax: torch.Tensor) -> torch.Tensor:
     return torch.ldexp(torch.ones_like(amax), e - 9 + (m > 0.875).to(e.dtype))
 
 
-def _rotate_append_plain(q, k, v, cache, table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps):
+def _rotate_append_plain(q, k, v, cache, table, cu_rows, lengths, cos_sin, interleaved, q_norm, k_norm, eps, given=None):
     page, pages = cache.page_size, cache.k.shape[0]
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     for s, row, n, first, tokens in _sequences(q.shape[0], cache, table, cu_rows, lengths):
         skip = max(-first, 0)  # rows before the first token
         if n <= skip:
             continue
-        positions = torch.arange(first + skip, first + n)
+        positions = torch.arange(first + skip, first + n) if given is None else given[row + skip: row + n].long()
         part = [x[row + skip: row + n].to(torch.float32) for x in (q, k, v)]
         if q_norm is not None:
             part[0] = _head_norm(part[0], q_norm, eps)
@@ -309,7 +368,22 @@ def _rotate_append_plain(q, k, v, cache, table, cu_rows, lengths, cos_sin, inter
     return out
 
 
-def _paged_attention_plain(q, cache, table, cu_rows, lengths, scale, causal, window):
+def _tree_seen(tree, row, n, first, tokens, window):
+    """Whether each of a sequence's rows sees each of its tokens."""
+
+    positions, words = tree.positions[row: row + n].long()[:, None], tree.mask[row: row + n].long()
+    token = torch.arange(tokens)
+    node = (token - first).expand(n, -1)
+    word = node >> 5
+    bit = words.gather(1, word.clamp(0, words.shape[1] - 1)) >> (node & 31) & 1
+    drafted = (node >= 0) & (word < words.shape[1]) & (bit == 1)
+    context = node < 0
+    if window:
+        context = context & (token > positions.clamp(min=first) - window)
+    return (positions >= 0) & (drafted | context)
+
+
+def _paged_attention_plain(q, cache, table, cu_rows, lengths, scale, causal, window, tree=None):
     heads, kv_heads, pages, page = q.shape[1], cache.k.shape[1], cache.k.shape[0], cache.page_size
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     for s, row, n, first, tokens in _sequences(q.shape[0], cache, table, cu_rows, lengths):
@@ -325,9 +399,11 @@ def _paged_attention_plain(q, cache, table, cu_rows, lengths, scale, causal, win
         position = torch.arange(first, first + n)[:, None]
         token = torch.arange(tokens)
         seen = there.expand(n, -1)
-        if causal:
+        if tree is not None:
+            seen = seen & _tree_seen(tree, row, n, first, tokens, window)
+        elif causal:
             seen = seen & (token <= position)
-        if window:
+        if window and tree is None:
             seen = seen & (token > position - window)
         x = q[row: row + n].to(torch.float32).unflatten(1, (kv_heads, heads // kv_heads))
         z = torch.einsum("nhgd,htd->hgnt", x, k) * scale

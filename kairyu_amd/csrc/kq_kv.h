@@ -153,7 +153,19 @@ struct KvLanes {
 // A value of the whole wave in a scalar register (quotients come out of the vector unit).
 KQ_DEV int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Host checks that append and attention share; set_error and a status on failure.
+// Four codes of stored tokens on a coarser scale: code * ratio (below 1), rounded again;
+// NaN codes stay.
+KQ_DEV uint32_t move4(uint32_t w, float ratio) {
+  uint32_t nan = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if ((w >> (8 * e) & 0x7fu) == 0x7fu) nan |= 0xffu << (8 * e);
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), true);
+  return (pack4_e4m3(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio) & ~nan) | (w & nan);
+}
+KQ_DEV u32x4 move16(u32x4 w, float ratio) { return u32x4{move4(w[0], ratio), move4(w[1], ratio), move4(w[2], ratio), move4(w[3], ratio)}; }
+
+// Host checks that the cache's entries share; set_error and a status on failure.
 int kv_check(const char* what, int dtype, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
              int64_t page_size, int64_t pages, int64_t seqs, int64_t table_width, int64_t table_ld);
 

@@ -29,6 +29,7 @@ struct AppendArgs {
   uint16_t* q_out;           // [rows][heads][D]
   const float* cos_sin;      // [positions][rotary]: cos, then sin
   int64_t positions;
+  const int32_t* at;         // [rows], or null: a row turns by its slot
   const uint16_t* q_norm;
   const uint16_t* k_norm;
   float eps;
@@ -70,13 +71,13 @@ KQ_DEV Pairing pairing(int u, const AppendArgs& a) {
   return p;
 }
 
-// cos and sin of the thread's 8 angles at a position; NaN past the table
+// cos and sin of the thread's 8 angles at a position; NaN before and past the table
 struct Angles {
   float co[8], si[8];
 };
 KQ_DEV Angles angles_at(const Pairing& p, int pos, const AppendArgs& a) {
   Angles g;
-  const bool there = pos < a.positions;
+  const bool there = pos >= 0 && pos < a.positions;
   const float* at = a.cos_sin + (int64_t)(there ? pos : 0) * a.rotary + p.angle;
   const int half = a.rotary >> 1;
 #pragma unroll
@@ -159,18 +160,6 @@ KQ_DEV u32x2 encode8(const float v[8], float inv) {
   return w;
 }
 
-// Four codes of earlier tokens on a coarser scale: code * ratio (below 1), rounded again;
-// NaN codes stay.
-KQ_DEV uint32_t move4(uint32_t w, float ratio) {
-  uint32_t nan = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if ((w >> (8 * e) & 0x7fu) == 0x7fu) nan |= 0xffu << (8 * e);
-  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(w & ~nan), true);
-  return (pack4_e4m3(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio) & ~nan) | (w & nan);
-}
-KQ_DEV u32x4 move16(u32x4 w, float ratio) { return u32x4{move4(w[0], ratio), move4(w[1], ratio), move4(w[2], ratio), move4(w[3], ratio)}; }
-
 // Workgroups [0, page_units): one page of one sequence and one kv head each, its new
 // tokens in registers (NCH pairs of chunks a thread, keys and values), so that the scale
 // is known before a code is written and each row is read once.  The others: query rows,
@@ -220,7 +209,7 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
       raw[i][1] = *(const u32x4*)(at + 8 * p.c1);
     }
     Angles g;
-    if (p.turned) g = angles_at(p, max(pos, 0), a);
+    if (p.turned) g = angles_at(p, a.at != nullptr ? a.at[row] : max(pos, 0), a);
 #pragma unroll
     for (int i = 0; i < HPT; ++i) {
       float x[2][8];
@@ -285,7 +274,7 @@ kv_append_kernel(AppendArgs a, KvCache cache, KvBatch batch, int dtype) {
     widen(raw[i][2], dtype, v[i][0]);
     widen(raw[i][3], dtype, v[i][1]);
     Angles g;
-    if (p.turned) g = angles_at(p, pos, a);
+    if (p.turned) g = angles_at(p, a.at != nullptr ? a.at[q.row0 + (pos - q.first)] : pos, a);
     if (a.k_norm != nullptr) head_norm<D>(p, a.k_norm, a.eps, dtype, k[i]);
     turn(p, g, a.interleaved, k[i]);
     int ok = finite8(k[i][0]) && finite8(k[i][1]) && finite8(v[i][0]) && finite8(v[i][1]);
@@ -430,14 +419,15 @@ static void pick_heads(const AppendArgs& a, const KvCache& c, const KvBatch& b, 
 
 using namespace kq;
 
-extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld, int64_t k_hs,
-                                   const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
-                                   int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
-                                   float* v_scale, int64_t pages, int64_t page_size, const int32_t* table, int64_t table_ld,
-                                   int64_t table_width, const int32_t* cu, const int32_t* lengths, int64_t seqs,
-                                   const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
-                                   const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream) {
-  const char* what = "kq_kv_rotate_append";
+extern "C" int kq_kv_rotate_append_at(const int32_t* at, const void* q, int64_t q_ld, int64_t q_hs, const void* k,
+                                      int64_t k_ld, int64_t k_hs, const void* v, int64_t v_ld, int64_t v_hs, int dtype,
+                                      int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, uint8_t* k_cache,
+                                      uint8_t* v_cache, float* k_scale, float* v_scale, int64_t pages, int64_t page_size,
+                                      const int32_t* table, int64_t table_ld, int64_t table_width, const int32_t* cu,
+                                      const int32_t* lengths, int64_t seqs, const float* cos_sin, int64_t positions,
+                                      int64_t rotary, int interleaved, const void* q_norm, const void* k_norm, float eps,
+                                      void* q_out, void* stream) {
+  const char* what = at != nullptr ? "kq_kv_rotate_append_at" : "kq_kv_rotate_append";
   int rc = kv_check(what, dtype, rows, heads, kv_heads, dim, page_size, pages, seqs, table_width, table_ld);
   if (rc) return rc;
   // (a table without positions has no address, but turns: every position is past it)
@@ -461,6 +451,7 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   a.q_out = (uint16_t*)q_out;
   a.cos_sin = cos_sin;
   a.positions = positions;
+  a.at = at;
   a.rotary = turns ? (int)rotary : 0;
   a.interleaved = interleaved;
   a.q_norm = (const uint16_t*)q_norm;
@@ -486,4 +477,17 @@ extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, co
   else
     pick_heads<256>(a, c, b, dtype, st);
   return check_launch(what);
+}
+
+extern "C" int kq_kv_rotate_append(const void* q, int64_t q_ld, int64_t q_hs, const void* k, int64_t k_ld, int64_t k_hs,
+                                   const void* v, int64_t v_ld, int64_t v_hs, int dtype, int64_t rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                                   float* v_scale, int64_t pages, int64_t page_size, const int32_t* table, int64_t table_ld,
+                                   int64_t table_width, const int32_t* cu, const int32_t* lengths, int64_t seqs,
+                                   const float* cos_sin, int64_t positions, int64_t rotary, int interleaved,
+                                   const void* q_norm, const void* k_norm, float eps, void* q_out, void* stream) {
+  return kq_kv_rotate_append_at(nullptr, q, q_ld, q_hs, k, k_ld, k_hs, v, v_ld, v_hs, dtype, rows, heads, kv_heads, dim,
+                                k_cache, v_cache, k_scale, v_scale, pages, page_size, table, table_ld, table_width, cu,
+                                lengths, seqs, cos_sin, positions, rotary, interleaved, q_norm, k_norm, eps, q_out,
+                                stream);
 }

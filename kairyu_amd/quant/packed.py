@@ -276,16 +276,18 @@ class QuantLinearPack:
     def attend(self, hidden: torch.Tensor, cache, block_table: torch.Tensor, cu_rows: torch.Tensor,
                lengths: torch.Tensor, cos_sin: torch.Tensor | None = None, *, scale: float | None = None,
                causal: bool = True, window: int = 0, interleaved: bool = False, q_norm: torch.Tensor | None = None,
-               k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+               k_norm: torch.Tensor | None = None, eps: float = 1e-6, tree=None) -> torch.Tensor:
         """What the output projection of a decoder layer takes, from a (q, k, v)
         pack's input: the projections, the rotation of queries and keys and the
         append of keys and values to ``cache``, and attention over it
         (:func:`kairyu_amd.attention.rotate_append` and
         :func:`~kairyu_amd.attention.paged_attention`, whose arguments these are).
         ``hidden [..., K]`` holds the batch's rows in order; returns ``[...,
-        q_features]``."""
+        q_features]``.  With a ``tree`` (:class:`~kairyu_amd.attention.DraftTree`) the rows
+        are drafted tokens that branch: they turn by its positions, and
+        :func:`~kairyu_amd.attention.tree_attention` attends."""
 
-        from kairyu_amd.attention import check_scores, paged_attention, rotate_append
+        from kairyu_amd.attention import check_scores, check_tree, paged_attention, rotate_append, tree_attention
 
         heads, dim = cache.k.shape[1], cache.k.shape[3]
         widths = self._out_features
@@ -295,11 +297,18 @@ class QuantLinearPack:
         if torch.is_grad_enabled() and hidden.requires_grad:
             raise RuntimeError("attend is for inference: the hidden states require a gradient")
         check_scores(scale, causal, window, dim)  # (before anything is stored)
+        if tree is not None:
+            if not causal:
+                raise ValueError("a tree of drafted tokens says what its rows see: causal must not be False")
+            check_tree(tree, hidden.shape[:-1].numel(), hidden.device)
         with torch.no_grad():
             q, k, v = (part.reshape(-1, part.shape[-1]).unflatten(-1, (-1, dim)) for part in self(hidden))
             q = rotate_append(q, k, v, cache, block_table, cu_rows, lengths, cos_sin, interleaved=interleaved,
-                              q_norm=q_norm, k_norm=k_norm, eps=eps)
-            out = paged_attention(q, cache, block_table, cu_rows, lengths, scale=scale, causal=causal, window=window)
+                              q_norm=q_norm, k_norm=k_norm, eps=eps, positions=None if tree is None else tree.positions)
+            if tree is None:
+                out = paged_attention(q, cache, block_table, cu_rows, lengths, scale=scale, causal=causal, window=window)
+            else:
+                out = tree_attention(q, cache, block_table, cu_rows, lengths, tree, scale=scale, window=window)
         return out.reshape(*hidden.shape[:-1], widths[0])
 
     def swiglu(self, hidden: torch.Tensor) -> torch.Tensor:

@@ -97,9 +97,10 @@ def append(q, k, v, cache, table, cu, lengths, cos_sin=None, interleaved=False, 
     return out, new
 
 
-def attend(q, cache, table, cu, lengths, scale=None, causal=True, window=0):
+def attend(q, cache, table, cu, lengths, scale=None, causal=True, window=0, seen_by=None):
     """``(o, bound)`` in fp64: attention, and what a kernel may be off by before its
-    output's own rounding.
+    output's own rounding.  ``seen_by(row, n, first, tokens)`` says in place of
+    ``causal`` and ``window`` which tokens a sequence's rows see.
 
     With weights ``p = exp(z - max)``, ``A = sum p |v| / sum p``:
 
@@ -131,9 +132,11 @@ def attend(q, cache, table, cu, lengths, scale=None, causal=True, window=0):
         at = at.clamp(0, pages - 1)
         position, token = torch.arange(first, first + n)[:, None], torch.arange(tokens)[None]
         seen = there[None].expand(n, -1).clone()
-        if causal:
+        if seen_by is not None:
+            seen &= seen_by(row, n, first, tokens)
+        elif causal:
             seen &= token <= position
-        if window:
+        if window and seen_by is None:
             seen &= token > position - window
         seen = seen.repeat_interleave(group, 0)  # [n * group, tokens]
         for h in range(kv_heads):
