@@ -53,8 +53,15 @@ struct TreeDeal {
   }
 };
 
-// Words `at` of a row's mask with all ones before it: tokens before the new ones are seen.
-KQ_DEV uint32_t mask_word(const uint32_t* mask, int words, int at) { return at < 0 ? ~0u : at < words ? mask[at] : 0u; }
+// A row's mask with all ones before it, for the tokens before the new ones, and none behind.
+// The load is always in range and may be on its way long before the word is asked for.
+KQ_DEV uint32_t load_word(const uint32_t* mask, int words, int at) { return mask[min(max(at, 0), words - 1)]; }
+KQ_DEV uint32_t word_at(uint32_t loaded, int words, int at) { return at < 0 ? ~0u : at < words ? loaded : 0u; }
+// 32 bits from bit `shift` of two words on.
+KQ_DEV uint32_t bits_at(uint32_t lo, uint32_t hi, int shift) { return (uint32_t)(((uint64_t)hi << 32 | lo) >> (shift & 31)); }
+
+// Bits of tokens 0..31 from the n-th on.
+KQ_DEV uint32_t tokens_from(int n) { return n <= 0 ? ~0u : n >= 32 ? 0u : ~0u << n; }
 
 // One workgroup: its run of blocks of one kv head, tile by tile; its four waves take a
 // tile's steps of 16 * NT tokens in turn, each for all of the tile's 16 * MT columns, so that
@@ -64,8 +71,8 @@ KQ_DEV uint32_t mask_word(const uint32_t* mask, int words, int at) { return at <
 // (l % 16, l / 16) holds scores of columns c of the MT tiles for tokens 4b..4b+3 of each 16,
 // which are what it hands over as its part of P^T.  Loads go from memory to registers through
 // resources of one page's tile that end at the sequence's last token.
-template <int D, int DT, int NT, int PP, int MT>
-__global__ void __launch_bounds__(256, D * MT <= 64 ? 3 : D * MT <= 256 ? 2 : 1)
+template <int D, int DT, int NT, int PP, int MT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : D * MT <= 64 ? 3 : D * MT <= 256 ? 2 : 1)
 kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
                const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
   constexpr int KS = D / 32;   // MFMA steps along a key
@@ -74,13 +81,13 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
   constexpr int ST = 16 * NT;  // tokens of a step
   constexpr int TW = 16 * MT;
   constexpr int LD = D + 4;
-  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * LD];
+  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * LD];
   const int lane = lane_id(), wave = scalar(wave_id()), c = lane & 15, b = lane >> 4;
   const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
   const int head = (int)blockIdx.y;
 
-  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 256);
   const KvLanes lanes(batch, shift);
+  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 64 * WAVES);
   const TreeDeal<TW> deal{a, group};
   const int run = deal.run(lanes), run_end = ((int)blockIdx.x + 1) * run;
   int block = (int)blockIdx.x * run;
@@ -157,7 +164,7 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
         }
     }
   };
-  auto begin_part = [&] {
+  auto begin_loads = [&] {
     hi = q.tokens;
     part_blocks = min(blocks - within, run_end - block);
     const int begin = deal.first(q) * 64 + (within << (6 + a.block_shift));
@@ -176,19 +183,36 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
       bits[m] = a.mask + (int64_t)(q.row0 + row) * a.words;
       from[m] = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) + 1 - a.window, 0), max(q.first, 0)) : 0;
       most_from = max(most_from, (uint32_t)from[m]);
+      // (columns past the rows compute the first one's again, and are not stored)
+      const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) qf[m][i] = u32x4{0, 0, 0, 0};
-      if (real) {
-        const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) qf[m][i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1)) ^ a.q_sign;
-      }
+      for (int i = 0; i < KS; ++i) qf[m][i] = *(const u32x4*)(src + 64 * (i >> 1) + 16 * b + 8 * (i & 1)) ^ a.q_sign;
     }
     lo_all = (int)wave_max_u32_dpp(most_from);
     place(t);
     load_keys(t);
     load_values(t);
-    pages_of(t + 4 * ST);
+    pages_of(t + WAVES * ST);
+  };
+
+  // a step's words of the masks, a step ahead, where it is not seen whole
+  int last;
+  uint32_t word[MT][NT / 2 + 1];
+  auto words_of = [&](int t) {
+    if (t + ST <= last) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int g = 0; g <= NT / 2; ++g) word[m][g] = load_word(bits[m], a.words, ((t - q.first) >> 5) + g);
+  };
+  auto begin_part = [&] {
+    begin_loads();
+    last = min(q.first, q.tokens);  // (steps that end at or before it are seen whole, but for a window)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int g = 0; g <= NT / 2; ++g) word[m][g] = 0;
+    words_of(lo + ST * wave);
   };
 
   f32x4 o[MT][OT];
@@ -224,22 +248,26 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
           for (int r = 0; r < 4; ++r) w[m][i][r] = fmaf(w[m][i][r], scale, shift_v);
     }
     // the keys' registers take the next step's while this one goes on, the values' then theirs
-    place(t + 4 * ST);
-    load_keys(t + 4 * ST);
-    pages_of(t + 8 * ST);
-    if (t < lo_all || t + ST > q.first) {
+    place(t + WAVES * ST);
+    load_keys(t + WAVES * ST);
+    pages_of(t + 2 * WAVES * ST);
+    if (t < lo_all || t + ST > last) {
+      const int node = t - q.first, at = node >> 5;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const int token = t + 16 * i + 4 * b, node = token - q.first, at = node >> 5;
-          const uint64_t both = (uint64_t)mask_word(bits[m], a.words, at + 1) << 32 | mask_word(bits[m], a.words, at);
-          const uint32_t seen = (uint32_t)(both >> (node & 31));
+        for (int g = 0; g < NT / 2; ++g) {  // 32 tokens
+          const int token = t + 32 * g;
+          uint32_t seen = bits_at(word_at(word[m][g], a.words, at + g), word_at(word[m][g + 1], a.words, at + g + 1), node);
+          seen = (seen & tokens_from(from[m] - token) & ~tokens_from(q.tokens - token)) >> (4 * b);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (token + r < from[m] || token + r >= q.tokens || !(seen >> r & 1)) w[m][i][r] = -__builtin_inff();
+          for (int e = 0; e < 8; ++e) {
+            const bool sees = seen & (1u << (16 * (e >> 2) + (e & 3)));
+            w[m][2 * g + (e >> 2)][e & 3] = sees ? w[m][2 * g + (e >> 2)][e & 3] : -__builtin_inff();
+          }
         }
     }
+    words_of(t + WAVES * ST);
     u32x4 p[MT][NT / 2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -285,7 +313,7 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
           for (int m = 0; m < MT; ++m) o[m][4 * d + j] = mfma16<KQ_DTYPE_F16>(value, p[m][g], o[m][4 * d + j]);
         }
       }
-    load_values(t + 4 * ST);
+    load_values(t + WAVES * ST);
   };
   // Whether a column sees any token of this part that is there (its sum is NaN).
   auto sees_any = [&](int m) {
@@ -293,7 +321,9 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
     if (from[m] == 0x7fffffff) return false;
     for (int t = max(max(q.first, 0), lo); t < hi; ++t) {
       const int node = t - q.first;
-      if ((mask_word(bits[m], a.words, node >> 5) >> (node & 31) & 1) && any_there(pages, cache.pages, t, t + 1, shift)) return true;
+      if ((word_at(load_word(bits[m], a.words, node >> 5), a.words, node >> 5) >> (node & 31) & 1) &&
+          any_there(pages, cache.pages, t, t + 1, shift))
+        return true;
     }
     return false;
   };
@@ -307,7 +337,7 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
       top[m] = -__builtin_inff();
       sum[m] = 0.0f;
     }
-    for (int t = lo + ST * wave; t < hi; t += 4 * ST) step(t);
+    for (int t = lo + ST * wave; t < hi; t += WAVES * ST) step(t);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       sum[m] = column_sum(sum[m]);
@@ -350,17 +380,17 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
         mine[D + 1] = sum[m];
       }
       meet();
-      for (int i = (int)threadIdx.x; i < 16 * (D / 2); i += 256) {
+      for (int i = (int)threadIdx.x; i < 16 * (D / 2); i += 64 * WAVES) {
         const int col = i / (D / 2), d = 2 * (i - col * (D / 2));
         const int it = old_tile * TW + 16 * m + col;
         if (it >= old.rows * group) break;
         float most = -__builtin_inff();
 #pragma unroll
-        for (int v = 0; v < 4; ++v) most = fmaxf(most, lds[(v * 16 + col) * LD + D]);
+        for (int v = 0; v < WAVES; ++v) most = fmaxf(most, lds[(v * 16 + col) * LD + D]);
         const float base = most == -__builtin_inff() ? 0.0f : most;
         float ox = 0.0f, oy = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int v = 0; v < WAVES; ++v) {
           const float* part = lds + (v * 16 + col) * LD;
           const float f = __builtin_amdgcn_exp2f(part[D] - base);
           ox += part[d] * f;
@@ -384,23 +414,417 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
   }
 }
 
-// The parts of split tiles joined in the order of their tokens, one wave per row and query
-// head.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+KQ_DEV f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if (DT == KQ_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// log2 of the weights' lift in these tiles, whose maximum moves only when a lane's 16 weights
+// may add up to more than fp16 holds, and the maximum's magnitude from which exponents are
+// formed as exact differences.
+constexpr float kTileLift = 9.0f, kTileMost = 65504.0f, kCoarse = 0x1p20f;
+
+// One workgroup: its run of blocks of one kv head, tile by tile, tiles of 32 * CG columns.
+// A step's tokens, 32 for each of TG = 4 / CG groups, are widened once for the whole
+// workgroup, keys to Q's type in rows of one token and values to fp16 in rows of one d; a
+// wave takes 32 columns and 32 tokens of it on 32x32x16 MFMAs.  So a wave's columns
+// bound what LDS and the widening cost, and the workgroup's what memory does.
+//
+// The transposed products keep scores in the lane that hands them over as weights: lane
+// (c, h) = (l % 32, l / 32) holds column c's scores of tokens 8 i + 4 h + 0..3, i < 4, which
+// is the order (of each 16: 0-3, 8-11, then 4-7, 12-15) that the rows of values have.
+//
+// A step's weights are computed between the products of the next step's scores.  Codes
+// travel two steps ahead in registers, keys reach LDS a step before values, and
+// one barrier ends a step: it has read keys i + 1 and values i, and written keys i + 2 and
+// values i + 1 where keys i and values i - 1 were.
+template <int D, int DT, int CG>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
+                     const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
+  constexpr int TG = 4 / CG, ST = 32 * TG, TW = 32 * CG;
+  constexpr int KS = D / 16;            // MFMA steps along a key
+  constexpr int OT = D / 32;            // output tiles
+  constexpr int KLD = 2 * D + 16;       // bytes of a key's row: 16 more spread eight lanes' reads over all banks
+  constexpr int VLD = 2 * ST + 16;      // bytes of a d's row of values
+  constexpr int KB = ST * KLD, VB = D * VLD + 64;  // a buffer of keys; of values, and per 16 tokens scale, log2 of the value scale, its inverse
+  constexpr int KT = 256 / ST, KC = D / KT / 8;    // threads of a token's key, and 8-byte chunks of a thread
+  constexpr int VT = 1024 / ST, VY = D / VT;       // threads of four tokens' values, and each one's bytes of a token
+  constexpr int VC = VY < 4 ? 1 : VY / 4;
+  constexpr int LD = D + 4;
+  constexpr int MERGE = 4 * 32 * LD * 4;  // every wave's columns at the end of a part
+  constexpr int LDS = 2 * (KB + VB) > MERGE ? 2 * (KB + VB) : MERGE;
+  __shared__ __attribute__((aligned(16))) char smem[LDS];
+  const int wave = scalar(wave_id()), cg = wave % CG, tg = wave / CG;
+  const int lane = lane_id(), c = lane & 31, h = lane >> 5, tid = (int)threadIdx.x;
+  const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
+  const int head = (int)blockIdx.y;
+  const KvLanes lanes(batch, shift);
+  zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 256);
+  const TreeDeal<TW> deal{a, group};
+  const int run = deal.run(lanes), run_end = ((int)blockIdx.x + 1) * run;
+  int block = (int)blockIdx.x * run;
+  int within = 0;  // blocks of the sequence, then of the tile, before `block`
+  int s = lanes.find(block, within, deal);
+  if (s < 0) return;
+  KvSeq q = lanes[s];
+  int blocks = deal.blocks(q), tile = scalar(within / blocks);
+  within -= tile * blocks;
+
+  // what this thread moves: D / KT bytes of a token's key, VY of four tokens' values; a
+  // wave's tokens lie in one page.  Row R of the values is d = R % VT * VY + R / VT, so that
+  // neighbouring lanes write neighbouring rows.
+  const int k_tok = tid / KT, v_grp = tid / VT, v_c = tid % VT;
+  const int k_lane = (k_tok % (ST / 4)) * D + (tid % KT) * (D / KT), v_lane = 4 * (v_grp % (ST / 16)) * D + v_c * VY;
+  const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
+  const int tile_shift = shift + (D == 64 ? 6 : D == 128 ? 7 : 8);  // log2 of a page's bytes
+  const int in_page = (1 << shift) - 1;
+
+  while (true) {
+    const int item = tile * TW + cg * 32 + c;
+    const bool real = item < q.rows * group;
+    const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
+    const int pos = a.positions[q.row0 + row];
+    const uint32_t* bits = a.mask + (int64_t)(q.row0 + row) * a.words;
+    const int from = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) + 1 - a.window, 0), max(q.first, 0)) : 0;
+    const int part_blocks = min(blocks - within, run_end - block);
+    const int lo = deal.first(q) * 64 + (within << (6 + a.block_shift));
+    const int hi = (int)min((int64_t)q.tokens, (int64_t)lo + ((int64_t)part_blocks << (6 + a.block_shift)));
+    const int32_t* pages = table + (int64_t)s * batch.table_ld;
+    u32x4 qf[KS];  // (columns past the rows compute the first one's again, and are not stored)
+    const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h);
+
+    auto page_at = [&](int t) { return pages[min(t + ST / 4 * wave, max(hi - 1, 0)) >> shift]; };
+    struct Place {
+      int head_tile, size, off;
+    };
+    auto place_of = [&](int t, int page_) {
+      const int page = __builtin_amdgcn_readfirstlane(page_), at = t + ST / 4 * wave;
+      const bool there = page >= 0 && page < (int)cache.pages && at < hi;
+      Place p;
+      p.head_tile = (there ? page : 0) * cache.kv_heads + head;
+      p.size = there ? min(q.tokens - (at & ~in_page), in_page + 1) * D : 0;
+      p.off = (at & in_page) * D;
+      return p;
+    };
+    uint32_t kr[2][2 * KC], vr[2][4][VC];
+    float sc_k[2], sc_v[2];
+    auto fetch_k = [&](const Place& p, auto w) {
+      const i32x4 src = make_rsrc(cache.k + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
+      if constexpr (KC == 1) {
+        const i32x2 x = kq_rbl_v2i32(src, k_lane, p.off, 0);
+        kr[w][0] = (uint32_t)x[0], kr[w][1] = (uint32_t)x[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < KC / 2; ++i) {
+          const i32x4 x = kq_rbl_v4i32(src, k_lane + 16 * i, p.off, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kr[w][4 * i + e] = (uint32_t)x[e];
+        }
+      }
+    };
+    auto fetch_v = [&](const Place& p, auto w) {
+      const i32x4 src = make_rsrc(cache.v + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (VY == 2) {
+          vr[w][r][0] = (uint16_t)kq_rbl_i16(src, v_lane + r * D, p.off, 0);
+        } else if constexpr (VC == 1) {
+          vr[w][r][0] = (uint32_t)kq_rbl_i32(src, v_lane + r * D, p.off, 0);
+        } else if constexpr (VC == 2) {
+          const i32x2 x = kq_rbl_v2i32(src, v_lane + r * D, p.off, 0);
+          vr[w][r][0] = (uint32_t)x[0], vr[w][r][1] = (uint32_t)x[1];
+        } else {
+          const i32x4 x = kq_rbl_v4i32(src, v_lane + r * D, p.off, 0);
+#pragma unroll
+          for (int i = 0; i < VC; ++i) vr[w][r][i] = (uint32_t)x[i];
+        }
+      }
+      // (vector loads, which the barriers do not wait for; 0 where there is no page)
+      sc_k[w] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
+      sc_v[w] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
+    };
+    auto put_k = [&](char* buf, auto w) {
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+        *(u32x4*)(buf + k_tok * KLD + 2 * ((tid % KT) * (D / KT) + 8 * i)) = widen_codes<DT>(kr[w][2 * i], kr[w][2 * i + 1]);
+    };
+    auto put_v = [&](char* buf, auto w) {
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        const uint32_t in[4] = {vr[w][0][i], vr[w][1][i], vr[w][2][i], vr[w][3][i]};
+        uint32_t out[4];
+        transpose4(in, out);
+#pragma unroll
+        for (int j = 0; j < (VY < 4 ? VY : 4); ++j) {
+          const u32x2 x = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, false)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, true))};
+          *(u32x2*)(buf + ((4 * i + j) * VT + v_c) * VLD + 2 * v_pos) = x;
+        }
+      }
+      // (a page holds whole tiles of 16 tokens: where a wave moves 8, every other one says)
+      if (lane == 0 && (ST / 4 * wave) % 16 == 0) {
+        float* dst = (float*)(buf + D * VLD) + ST / 4 * wave / 16;
+        dst[0] = sc_k[w] > 0.0f ? sc_k[w] * a.scale : 1.0f;
+        dst[4] = __builtin_amdgcn_logf(sc_v[w]);
+        dst[8] = sc_v[w] > 0.0f ? __builtin_amdgcn_rcpf(sc_v[w]) : 0.0f;
+      }
+    };
+    f32x16 o[OT];
+#pragma unroll
+    for (int j = 0; j < OT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
+    float top = -__builtin_inff(), sum = 0.0f;
+    float ref = -kTileLift;  // what exponents are formed against: top (0 while there is none) - kTileLift
+
+    auto key_of = [&](const char* buf, int k) { return *(const u32x4*)(buf + (32 * tg + c) * KLD + 32 * k + 16 * h); };
+    auto value_of = [&](const char* buf, int k, int j) { return *(const u32x4*)(buf + (32 * j + c) * VLD + 64 * tg + 32 * k + 16 * h); };
+    // Weights by an earlier maximum, which only has to keep them from overflowing; l adds up
+    // the denominator's share in fp32, weights times 1 / value scale.
+    auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, f32x2_t iv, const f32x16& w, float& l) {
+      const int g = i >> 2;
+      const float x = __builtin_amdgcn_exp2f(fmaf(w[2 * i], ks[g], shift_v[g]));
+      const float y = __builtin_amdgcn_exp2f(fmaf(w[2 * i + 1], ks[g], shift_v[g]));
+      l = i == 0 ? (x + y) * iv[g] : fmaf(x + y, iv[g], l);
+      return pack_act2(x, y, KQ_DTYPE_F16);
+    };
+    auto base_of = [](float m) { return m == -__builtin_inff() ? 0.0f : m; };
+    // (a tile's scale is positive, so its largest score is its largest dot product's)
+    auto limit = [&](f32x2_t ks, f32x2_t lv, f32x2_t iv, const f32x16& w, u32x4 (&p)[2], float& l) {
+      if (__ballot(l > kTileMost * fminf(iv[0], iv[1]) || !(fabsf(top) <= kCoarse)) == 0) return;
+      float x[2] = {w[0], w[8]};
+#pragma unroll
+      for (int e = 1; e < 8; ++e) {
+        x[0] = fmaxf(x[0], w[e]);
+        x[1] = fmaxf(x[1], w[8 + e]);
+      }
+      float m = fmaxf(fmaf(x[0], ks[0], lv[0]), fmaf(x[1], ks[1], lv[1]));
+      const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+      m = fmaxf(top, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+      const float keep = __builtin_amdgcn_exp2f(top - base_of(m));
+      sum *= keep;
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[j] *= keep;
+      top = m;
+      const float base = base_of(m);
+      ref = base - kTileLift;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // (exact differences, of at most kTileLift with it)
+        const int g = i >> 2;
+        const float u = __builtin_amdgcn_exp2f((fmaf(w[2 * i], ks[g], lv[g]) - base) + kTileLift);
+        const float v = __builtin_amdgcn_exp2f((fmaf(w[2 * i + 1], ks[g], lv[g]) - base) + kTileLift);
+        l = i == 0 ? (u + v) * iv[g] : fmaf(u + v, iv[g], l);
+        p[i >> 2][i & 3] = pack_act2(u, v, KQ_DTYPE_F16);
+      }
+    };
+
+    char* const keys[2] = {smem, smem + KB};
+    char* const values[2] = {smem + 2 * KB, smem + 2 * KB + VB};
+    f32x16 x, y;
+    if (lo < hi) {
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
+      const int last = min(q.first, q.tokens);  // (steps that end at or before it are seen whole)
+      const int lo_all = (int)wave_max_u32_dpp((uint32_t)from);
+      Place at0 = place_of(lo, page_at(lo)), at1 = place_of(lo + ST, page_at(lo + ST));
+      fetch_k(at0, even);
+      fetch_v(at0, even);
+      fetch_k(at1, odd);
+      fetch_v(at1, odd);
+      int page2 = page_at(lo + 2 * ST), page3 = page_at(lo + 3 * ST), next_page = page_at(lo + 4 * ST);
+      put_k(keys[0], even);
+      put_v(values[0], even);
+      at0 = place_of(lo + 2 * ST, page2);
+      fetch_k(at0, even);
+      fetch_v(at0, even);
+      put_k(keys[1], odd);
+      Place ahead = place_of(lo + 3 * ST, page3);  // of the next values
+      fetch_k(ahead, odd);
+      meet();
+#pragma unroll
+      for (int i = 0; i < KS; ++i) qf[i] ^= a.q_sign;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) x = mfma32<DT>(key_of(keys[0], k), qf[k], x);
+      meet();
+      // a step's words of the mask, a step ahead
+      uint32_t word0 = 0, word1 = 0;
+      auto words_of = [&](int t) {
+        if (t + ST <= last) return;
+        const int at = (t + 32 * tg - q.first) >> 5;
+        word0 = load_word(bits, a.words, at);
+        word1 = load_word(bits, a.words, at + 1);
+      };
+      words_of(lo);
+      // step i of parity p: scores in `now`, the next step's go to `next`
+      auto step = [&](int t, f32x16& now, f32x16& next, auto p_) {
+        constexpr int p = decltype(p_)::value;
+        constexpr std::integral_constant<int, p> same{};
+        constexpr std::integral_constant<int, 1 - p> other{};
+        const char* scales = values[p] + D * VLD + 8 * tg;
+        const f32x2_t ks = *(const f32x2_t*)scales, lv = *(const f32x2_t*)(scales + 16), iv = *(const f32x2_t*)(scales + 32);
+        u32x4 kx[4];  // (four of the operands ahead)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) kx[k] = key_of(keys[1 - p], k);
+        if (t < lo_all || t + ST > last) {
+          const int token = t + 32 * tg, node = token - q.first, at = node >> 5;
+          const uint32_t seen = bits_at(word_at(word0, a.words, at), word_at(word1, a.words, at + 1), node) & tokens_from(from - token) &
+                                ~tokens_from(q.tokens - token);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) now[e] = seen >> (4 * h) & (1u << (8 * (e >> 2) + (e & 3))) ? now[e] : -__builtin_inff();
+        }
+        words_of(t + ST);
+        u32x4 w[2];
+        float l;
+        const f32x2_t shift_v = {lv[0] - ref, lv[1] - ref};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) next[e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          next = mfma32<DT>(kx[k & 3], qf[k], next);
+          if (k + 4 < KS) kx[k & 3] = key_of(keys[1 - p], k + 4);
+#pragma unroll
+          for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) w[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, now, l);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(l));  // (not behind the branch that may compute them anew)
+        u32x4 vx[2][OT];
+#pragma unroll
+        for (int j = 0; j < OT; ++j) vx[0][j] = value_of(values[p], 0, j);
+        limit(ks, lv, iv, now, w, l);
+#pragma unroll
+        for (int j = 0; j < OT; ++j) vx[1][j] = value_of(values[p], 1, j);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < OT; ++j) o[j] = mfma32<KQ_DTYPE_F16>(vx[k][j], w[k], o[j]);
+        sum += l;
+        put_k(keys[p], same);
+        put_v(values[1 - p], other);
+        fetch_v(ahead, other);
+        ahead = place_of(t + 4 * ST, next_page);
+        fetch_k(ahead, same);
+        next_page = page_at(t + 5 * ST);
+        meet();
+      };
+      for (int t = lo; t < hi; t += 2 * ST) {  // (a step past the end finds no page and adds nothing)
+        step(t, x, y, even);
+        step(t + ST, y, x, odd);
+      }
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (sum != sum) {
+      bool any = any_there(pages, cache.pages, max(from, lo), min(max(q.first, 0), hi), shift);
+      for (int t = max(max(q.first, 0), lo); !any && from != 0x7fffffff && t < hi; ++t) {
+        const int node = t - q.first;
+        any = (word_at(load_word(bits, a.words, node >> 5), a.words, node >> 5) >> (node & 31) & 1) &&
+              any_there(pages, cache.pages, t, t + 1, shift);
+      }
+      if (!any) {
+        sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < OT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
+      }
+    }
+    // The waves' columns meet in LDS in the order of d, and are added in the order of their
+    // tokens by threads that write whole rows.  Element e of tile j is row R = 32 j + 8 (e / 4) +
+    // 4 h + e % 4 of the values: N neighbouring d are elements e of all tiles, or e and e + 8.
+    constexpr int N = VT == 32 ? OT : 2 * OT;
+    float* mine = (float*)smem + (wave * 32 + c) * LD;
+#pragma unroll
+    for (int e = 0; e < 16 * OT / N; ++e) {
+      float v[N];
+#pragma unroll
+      for (int j = 0; j < OT; ++j) {
+        if constexpr (VT == 32) {
+          v[j] = o[j][e];
+        } else {
+          v[2 * j] = o[j][e];
+          v[2 * j + 1] = o[j][8 + e];
+        }
+      }
+      float* dst = mine + (8 * (e >> 2) + 4 * h + (e & 3)) * VY;
+      if constexpr (N == 2) {
+        *(f32x2_t*)dst = f32x2_t{v[0], v[1]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *(f32x4*)(dst + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+      }
+    }
+    if (h == 0) mine[D] = top, mine[D + 1] = sum;
+    meet();
+    const bool whole = part_blocks == blocks;
+    float* part = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (within == 0)) * TW) * LD;
+#pragma unroll 1
+    for (int i = tid; i < TW * (D / 4); i += 256) {
+      const int col = i / (D / 4), d = 4 * (i - col * (D / 4)), it = tile * TW + col;
+      if (it >= q.rows * group) break;
+      const float* from_ = (const float*)smem + col * LD;
+      float most = from_[D];
+#pragma unroll
+      for (int g = 1; g < TG; ++g) most = fmaxf(most, from_[g * TW * LD + D]);
+      f32x4 v = {0, 0, 0, 0};
+      float l = 0.0f;
+#pragma unroll
+      for (int g = 0; g < TG; ++g) {
+        const float f = TG == 1 ? 1.0f : __builtin_amdgcn_exp2f(from_[g * TW * LD + D] - base_of(most));
+        const f32x4 more = *(const f32x4*)(from_ + g * TW * LD + d);
+        l += from_[g * TW * LD + D + 1] * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += more[e] * f;
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees no token is zero)
+        const int rw = it / group;
+        uint16_t* dst = a.out + ((int64_t)(q.row0 + rw) * a.heads + head * group + (it - rw * group)) * D + d;
+        *(u32x2*)dst = u32x2{pack_act2(v[0] * inv, v[1] * inv, DT), pack_act2(v[2] * inv, v[3] * inv, DT)};
+      } else {
+        *(f32x4*)(part + (int64_t)col * LD + d) = v;
+        if (d == 0) *(f32x2_t*)(part + (int64_t)col * LD + D) = f32x2_t{most, l};
+      }
+    }
+    block += part_blocks;
+    within = 0;
+    if (block >= run_end) return;
+    if (++tile >= deal.tiles(q)) {
+      tile = 0;
+      do {
+        if (++s >= batch.seqs) return;
+        q = lanes[s];
+      } while (deal.tiles(q) == 0);
+      blocks = deal.blocks(q);
+    }
+    meet();  // (LDS is read to the end)
+  }
+}
+
+// The parts of split tiles joined in the order of their tokens: a workgroup takes COLS columns
+// of one tile, a thread four neighbouring d of each of E columns.
 template <int D, int DT, int TW>
 __global__ void __launch_bounds__(256)
 kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
-  constexpr int LD = D + 4, PER = D / 64;
+  constexpr int LD = D + 4, PER = D / 4, E = TW * PER >= 512 ? 2 : 1, COLS = 256 * E / PER;
   const int shift = cache.page_shift, group = scalar(a.heads / cache.kv_heads);
-  const int at = (int)blockIdx.x * 4 + scalar(wave_id());
+  const int head = (int)blockIdx.y, column0 = (int)blockIdx.z * COLS;
   const KvLanes lanes(batch, shift);
   const TreeDeal<TW> deal{a, group};
-  const int row = scalar(at / a.heads), qh = at - row * a.heads, head = scalar(qh / group);
-  if (row >= batch.rows) return;
-  int block = 0;  // blocks of the sequences before s
-  const int s = lanes.of_row(row, block, deal);
+  int tile;
+  const int s = lanes.find((int)blockIdx.x, tile, [&](const KvSeq& q) { return deal.tiles(q); });
   if (s < 0) return;
   const KvSeq q = lanes[s];
-  const int item = (row - q.row0) * group + (qh - head * group), tile = scalar(item / TW);
+  if (tile * TW + column0 >= q.rows * group) return;
+  int block = 0;  // blocks before the tile's
+  lanes.of_row(q.row0, block, deal);
   const int run = max(deal.run(lanes), 1), blocks = deal.blocks(q);
   block += tile * blocks;
   // (within the shares also where row bounds that go back make counts wrap)
@@ -408,34 +832,69 @@ kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
   const int chunks = min(max(scalar((block + blocks - 1) / run), x0), a.shares - 1) - x0 + 1;
   if (chunks == 1) return;  // written already
   // part 1 of the run it begins in, then part 0 of those behind
-  const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * TW + (item - tile * TW)) * LD;
+  const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * TW + column0) * LD;
   auto at_part = [&](int i) { return src + (i == 0 ? 0 : (int64_t)(2 * i - 1) * TW) * LD; };
-  float m = -__builtin_inff();
-  for (int i = lane_id(); i < chunks; i += 64) m = fmaxf(m, at_part(i)[D]);
-  m = wave_max(m);
-  const float base = m == -__builtin_inff() ? 0.0f : m;
-  float x[PER], l = 0.0f;
+  float m[E], l[E];
+  f32x4 x[E];
 #pragma unroll
-  for (int d = 0; d < PER; ++d) x[d] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < chunks; ++i) {
-    const float* p = at_part(i);
-    const float f = __builtin_amdgcn_exp2f(p[D] - base);
-    l += p[D + 1] * f;
-#pragma unroll
-    for (int d = 0; d < PER; ++d) x[d] += p[PER * lane_id() + d] * f;
+  for (int e = 0; e < E; ++e) {
+    m[e] = -__builtin_inff(), l[e] = 0.0f;
+    x[e] = f32x4{0, 0, 0, 0};
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* dst = a.out + ((int64_t)row * a.heads + qh) * D + PER * lane_id();
+  constexpr int U = 8 / E;  // parts on their way at once
+  for (int i0 = 0; i0 < chunks; i0 += U) {
+    f32x4 v[U][E];
+    f32x2_t has[U][E];  // a part's maximum and denominator
 #pragma unroll
-  for (int d = 0; d < PER; ++d) dst[d] = f32_to_out(x[d] * inv, DT);
+    for (int i = 0; i < U; ++i) {
+      if (i0 + i >= chunks) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = (int)threadIdx.x + 256 * e, col = at / PER;
+        const float* p = at_part(i0 + i) + col * LD;
+        has[i][e] = *(const f32x2_t*)(p + D);
+        v[i][e] = *(const f32x4*)(p + 4 * (at - col * PER));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (i0 + i >= chunks) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float most = fmaxf(m[e], has[i][e][0]), base = most == -__builtin_inff() ? 0.0f : most;
+        const float keep = __builtin_amdgcn_exp2f(m[e] - base), f = __builtin_amdgcn_exp2f(has[i][e][0] - base);
+        m[e] = most;
+        l[e] = l[e] * keep + has[i][e][1] * f;
+        x[e] = x[e] * keep + v[i][e] * f;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int at = (int)threadIdx.x + 256 * e, col = at / PER, item = tile * TW + column0 + col;
+    if (item >= q.rows * group) return;
+    const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+    const int row = item / group;
+    uint16_t* dst = a.out + ((int64_t)(q.row0 + row) * a.heads + head * group + (item - row * group)) * D + 4 * (at - col * PER);
+    *(u32x2*)dst = u32x2{pack_act2(x[e][0] * inv, x[e][1] * inv, DT), pack_act2(x[e][2] * inv, x[e][3] * inv, DT)};
+  }
 }
 
-// Tokens up to which one workgroup reads a tile's whole, which saves the second launch.
-constexpr int64_t kWhole = 1024;
+// Blocks of 16 columns and 256 tokens up to which the tiles are of 16 columns whatever the trees
+// are: a step of theirs is the shortest, and they fill the chip with the least (one tree of 64
+// rows x heads behind 4000 and 16000 tokens, 8 kv heads of 128: 19 and 27 us, in tiles of 64 28
+// and 39; one of 256 behind 4000 24 and 32; but 16 of up to 96 behind 3000 65, in tiles of 128 44).
+constexpr int64_t kFewBlocks = 2560;
+// Tokens up to which one workgroup reads a tile's whole and nothing is joined, where that leaves
+// tiles of 16 (one tree of 48 behind 900 tokens 13 us, cut 14; 48 of 64 behind up to 900, in tiles of
+// 64, 39 and 51), and under a window, which makes the tiles alike, where they fill the chip (24
+// windows of 1024, 16 heads of 64: 16 us whole, 23 cut).  By the table's width, which is all that
+// the host knows.
+constexpr int64_t kWhole = 1024, kWholeMany = 2048;
 
 struct TreePlan {
-  int columns;  // tiles of 16 that a wave holds at once
+  int columns;  // of a tile: 16 or 32 (a wave holds them all), 64 or 128 (the workgroup does)
+  int waves;    // of a workgroup
   int shares, block_shift;
   size_t part;  // bytes
 };
@@ -445,46 +904,74 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
                           int64_t seqs, int64_t window) {
   TreePlan p{};
   const int64_t items = rows * (heads / kv_heads), each = (items + std::max<int64_t>(seqs, 1) - 1) / std::max<int64_t>(seqs, 1);
-  p.columns = each <= 16 ? 1 : each <= 32 || dim == 256 ? 2 : 4;
-  const int64_t slots = 256 * (dim * p.columns <= 64 ? 3 : dim * p.columns <= 256 ? 2 : 1);
-  p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
   const int64_t tokens = width * page_size, span = window > 0 ? std::min(tokens, window + rows + 64) : tokens;
-  p.block_shift = 2;
-  const bool whole = span <= kWhole;
+  auto tiles = [&](int64_t columns) { return (items / columns + seqs) * kv_heads; };
+  if (tiles(16) * ((span + 255) / 256) <= kFewBlocks)
+    p.columns = 16;
+  else
+    p.columns = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+  const bool whole = (span <= kWhole && (p.columns == 16 || tiles(p.columns) >= 256)) ||
+                     (window > 0 && span <= kWholeMany && p.columns == 16 && tiles(16) >= 256);
+  // eight waves to a tile while there is at most one for a CU (four trees of 64 behind 900 tokens 14
+  // us, with four waves 19; 16 of them 26 and 24)
+  p.waves = whole && p.columns == 16 && tiles(16) <= 256 ? 8 : 4;
+  // workgroups that registers and LDS let a CU hold
+  const int64_t slots = 256 * (p.columns > 32 ? (dim == 256 ? 1 : 2) : p.waves == 8 ? 1 : dim * p.columns <= 1024 ? 3 : dim * p.columns <= 4096 ? 2 : 1);
+  p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
+  // blocks of 256 tokens, or of 512 where those still give every workgroup one: tiles are cut less
+  // often (one tree of 64 behind 16000 tokens 31 -> 27 us, 16 of up to 96 behind 3000 43 -> 39)
+  p.block_shift = tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
-  if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * 16 * p.columns * (dim + 4));
+  if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * p.columns * (dim + 4));
   return p;
 }
 
-template <int D, int DT, int NT, int PP, int MT>
-static void launch_columns(const TreeArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  hipLaunchKernelGGL((kv_tree_kernel<D, DT, NT, PP, MT>), dim3((unsigned)a.shares, (unsigned)c.kv_heads), dim3(256), 0, st, a, c,
-                     b, b.table, c.k_scale, c.v_scale);
-  if (a.part != nullptr)
-    hipLaunchKernelGGL((kv_tree_join_kernel<D, DT, 16 * MT>), dim3((unsigned)(((int64_t)b.rows * a.heads + 3) / 4)), dim3(256), 0,
-                       st, a, c, b);
+template <int D, int DT, int MT, int WAVES>
+static void launch_rows(const TreeArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  constexpr int NT = D == 256 || MT > 1 ? 2 : 4;  // (registers)
+  const int page = 1 << c.page_shift;
+  const dim3 grid((unsigned)a.shares, (unsigned)c.kv_heads);
+  if (page >= 16 * NT)
+    hipLaunchKernelGGL((kv_tree_kernel<D, DT, NT, 1, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, a, c, b, b.table, c.k_scale, c.v_scale);
+  else if (page == 8 * NT)
+    hipLaunchKernelGGL((kv_tree_kernel<D, DT, NT, 2, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, a, c, b, b.table, c.k_scale, c.v_scale);
+  else if constexpr (NT == 4)
+    hipLaunchKernelGGL((kv_tree_kernel<D, DT, NT, 4, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, a, c, b, b.table, c.k_scale, c.v_scale);
 }
 
-template <int D, int DT, int NT, int PP>
-static void launch_pages(const TreeArgs& a, const TreePlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  if (p.columns == 1)
-    launch_columns<D, DT, NT, PP, 1>(a, c, b, st);
-  else if (p.columns == 2)
-    launch_columns<D, DT, NT, PP, 2>(a, c, b, st);
-  else if constexpr (D < 256)
-    launch_columns<D, DT, NT, PP, 4>(a, c, b, st);
+template <int D, int DT, int CG>
+static void launch_tiles(const TreeArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  hipLaunchKernelGGL((kv_tree_tiles_kernel<D, DT, CG>), dim3((unsigned)a.shares, (unsigned)c.kv_heads), dim3(256), 0, st, a, c, b,
+                     b.table, c.k_scale, c.v_scale);
+}
+
+template <int D, int DT, int TW>
+static void launch_join(const TreeArgs& a, const KvCache& c, const KvBatch& b, hipStream_t st) {
+  if (a.part == nullptr) return;
+  constexpr int COLS = 1024 * (TW * D >= 2048 ? 2 : 1) / D;
+  const int64_t tiles = std::min<int64_t>((int64_t)b.rows * (a.heads / c.kv_heads) / TW + b.seqs, b.rows * (int64_t)a.heads);
+  hipLaunchKernelGGL((kv_tree_join_kernel<D, DT, TW>), dim3((unsigned)tiles, (unsigned)c.kv_heads, (TW + COLS - 1) / COLS), dim3(256),
+                     0, st, a, c, b);
 }
 
 template <int D, int DT>
 static void launch_tree(const TreeArgs& a, const TreePlan& p, const KvCache& c, const KvBatch& b, hipStream_t st) {
-  constexpr int NT = D == 256 ? 2 : 4;  // (registers)
-  const int page = 1 << c.page_shift;
-  if (page >= 16 * NT)
-    launch_pages<D, DT, NT, 1>(a, p, c, b, st);
-  else if (page == 8 * NT)
-    launch_pages<D, DT, NT, 2>(a, p, c, b, st);
-  else if constexpr (NT == 4)
-    launch_pages<D, DT, NT, 4>(a, p, c, b, st);
+  if (p.columns == 16) {
+    if (p.waves == 8)
+      launch_rows<D, DT, 1, 8>(a, c, b, st);
+    else
+      launch_rows<D, DT, 1, 4>(a, c, b, st);
+    launch_join<D, DT, 16>(a, c, b, st);
+  } else if (p.columns == 32) {
+    launch_rows<D, DT, 2, 4>(a, c, b, st);
+    launch_join<D, DT, 32>(a, c, b, st);
+  } else if (p.columns == 64) {
+    launch_tiles<D, DT, 2>(a, c, b, st);
+    launch_join<D, DT, 64>(a, c, b, st);
+  } else {
+    launch_tiles<D, DT, 4>(a, c, b, st);
+    launch_join<D, DT, 128>(a, c, b, st);
+  }
 }
 
 template <int D>
@@ -537,7 +1024,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
     return KQ_EWORKSPACE;
   }
   // threads of one launch, and blocks of all tiles
-  const int64_t tiles = empty ? 0 : rows * (heads / kv_heads) / (16 * p.columns) + seqs;
+  const int64_t tiles = empty ? 0 : rows * (heads / kv_heads) / p.columns + seqs;
   const int64_t blocks = tiles * ((table_width * page_size + 255) / 256);
   if (rows * heads * 64 >= (1LL << 32) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,

@@ -12,6 +12,7 @@ import kv_helpers as kv
 from gpu_helpers import banner
 from kairyu_amd.attention import DraftTree, PagedKvCache, paged_attention, rotary_table, rotate_append, tree_attention
 from kairyu_amd.drafts import accept_drafts, draft_tree, keep_tokens
+from kairyu_amd.kernels import kv_cache_hip as hip
 from kairyu_amd.pages import KvCaches, fork_sequences
 from kairyu_amd.quant.packed import QuantLinearPack
 from oracle import attention as oatt
@@ -262,6 +263,80 @@ def test_lengths_and_bounds_that_are_wrong_stay_in_range(cuda):
     torch.cuda.synchronize()
     out = tree_attention(q, pool, table, cu, lengths, tree)
     assert out.isfinite().all()
+
+
+def _columns(q, pool, table, lengths):
+    """Columns of the tiles that a call without a window runs in, from its scratch (0: none)."""
+    pages, kv_heads, page, dim = pool.k.shape
+    need = hip._tree_bytes(*q.shape[:2], kv_heads, dim, page, table.shape[1], lengths.shape[0])
+    return need // (8 * (dim + 4) * kv_heads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("batch", BATCHES)
+def test_attention_in_wide_tables(cuda, batch, heads, dtype):
+    """A table for a million tokens: tiles of as many columns as the trees have, cut along the
+    tokens where there are enough, and bounds that say nothing of the lengths."""
+    page = {64: 16, 128: 64, 256: 32}[HEADS[heads][2]]
+    banner(f"tree attention wide {batch} {heads} page {page} {dtype}")
+    q, pool, table, cu, lengths, tree, seen = _case(cuda, batch, heads, page, dtype, seed=21)
+    table = torch.nn.functional.pad(table, (0, (1 << 20) // page - table.shape[1]), value=-1)
+    out = tree_attention(q, pool, table, cu, lengths, tree)
+    torch.cuda.synchronize()
+    dh.check_attention(out, q, pool, table, cu, lengths, seen, tree.positions, batch)
+    assert not out[-2:].any()
+
+
+@pytest.mark.parametrize("group", [1, 3, 8], ids=lambda g: f"group {g}")
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_every_tile(cuda, dim, page, group):
+    """Trees of 13 and 40 rows, 13 to 320 rows x heads, in tiles of 16, 32, 64 and 128 columns;
+    whole ones, cut ones, holes and NaN queries among them."""
+    banner(f"tree attention tiles {dim} page {page} group {group}")
+    seen_columns = set()
+    for new, holes in (([13, 9], [(0, 1)]), ([40, 33], [(1, 0), (1, 3)])):
+        q, pool, table, cu, lengths, tree, seen = _case(cuda, (new, [2500, 700]), (2 * group, 2, dim), page, torch.bfloat16,
+                                                        seed=22, holes=holes)
+        q[3, 0], q[5, -1] = float("nan"), float("inf")
+        table = torch.nn.functional.pad(table, (0, (1 << 20) // page - table.shape[1]), value=-1)
+        shares = {64: {16: 768, 32: 512, 64: 512, 128: 512}, 128: {16: 512, 32: 512, 64: 512, 128: 512},
+                  256: {16: 512, 32: 256, 64: 256, 128: 256}}[dim]
+        need = _columns(q, pool, table, lengths)
+        seen_columns |= {c for c, s in shares.items() if c * (s // 2) == need}
+        out = tree_attention(q, pool, table, cu, lengths, tree)
+        torch.cuda.synchronize()
+        dh.check_attention(out, q, pool, table, cu, lengths, seen, tree.positions)
+    assert seen_columns >= {1: {16, 64}, 3: {64, 128}, 8: {128}}[group]
+
+
+@pytest.mark.parametrize("heads", [(4, 4, 64), (8, 4, 64), (16, 4, 64), (16, 4, 128), (8, 4, 128)], ids=str)
+@pytest.mark.parametrize("window", [7, 300, 1500])
+def test_attention_windows_in_every_tile(cuda, heads, window):
+    """Many trees under a window: tiles whole and cut, from 16 to 128 columns."""
+    banner(f"tree attention windows {heads} {window}")
+    new = [8 + (5 * i) % 19 for i in range(48)]
+    total = [n + (331 * i) % 2000 for i, n in enumerate(new)]
+    q, pool, table, cu, lengths, tree, seen = _case(cuda, (new, total), heads, 32, torch.float16, seed=23, window=window)
+    out = tree_attention(q, pool, table, cu, lengths, tree, window=window)
+    torch.cuda.synchronize()
+    dh.check_attention(out, q, pool, table, cu, lengths, seen, tree.positions, window=window)
+
+
+def test_attention_of_lengths_past_the_table(cuda):
+    """Tokens past the table are not there: rows see those of the context that are."""
+    banner("tree attention lengths past the table")
+    for wide in (6, 4096):
+        q, pool, table, cu, lengths, tree, _ = _case(cuda, ([9, 30], [90, 96]), "32 of 4, 128", 16, torch.bfloat16, seed=24)
+        table = torch.nn.functional.pad(table, (0, max(wide - table.shape[1], 0)), value=-1)[:, :wide].contiguous()
+        long = lengths + torch.tensor([40, 5000], dtype=torch.int32, device=cuda)
+        tree, seen = dh.oracle_tree(dh.parents([9, 30], 24, pad=2), cu.cpu(), long.cpu(), 30)
+        pool.v.view(torch.uint8).copy_(torch.where((pool.v.view(torch.uint8) & 0x7F) == 0x7F, 0, pool.v.view(torch.uint8)))
+        pool.k.view(torch.uint8).copy_(torch.where((pool.k.view(torch.uint8) & 0x7F) == 0x7F, 0, pool.k.view(torch.uint8)))
+        out = tree_attention(q, pool, table, cu, long, DraftTree(*(t.to(cuda) for t in tree)))
+        torch.cuda.synchronize()
+        dh.check_attention(out, q, pool, table, cu, long, seen, tree.positions)
 
 
 # ------------------------------------------------------------------ kept tokens
