@@ -26,17 +26,19 @@ struct KvLayers {
 KQ_DEV bool is_page(int p, int64_t pages) { return p >= 0 && p < pages; }
 
 // ---------------------------------------------------------------- copies
-// Bytes of `src` to `dst` by one workgroup, both 16-byte aligned, `bytes` a multiple of 16:
-// four chunks a thread in flight.
+// Bytes of `src` to `dst` by a workgroup or a wave, both 16-byte aligned, `bytes` a multiple
+// of 16: four chunks a thread in flight.
+template <int THREADS>
 KQ_DEV void copy_bytes(const uint8_t* src, uint8_t* dst, int bytes) {
-  for (int at = (int)threadIdx.x * 16; at < bytes; at += 256 * 64) {
+  constexpr int STEP = 16 * THREADS;
+  for (int at = (int)(threadIdx.x % THREADS) * 16; at < bytes; at += 4 * STEP) {
     u32x4 w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (at + i * 4096 < bytes) w[i] = *(const u32x4*)(src + at + i * 4096);
+      if (at + i * STEP < bytes) w[i] = *(const u32x4*)(src + at + i * STEP);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (at + i * 4096 < bytes) *(u32x4*)(dst + at + i * 4096) = w[i];
+      if (at + i * STEP < bytes) *(u32x4*)(dst + at + i * STEP) = w[i];
   }
 }
 
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(KvLayers c, const in
   uint8_t* codes = values ? layer.v : layer.k;
   const int64_t bytes = (int64_t)c.kv_heads << (c.page_shift + c.dim_shift);
   const int64_t at = (int64_t)part * kCopyBytes;
-  copy_bytes(codes + from * bytes + at, codes + to * bytes + at, (int)min((int64_t)kCopyBytes, bytes - at));
+  copy_bytes<256>(codes + from * bytes + at, codes + to * bytes + at, (int)min((int64_t)kCopyBytes, bytes - at));
   if (part == 0) {
     float* scales = values ? layer.v_scale : layer.k_scale;
     for (int h = (int)threadIdx.x; h < c.kv_heads; h += 256)
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(ForkArgs a, int64_t 
 }
 
 // The first `tables` workgroups: the other entries of the new table, and the holders (sums
-// of whole numbers, in any order).  The others: half-filled pages, a kv head's tokens each.
+// of whole numbers, in any order).  The others: half-filled pages, keys or values of one layer each.
 __global__ void __launch_bounds__(256) kv_fork_kernel(ForkArgs a, KvLayers c, int tables, int layers) {
   const int shift = c.page_shift;
   if ((int)blockIdx.x < tables) {
@@ -207,10 +209,8 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(ForkArgs a, KvLayers c, in
     }
     return;
   }
-  // (row, layer, keys or values, head), the heads next to each other
+  // (row, layer, keys or values); a wave copies every fourth head's tokens
   int unit = (int)blockIdx.x - tables;
-  const int head = unit % c.kv_heads;
-  unit /= c.kv_heads;
   const int values = unit & 1;
   unit >>= 1;
   const int row = unit / layers;
@@ -218,14 +218,13 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(ForkArgs a, KvLayers c, in
   if (from < 0) return;
   const int to = a.copies[2 * row + 1];
   const KvLayer& layer = c.at[unit - row * layers];
-  const int held = a.new_lengths[row] & ((1 << shift) - 1);
+  const int bytes = (a.new_lengths[row] & ((1 << shift) - 1)) << c.dim_shift;
   uint8_t* codes = values ? layer.v : layer.k;
-  const int64_t src = (int64_t)from * c.kv_heads + head, dst = (int64_t)to * c.kv_heads + head;
-  copy_bytes(codes + (src << (shift + c.dim_shift)), codes + (dst << (shift + c.dim_shift)), held << c.dim_shift);
-  if (threadIdx.x == 0) {
-    float* scales = values ? layer.v_scale : layer.k_scale;
-    scales[dst] = scales[src];
-  }
+  float* scales = values ? layer.v_scale : layer.k_scale;
+  const int64_t src = (int64_t)from * c.kv_heads, dst = (int64_t)to * c.kv_heads;
+  for (int h = (int)threadIdx.x; h < c.kv_heads; h += 256) scales[dst + h] = scales[src + h];
+  for (int h = scalar(wave_id()); h < c.kv_heads; h += 4)
+    copy_bytes<64>(codes + ((src + h) << (shift + c.dim_shift)), codes + ((dst + h) << (shift + c.dim_shift)), bytes);
 }
 
 // ------------------------------------------------- kept tokens behind their context
@@ -421,7 +420,7 @@ extern "C" int kq_kv_fork_sequences(const uint64_t* caches, int64_t layers, int6
   const int64_t slots = std::min(fork_slots(page_size, room), table_width);
   const int64_t tables = (std::max(seqs, rows) * table_width + 255) / 256;
   if (rows < 0 || room < 0 || room > (1 << 24) || rows * slots >= (1LL << 30) || tables >= (1LL << 23) ||
-      rows * 2 * std::min<int64_t>(layers, kMostLayers) * kv_heads >= (1LL << 23)) {
+      rows * 2 * std::min<int64_t>(layers, kMostLayers) >= (1LL << 23)) {
     set_error("%s: %lld rows of %lld pages, room for %lld tokens are past the supported range", what, (long long)rows,
               (long long)table_width, (long long)room);
     return KQ_EINVAL;
@@ -441,7 +440,7 @@ extern "C" int kq_kv_fork_sequences(const uint64_t* caches, int64_t layers, int6
   for (int64_t begin = 0; begin < layers; begin += kMostLayers) {
     const KvLayers c = some_layers(caches, layers, begin, pages, kv_heads, page_size, dim);
     const int n = (int)std::min<int64_t>(kMostLayers, layers - begin);
-    const int64_t own = begin == 0 ? tables : 0, blocks = own + (slots > 0 ? rows * 2 * n * kv_heads : 0);
+    const int64_t own = begin == 0 ? tables : 0, blocks = own + (slots > 0 ? rows * 2 * n : 0);
     if (begin == 0) hipLaunchKernelGGL(kv_fork_plan_kernel, dim3(1), dim3(1024), 0, st, a, pages, c.page_shift);
     if (blocks > 0) hipLaunchKernelGGL(kv_fork_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a, c, (int)own, n);
   }

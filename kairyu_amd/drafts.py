@@ -22,19 +22,11 @@ from __future__ import annotations
 
 import torch
 
-from kairyu_amd.attention import E4M3, MOST_NODES, DraftTree, PagedKvCache, _rows_apart
+from kairyu_amd.attention import E4M3, MOST_NODES, DraftTree, PagedKvCache
 from kairyu_amd.kernels import kv_cache_hip as hip
-from kairyu_amd.pages import KvCaches, caches_of
+from kairyu_amd.pages import KvCaches, caches_of, check_ints, check_table
 
 __all__ = ["DraftTree", "accept_drafts", "draft_tree", "keep_tokens"]
-
-
-def _check_ints(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dim() != 1 or t.dtype is not torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous int32 of one dimension, got {t.dtype} {tuple(t.shape)}")
-        if t.device != device:
-            raise RuntimeError(f"{name} must be on {device}; found {t.device}")
 
 
 def _check_most(most: int) -> None:
@@ -59,7 +51,7 @@ def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, lengths: torch.Tens
     _check_most(most)
     if not 0 <= window <= 1 << 30:
         raise ValueError(f"window must be 0 or a positive number of tokens, got {window}")
-    _check_ints(parents.device, parents=parents, cu_rows=cu_rows, lengths=lengths)
+    check_ints(parents.device, parents=parents, cu_rows=cu_rows, lengths=lengths)
     if cu_rows.shape[0] != lengths.shape[0] + 1:
         raise ValueError(f"cu_rows {tuple(cu_rows.shape)} does not match {lengths.shape[0]} lengths")
     if not parents.is_cuda:
@@ -87,7 +79,7 @@ def accept_drafts(tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Te
         raise ValueError(f"targets must be like tokens, got {targets.dtype} {tuple(targets.shape)}")
     if targets.device != tokens.device:
         raise RuntimeError(f"targets must be on {tokens.device}; found {targets.device}")
-    _check_ints(tokens.device, parents=parents, cu_rows=cu_rows)
+    check_ints(tokens.device, parents=parents, cu_rows=cu_rows)
     if parents.shape != tokens.shape or not cu_rows.shape[0]:
         raise ValueError(f"parents {tuple(parents.shape)} and cu_rows {tuple(cu_rows.shape)} do not match {tokens.shape[0]} rows")
     if not tokens.is_cuda:
@@ -111,16 +103,13 @@ def keep_tokens(caches: PagedKvCache | KvCaches, block_table: torch.Tensor, cu_r
     as they are.  A page is appended to by one sequence, as in an append."""
 
     caches = caches_of(caches)
-    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or not (block_table.is_contiguous() or _rows_apart(block_table)):
-        raise ValueError("block_table must be int32 [S, W] with contiguous rows that do not overlap")
-    device, seqs = caches.device, block_table.shape[0]
-    if block_table.device != device:
-        raise RuntimeError(f"block_table must be on {device}; found {block_table.device}")
-    _check_ints(device, cu_rows=cu_rows, lengths=lengths, counts=counts)
+    device = caches.device
+    seqs = check_table(block_table, device)[0]
+    check_ints(device, cu_rows=cu_rows, lengths=lengths, counts=counts)
     if lengths.shape[0] != seqs or cu_rows.shape[0] != seqs + 1 or counts.shape[0] != seqs:
         raise ValueError(f"cu_rows {tuple(cu_rows.shape)}, lengths {tuple(lengths.shape)} and counts {tuple(counts.shape)} "
                          f"do not match {seqs} sequences")
-    if kept.dim() != 2 or kept.shape[0] != seqs or kept.dtype is not torch.int32 or not kept.is_contiguous():
+    if len(kept.shape) != 2 or kept.shape[0] != seqs or kept.dtype is not torch.int32 or not kept.is_contiguous():
         raise ValueError(f"kept must be contiguous int32 [{seqs}, most], got {kept.dtype} {tuple(kept.shape)}")
     if kept.shape[1] > MOST_NODES:
         raise ValueError(f"kept must name at most {MOST_NODES} tokens of a sequence, got {kept.shape[1]}")

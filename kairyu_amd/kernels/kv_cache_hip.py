@@ -31,11 +31,15 @@ def require_device(device: torch.device, what: str) -> None:
         raise RuntimeError(f"{what} requires {REQUIRED_ARCH}, got {arch}")
 
 
+# (torch.cuda.current_device, which this device's tensors have initialised, without its checks)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def call_on(device: torch.device, entry: str, *args) -> None:
     """``entry`` on torch's current stream of ``device``, with that device current
     for the launch."""
 
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         _native.call(entry, *args, _native.stream_handle(device))
         return
     with torch.cuda.device(device):
@@ -146,8 +150,7 @@ def draft_tree(parents, cu_rows, lengths, most, window):
     device = parents.device
     require_device(device, "a tree of drafts")
     rows, seqs = parents.shape[0], lengths.shape[0]
-    mask = torch.empty((rows, -(-most // 32)), device=device, dtype=torch.int32)
-    positions = torch.empty(rows, device=device, dtype=torch.int32)
+    mask, positions = parents.new_empty((rows, -(-most // 32))), parents.new_empty(rows)
     call_on(device, "kq_draft_tree", parents.data_ptr(), rows, cu_rows.data_ptr(), lengths.data_ptr(), seqs, most, window,
             mask.data_ptr(), positions.data_ptr())
     return mask, positions
@@ -157,9 +160,7 @@ def accept_drafts(tokens, targets, parents, cu_rows, most):
     device = tokens.device
     require_device(device, "the walk along drafts")
     rows, seqs = tokens.shape[0], cu_rows.shape[0] - 1
-    kept = torch.empty((seqs, most), device=device, dtype=torch.int32)
-    counts = torch.empty(seqs, device=device, dtype=torch.int32)
-    following = torch.empty(seqs, device=device, dtype=tokens.dtype)
+    kept, counts, following = parents.new_empty((seqs, most)), parents.new_empty(seqs), tokens.new_empty(seqs)
     call_on(device, "kq_draft_accept", tokens.data_ptr(), targets.data_ptr(), tokens.dtype is torch.int64, parents.data_ptr(),
             rows, cu_rows.data_ptr(), seqs, most, kept.data_ptr(), counts.data_ptr(), following.data_ptr())
     return kept, counts, following
@@ -196,10 +197,9 @@ def fork_sequences(caches, holders, table, lengths, parents, room):
     pages, kv_heads, page, dim = caches.shape
     seqs, width = table.shape
     rows = parents.shape[0]
-    new_table = torch.empty((rows, width), device=device, dtype=torch.int32)
-    new_lengths, missing = torch.empty(rows + 1, device=device, dtype=torch.int32).split((rows, 1))
+    new_table, new_lengths, missing = table.new_empty((rows, width)), table.new_empty(rows), table.new_empty(1)
     need = _fork_bytes(seqs, rows, width, page, room)
-    scratch = torch.empty(need, device=device, dtype=torch.uint8)
+    scratch = table.new_empty(need // 4)
     call_on(device, "kq_kv_fork_sequences", caches.pointers, len(caches.layers), pages, kv_heads, page, dim, holders.data_ptr(),
             table.data_ptr(), _pitch(table, seqs, width), width, lengths.data_ptr(), seqs, parents.data_ptr(), rows, room,
             new_table.data_ptr(), new_lengths.data_ptr(), missing.data_ptr(), scratch.data_ptr(), need)

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 from collections.abc import Sequence
+from functools import lru_cache
 
 import torch
 
@@ -41,7 +42,7 @@ class KvCaches:
             raise ValueError("KvCaches needs at least one layer's cache")
         self.shape, self.device = _check_cache(self.layers[0]), self.layers[0].k.device
         for cache in self.layers:
-            if _check_cache(cache) != self.shape:
+            if cache is not self.layers[0] and _check_cache(cache) != self.shape:
                 raise ValueError(f"caches must be alike: {tuple(cache.k.shape)} beside {tuple(self.shape)}")
             for t in cache:
                 if t.device != self.device:
@@ -49,19 +50,33 @@ class KvCaches:
         at = [t.data_ptr() for cache in self.layers for t in cache]
         if self.shape[0] and len(set(at)) != len(at):
             raise ValueError("the layers' caches must be different tensors")
-        self.pointers = (ctypes.c_uint64 * len(at))(*at)
+        self.pointers = _addresses(len(at))(*at)
+
+
+@lru_cache(maxsize=None)
+def _addresses(n: int):
+    return ctypes.c_uint64 * n
 
 
 def caches_of(caches: PagedKvCache | KvCaches) -> KvCaches:
-    return caches if isinstance(caches, KvCaches) else KvCaches([caches])
+    return caches if isinstance(caches, KvCaches) else KvCaches((caches,))
 
 
-def _check_ints(device: torch.device, **tensors) -> None:
+def check_ints(device: torch.device, **tensors) -> None:
     for name, t in tensors.items():
-        if t.dim() != 1 or t.dtype is not torch.int32 or not t.is_contiguous():
+        if len(t.shape) != 1 or t.dtype is not torch.int32 or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 of one dimension, got {t.dtype} {tuple(t.shape)}")
         if t.device != device:
             raise RuntimeError(f"{name} must be on {device}; found {t.device}")
+
+
+def check_table(table: torch.Tensor, device: torch.device) -> torch.Size:
+    shape = table.shape
+    if len(shape) != 2 or table.dtype is not torch.int32 or not (table.is_contiguous() or _rows_apart(table)):
+        raise ValueError("block_table must be int32 [S, W] with contiguous rows that do not overlap")
+    if table.device != device:
+        raise RuntimeError(f"block_table must be on {device}; found {table.device}")
+    return shape
 
 
 def copy_pages(caches: PagedKvCache | KvCaches, sources: torch.Tensor, targets: torch.Tensor) -> None:
@@ -70,7 +85,7 @@ def copy_pages(caches: PagedKvCache | KvCaches, sources: torch.Tensor, targets: 
     be the target of two pairs, nor the target of one and the source of another."""
 
     caches = caches_of(caches)
-    _check_ints(caches.device, sources=sources, targets=targets)
+    check_ints(caches.device, sources=sources, targets=targets)
     if sources.shape != targets.shape:
         raise ValueError(f"{sources.shape[0]} sources and {targets.shape[0]} targets")
     if not sources.is_cuda:
@@ -102,15 +117,12 @@ def fork_sequences(caches: PagedKvCache | KvCaches, holders: torch.Tensor, block
 
     caches = caches_of(caches)
     pages = caches.shape[0]
-    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or not (block_table.is_contiguous() or _rows_apart(block_table)):
-        raise ValueError("block_table must be int32 [S, W] with contiguous rows that do not overlap")
-    if block_table.device != caches.device:
-        raise RuntimeError(f"block_table must be on {caches.device}; found {block_table.device}")
-    _check_ints(caches.device, holders=holders, lengths=lengths, parents=parents)
+    table_shape = check_table(block_table, caches.device)
+    check_ints(caches.device, holders=holders, lengths=lengths, parents=parents)
     if holders.shape[0] != pages:
         raise ValueError(f"holders must count {pages} pages, got {holders.shape[0]}")
-    if lengths.shape[0] != block_table.shape[0]:
-        raise ValueError(f"block_table {tuple(block_table.shape)} does not match {lengths.shape[0]} lengths")
+    if lengths.shape[0] != table_shape[0]:
+        raise ValueError(f"block_table {tuple(table_shape)} does not match {lengths.shape[0]} lengths")
     if not 0 <= room <= 1 << 24:
         raise ValueError(f"room must be 0 to 2^24 tokens, got {room}")
     if not block_table.is_cuda:
