@@ -446,15 +446,14 @@ template <int D, int DT, int CG>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
                      const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
-  constexpr int TG = 4 / CG, ST = 32 * TG, TW = 32 * CG;
+  constexpr int TG = 4 / CG, ST = 64, TW = 32 * CG;
   constexpr int KS = D / 16;            // MFMA steps along a key
   constexpr int OT = D / 32;            // output tiles
   constexpr int KLD = 2 * D + 16;       // bytes of a key's row: 16 more spread eight lanes' reads over all banks
   constexpr int VLD = 2 * ST + 16;      // bytes of a d's row of values
   constexpr int KB = ST * KLD, VB = D * VLD + 64;  // a buffer of keys; of values, and per 16 tokens scale, log2 of the value scale, its inverse
-  constexpr int KT = 256 / ST, KC = D / KT / 8;    // threads of a token's key, and 8-byte chunks of a thread
-  constexpr int VT = 1024 / ST, VY = D / VT;       // threads of four tokens' values, and each one's bytes of a token
-  constexpr int VC = VY < 4 ? 1 : VY / 4;
+  constexpr int KC = D / 64;            // 16-byte chunks of one token's key a thread moves
+  constexpr int VY = D / 16, VC = VY / 4;  // bytes and dwords of each of four tokens' values a thread moves
   constexpr int LD = D + 4;
   constexpr int MERGE = 4 * 32 * LD * 4;  // every wave's columns at the end of a part
   constexpr int LDS = 2 * (KB + VB) > MERGE ? 2 * (KB + VB) : MERGE;
@@ -475,11 +474,11 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
   int blocks = deal.blocks(q), tile = scalar(within / blocks);
   within -= tile * blocks;
 
-  // what this thread moves: D / KT bytes of a token's key, VY of four tokens' values; a
-  // wave's tokens lie in one page.  Row R of the values is d = R % VT * VY + R / VT, so that
-  // neighbouring lanes write neighbouring rows.
-  const int k_tok = tid / KT, v_grp = tid / VT, v_c = tid % VT;
-  const int k_lane = (k_tok % (ST / 4)) * D + (tid % KT) * (D / KT), v_lane = 4 * (v_grp % (ST / 16)) * D + v_c * VY;
+  // what this thread moves: D / 4 bytes of a token's key, D / 16 of four tokens' values; a
+  // wave moves 16 tokens, which lie in one page.  Row R of the values is d = R % 16 * VY + R / 16,
+  // so that neighbouring lanes write neighbouring rows.
+  const int k_tok = tid / 4, v_grp = tid / 16, v_c = tid % 16;
+  const int k_lane = (k_tok % 16) * D + (tid % 4) * (D / 4), v_lane = 4 * (v_grp % 4) * D + v_c * VY;
   const int v_pos = (v_grp >> 2) * 16 + (v_grp & 1) * 8 + ((v_grp >> 1) & 1) * 4;
   const int tile_shift = shift + (D == 64 ? 6 : D == 128 ? 7 : 8);  // log2 of a page's bytes
   const int in_page = (1 << shift) - 1;
@@ -500,12 +499,12 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
 #pragma unroll
     for (int i = 0; i < KS; ++i) qf[i] = *(const u32x4*)(src + 16 * i + 8 * h);
 
-    auto page_at = [&](int t) { return pages[min(t + ST / 4 * wave, max(hi - 1, 0)) >> shift]; };
+    auto page_at = [&](int t) { return pages[min(t + 16 * wave, max(hi - 1, 0)) >> shift]; };
     struct Place {
       int head_tile, size, off;
     };
     auto place_of = [&](int t, int page_) {
-      const int page = __builtin_amdgcn_readfirstlane(page_), at = t + ST / 4 * wave;
+      const int page = __builtin_amdgcn_readfirstlane(page_), at = t + 16 * wave;
       const bool there = page >= 0 && page < (int)cache.pages && at < hi;
       Place p;
       p.head_tile = (there ? page : 0) * cache.kv_heads + head;
@@ -513,67 +512,59 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
       p.off = (at & in_page) * D;
       return p;
     };
-    uint32_t kr[2][2 * KC], vr[2][4][VC];
-    float sc_k[2], sc_v[2];
-    auto fetch_k = [&](const Place& p, auto w) {
+    u32x4 kr[KC];
+    uint32_t vr[4][VC];
+    float sc_k = 0.0f, sc_v = 0.0f;
+    auto fetch_k = [&](const Place& p) {
       const i32x4 src = make_rsrc(cache.k + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
-      if constexpr (KC == 1) {
-        const i32x2 x = kq_rbl_v2i32(src, k_lane, p.off, 0);
-        kr[w][0] = (uint32_t)x[0], kr[w][1] = (uint32_t)x[1];
-      } else {
 #pragma unroll
-        for (int i = 0; i < KC / 2; ++i) {
-          const i32x4 x = kq_rbl_v4i32(src, k_lane + 16 * i, p.off, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) kr[w][4 * i + e] = (uint32_t)x[e];
-        }
-      }
+      for (int i = 0; i < KC; ++i) kr[i] = __builtin_bit_cast(u32x4, kq_rbl_v4i32(src, k_lane + 16 * i, p.off, 0));
     };
-    auto fetch_v = [&](const Place& p, auto w) {
+    auto fetch_v = [&](const Place& p) {
       const i32x4 src = make_rsrc(cache.v + ((int64_t)p.head_tile << tile_shift), (uint32_t)p.size);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if constexpr (VY == 2) {
-          vr[w][r][0] = (uint16_t)kq_rbl_i16(src, v_lane + r * D, p.off, 0);
-        } else if constexpr (VC == 1) {
-          vr[w][r][0] = (uint32_t)kq_rbl_i32(src, v_lane + r * D, p.off, 0);
+        if constexpr (VC == 1) {
+          vr[r][0] = (uint32_t)kq_rbl_i32(src, v_lane + r * D, p.off, 0);
         } else if constexpr (VC == 2) {
           const i32x2 x = kq_rbl_v2i32(src, v_lane + r * D, p.off, 0);
-          vr[w][r][0] = (uint32_t)x[0], vr[w][r][1] = (uint32_t)x[1];
+          vr[r][0] = (uint32_t)x[0], vr[r][1] = (uint32_t)x[1];
         } else {
           const i32x4 x = kq_rbl_v4i32(src, v_lane + r * D, p.off, 0);
 #pragma unroll
-          for (int i = 0; i < VC; ++i) vr[w][r][i] = (uint32_t)x[i];
+          for (int i = 0; i < VC; ++i) vr[r][i] = (uint32_t)x[i];
         }
       }
       // (vector loads, which the barriers do not wait for; 0 where there is no page)
-      sc_k[w] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
-      sc_v[w] = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
+      sc_k = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(k_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
+      sc_v = __builtin_bit_cast(float, kq_rbl_i32(make_rsrc(v_scale + p.head_tile, p.size != 0 ? 4 : 0), 0, 0, 0));
     };
-    auto put_k = [&](char* buf, auto w) {
+    auto put_k = [&](char* buf) {
 #pragma unroll
-      for (int i = 0; i < KC; ++i)
-        *(u32x4*)(buf + k_tok * KLD + 2 * ((tid % KT) * (D / KT) + 8 * i)) = widen_codes<DT>(kr[w][2 * i], kr[w][2 * i + 1]);
+      for (int i = 0; i < KC; ++i) {
+        char* dst = buf + k_tok * KLD + 2 * ((tid % 4) * (D / 4) + 16 * i);
+        *(u32x4*)dst = widen_codes<DT>(kr[i][0], kr[i][1]);
+        *(u32x4*)(dst + 16) = widen_codes<DT>(kr[i][2], kr[i][3]);
+      }
     };
-    auto put_v = [&](char* buf, auto w) {
+    auto put_v = [&](char* buf) {
 #pragma unroll
       for (int i = 0; i < VC; ++i) {
-        const uint32_t in[4] = {vr[w][0][i], vr[w][1][i], vr[w][2][i], vr[w][3][i]};
+        const uint32_t in[4] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i]};
         uint32_t out[4];
         transpose4(in, out);
 #pragma unroll
-        for (int j = 0; j < (VY < 4 ? VY : 4); ++j) {
+        for (int j = 0; j < 4; ++j) {
           const u32x2 x = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, false)),
                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(out[j], 1.0f, true))};
-          *(u32x2*)(buf + ((4 * i + j) * VT + v_c) * VLD + 2 * v_pos) = x;
+          *(u32x2*)(buf + ((4 * i + j) * 16 + v_c) * VLD + 2 * v_pos) = x;
         }
       }
-      // (a page holds whole tiles of 16 tokens: where a wave moves 8, every other one says)
-      if (lane == 0 && (ST / 4 * wave) % 16 == 0) {
-        float* dst = (float*)(buf + D * VLD) + ST / 4 * wave / 16;
-        dst[0] = sc_k[w] > 0.0f ? sc_k[w] * a.scale : 1.0f;
-        dst[4] = __builtin_amdgcn_logf(sc_v[w]);
-        dst[8] = sc_v[w] > 0.0f ? __builtin_amdgcn_rcpf(sc_v[w]) : 0.0f;
+      if (lane == 0) {
+        float* dst = (float*)(buf + D * VLD) + wave;
+        dst[0] = sc_k > 0.0f ? sc_k * a.scale : 1.0f;
+        dst[4] = __builtin_amdgcn_logf(sc_v);
+        dst[8] = sc_v > 0.0f ? __builtin_amdgcn_rcpf(sc_v) : 0.0f;
       }
     };
     f32x16 o[OT];
@@ -584,8 +575,9 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
     float top = -__builtin_inff(), sum = 0.0f;
     float ref = -kTileLift;  // what exponents are formed against: top (0 while there is none) - kTileLift
 
-    auto key_of = [&](const char* buf, int k) { return *(const u32x4*)(buf + (32 * tg + c) * KLD + 32 * k + 16 * h); };
-    auto value_of = [&](const char* buf, int k, int j) { return *(const u32x4*)(buf + (32 * j + c) * VLD + 64 * tg + 32 * k + 16 * h); };
+    // operands of 32 tokens of a step, its half `i`
+    auto key_of = [&](const char* buf, int i, int k) { return *(const u32x4*)(buf + (32 * i + c) * KLD + 32 * k + 16 * h); };
+    auto value_of = [&](const char* buf, int i, int k, int j) { return *(const u32x4*)(buf + (32 * j + c) * VLD + 64 * i + 32 * k + 16 * h); };
     // Weights by an earlier maximum, which only has to keep them from overflowing; l adds up
     // the denominator's share in fp32, weights times 1 / value scale.
     auto weight_pair = [&](int i, f32x2_t ks, f32x2_t shift_v, f32x2_t iv, const f32x16& w, float& l) {
@@ -625,63 +617,62 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
       }
     };
 
-    char* const keys[2] = {smem, smem + KB};
-    char* const values[2] = {smem + 2 * KB, smem + 2 * KB + VB};
+    auto keys = [&](int which) { return smem + which * KB; };
+    auto values = [&](int which) { return smem + 2 * KB + which * VB; };
     f32x16 x, y;
     if (lo < hi) {
-      constexpr std::integral_constant<int, 0> even{};
-      constexpr std::integral_constant<int, 1> odd{};
-      const int last = min(q.first, q.tokens);  // (steps that end at or before it are seen whole)
+      const int last = min(q.first, q.tokens);  // (what ends at or before it is seen whole)
       const int lo_all = (int)wave_max_u32_dpp((uint32_t)from);
-      Place at0 = place_of(lo, page_at(lo)), at1 = place_of(lo + ST, page_at(lo + ST));
-      fetch_k(at0, even);
-      fetch_v(at0, even);
-      fetch_k(at1, odd);
-      fetch_v(at1, odd);
-      int page2 = page_at(lo + 2 * ST), page3 = page_at(lo + 3 * ST), next_page = page_at(lo + 4 * ST);
-      put_k(keys[0], even);
-      put_v(values[0], even);
-      at0 = place_of(lo + 2 * ST, page2);
-      fetch_k(at0, even);
-      fetch_v(at0, even);
-      put_k(keys[1], odd);
-      Place ahead = place_of(lo + 3 * ST, page3);  // of the next values
-      fetch_k(ahead, odd);
-      meet();
+      Place at = place_of(lo, page_at(lo));
+      fetch_k(at);
+      fetch_v(at);
+      int next_page = page_at(lo + ST), page = page_at(lo + 2 * ST);
+      // the words of the mask for 32 tokens, asked for while those before are at work
+      uint32_t word0 = 0, word1 = 0;
+      auto words_of = [&](int t) {
+        if (t + 32 <= last) return;
+        const int at = (t - q.first) >> 5;
+        word0 = load_word(bits, a.words, at);
+        word1 = load_word(bits, a.words, at + 1);
+      };
+      words_of(lo + 32 * tg);
+      put_k(keys(0));
+      put_v(values(0));
+      at = place_of(lo + ST, next_page);
+      fetch_k(at);
+      if constexpr (TG > 1) {
+        put_k(keys(1));
+        fetch_v(at);
+        at = place_of(lo + 2 * ST, page);
+        fetch_k(at);
+        next_page = page_at(lo + 3 * ST);
+      } else {
+        fetch_v(at);
+        next_page = page;
+      }
 #pragma unroll
       for (int i = 0; i < KS; ++i) qf[i] ^= a.q_sign;
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) x = mfma32<DT>(key_of(keys[0], k), qf[k], x);
       meet();
-      // a step's words of the mask, a step ahead
-      uint32_t word0 = 0, word1 = 0;
-      auto words_of = [&](int t) {
-        if (t + ST <= last) return;
-        const int at = (t + 32 * tg - q.first) >> 5;
-        word0 = load_word(bits, a.words, at);
-        word1 = load_word(bits, a.words, at + 1);
-      };
-      words_of(lo);
-      // step i of parity p: scores in `now`, the next step's go to `next`
-      auto step = [&](int t, f32x16& now, f32x16& next, auto p_) {
-        constexpr int p = decltype(p_)::value;
-        constexpr std::integral_constant<int, p> same{};
-        constexpr std::integral_constant<int, 1 - p> other{};
-        const char* scales = values[p] + D * VLD + 8 * tg;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) x = mfma32<DT>(key_of(keys(0), tg, k), qf[k], x);
+      // 32 tokens from t on, half i of a step whose values are in `vals`: their weights from the
+      // scores `now`, between the products that give the next ones' scores
+      auto half = [&](int t, int i, const char* vals, f32x16& now, f32x16& next, const char* next_keys, int next_i, int next_t) {
+        const char* scales = vals + D * VLD + 8 * i;
         const f32x2_t ks = *(const f32x2_t*)scales, lv = *(const f32x2_t*)(scales + 16), iv = *(const f32x2_t*)(scales + 32);
         u32x4 kx[4];  // (four of the operands ahead)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) kx[k] = key_of(keys[1 - p], k);
-        if (t < lo_all || t + ST > last) {
-          const int token = t + 32 * tg, node = token - q.first, at = node >> 5;
-          const uint32_t seen = bits_at(word_at(word0, a.words, at), word_at(word1, a.words, at + 1), node) & tokens_from(from - token) &
-                                ~tokens_from(q.tokens - token);
+        for (int k = 0; k < 4; ++k) kx[k] = key_of(next_keys, next_i, k);
+        if (t < lo_all || t + 32 > last) {
+          const int node = t - q.first, at = node >> 5;
+          const uint32_t seen = bits_at(word_at(word0, a.words, at), word_at(word1, a.words, at + 1), node) & tokens_from(from - t) &
+                                ~tokens_from(q.tokens - t);
 #pragma unroll
           for (int e = 0; e < 16; ++e) now[e] = seen >> (4 * h) & (1u << (8 * (e >> 2) + (e & 3))) ? now[e] : -__builtin_inff();
         }
-        words_of(t + ST);
+        words_of(next_t);
         u32x4 w[2];
         float l;
         const f32x2_t shift_v = {lv[0] - ref, lv[1] - ref};
@@ -690,34 +681,59 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           next = mfma32<DT>(kx[k & 3], qf[k], next);
-          if (k + 4 < KS) kx[k & 3] = key_of(keys[1 - p], k + 4);
+          if (k + 4 < KS) kx[k & 3] = key_of(next_keys, next_i, k + 4);
 #pragma unroll
-          for (int i = 8 * k / KS; i < 8 * (k + 1) / KS; ++i) w[i >> 2][i & 3] = weight_pair(i, ks, shift_v, iv, now, l);
+          for (int j = 8 * k / KS; j < 8 * (k + 1) / KS; ++j) w[j >> 2][j & 3] = weight_pair(j, ks, shift_v, iv, now, l);
           __builtin_amdgcn_sched_barrier(0);
         }
         asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(l));  // (not behind the branch that may compute them anew)
         u32x4 vx[2][OT];
 #pragma unroll
-        for (int j = 0; j < OT; ++j) vx[0][j] = value_of(values[p], 0, j);
+        for (int j = 0; j < OT; ++j) vx[0][j] = value_of(vals, i, 0, j);
         limit(ks, lv, iv, now, w, l);
 #pragma unroll
-        for (int j = 0; j < OT; ++j) vx[1][j] = value_of(values[p], 1, j);
+        for (int j = 0; j < OT; ++j) vx[1][j] = value_of(vals, i, 1, j);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int j = 0; j < OT; ++j) o[j] = mfma32<KQ_DTYPE_F16>(vx[k][j], w[k], o[j]);
         sum += l;
-        put_k(keys[p], same);
-        put_v(values[1 - p], other);
-        fetch_v(ahead, other);
-        ahead = place_of(t + 4 * ST, next_page);
-        fetch_k(ahead, same);
-        next_page = page_at(t + 5 * ST);
-        meet();
       };
-      for (int t = lo; t < hi; t += 2 * ST) {  // (a step past the end finds no page and adds nothing)
-        step(t, x, y, even);
-        step(t + ST, y, x, odd);
+      if constexpr (TG > 1) {
+        meet();  // (keys 0 are read)
+        // step n of parity p: reads keys n + 1 and values n, writes keys n + 2 and values n + 1
+        // where keys n and values n - 1 were
+        auto step = [&](int t, f32x16& now, f32x16& next, auto p_) {
+          constexpr int p = decltype(p_)::value;
+          half(t + 32 * tg, tg, values(p), now, next, keys(1 - p), tg, t + ST + 32 * tg);
+          put_k(keys(p));
+          put_v(values(1 - p));
+          fetch_v(at);
+          at = place_of(t + 3 * ST, next_page);
+          fetch_k(at);
+          next_page = page_at(t + 4 * ST);
+          meet();
+        };
+        for (int t = lo; t < hi; t += 2 * ST) {  // (a step past the end finds no page and adds nothing)
+          step(t, x, y, std::integral_constant<int, 0>{});
+          step(t + ST, y, x, std::integral_constant<int, 1>{});
+        }
+      } else {
+        // both halves of a step: keys n + 1 reach LDS between them, values n + 1 at the end
+        int which = 0;
+        for (int t = lo; t < hi; t += ST) {
+          half(t, 0, values(which), x, y, keys(which), 1, t + 32);
+          put_k(keys(which ^ 1));
+          at = place_of(t + 2 * ST, next_page);
+          fetch_k(at);
+          next_page = page_at(t + 3 * ST);
+          meet();
+          half(t + 32, 1, values(which), y, x, keys(which ^ 1), 0, t + 64);
+          put_v(values(which ^ 1));
+          fetch_v(at);
+          meet();
+          which ^= 1;
+        }
       }
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -738,28 +754,20 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
     }
     // The waves' columns meet in LDS in the order of d, and are added in the order of their
     // tokens by threads that write whole rows.  Element e of tile j is row R = 32 j + 8 (e / 4) +
-    // 4 h + e % 4 of the values: N neighbouring d are elements e of all tiles, or e and e + 8.
-    constexpr int N = VT == 32 ? OT : 2 * OT;
+    // 4 h + e % 4 of the values: elements e and e + 8 of all tiles are neighbouring d.
+    constexpr int N = 2 * OT;
     float* mine = (float*)smem + (wave * 32 + c) * LD;
 #pragma unroll
-    for (int e = 0; e < 16 * OT / N; ++e) {
+    for (int e = 0; e < 8; ++e) {
       float v[N];
 #pragma unroll
       for (int j = 0; j < OT; ++j) {
-        if constexpr (VT == 32) {
-          v[j] = o[j][e];
-        } else {
-          v[2 * j] = o[j][e];
-          v[2 * j + 1] = o[j][8 + e];
-        }
+        v[2 * j] = o[j][e];
+        v[2 * j + 1] = o[j][8 + e];
       }
       float* dst = mine + (8 * (e >> 2) + 4 * h + (e & 3)) * VY;
-      if constexpr (N == 2) {
-        *(f32x2_t*)dst = f32x2_t{v[0], v[1]};
-      } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) *(f32x4*)(dst + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-      }
+      for (int i = 0; i < N; i += 4) *(f32x4*)(dst + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
     }
     if (h == 0) mine[D] = top, mine[D + 1] = sum;
     meet();
