@@ -4,9 +4,10 @@
 // sees: those before its sequence's new ones (from its position less the window on), and
 // the new ones whose bit its mask holds.  Scores, scales and weights are formed as in
 // attention over prompts and single tokens: w_t = log2(e) scale k_scale (q . code_t) +
-// log2 v_scale, exp2(w_t - max w + lift) in fp16 (11 bits down to 2^-29 of the largest,
-// some down to 2^-40) times the value's codes, the denominator in fp32 from weights not yet
-// rounded over v_scale, maxima, denominators and outputs in fp32.
+// log2 v_scale, exp2(w_t - max w + lift) in fp16 (11 bits down to 2^-29 of the largest and
+// some down to 2^-40, in tiles of 64 and 128 columns 2^-23 and 2^-34) times the value's codes,
+// the denominator in fp32 from weights not yet rounded over v_scale, maxima, denominators and
+// outputs in fp32.
 #include "kq_kv_attend.h"
 
 #include <algorithm>
@@ -181,7 +182,7 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
       const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
       const int pos = a.positions[q.row0 + row];
       bits[m] = a.mask + (int64_t)(q.row0 + row) * a.words;
-      from[m] = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) + 1 - a.window, 0), max(q.first, 0)) : 0;
+      from[m] = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) - (a.window - 1), 0), max(q.first, 0)) : 0;
       most_from = max(most_from, (uint32_t)from[m]);
       // (columns past the rows compute the first one's again, and are not stored)
       const uint16_t* src = a.q + (int64_t)(q.row0 + row) * a.q_ld + (int64_t)(head * group + qh) * a.q_hs;
@@ -489,7 +490,7 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
     const int row = real ? item / group : 0, qh = real ? item - row * group : 0;
     const int pos = a.positions[q.row0 + row];
     const uint32_t* bits = a.mask + (int64_t)(q.row0 + row) * a.words;
-    const int from = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) + 1 - a.window, 0), max(q.first, 0)) : 0;
+    const int from = !real ? 0 : pos < 0 ? 0x7fffffff : a.window > 0 ? min(max(max(pos, q.first) - (a.window - 1), 0), max(q.first, 0)) : 0;
     const int part_blocks = min(blocks - within, run_end - block);
     const int lo = deal.first(q) * 64 + (within << (6 + a.block_shift));
     const int hi = (int)min((int64_t)q.tokens, (int64_t)lo + ((int64_t)part_blocks << (6 + a.block_shift)));

@@ -324,6 +324,22 @@ def test_attention_windows_in_every_tile(cuda, heads, window):
     dh.check_attention(out, q, pool, table, cu, lengths, seen, tree.positions, window=window)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_of_positions_far_off(cuda, wide):
+    """Under a window, positions before the first drafted slot count as it, and the largest
+    leave nothing of the context."""
+    banner(f"tree attention far positions {wide}")
+    q, pool, table, cu, lengths, tree, seen = _case(cuda, ([12, 40], [90, 400]), "32 of 4, 128", 16, torch.bfloat16, seed=25)
+    if wide:
+        table = torch.nn.functional.pad(table, (0, 65536 - table.shape[1]), value=-1)
+    positions = tree.positions.cpu()
+    positions[::3], positions[1::3] = 0, 2**31 - 1
+    for window in (1, 50, 1 << 30):
+        out = tree_attention(q, pool, table, cu, lengths, DraftTree(tree.mask, positions.to(cuda)), window=window)
+        torch.cuda.synchronize()
+        dh.check_attention(out, q, pool, table, cu, lengths, seen, positions, window=window)
+
+
 def test_attention_of_lengths_past_the_table(cuda):
     """Tokens past the table are not there: rows see those of the context that are."""
     banner("tree attention lengths past the table")
