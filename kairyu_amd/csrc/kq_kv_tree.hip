@@ -28,15 +28,19 @@ struct TreeArgs {
   int most_blocks;  // no batch has more
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
   int block_shift;  // log2 of the 64-token steps of a block
+  int alike;      // whether every workgroup gets one part of one tile
 };
 
 constexpr float kLift = 15.0f;  // log2 of the largest weight
 
 // A sequence's rows (drafted tokens x the group's query heads) go to tiles of TW, the
-// tokens that they see to blocks, and the blocks of all tiles, one after the other, to
-// `shares` workgroups per kv head in equal runs: whole tiles, written at once, and at most two
-// parts of tiles, the end of one begun before (part 0) and the beginning of one that goes on
-// (part 1).
+// tokens that they see to blocks.  Where no batch has more tiles than there are workgroups to a
+// kv head, tiles are cut into parts of as few blocks as gives every part a workgroup of its
+// own.  Otherwise the blocks of all tiles, one after the other, are dealt to the workgroups in
+// equal runs: whole tiles, and at most two parts of tiles.  Parts that are not whole go through
+// memory: those that do not begin their tile to a workgroup's place 0, the others to place 1.
+// (In runs a workgroup with two parts begins twice, 8 us: two trees of 48 rows behind 100003
+// tokens, 28 heads over 4, 200 us, and in parts of one length 186.)
 template <int TW>
 struct TreeDeal {
   const TreeArgs& a;
@@ -47,12 +51,60 @@ struct TreeDeal {
   KQ_DEV int blocks(const KvSeq& q) const { return (max(((q.tokens + 63) >> 6) - first(q), 1) + (1 << a.block_shift) - 1) >> a.block_shift; }
   KQ_DEV int tiles(const KvSeq& q) const { return (q.rows * group + TW - 1) / TW; }
   KQ_DEV int operator()(const KvSeq& q) const { return tiles(q) * blocks(q); }
-  KQ_DEV int run(const KvLanes& lanes) const {
-    // (held to what a batch can have, whatever the row bounds say)
-    const uint32_t all = min((uint32_t)lanes.total(*this), (uint32_t)a.most_blocks);
-    return scalar((int)((all + (uint32_t)a.shares - 1) / (uint32_t)a.shares));
+  KQ_DEV int parts(const KvSeq& q, int length) const { return (int)((uint32_t)(blocks(q) + length - 1) / (uint32_t)length); }
+  // blocks of all tiles (held to what a batch can have, whatever the row bounds say)
+  KQ_DEV int all(const KvLanes& lanes) const { return (int)min((uint32_t)lanes.total(*this), (uint32_t)a.most_blocks); }
+  KQ_DEV int run(const KvLanes& lanes) const { return scalar((int)(((uint32_t)all(lanes) + (uint32_t)a.shares - 1) / (uint32_t)a.shares)); }
+  // blocks of a part: the fewest that need no more parts than there are workgroups
+  KQ_DEV int length(const KvLanes& lanes) const {
+    const int blocks_ = all(lanes), tiles_ = lanes.total([&](const KvSeq& q) { return tiles(q); }), spare = a.shares - tiles_;
+    int lo = max((blocks_ + a.shares - 1) / a.shares, 1);
+    // (a tile has at most one part that is not full; without spare workgroups every tile is one)
+    int hi = max(spare > 0 ? (blocks_ + spare - 1) / spare : (int)(((int64_t)lanes.b.table_width << lanes.shift) >> (6 + a.block_shift)) + 2, lo);
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (lanes.total([&](const KvSeq& q) { return tiles(q) * parts(q, mid); }) <= a.shares)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    return scalar(lo);
   }
 };
+
+// A workgroup's blocks: from `within` of `tile` of sequence s (-1: none) on, `end` - `block` of them.
+struct TreeRun {
+  int s, tile, within, blocks, block, end;
+  KvSeq q;
+};
+template <int TW>
+KQ_DEV TreeRun run_of(const TreeArgs& a, const KvLanes& lanes, const TreeDeal<TW>& deal, int share) {
+  TreeRun r{};
+  if (a.alike) {
+    const int length = deal.length(lanes);
+    int unit;
+    r.s = lanes.find(share, unit, [&](const KvSeq& q) { return deal.tiles(q) * deal.parts(q, length); });
+    if (r.s < 0) return r;
+    r.q = lanes[r.s];
+    r.blocks = deal.blocks(r.q);
+    const int parts = scalar(deal.parts(r.q, length));
+    r.tile = scalar(unit / parts);
+    r.within = (unit - r.tile * parts) * length;
+    r.end = min(length, r.blocks - r.within);
+    return r;
+  }
+  const int run = deal.run(lanes);
+  r.block = share * run;
+  r.end = r.block + run;
+  int unit;
+  r.s = lanes.find(r.block, unit, deal);
+  if (r.s < 0) return r;
+  r.q = lanes[r.s];
+  r.blocks = deal.blocks(r.q);
+  r.tile = scalar(unit / r.blocks);
+  r.within = unit - r.tile * r.blocks;
+  return r;
+}
 
 // A row's mask with all ones before it, for the tokens before the new ones, and none behind.
 // The load is always in range and may be on its way long before the word is asked for.
@@ -90,14 +142,11 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
   const KvLanes lanes(batch, shift);
   zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 64 * WAVES);
   const TreeDeal<TW> deal{a, group};
-  const int run = deal.run(lanes), run_end = ((int)blockIdx.x + 1) * run;
-  int block = (int)blockIdx.x * run;
-  int within = 0;  // blocks of the sequence, then of the tile, before `block`
-  int s = lanes.find(block, within, deal);
-  if (s < 0) return;
-  KvSeq q = lanes[s];
-  int blocks = deal.blocks(q), tile = scalar(within / blocks);
-  within -= tile * blocks;
+  const TreeRun given = run_of(a, lanes, deal, (int)blockIdx.x);
+  if (given.s < 0) return;
+  KvSeq q = given.q;
+  int s = given.s, tile = given.tile, within = given.within, blocks = given.blocks, block = given.block;
+  const int run_end = given.end;
   const int64_t tile_bytes = (int64_t)D << shift;
   const int in_page = (1 << shift) - 1;
   const int k_lane = c * D + 16 * b, v_lane = 4 * b * D + c * (D / 16);
@@ -466,14 +515,11 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
   const KvLanes lanes(batch, shift);
   zero_padding<D>(a, batch, head, group, (int)blockIdx.x, (int)gridDim.x, 256);
   const TreeDeal<TW> deal{a, group};
-  const int run = deal.run(lanes), run_end = ((int)blockIdx.x + 1) * run;
-  int block = (int)blockIdx.x * run;
-  int within = 0;  // blocks of the sequence, then of the tile, before `block`
-  int s = lanes.find(block, within, deal);
-  if (s < 0) return;
-  KvSeq q = lanes[s];
-  int blocks = deal.blocks(q), tile = scalar(within / blocks);
-  within -= tile * blocks;
+  const TreeRun given = run_of(a, lanes, deal, (int)blockIdx.x);
+  if (given.s < 0) return;
+  KvSeq q = given.q;
+  int s = given.s, tile = given.tile, within = given.within, blocks = given.blocks, block = given.block;
+  const int run_end = given.end;
 
   // what this thread moves: D / 4 bytes of a token's key, D / 16 of four tokens' values; a
   // wave moves 16 tokens, which lie in one page.  Row R of the values is d = R % 16 * VY + R / 16,
@@ -832,15 +878,25 @@ kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
   if (s < 0) return;
   const KvSeq q = lanes[s];
   if (tile * TW + column0 >= q.rows * group) return;
-  int block = 0;  // blocks before the tile's
-  lanes.of_row(q.row0, block, deal);
-  const int run = max(deal.run(lanes), 1), blocks = deal.blocks(q);
-  block += tile * blocks;
-  // (within the shares also where row bounds that go back make counts wrap)
-  const int x0 = min(max(scalar(block / run), 0), a.shares - 1);
-  const int chunks = min(max(scalar((block + blocks - 1) / run), x0), a.shares - 1) - x0 + 1;
+  // its parts and the workgroup of the first (within the shares also where row bounds that go
+  // back make counts wrap)
+  int x0 = 0, chunks = 0;
+  const int blocks = deal.blocks(q);
+  if (a.alike) {
+    const int length = deal.length(lanes), parts = scalar(deal.parts(q, length));
+    lanes.of_row(q.row0, x0, [&](const KvSeq& p) { return deal.tiles(p) * deal.parts(p, length); });
+    x0 = min(max(x0 + tile * parts, 0), a.shares - 1);
+    chunks = min(parts, a.shares - x0);
+  } else {
+    const int run = max(deal.run(lanes), 1);
+    int block = 0;  // blocks before the tile's
+    lanes.of_row(q.row0, block, deal);
+    block += tile * blocks;
+    x0 = min(max(scalar(block / run), 0), a.shares - 1);
+    chunks = min(max(scalar((block + blocks - 1) / run), x0), a.shares - 1) - x0 + 1;
+  }
   if (chunks == 1) return;  // written already
-  // part 1 of the run it begins in, then part 0 of those behind
+  // place 1 of the workgroup it begins in, then place 0 of those behind
   const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * TW + column0) * LD;
   auto at_part = [&](int i) { return src + (i == 0 ? 0 : (int64_t)(2 * i - 1) * TW) * LD; };
   float m[E], l[E];
@@ -905,6 +961,7 @@ struct TreePlan {
   int columns;  // of a tile: 16 or 32 (a wave holds them all), 64 or 128 (the workgroup does)
   int waves;    // of a workgroup
   int shares, block_shift;
+  bool alike;
   size_t part;  // bytes
 };
 
@@ -927,9 +984,10 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   // workgroups that registers and LDS let a CU hold
   const int64_t slots = 256 * (p.columns > 32 ? (dim == 256 ? 1 : 2) : p.waves == 8 ? 1 : dim * p.columns <= 1024 ? 3 : dim * p.columns <= 4096 ? 2 : 1);
   p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
-  // blocks of 256 tokens, or of 512 where those still give every workgroup one: tiles are cut less
-  // often (one tree of 64 behind 16000 tokens 31 -> 27 us, 16 of up to 96 behind 3000 43 -> 39)
-  p.block_shift = tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
+  p.alike = tiles(p.columns) <= p.shares * kv_heads;
+  // parts of one length: blocks of a workgroup's two steps or so.  Runs: of 256 tokens, or of 512 where
+  // those still give every workgroup one, so that tiles are cut less often
+  p.block_shift = p.alike ? (p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
   if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * p.columns * (dim + 4));
   return p;
@@ -1034,7 +1092,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
   }
   // threads of one launch, and blocks of all tiles
   const int64_t tiles = empty ? 0 : rows * (heads / kv_heads) / p.columns + seqs;
-  const int64_t blocks = tiles * ((table_width * page_size + 255) / 256);
+  const int64_t blocks = tiles * ((table_width * page_size + 127) / 128);
   if (rows * heads * 64 >= (1LL << 32) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
@@ -1050,7 +1108,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.window = (int)window;
   a.most_blocks = (int)blocks;
-  a.shares = p.shares, a.block_shift = p.block_shift;
+  a.shares = p.shares, a.block_shift = p.block_shift, a.alike = p.alike;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};
