@@ -36,11 +36,12 @@ constexpr float kLift = 15.0f;  // log2 of the largest weight
 // A sequence's rows (drafted tokens x the group's query heads) go to tiles of TW, the
 // tokens that they see to blocks.  Where no batch has more tiles than there are workgroups to a
 // kv head, tiles are cut into parts of as few blocks as gives every part a workgroup of its
-// own.  Otherwise the blocks of all tiles, one after the other, are dealt to the workgroups in
-// equal runs: whole tiles, and at most two parts of tiles.  Parts that are not whole go through
-// memory: those that do not begin their tile to a workgroup's place 0, the others to place 1.
-// (In runs a workgroup with two parts begins twice, 8 us: two trees of 48 rows behind 100003
-// tokens, 28 heads over 4, 200 us, and in parts of one length 186.)
+// own.  Otherwise, and in tiles of 16 columns, the blocks of all tiles, one after the other, are
+// dealt to the workgroups in equal runs: whole tiles, and at most two parts of tiles.  Parts that
+// are not whole go through memory: those that do not begin their tile to a workgroup's place 0,
+// the others to place 1.  (A workgroup with two parts begins twice, 8 us, and finding the length
+// of parts takes 1: 32 trees of up to 32 rows behind 6000 tokens, 32 heads over 4, in runs 102 us,
+// in parts of one length 96; one tree of 16 rows behind 4000, 32 heads over 8, 18.9 and 19.9.)
 template <int TW>
 struct TreeDeal {
   const TreeArgs& a;
@@ -57,13 +58,18 @@ struct TreeDeal {
   KQ_DEV int run(const KvLanes& lanes) const { return scalar((int)(((uint32_t)all(lanes) + (uint32_t)a.shares - 1) / (uint32_t)a.shares)); }
   // blocks of a part: the fewest that need no more parts than there are workgroups
   KQ_DEV int length(const KvLanes& lanes) const {
-    const int blocks_ = all(lanes), tiles_ = lanes.total([&](const KvSeq& q) { return tiles(q); }), spare = a.shares - tiles_;
-    int lo = max((blocks_ + a.shares - 1) / a.shares, 1);
+    const KvSeq q = lanes.at_lane(0);
+    const int tiles_ = tiles(q), blocks_ = blocks(q);  // (of the lane's sequence, while a wave holds them all)
+    const int most = all(lanes), spare = a.shares - lanes.total([&](const KvSeq& p) { return tiles(p); });
+    int lo = max((int)((uint32_t)(most + a.shares - 1) / (uint32_t)a.shares), 1);
     // (a tile has at most one part that is not full; without spare workgroups every tile is one)
-    int hi = max(spare > 0 ? (blocks_ + spare - 1) / spare : (int)(((int64_t)lanes.b.table_width << lanes.shift) >> (6 + a.block_shift)) + 2, lo);
+    int hi = max(spare > 0 ? (int)((uint32_t)(most + spare - 1) / (uint32_t)spare)
+                           : (int)(((int64_t)lanes.b.table_width << lanes.shift) >> (6 + a.block_shift)) + 2, lo);
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (lanes.total([&](const KvSeq& q) { return tiles(q) * parts(q, mid); }) <= a.shares)
+      const int parts_ = lanes.held ? __builtin_amdgcn_readlane(wave_scan(tiles_ * (int)((uint32_t)(blocks_ + mid - 1) / (uint32_t)mid)), 63)
+                                    : lanes.total([&](const KvSeq& p) { return tiles(p) * parts(p, mid); });
+      if (parts_ <= a.shares)
         hi = mid;
       else
         lo = mid + 1;
@@ -984,7 +990,7 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   // workgroups that registers and LDS let a CU hold
   const int64_t slots = 256 * (p.columns > 32 ? (dim == 256 ? 1 : 2) : p.waves == 8 ? 1 : dim * p.columns <= 1024 ? 3 : dim * p.columns <= 4096 ? 2 : 1);
   p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
-  p.alike = tiles(p.columns) <= p.shares * kv_heads;
+  p.alike = p.columns > 16 && tiles(p.columns) <= p.shares * kv_heads;
   // parts of one length: blocks of a workgroup's two steps or so.  Runs: of 256 tokens, or of 512 where
   // those still give every workgroup one, so that tiles are cut less often
   p.block_shift = p.alike ? (p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
