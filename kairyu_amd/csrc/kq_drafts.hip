@@ -9,21 +9,25 @@ namespace kq {
 constexpr int kMostNodes = 1024;
 
 // One workgroup a sequence.  A node's parent lies before it, so a walk upwards ends, and
-// meets the words of its mask from the last to the first: each is written once.
+// meets the words of its mask from the last to the first: each is written once.  What a node
+// has above it among the 32 nodes of its own word is found first, with the node that it leaves
+// the word to; then each row goes from word to word, which makes 64 steps of 1024.
 //
-// Latency: bounds, parents, LDS, and a step of some 100 cycles for each level.
-__global__ void __launch_bounds__(256)
+// Latency: bounds, parents, LDS, and a step of some 200 cycles for each level: one tree of 8 rows
+// 2.2 us, a chain of 1024 21 (every row from node to node 281).
+__global__ void __launch_bounds__(kMostNodes)
 draft_tree_kernel(KvBatch batch, const int32_t* __restrict__ parents, int most, int window, uint32_t* __restrict__ mask,
                   int32_t* __restrict__ positions) {
-  __shared__ int16_t parent[kMostNodes];
-  const int tid = (int)threadIdx.x, words = (most + 31) >> 5;
+  __shared__ int16_t parent[kMostNodes], leaves_to[kMostNodes];
+  __shared__ uint32_t inside[kMostNodes];
+  const int tid = (int)threadIdx.x, threads = (int)blockDim.x, words = (most + 31) >> 5;
   auto none = [&](int64_t row, int from_word) {
     for (int w = from_word; w >= 0; --w) mask[row * words + w] = 0;
   };
   // rows of no sequence, dealt to the workgroups
   const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
   const int begin = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
-  for (int i = (int)blockIdx.x * 256 + tid; i < begin + batch.rows - last; i += (int)gridDim.x * 256) {
+  for (int i = (int)blockIdx.x * threads + tid; i < begin + batch.rows - last; i += (int)gridDim.x * threads) {
     const int row = i < begin ? i : last + (i - begin);
     none(row, words - 1);
     positions[row] = -1;
@@ -31,73 +35,93 @@ draft_tree_kernel(KvBatch batch, const int32_t* __restrict__ parents, int most, 
   if ((int)blockIdx.x >= batch.seqs) return;
   const KvSeq q = kv_seq(batch, (int)blockIdx.x, 4);
   const int n = min(q.rows, most);
-  for (int i = tid; i < n; i += 256) {
+  for (int i = tid; i < n; i += threads) {
     const int p = parents[q.row0 + i];
     parent[i] = (int16_t)(p >= 0 && p < i ? p : -1);
   }
   __syncthreads();
-  for (int i = tid; i < q.rows; i += 256) {
-    const int64_t row = q.row0 + i;
-    int depth = -1, at = i < n ? i : -1, word = words - 1;
+  for (int i = tid; i < n; i += threads) {
     uint32_t bits = 0;
-    // the levels above; whether the row has a token is known when its depth is
-    for (; at >= 0; at = parent[at]) {
-      ++depth;
-      if (window > 0 && depth >= window) continue;
-      for (; word > at >> 5; --word, bits = 0) mask[row * words + word] = bits;
+    int at = i;
+    do {
       bits |= 1u << (at & 31);
+      at = parent[at];
+    } while (at >= (i & ~31));
+    inside[i] = bits;
+    leaves_to[i] = (int16_t)at;
+  }
+  __syncthreads();
+  for (int i = tid; i < q.rows; i += threads) {
+    const int64_t row = q.row0 + i;
+    int nodes = 0, word = words - 1;
+    if (i < n && q.first + i >= 0) {
+      for (int at = i; at >= 0; at = leaves_to[at]) {
+        uint32_t bits = inside[at];
+        const int here = __popc(bits);
+        // (the nearest are the highest)
+        for (int far = window > 0 ? min(nodes + here - window, here) : 0; far > 0; --far) bits &= bits - 1;
+        nodes += here;
+        for (; word > at >> 5; --word) mask[row * words + word] = 0;
+        mask[row * words + word--] = bits;
+      }
     }
-    for (; word >= 0; --word, bits = 0) mask[row * words + word] = bits;
-    const int position = q.first + depth;
-    const bool there = i < n && q.first + i >= 0 && position >= 0;
-    if (!there) none(row, words - 1);
-    positions[row] = there ? position : -1;
+    none(row, word);
+    const int position = q.first + nodes - 1;
+    if (nodes > 0 && position < 0) none(row, words - 1);
+    positions[row] = nodes > 0 && position >= 0 ? position : -1;
   }
 }
 
-// One wave a sequence: its rows' parents and tokens in LDS, then step by step the lowest
-// child that has the token that the model says, 64 rows at a look.
+// One workgroup a sequence: the lowest child of each row that has the token that the model says
+// there (a minimum in LDS, the same in any order), then the walk from child to child.
+//
+// Latency, as above: one tree of 8 rows 2.2 us, a chain of 1024 that is kept whole 56 (with a look at
+// all rows for each step 236).
 template <typename T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(256)
 draft_accept_kernel(KvBatch batch, const T* __restrict__ tokens, const T* __restrict__ targets,
                     const int32_t* __restrict__ parents, int most, int32_t* __restrict__ kept, int32_t* __restrict__ counts,
                     T* __restrict__ following) {
-  __shared__ T token[kMostNodes], target[kMostNodes];
-  __shared__ int16_t parent[kMostNodes];
-  const int s = (int)blockIdx.x, lane = lane_id();
+  __shared__ T target[kMostNodes];
+  __shared__ int child[kMostNodes], path[kMostNodes];
+  __shared__ int length;
+  constexpr int kNone = 0x7fffffff, U = kMostNodes / 256;
+  const int s = (int)blockIdx.x, tid = (int)threadIdx.x, threads = (int)blockDim.x;
   const int lo = min(max(batch.cu[s], 0), batch.rows), hi = min(max(batch.cu[s + 1], lo), batch.rows);
   const int n = scalar(min(hi - lo, most));
-  for (int i = lane; i < n; i += 64) {
-    const int p = parents[lo + i];
-    parent[i] = (int16_t)(p >= 0 && p < i ? p : -1);
-    token[i] = tokens[lo + i];
+  T token[U];
+  int parent[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = tid + u * threads;
+    if (i >= n) break;
+    parent[u] = parents[lo + i];
+    token[u] = tokens[lo + i];
     target[i] = targets[lo + i];
+    child[i] = kNone;
   }
   __syncthreads();
-  int count = 0, at = n > 0 ? 0 : -1;
-  T said = (T)-1;
-  int32_t* out = kept + (int64_t)s * most;
-  while (at >= 0) {
-    if (lane == 0) out[count] = at;
-    ++count;
-    said = target[at];
-    int next = -1;
-    for (int base = (at + 1) & ~63; base < n && next < 0; base += 64) {
-      const int i = base + lane;
-      const uint64_t right = __ballot(i < n && parent[i < n ? i : 0] == at && token[i < n ? i : 0] == said);
-      if (right != 0) next = base + (int)__builtin_ctzll(right);
-    }
-    at = scalar(next);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = tid + u * threads;
+    if (i >= n) break;
+    if (parent[u] >= 0 && parent[u] < i && token[u] == target[parent[u]]) atomicMin(&child[parent[u]], i);
   }
-  for (int i = count + lane; i < most; i += 64) out[i] = -1;
-  if (lane == 0) {
+  __syncthreads();
+  if (tid == 0) {
+    int count = 0;
+    for (int at = 0; at < n; at = child[at]) path[count++] = at;
+    length = count;
     counts[s] = count;
-    following[s] = said;
+    following[s] = count > 0 ? target[path[count - 1]] : (T)-1;
   }
+  __syncthreads();
+  const int count = length;
+  for (int i = tid; i < most; i += threads) kept[(int64_t)s * most + i] = i < count ? path[i] : -1;
 }
 
 static int check_drafts(const char* what, int64_t rows, int64_t seqs, int64_t most) {
-  if (rows < 0 || seqs < 0 || rows > (1 << 24) || seqs > (1 << 24)) {
+  if (rows < 0 || seqs < 0 || rows > (1 << 24) || seqs >= (1 << 24)) {
     set_error("%s: bad shape rows=%lld seqs=%lld", what, (long long)rows, (long long)seqs);
     return KQ_EINVAL;
   }
@@ -122,8 +146,10 @@ extern "C" int kq_draft_tree(const int32_t* parents, int64_t rows, const int32_t
   }
   if (rows == 0) return KQ_OK;
   const KvBatch b{nullptr, cu, lengths, 0, (int)seqs, 0, (int)rows};
-  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)std::max<int64_t>(seqs, 1)), dim3(256), 0, (hipStream_t)stream, b, parents,
-                     (int)most, (int)window, (uint32_t*)mask, positions);
+  // (a thread a row, and fewer than 2^32 of them)
+  const int64_t threads = std::min<int64_t>((most + 63) / 64 * 64, seqs < (1 << 22) ? kMostNodes : 128);
+  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)std::max<int64_t>(seqs, 1)), dim3((unsigned)threads), 0, (hipStream_t)stream, b,
+                     parents, (int)most, (int)window, (uint32_t*)mask, positions);
   return check_launch(what);
 }
 
@@ -135,11 +161,12 @@ extern "C" int kq_draft_accept(const void* tokens, const void* targets, int wide
   if (seqs == 0) return KQ_OK;
   const KvBatch b{nullptr, cu, nullptr, 0, (int)seqs, 0, (int)rows};
   hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)seqs), block((unsigned)std::min<int64_t>((most + 63) / 64 * 64, 256));
   if (wide)
-    hipLaunchKernelGGL((draft_accept_kernel<int64_t>), dim3((unsigned)seqs), dim3(64), 0, st, b, (const int64_t*)tokens,
+    hipLaunchKernelGGL((draft_accept_kernel<int64_t>), grid, block, 0, st, b, (const int64_t*)tokens,
                        (const int64_t*)targets, parents, (int)most, kept, counts, (int64_t*)following);
   else
-    hipLaunchKernelGGL((draft_accept_kernel<int32_t>), dim3((unsigned)seqs), dim3(64), 0, st, b, (const int32_t*)tokens,
+    hipLaunchKernelGGL((draft_accept_kernel<int32_t>), grid, block, 0, st, b, (const int32_t*)tokens,
                        (const int32_t*)targets, parents, (int)most, kept, counts, (int32_t*)following);
   return check_launch(what);
 }

@@ -130,6 +130,11 @@ KQ_DEV uint32_t tokens_from(int n) { return n <= 0 ? ~0u : n >= 32 ? 0u : ~0u <<
 // (l % 16, l / 16) holds scores of columns c of the MT tiles for tokens 4b..4b+3 of each 16,
 // which are what it hands over as its part of P^T.  Loads go from memory to registers through
 // resources of one page's tile that end at the sequence's last token.
+//
+// Bound by its chain of steps, not by bytes: the first loads wait for bounds, tiles and table
+// (4 us), a step takes 1.3 us and the merge 2.  One tree of 12 rows behind 900 tokens, 32 heads
+// over 8 of 128, eight waves to a tile: 13 us (1.9 MB, which 0.4 would do); 24 windows of 1024, 16
+// heads of 64: 16 us, 2.7 TB/s.
 template <int D, int DT, int NT, int PP, int MT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : D * MT <= 64 ? 3 : D * MT <= 256 ? 2 : 1)
 kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -498,6 +503,12 @@ constexpr float kTileLift = 9.0f, kTileMost = 65504.0f, kCoarse = 0x1p20f;
 // travel two steps ahead in registers, keys reach LDS a step before values, and
 // one barrier ends a step: it has read keys i + 1 and values i, and written keys i + 2 and
 // values i + 1 where keys i and values i - 1 were.
+//
+// MFMAs (39% busy), vector instructions (48%) and LDS (44%) bound it in turn, with two workgroups
+// to a CU by their registers: 32 tokens of 128 columns take a CU 1310 cycles of some 512 of MFMA.
+// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 210 us, 0.65 PFLOP/s
+// (0.75 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
+// 93 us, 0.46 PFLOP/s, as parts end unevenly and tiles are padded to 128.
 template <int D, int DT, int CG>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -870,7 +881,8 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
 }
 
 // The parts of split tiles joined in the order of their tokens: a workgroup takes COLS columns
-// of one tile, a thread four neighbouring d of each of E columns.
+// of one tile, a thread four neighbouring d of each of E columns.  Latency: finding the tile's parts,
+// then their loads, eight a thread on their way: 7 us for 16 trees, 11 for 32 with parts of 68 MB.
 template <int D, int DT, int TW>
 __global__ void __launch_bounds__(256)
 kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
@@ -1099,7 +1111,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
   // threads of one launch, and blocks of all tiles
   const int64_t tiles = empty ? 0 : rows * (heads / kv_heads) / p.columns + seqs;
   const int64_t blocks = tiles * ((table_width * page_size + 127) / 128);
-  if (rows * heads * 64 >= (1LL << 32) || blocks >= (1LL << 30)) {
+  if (rows * heads * 64 >= (1LL << 32) || tiles >= (1LL << 24) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
     return KQ_EINVAL;
