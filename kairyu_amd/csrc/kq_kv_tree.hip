@@ -29,6 +29,7 @@ struct TreeArgs {
   int shares;     // workgroups per kv head that the batch's tokens are dealt to
   int block_shift;  // log2 of the 64-token steps of a block
   int alike;      // whether every workgroup gets one part of one tile
+  int near;       // whether neighbouring shares go to one XCD
 };
 
 constexpr float kLift = 15.0f;  // log2 of the largest weight
@@ -78,29 +79,42 @@ struct TreeDeal {
   }
 };
 
+// Workgroups go to the 8 XCDs in turn: those of one take neighbouring shares, so that the tiles of
+// a tree that read the same tokens at the same time do so through one L2 (16 trees of 64 columns
+// behind 900 tokens 20.8 us, 24.1 in turn; 16 of 512 behind 6000 134 and 137).  Where several tiles of
+// a sequence are cut by runs, equal parts of them are far apart, and meet more often in turn (one tree
+// of 64 columns behind 16000 tokens 32 and 27).
+KQ_DEV int share_of(const TreeArgs& a, int x, int shares) {
+  if (!a.near || x >= shares) return x;
+  const int xcd = x & 7, each = shares >> 3, more = shares & 7;
+  return xcd * each + min(xcd, more) + (x >> 3);
+}
+
 // A workgroup's blocks: from `within` of `tile` of sequence s (-1: none) on, `end` - `block` of them.
 struct TreeRun {
-  int s, tile, within, blocks, block, end;
+  int share, s, tile, within, blocks, block, end;
   KvSeq q;
 };
 template <int TW>
-KQ_DEV TreeRun run_of(const TreeArgs& a, const KvLanes& lanes, const TreeDeal<TW>& deal, int share) {
+KQ_DEV TreeRun run_of(const TreeArgs& a, const KvLanes& lanes, const TreeDeal<TW>& deal, int x) {
   TreeRun r{};
   if (a.alike) {
     const int length = deal.length(lanes);
     int unit;
-    r.s = lanes.find(share, unit, [&](const KvSeq& q) { return deal.tiles(q) * deal.parts(q, length); });
+    r.share = share_of(a, x, a.shares);
+    r.s = lanes.find(r.share, unit, [&](const KvSeq& q) { return deal.tiles(q) * deal.parts(q, length); });
     if (r.s < 0) return r;
     r.q = lanes[r.s];
     r.blocks = deal.blocks(r.q);
-    const int parts = scalar(deal.parts(r.q, length));
-    r.tile = scalar(unit / parts);
-    r.within = (unit - r.tile * parts) * length;
+    const int tiles = scalar(deal.tiles(r.q)), nth = scalar(unit / tiles);  // (all tiles' first parts, then their second)
+    r.tile = unit - nth * tiles;
+    r.within = nth * length;
     r.end = min(length, r.blocks - r.within);
     return r;
   }
-  const int run = deal.run(lanes);
-  r.block = share * run;
+  const int all = deal.all(lanes), run = max(scalar((int)(((uint32_t)all + (uint32_t)a.shares - 1) / (uint32_t)a.shares)), 1);
+  r.share = share_of(a, x, scalar((int)((uint32_t)(all + run - 1) / (uint32_t)run)));  // (of those with blocks)
+  r.block = r.share * run;
   r.end = r.block + run;
   int unit;
   r.s = lanes.find(r.block, unit, deal);
@@ -459,7 +473,7 @@ kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restri
           l += part[D + 1] * f;
         }
         if (!whole) {
-          float* dst = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (old_within == 0)) * TW + 16 * m + col) * LD;
+          float* dst = a.part + ((((int64_t)head * a.shares + given.share) * 2 + (old_within == 0)) * TW + 16 * m + col) * LD;
           *(f32x2_t*)(dst + d) = f32x2_t{ox, oy};
           if (d == 0) *(f32x2_t*)(dst + D) = f32x2_t{most, l};
           continue;
@@ -836,7 +850,7 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
     if (h == 0) mine[D] = top, mine[D + 1] = sum;
     meet();
     const bool whole = part_blocks == blocks;
-    float* part = a.part + ((((int64_t)head * a.shares + (int)blockIdx.x) * 2 + (within == 0)) * TW) * LD;
+    float* part = a.part + ((((int64_t)head * a.shares + given.share) * 2 + (within == 0)) * TW) * LD;
 #pragma unroll 1
     for (int i = tid; i < TW * (D / 4); i += 256) {
       const int col = i / (D / 4), d = 4 * (i - col * (D / 4)), it = tile * TW + col;
@@ -898,13 +912,14 @@ kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
   if (tile * TW + column0 >= q.rows * group) return;
   // its parts and the workgroup of the first (within the shares also where row bounds that go
   // back make counts wrap)
-  int x0 = 0, chunks = 0;
+  int x0 = 0, chunks = 0, apart = 1;
   const int blocks = deal.blocks(q);
   if (a.alike) {
     const int length = deal.length(lanes), parts = scalar(deal.parts(q, length));
     lanes.of_row(q.row0, x0, [&](const KvSeq& p) { return deal.tiles(p) * deal.parts(p, length); });
-    x0 = min(max(x0 + tile * parts, 0), a.shares - 1);
-    chunks = min(parts, a.shares - x0);
+    x0 = min(max(x0 + tile, 0), a.shares - 1);
+    apart = scalar(deal.tiles(q));
+    chunks = min(parts, (int)((uint32_t)(a.shares - 1 - x0) / (uint32_t)apart) + 1);
   } else {
     const int run = max(deal.run(lanes), 1);
     int block = 0;  // blocks before the tile's
@@ -916,7 +931,7 @@ kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
   if (chunks == 1) return;  // written already
   // place 1 of the workgroup it begins in, then place 0 of those behind
   const float* src = a.part + ((((int64_t)head * a.shares + x0) * 2 + 1) * TW + column0) * LD;
-  auto at_part = [&](int i) { return src + (i == 0 ? 0 : (int64_t)(2 * i - 1) * TW) * LD; };
+  auto at_part = [&](int i) { return src + (i == 0 ? 0 : (int64_t)(2 * i * apart - 1) * TW) * LD; };
   float m[E], l[E];
   f32x4 x[E];
 #pragma unroll
@@ -979,7 +994,7 @@ struct TreePlan {
   int columns;  // of a tile: 16 or 32 (a wave holds them all), 64 or 128 (the workgroup does)
   int waves;    // of a workgroup
   int shares, block_shift;
-  bool alike;
+  bool alike, near;
   size_t part;  // bytes
 };
 
@@ -1003,6 +1018,7 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   const int64_t slots = 256 * (p.columns > 32 ? (dim == 256 ? 1 : 2) : p.waves == 8 ? 1 : dim * p.columns <= 1024 ? 3 : dim * p.columns <= 4096 ? 2 : 1);
   p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
   p.alike = p.columns > 16 && tiles(p.columns) <= p.shares * kv_heads;
+  p.near = p.alike || (whole ? each > p.columns : each <= p.columns);
   // parts of one length: blocks of a workgroup's two steps or so.  Runs: of 256 tokens, or of 512 where
   // those still give every workgroup one, so that tiles are cut less often
   p.block_shift = p.alike ? (p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
@@ -1126,7 +1142,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.heads = (int)heads, a.window = (int)window;
   a.most_blocks = (int)blocks;
-  a.shares = p.shares, a.block_shift = p.block_shift, a.alike = p.alike;
+  a.shares = p.shares, a.block_shift = p.block_shift, a.alike = p.alike, a.near = p.near;
   int shift = 4;
   while ((1 << shift) < page_size) ++shift;
   const KvCache c{(uint8_t*)k_cache, (uint8_t*)v_cache, (float*)k_scale, (float*)v_scale, pages, (int)kv_heads, shift};

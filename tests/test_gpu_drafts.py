@@ -78,6 +78,18 @@ def test_the_largest_tree(cuda, kind):
         assert kept[s, : len(nodes)].tolist() == nodes and int(counts[s]) == len(nodes) and int(following[s]) == after
 
 
+@pytest.mark.parametrize("window", [1, 31, 33, 500, 1 << 30])
+@pytest.mark.parametrize("most", [1024, 700, 65])
+def test_large_trees_in_windows(cuda, most, window):
+    banner(f"large draft trees {most} window {window}")
+    cu, lengths = dh.ints(0, 800, 1900, 1903), dh.ints(900, 1090, 3)  # (rows before the first token in the second)
+    for kind in ("tree", "chain"):
+        par = dh.parents([800, 1100, 3], 5, kind)
+        got = draft_tree(par.to(cuda), cu.to(cuda), lengths.to(cuda), most, window=window)
+        seen, positions = odr.tree(par, cu, lengths, most, window)
+        assert got.positions.tolist() == positions and torch.equal(got.mask.cpu(), odr.pack(seen, -(-most // 32)))
+
+
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("kind", ["tree", "chain", "star"])
 @pytest.mark.parametrize("batch", BATCHES)
