@@ -247,6 +247,7 @@ struct KeepArgs {
 };
 
 constexpr int kMostNodes = 1024;
+constexpr int kScales = 1024;  // of a sequence's pages that a workgroup holds in LDS
 
 // One workgroup a sequence and layer.  Token first + kept[i] goes to slot first + i, i in
 // steps of what the workgroup's threads hold: a step's codes are all in registers before
@@ -255,12 +256,12 @@ constexpr int kMostNodes = 1024;
 // A page's new scale is the largest of its tokens' old ones, so code * (old / new) is
 // rounded once, and is exact between powers of two but for codes that fall below e4m3's
 // normal range.  Which old pages a page's tokens come from is found once for all heads
-// (`sources`, a bit for each page behind the first), scales are read by those who need
-// them, and written last.
+// (`sources`, a bit for each page behind the first); scales are held in LDS where they fit (64
+// pages of 8 heads), else read by those who need them, and written last.
 //
-// Latency: bounds, kept tokens and pages, checks, codes and scales, one after the other.  One
-// sequence in 32 layers 7.8 us, 64 in 28 layers 10.6 (a workgroup to several heads' moves of all
-// tokens: 1792 of them, where bytes alone would take 2.4).
+// Latency: bounds, kept tokens and pages, checks and scales, codes, one after the other.  One
+// sequence in 32 layers 6.4 us, 64 in 28 layers 9.5, where bytes alone would take 2.4 (with scales
+// read where they are needed, four times in turn, 7.2 and 10.2).
 template <int DS>
 __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, KvBatch batch) {
   constexpr int CH = 1 << (DS - 4);  // 16-byte chunks of a token
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, Kv
   __shared__ int kept[kMostNodes];
   __shared__ int pages[SPAN];
   __shared__ uint32_t sources[SPAN][3];
+  __shared__ float olds[kScales], growns[kScales];  // [page][head][keys, values], where they fit
   __shared__ int stop;
   const int tid = (int)threadIdx.x, s = (int)blockIdx.x, shift = c.page_shift, in_page = (1 << shift) - 1;
   const KvSeq q = kv_seq_uniform(batch, s, shift);
@@ -285,6 +287,14 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, Kv
   }
   __syncthreads();
   auto slot_of = [&](int node) { return ((first + node) >> shift) - slot0; };
+  const KvLayer& layer = c.at[blockIdx.y];
+  const int heads = c.kv_heads, span = count > 0 && n > 0 ? slot_of(n - 1) + 1 : 0;
+  const bool fits = (int64_t)span * 2 * heads <= kScales;
+  if (fits)
+    for (int i = tid; i < span * 2 * heads; i += 256) {
+      const int page = pages[i / (2 * heads)], u = i % (2 * heads);
+      olds[i] = page < 0 ? 0.0f : (u & 1 ? layer.v_scale : layer.k_scale)[(int64_t)page * heads + (u >> 1)];
+    }
   for (int i = tid; i < count; i += 256) {
     const int node = kept[i];
     const bool good = node >= 0 && node < n && (i == 0 || kept[i - 1] < node) && i < n && pages[slot_of(node)] >= 0 && pages[slot_of(i)] >= 0;
@@ -299,28 +309,31 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, Kv
     atomicOr(&sources[slot_of(i)][from >> 5], 1u << (from & 31));
   }
   const int before = first & in_page, last_slot = slot_of(keep - 1);
-  __syncthreads();
-  if (tid == 0 && before > 0) sources[0][0] |= 1u;  // (its own earlier tokens)
+  if (tid == 0 && before > 0) atomicOr(&sources[0][0], 1u);  // (its own earlier tokens)
   __syncthreads();
 
-  const KvLayer& layer = c.at[blockIdx.y];
-  const int heads = c.kv_heads;
-  // the scale that page `to` gets
-  auto scale_of = [&](const float* scales, int to, int head) {
+  // u: 2 head, or 2 head + 1 for values.  The scale that a page has, and the one it gets.
+  auto old_of = [&](int slot, int u) {
+    if (fits) return olds[slot * 2 * heads + u];
+    return (u & 1 ? layer.v_scale : layer.k_scale)[(int64_t)pages[slot] * heads + (u >> 1)];
+  };
+  auto largest = [&](int to, int u) {
     float m = 0.0f;
 #pragma unroll
     for (int w = 0; w < 3; ++w)
-      for (uint32_t bits = sources[to][w]; bits != 0; bits &= bits - 1)
-        m = fmaxf(m, scales[(int64_t)pages[32 * w + __builtin_ctz(bits)] * heads + head]);
+      for (uint32_t bits = sources[to][w]; bits != 0; bits &= bits - 1) m = fmaxf(m, old_of(32 * w + __builtin_ctz(bits), u));
     return m;
   };
+  if (fits) {
+    for (int i = tid; i < (last_slot + 1) * 2 * heads; i += 256) growns[i] = largest(i / (2 * heads), i % (2 * heads));
+    __syncthreads();
+  }
+  auto grown_of = [&](int slot, int u) { return fits ? growns[slot * 2 * heads + u] : largest(slot, u); };
   // earlier tokens of the first page, where its scale grows
   if (before > 0) {
     for (int u = wave_id(); u < 2 * heads; u += 4) {
-      const int head = u >> 1;
-      const float* scales = u & 1 ? layer.v_scale : layer.k_scale;
-      const int64_t tile = (int64_t)pages[0] * heads + head;
-      const float old = scales[tile], grown = scale_of(scales, 0, head);
+      const int64_t tile = (int64_t)pages[0] * heads + (u >> 1);
+      const float old = old_of(0, u), grown = grown_of(0, u);
       if (old == grown) continue;
       uint8_t* codes = (u & 1 ? layer.v : layer.k) + (tile << (shift + DS));
       for (int i = lane_id(); i < before * CH; i += 64) *(u32x4*)(codes + 16 * i) = move16(*(const u32x4*)(codes + 16 * i), old / grown);
@@ -338,9 +351,8 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, Kv
       const int chunk = unit & (CH - 1), which = (unit >> (DS - 4)) & 1, rest = unit >> (DS - 3);
       const int i = rest / heads, head = rest - i * heads;
       const int node = kept[i], from = slot_of(node), to = slot_of(i);
-      const float* scales = which ? layer.v_scale : layer.k_scale;
       const int64_t src = (int64_t)pages[from] * heads + head, to_tile = (int64_t)pages[to] * heads + head;
-      const float old = scales[src], grown = scale_of(scales, to, head);
+      const float old = old_of(from, 2 * head + which), grown = grown_of(to, 2 * head + which);
       if (node == i && old == grown) continue;
       uint8_t* codes = which ? layer.v : layer.k;
       w[k] = *(const u32x4*)(codes + (src << (shift + DS)) + ((((first + node) & in_page) << DS) + 16 * chunk));
@@ -358,7 +370,7 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, Kv
   for (int u = tid; u < 2 * heads; u += 256) {
     float* scales = u & 1 ? layer.v_scale : layer.k_scale;
     for (int to = 0; to <= last_slot; ++to) {
-      const float grown = scale_of(scales, to, u >> 1);
+      const float grown = grown_of(to, u);
       scales[(int64_t)pages[to] * heads + (u >> 1)] = grown;
     }
   }
