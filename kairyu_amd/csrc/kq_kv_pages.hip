@@ -110,16 +110,16 @@ KQ_DEV WaveSums wave_sums(int mine, int* lds) {
 // order of rows and slots and free pages in their own, so that the result does not depend
 // on any order of threads.  Only reads the holders, which the second launch changes.
 //
-// Latency, some five trips to memory and as many barriers: 4.6 us for 8 new rows, 6 for 128.
-// One workgroup needs no order among several, but reads 8192 holders a step: where the first free
-// page is the last of a million, 231 us.
+// Latency, some five trips to memory and as many barriers: 5 us for 8 new rows, 6 for 128.
+// One workgroup needs no order among several, but reads 4096 holders a step: where the first free
+// pages are the last of a million, 298 us (231 with eight loads a thread, which cost 0.5 us in small pools).
 __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(ForkArgs a, int64_t pages, int shift) {
   __shared__ int lds[16];
   const int tid = (int)threadIdx.x, wave = scalar(wave_id());
   for (int s = tid; s < a.seqs; s += 1024) a.eldest[s] = 0x7fffffff;
   const int items = a.rows * a.slots;
   int found = 0;
-  constexpr int K = 8, SPAN = 1024 * K;
+  constexpr int K = 4, SPAN = 1024 * K;
   for (int64_t base = 0; base < pages && found < items; base += SPAN) {
     uint64_t free[K];
     int n = 0, held[K];  // (all on their way at once)

@@ -520,9 +520,9 @@ constexpr float kTileLift = 9.0f, kTileMost = 65504.0f, kCoarse = 0x1p20f;
 //
 // MFMAs (39% busy), vector instructions (48%) and LDS (44%) bound it in turn, with two workgroups
 // to a CU by their registers: 32 tokens of 128 columns take a CU 1310 cycles of some 512 of MFMA.
-// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 210 us, 0.65 PFLOP/s
-// (0.75 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
-// 93 us, 0.46 PFLOP/s, as parts end unevenly and tiles are padded to 128.
+// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 206 us, 0.67 PFLOP/s
+// (0.76 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
+// 92 us, 0.46 PFLOP/s, as parts end unevenly and tiles are padded to 128.
 template <int D, int DT, int CG>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -896,7 +896,8 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
 
 // The parts of split tiles joined in the order of their tokens: a workgroup takes COLS columns
 // of one tile, a thread four neighbouring d of each of E columns.  Latency: finding the tile's parts,
-// then their loads, eight a thread on their way: 7 us for 16 trees, 11 for 32 with parts of 68 MB.
+// then their loads, eight a thread on their way: 7 us for 16 trees of up to 24 rows, 11 for 32 of up to
+// 32 (28 MB of parts).
 template <int D, int DT, int TW>
 __global__ void __launch_bounds__(256)
 kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
