@@ -1020,9 +1020,9 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
   p.alike = p.columns > 16 && tiles(p.columns) <= p.shares * kv_heads;
   p.near = p.alike || (whole ? each > p.columns : each <= p.columns);
-  // parts of one length: blocks of a workgroup's two steps or so.  Runs: of 256 tokens, or of 512 where
+  // parts of one length: blocks of what a workgroup's loop takes at once.  Runs: of 256 tokens, or of 512 where
   // those still give every workgroup one, so that tiles are cut less often
-  p.block_shift = p.alike ? (p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
+  p.block_shift = p.alike ? (p.columns > 64 ? 0 : p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
   if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * p.columns * (dim + 4));
   return p;
@@ -1127,7 +1127,7 @@ extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, i
   }
   // threads of one launch, and blocks of all tiles
   const int64_t tiles = empty ? 0 : rows * (heads / kv_heads) / p.columns + seqs;
-  const int64_t blocks = tiles * ((table_width * page_size + 127) / 128);
+  const int64_t blocks = tiles * (((table_width * page_size - 1) >> (6 + p.block_shift)) + 1);
   if (rows * heads * 64 >= (1LL << 32) || tiles >= (1LL << 24) || blocks >= (1LL << 30)) {
     set_error("%s: %lld rows of %lld heads over up to %lld tokens are past the supported range", what, (long long)rows,
               (long long)heads, (long long)(table_width * page_size));
