@@ -1022,7 +1022,7 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   p.near = p.alike || (whole ? each > p.columns : each <= p.columns);
   // parts of one length: blocks of what a workgroup's loop takes at once.  Runs: of 256 tokens, or of 512 where
   // those still give every workgroup one, so that tiles are cut less often
-  p.block_shift = p.alike ? (p.columns > 64 ? 0 : p.columns > 32 ? 1 : 2) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
+  p.block_shift = p.alike ? (p.columns > 64 ? 0 : 1) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
   if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * p.columns * (dim + 4));
   return p;
