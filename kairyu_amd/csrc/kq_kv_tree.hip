@@ -163,7 +163,7 @@ KQ_DEV void give_way(int done, int all) {
 // Bound by its chain of steps, not by bytes: the first loads wait for bounds, tiles and table
 // (4 us), a step takes 1.3 us and the merge 2.  One tree of 12 rows behind 900 tokens, 32 heads
 // over 8 of 128, eight waves to a tile: 13 us (1.9 MB, which 0.4 would do); 24 windows of 1024, 16
-// heads of 64: 16 us, 2.7 TB/s.
+// heads of 64: 15.7 us, 2.8 TB/s.
 template <int D, int DT, int NT, int PP, int MT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : D * MT <= 64 ? 3 : D * MT <= 256 ? 2 : 1)
 kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -538,9 +538,9 @@ constexpr float kTileLift = 9.0f, kTileMost = 65504.0f, kCoarse = 0x1p20f;
 //
 // MFMAs (39% busy), vector instructions (48%) and LDS (44%) bound it in turn, with two workgroups
 // to a CU by their registers: 32 tokens of 128 columns take a CU 1310 cycles of some 512 of MFMA.
-// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 206 us, 0.67 PFLOP/s
-// (0.76 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
-// 92 us, 0.46 PFLOP/s, as parts end unevenly and tiles are padded to 128.
+// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 203 us, 0.68 PFLOP/s
+// (0.77 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
+// 91 us, 0.47 PFLOP/s, as parts end unevenly and tiles are padded to 128.
 template <int D, int DT, int CG>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
