@@ -24,11 +24,11 @@ draft_tree_kernel(KvBatch batch, const int32_t* __restrict__ parents, int most, 
   auto none = [&](int64_t row, int from_word) {
     for (int w = from_word; w >= 0; --w) mask[row * words + w] = 0;
   };
-  // rows of no sequence, dealt to the workgroups
+  // rows of no sequence, dealt to the workgroups (up to 2^32 threads, past what an int counts)
   const int last = batch.seqs > 0 ? min(max(batch.cu[batch.seqs], 0), batch.rows) : 0;
   const int begin = batch.seqs > 0 ? min(max(batch.cu[0], 0), last) : 0;
-  for (int i = (int)blockIdx.x * threads + tid; i < begin + batch.rows - last; i += (int)gridDim.x * threads) {
-    const int row = i < begin ? i : last + (i - begin);
+  for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < begin + batch.rows - last; i += (int64_t)gridDim.x * threads) {
+    const int64_t row = i < begin ? i : last + (i - begin);
     none(row, words - 1);
     positions[row] = -1;
   }
