@@ -485,7 +485,8 @@ size_t kq_kv_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_he
  * up to 32 words) is set.  A row whose position is negative sees nothing, and a row
  * that sees nothing is zero.  What kq_kv_attention says of values, scales, NaN keys
  * and ranges holds here (blocks: of all sequences, of 16, 32 or 64 rows).
- * Workspace: kq_kv_tree_attention_workspace_size bytes, of the call's own. */
+ * Workspace: kq_kv_tree_attention_workspace_size bytes (enough for any window), of the
+ * call's own. */
 int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,
                          int64_t kv_heads, int64_t dim, const uint8_t* k_cache, const uint8_t* v_cache,
                          const float* k_scale, const float* v_scale, int64_t pages, int64_t page_size,

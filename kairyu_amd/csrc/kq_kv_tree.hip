@@ -1019,6 +1019,16 @@ struct TreePlan {
   size_t part;  // bytes
 };
 
+// Workgroups that registers and LDS let a CU hold, on all of them.
+static int64_t tree_slots(int columns, int waves, int64_t dim) {
+  return 256 * (columns > 32 ? (dim == 256 ? 1 : 2) : waves == 8 ? 1 : dim * columns <= 1024 ? 3 : dim * columns <= 4096 ? 2 : 1);
+}
+static int tree_shares(int64_t slots, int64_t kv_heads) { return (int)std::max<int64_t>(slots / kv_heads, 1); }
+// Bytes of the parts of split tiles.
+static size_t tree_parts(int shares, int64_t kv_heads, int columns, int64_t dim) {
+  return sizeof(float) * (size_t)(shares * kv_heads * 2 * columns * (dim + 4));
+}
+
 // From what the host knows: rows and sequences, not their lengths.
 static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page_size, int64_t width,
                           int64_t seqs, int64_t window) {
@@ -1035,16 +1045,15 @@ static TreePlan tree_plan(int64_t rows, int64_t heads, int64_t kv_heads, int64_t
   // eight waves to a tile while there is at most one for a CU (four trees of 64 behind 900 tokens 14
   // us, with four waves 19; 16 of them 26 and 24)
   p.waves = whole && p.columns == 16 && tiles(16) <= 256 ? 8 : 4;
-  // workgroups that registers and LDS let a CU hold
-  const int64_t slots = 256 * (p.columns > 32 ? (dim == 256 ? 1 : 2) : p.waves == 8 ? 1 : dim * p.columns <= 1024 ? 3 : dim * p.columns <= 4096 ? 2 : 1);
-  p.shares = (int)std::max<int64_t>(slots / kv_heads, 1);
+  const int64_t slots = tree_slots(p.columns, p.waves, dim);
+  p.shares = tree_shares(slots, kv_heads);
   p.alike = p.columns > 16 && tiles(p.columns) <= p.shares * kv_heads;
   p.near = p.alike || (whole ? each > p.columns : each <= p.columns);
   // parts of one length: blocks of what a workgroup's loop takes at once.  Runs: of 256 tokens, or of 512 where
   // those still give every workgroup one, so that tiles are cut less often
   p.block_shift = p.alike ? (p.columns > 64 ? 0 : 1) : tiles(p.columns) * ((span + 511) / 512) >= slots ? 3 : 2;
   while (whole && (64LL << p.block_shift) < span) ++p.block_shift;  // (no tile in two blocks: they would need `part`)
-  if (!whole) p.part = sizeof(float) * (size_t)(p.shares * kv_heads * 2 * p.columns * (dim + 4));
+  if (!whole) p.part = tree_parts(p.shares, kv_heads, p.columns, dim);
   return p;
 }
 
@@ -1111,7 +1120,11 @@ using namespace kq;
 extern "C" size_t kq_kv_tree_attention_workspace_size(int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                                       int64_t page_size, int64_t table_width, int64_t seqs) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || dim < 1 || page_size < 1 || table_width < 0 || seqs < 0) return 0;
-  return tree_plan(rows, heads, kv_heads, dim, page_size, table_width, seqs, 0).part;  // (a window needs no more than none)
+  // A window changes the plan in two ways: tiles are read whole and need nothing (as all are that are
+  // whole without one), or they are of 16 columns where wider ones would be taken without it, which have
+  // more workgroups where the kv heads do not divide them (10 heads of 256: 51 of 16 columns, 25 of 32).
+  const size_t part = tree_plan(rows, heads, kv_heads, dim, page_size, table_width, seqs, 0).part;
+  return part == 0 ? 0 : std::max(part, tree_parts(tree_shares(tree_slots(16, 4, dim), kv_heads), kv_heads, 16, dim));
 }
 
 extern "C" int kq_kv_tree_attention(const void* q, int64_t q_ld, int64_t q_hs, int dtype, int64_t rows, int64_t heads,

@@ -1,4 +1,5 @@
-"""Drafts in the largest batches, where indices of threads pass 31 bits."""
+"""Calls of drafts at the ends of their ranges: the largest batches, where indices of threads pass
+31 bits, and heads that do not divide the workgroups."""
 
 from __future__ import annotations
 
@@ -6,7 +7,9 @@ import pytest
 import torch
 
 import draft_helpers as dh
+import kv_helpers as kv
 from gpu_helpers import banner
+from kairyu_amd.attention import DraftTree, tree_attention
 from kairyu_amd.drafts import draft_tree
 from oracle import drafts as odr
 
@@ -31,3 +34,21 @@ def test_trees_of_two_million_sequences(cuda, seqs):
         few = torch.tensor([0, *new]).cumsum(0) + lead  # (sequences without rows leave nothing)
         seen, positions = odr.tree(par, few, dh.ints(*total), 1024)
         assert got.positions.tolist() == positions and torch.equal(got.mask.cpu(), odr.pack(seen, 32))
+
+
+@pytest.mark.parametrize("heads", [(20, 10, 256), (12, 6, 256), (7, 7, 256)], ids=str)
+@pytest.mark.parametrize("window", [0, 64, 1024])
+def test_attention_where_kv_heads_do_not_divide_the_workgroups(cuda, heads, window):
+    """A window takes tiles of 16 columns, more of them than the wider ones without it."""
+    banner(f"tree attention {heads} window {window}")
+    (hq, hk, dim), new, total, page = heads, [20, 12], [1500, 300], 64
+    table, cu, lengths, rows, pages = kv.batch(new, total, page, seed=1)
+    pool = kv.cache(pages, hk, page, dim, seed=2)
+    kv.stain(pool, table, lengths)
+    tree, seen = dh.oracle_tree(dh.parents(new, 3), cu, lengths, max(new), window)
+    q = (torch.randn(rows, hq, dim, generator=kv.gen(4)) * 2).to(torch.bfloat16)
+    table = torch.nn.functional.pad(table, (0, 65536 // page - table.shape[1]), value=-1)
+    out = tree_attention(q.to(cuda), kv.to(pool, cuda), table.to(cuda), cu.to(cuda), lengths.to(cuda),
+                         DraftTree(*(t.to(cuda) for t in tree)), window=window)
+    torch.cuda.synchronize()
+    dh.check_attention(out, q, pool, table, cu, lengths, seen, tree.positions, window=window)
