@@ -32,12 +32,20 @@ __all__ = ["KvCaches", "copy_pages", "fork_sequences"]
 
 class KvCaches:
     """The caches of a model's layers, alike in shape and device, made once and kept by
-    the program: pages, tables and lengths are the same for all of them."""
+    the program: pages, tables and lengths are the same for all of them.
+
+    It stands for the memory that the tensors have when it is made, and keeps that alive: a tensor
+    that is given other memory afterwards (``.data =``, ``set_``, a move to another device) needs
+    a new one, and the memory itself must not be resized under it."""
 
     __slots__ = ("layers", "shape", "device", "pointers")
 
     def __init__(self, layers: Sequence[PagedKvCache]) -> None:
-        self.layers = tuple(layers)
+        self._take(tuple(layers))
+        self.layers = tuple(PagedKvCache._make([t.detach() for t in cache]) for cache in self.layers)
+
+    def _take(self, layers: tuple[PagedKvCache, ...]) -> None:
+        self.layers = layers
         if not self.layers:
             raise ValueError("KvCaches needs at least one layer's cache")
         self.shape, self.device = _check_cache(self.layers[0]), self.layers[0].k.device
@@ -59,7 +67,11 @@ def _addresses(n: int):
 
 
 def caches_of(caches: PagedKvCache | KvCaches) -> KvCaches:
-    return caches if isinstance(caches, KvCaches) else KvCaches((caches,))
+    if isinstance(caches, KvCaches):
+        return caches
+    one = KvCaches.__new__(KvCaches)  # (of this call only, so over the tensors themselves)
+    one._take((caches,))
+    return one
 
 
 def check_ints(device: torch.device, **tensors) -> None:
