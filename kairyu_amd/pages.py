@@ -34,18 +34,14 @@ class KvCaches:
     """The caches of a model's layers, alike in shape and device, made once and kept by
     the program: pages, tables and lengths are the same for all of them.
 
-    It stands for the memory that the tensors have when it is made, and keeps that alive: a tensor
-    that is given other memory afterwards (``.data =``, ``set_``, a move to another device) needs
-    a new one, and the memory itself must not be resized under it."""
+    Launches go by the addresses that the tensors have when it is made, and it keeps that memory
+    alive.  Where a tensor is given other memory afterwards (``.data =``, ``set_``, a move to another
+    device) a new one has to be made, and the memory itself must not be resized under it."""
 
-    __slots__ = ("layers", "shape", "device", "pointers")
+    __slots__ = ("layers", "shape", "device", "pointers", "memory")
 
     def __init__(self, layers: Sequence[PagedKvCache]) -> None:
-        self._take(tuple(layers))
-        self.layers = tuple(PagedKvCache._make([t.detach() for t in cache]) for cache in self.layers)
-
-    def _take(self, layers: tuple[PagedKvCache, ...]) -> None:
-        self.layers = layers
+        self.layers = tuple(layers)
         if not self.layers:
             raise ValueError("KvCaches needs at least one layer's cache")
         self.shape, self.device = _check_cache(self.layers[0]), self.layers[0].k.device
@@ -59,6 +55,7 @@ class KvCaches:
         if self.shape[0] and len(set(at)) != len(at):
             raise ValueError("the layers' caches must be different tensors")
         self.pointers = _addresses(len(at))(*at)
+        self.memory = [t.untyped_storage() for cache in self.layers for t in cache]
 
 
 @lru_cache(maxsize=None)
@@ -67,11 +64,7 @@ def _addresses(n: int):
 
 
 def caches_of(caches: PagedKvCache | KvCaches) -> KvCaches:
-    if isinstance(caches, KvCaches):
-        return caches
-    one = KvCaches.__new__(KvCaches)  # (of this call only, so over the tensors themselves)
-    one._take((caches,))
-    return one
+    return caches if isinstance(caches, KvCaches) else KvCaches((caches,))
 
 
 def check_ints(device: torch.device, **tensors) -> None:
