@@ -112,7 +112,8 @@ KQ_DEV WaveSums wave_sums(int mine, int* lds) {
 //
 // Latency, some five trips to memory and as many barriers: 4.4 us for 8 new rows, 5 for 128.
 // One workgroup needs no order among several, but reads 4096 holders a step: where the first free
-// pages are the last of a million, 298 us (231 with eight loads a thread, which cost 0.5 us in small pools).
+// pages are the last of 65536, a whole call takes 24 us in a graph (9 with free pages in front), of a million
+// 298 (231 with eight loads a thread, which cost 0.5 us in small pools).
 __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(ForkArgs a, int64_t pages, int shift) {
   __shared__ int lds[16];
   const int tid = (int)threadIdx.x, wave = scalar(wave_id());
@@ -184,7 +185,8 @@ __global__ void __launch_bounds__(1024) kv_fork_plan_kernel(ForkArgs a, int64_t 
 
 // The first `tables` workgroups: the other entries of the new table, and the holders (sums
 // of whole numbers, in any order).  The others: half-filled pages, keys or values of one layer each.
-// Latency for few rows (8 in 32 layers 5.8 us), then HBM: 128 rows in 16 layers 12.5 us.
+// Latency for few rows (8 in 32 layers 5.8 us), then HBM: 128 rows in 16 layers 12.9 us.  These, and the
+// plan's above, are one kernel's times under the profiler; both launches in a graph take 9.0 and 20.
 __global__ void __launch_bounds__(256) kv_fork_kernel(ForkArgs a, KvLayers c, int tables, int layers) {
   const int shift = c.page_shift;
   if ((int)blockIdx.x < tables) {
@@ -260,8 +262,8 @@ constexpr int kScales = 1024;  // of a sequence's pages that a workgroup holds i
 // pages of 8 heads), else read by those who need them, and written last.
 //
 // Latency: bounds, kept tokens and pages, checks and scales, codes, one after the other.  One
-// sequence in 32 layers 6.4 us, 64 in 28 layers 9.5, where bytes alone would take 2.4 (with scales
-// read where they are needed, four times in turn, 7.2 and 10.2).
+// sequence in 32 layers 6.3 us, 64 in 28 layers 9.3, where bytes alone would take 2.4 (with scales
+// read where they are needed, four times in turn, 7.2 and 10.2), in a graph.
 template <int DS>
 __global__ void __launch_bounds__(256) kv_keep_kernel(KeepArgs a, KvLayers c, KvBatch batch) {
   constexpr int CH = 1 << (DS - 4);  // 16-byte chunks of a token

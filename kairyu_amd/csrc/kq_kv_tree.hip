@@ -7,7 +7,11 @@
 // log2 v_scale, exp2(w_t - max w + lift) in fp16 (11 bits down to 2^-29 of the largest and
 // some down to 2^-40, in tiles of 64 and 128 columns 2^-23 and 2^-34) times the value's codes,
 // the denominator in fp32 from weights not yet rounded over v_scale, maxima, denominators and
-// outputs in fp32.
+// outputs in fp32.  The width of a tile follows the batch, so that a tree's last bits may differ
+// from one batch to another.
+//
+// Times are of calls in a captured graph, joins included, unless they are said to be of one kernel
+// under the profiler, where kernels take up to a tenth longer.
 #include "kq_kv_attend.h"
 
 #include <algorithm>
@@ -160,10 +164,12 @@ KQ_DEV void give_way(int done, int all) {
 // which are what it hands over as its part of P^T.  Loads go from memory to registers through
 // resources of one page's tile that end at the sequence's last token.
 //
-// Bound by its chain of steps, not by bytes: the first loads wait for bounds, tiles and table
-// (4 us), a step takes 1.3 us and the merge 2.  One tree of 12 rows behind 900 tokens, 32 heads
-// over 8 of 128, eight waves to a tile: 13 us (1.9 MB, which 0.4 would do); 24 windows of 1024, 16
-// heads of 64: 15.7 us, 2.8 TB/s.
+// Bound by its chain of steps, not by bytes.  One tree of 12 rows behind 900 tokens, 32 heads over
+// 8 of 128, eight waves to a tile: 13.2 us (1.9 MB, which 0.4 would do).  Of them, by time stamps, 0.5 are
+// bounds and padding, 0.7 the deal, 2.4 table, pages and the first keys, 2.2 the rest of the first step (its
+// values, the next step's keys), 2.0 the second, 2.1 until all waves' parts are in LDS, 1.0 merge and
+// store, and 2.2 lie between the end of one launch and the start of the next.  24 windows of 1024, 16 heads of
+// 64: 15.5 us, 3.0 TB/s.
 template <int D, int DT, int NT, int PP, int MT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : D * MT <= 64 ? 3 : D * MT <= 256 ? 2 : 1)
 kv_tree_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -538,9 +544,10 @@ constexpr float kTileLift = 9.0f, kTileMost = 65504.0f, kCoarse = 0x1p20f;
 //
 // MFMAs (39% busy), vector instructions (48%) and LDS (44%) bound it in turn, with two workgroups
 // to a CU by their registers: 32 tokens of 128 columns take a CU 1310 cycles of some 512 of MFMA.
-// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 203 us, 0.68 PFLOP/s
-// (0.77 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32 over 4:
-// 91 us, 0.47 PFLOP/s, as parts end unevenly and tiles are padded to 128.
+// Two trees of 48 rows behind 100000 tokens, 28 heads over 4 of 128: 186 to 192 us on different cards,
+// 0.72 PFLOP/s in the middle (0.83 with the columns past 336 that pad the last tile); 32 of up to 32 behind up to 6000, 32
+// over 4: 93 us, 0.46 PFLOP/s, as parts end unevenly and tiles are padded to 128.  Joins are 11 us of each
+// under the profiler.
 template <int D, int DT, int CG>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __restrict__ table,
@@ -916,8 +923,8 @@ kv_tree_tiles_kernel(TreeArgs a, KvCache cache, KvBatch batch, const int32_t* __
 
 // The parts of split tiles joined in the order of their tokens: a workgroup takes COLS columns
 // of one tile, a thread four neighbouring d of each of E columns.  Latency: finding the tile's parts,
-// then their loads, eight a thread on their way: 7 us for 16 trees of up to 24 rows, 11 for 32 of up to
-// 32 (28 MB of parts).
+// then their loads, eight a thread on their way: 7.5 us for 16 trees of up to 24 rows, 12 for 32 of up to
+// 32 (28 MB of parts), both under the profiler.
 template <int D, int DT, int TW>
 __global__ void __launch_bounds__(256)
 kv_tree_join_kernel(TreeArgs a, KvCache cache, KvBatch batch) {
@@ -1008,7 +1015,8 @@ constexpr int64_t kFewBlocks = 2560;
 // tiles of 16 (one tree of 48 behind 900 tokens 13 us, cut 14; 48 of 64 behind up to 900, in tiles of
 // 64, 39 and 51), and under a window, which makes the tiles alike, where they fill the chip (24
 // windows of 1024, 16 heads of 64: 16 us whole, 23 cut).  By the table's width, which is all that
-// the host knows.
+// the host knows; under a window by the batch's rows in place of a sequence's, so that the form changes with
+// the batch (of such trees of 16 rows 60 are whole, 29.3 us, and 61 cut, 32.5; 128 take 67, their bytes 58).
 constexpr int64_t kWhole = 1024, kWholeMany = 2048;
 
 struct TreePlan {
